@@ -2,7 +2,8 @@
 (attention launchers, dense and paged), include/crane_layer.h (the decoder
 layer's row kernels), include/crane_gemm.h (the QKV / o_proj projections), include/crane_sampling.h
 (argmax, top-k), include/crane_few.h (a decode step's projections at one
-sequence), include/crane_kv.h (host-side KV-cache manager) and
+sequence), include/crane_shared.h (attention over pages that sequences share,
+page copies), include/crane_kv.h (host-side KV-cache manager) and
 include/crane_pkv.h (paged KV-cache manager).
 
 The library is the only compute path: there is no CPU fallback.  Loading
@@ -102,6 +103,12 @@ SIGNATURES = {
     "crane_few_attn_linear_supported": ([_i64, _i, _i64, _i], _i),
     "crane_few_attn_linear": ([_vp, _vp, _vp, _i64, _vp, _i64, _i, _i, _i, _f, _i, _vp, _sz, _vp, _vp, _vp, _i64, _i, _vp],
                               _i),
+    # include/crane_shared.h
+    "crane_hip_attn_shared_workspace": ([_i, _i, _i64, _i64, _i, _i, _i, _i, _i, _i], _sz),
+    "crane_hip_attn_shared_paged": (
+        [_vp, _vp, _vp, _i64, _i, _i32p, _i64, _i32p, _i64, _i32p, _i32p, _i32p, _i, _i, _i64, _i64,
+         _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp, _i, _vp], _i),
+    "crane_hip_copy_pages": ([_vpp, _i, _i64, _i, _i, _i, _i32p, _i32p, _i32p, _i, _i, _vp], _i),
     # include/crane_pkv.h
     "crane_pkv_create": ([_i, _i, _i, _i, _i64, _i, _i, _vpp], _i),
     "crane_pkv_destroy": ([_vp], None),

@@ -11,9 +11,10 @@ fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -461,6 +462,131 @@ def attention_prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
         out.data_ptr(), dt, _stream(dev))
     check(rc, "attention_prefill_paged")
     return out
+
+
+# ----------------------------------------------------- sequences that share pages
+# include/crane_shared.h: attention in which the rows a group of sequences has in
+# common are read once for the group, and copies of rows between pages.
+
+class PrefixGroups:
+    """Which sequences of a batch share their first rows (prefix_groups makes and
+    checks it): per-sequence shared rows and the groups' members on the device, and
+    their host-side bounds.  Kept for as long as the batch and its sharing stay."""
+
+    def __init__(self, batch: int, shared_rows, group_start, group_seq, n_groups: int, max_group: int,
+                 max_shared: int, min_shared: int):
+        self.batch, self.shared_rows, self.group_start, self.group_seq = batch, shared_rows, group_start, group_seq
+        self.n_groups, self.max_group = n_groups, max_group
+        self.max_shared, self.min_shared = max_shared, min_shared
+
+
+def prefix_groups(groups: Sequence[Sequence[int]], rows: Sequence[int], batch: int,
+                  device: Optional[torch.device] = None) -> PrefixGroups:
+    """groups[g]: the batch rows whose first rows[g] cache rows are the same rows
+    (their block tables name the same pages there).  A sequence is in one group at
+    most; sequences in none share nothing.  Copies three small arrays to the device
+    and waits for them."""
+    if len(groups) != len(rows):
+        raise CraneHipError(_lib.E_INVALID, f"{len(groups)} groups, {len(rows)} row counts")
+    shared, start, seq, seen = [0] * batch, [0], [], set()
+    for members, n in zip(groups, rows):
+        if n < 0 or n > 0x7fffffff or not len(members):
+            raise CraneHipError(_lib.E_INVALID, "a group has members and shares 0 or more rows")
+        for b in members:
+            if not 0 <= b < batch or b in seen:
+                raise CraneHipError(_lib.E_INVALID, f"sequence {b}: not in a batch of {batch}, or in two groups")
+            seen.add(b)
+            shared[b] = int(n)
+            seq.append(int(b))
+        start.append(len(seq))
+    dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    flat = torch.tensor(shared + start + seq, dtype=torch.int32).to(dev)
+    return PrefixGroups(batch, flat[:batch], flat[batch:batch + len(start)], flat[batch + len(start):], len(groups),
+                        max(map(len, groups), default=0), max(shared, default=0), min(shared, default=0))
+
+
+def _on_device(dev: torch.device):
+    """The device of a launch made current: a default stream's handle does not say
+    which device it is on."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                           kv_len: torch.Tensor, max_kv: int, groups: PrefixGroups, scale: Optional[float] = None,
+                           causal: bool = True, max_own: Optional[int] = None,
+                           workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of every sequence's last tokens over a paged cache whose sequences
+    share their first rows: q [B, Hq, D] (one token each, a decode step) gives
+    [B, 1, Hq*D], q [B, Hq, S, D] gives [B, S, Hq*D].  kv_len counts the S new rows;
+    with causal query i sees the rows up to its own, else all kv_len.  max_own:
+    host-side bound of kv_len - shared rows (default: what max_kv leaves).
+
+    The shared rows are read once per group.  Scores and softmax stay in f32, where
+    attention_decode_paged rounds every score as candle does."""
+    dev = _dev(q, k_pool, v_pool, block_table, kv_len, groups.shared_rows, workspace)
+    if q.dim() not in (3, 4) or q.shape[-1] != HEAD_DIM:
+        raise CraneHipError(_lib.E_HEAD_DIM if q.dim() in (3, 4) else _lib.E_INVALID,
+                            "q must be [B, Hq, 128] or [B, Hq, S, 128]")
+    B, Hq = q.shape[:2]
+    S = q.shape[2] if q.dim() == 4 else 1
+    n_pages, Hkv, page_rows, stride = _paged_args(k_pool, v_pool, block_table, B, q.dtype)
+    _contig(q, "q")
+    dt = _dtype_code(q)
+    _i32(kv_len, B, "kv_len")
+    if groups.batch != B:
+        raise CraneHipError(_lib.E_INVALID, f"groups of a batch of {groups.batch}, q of {B}")
+    if max_own is None:
+        max_own = max(max_kv - groups.min_shared, 0)
+    scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+    need = int(_lib.lib().crane_hip_attn_shared_workspace(groups.n_groups, groups.max_group, groups.max_shared, max_own,
+                                                          B, S, Hq, Hkv, HEAD_DIM, dt))
+    # Allocated per call, not kept per stream: a captured graph keeps its own.
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    out = torch.empty((B, S, Hq * HEAD_DIM), dtype=q.dtype, device=dev)
+    with _on_device(dev):
+        rc = _lib.lib().crane_hip_attn_shared_paged(
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, page_rows, block_table.data_ptr(), stride,
+            kv_len.data_ptr(), max_kv, groups.shared_rows.data_ptr(), groups.group_start.data_ptr(),
+            groups.group_seq.data_ptr(), groups.n_groups, groups.max_group, groups.max_shared, max_own, B, S, Hq, Hkv,
+            HEAD_DIM, scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace),
+            workspace.numel() * workspace.element_size() if workspace is not None else 0, out.data_ptr(), dt,
+            _stream(dev))
+    check(rc, "attention_shared_paged")
+    return out
+
+
+def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int],
+               rows: Optional[Sequence[int]] = None) -> None:
+    """Copy the first rows[i] rows (default: all) of page src[i] to page dst[i] in
+    every pool [n_pages, Hkv, page_rows, D]: the K and V pools of one layer or of
+    all.  A page may be copied to several; a destination is named once and is no
+    copy's source.  src, dst and rows are host lists."""
+    if len(src) != len(dst) or (rows is not None and len(rows) != len(src)):
+        raise CraneHipError(_lib.E_INVALID, "src, dst and rows must have one entry per copy")
+    if not len(pools) or not len(src):
+        return
+    first = pools[0]
+    dev = _dev(*pools)
+    if first.dim() != 4 or first.shape[3] != HEAD_DIM:
+        raise CraneHipError(_lib.E_INVALID, "pools must be [n_pages, Hkv, page_rows, D]")
+    for p in pools:
+        _contig(p, "pool")
+        if p.dtype != first.dtype:
+            raise CraneHipError(_lib.E_DTYPE, f"pool dtypes {p.dtype} and {first.dtype}")
+        if p.shape != first.shape:
+            raise CraneHipError(_lib.E_INVALID, "pools must have one shape")
+    n_pages, Hkv, page_rows, _ = first.shape
+    for ids, most in ((src, n_pages - 1), (dst, n_pages - 1), (rows or (), page_rows)):
+        if len(ids) and not 0 <= min(ids) <= max(ids) <= most:
+            raise CraneHipError(_lib.E_INVALID, f"{n_pages} pages of {page_rows} rows: {list(ids)}")
+    ints = lambda x: (ctypes.c_int32 * len(x))(*x)  # noqa: E731
+    ptrs = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
+    with _on_device(dev):
+        rc = _lib.lib().crane_hip_copy_pages(ptrs, len(pools), n_pages, page_rows, Hkv, HEAD_DIM, ints(src), ints(dst),
+                                             ints(rows) if rows is not None else None, len(src), _dtype_code(first),
+                                             _stream(dev))
+    check(rc, "copy_pages")
 
 
 # ------------------------------------------------------- decoder-layer rows

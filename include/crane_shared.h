@@ -1,0 +1,91 @@
+/*
+ * crane_shared.h -- C ABI of the operators for sequences that share pages of a
+ * paged KV cache (gfx950): attention in which the rows a group of sequences has
+ * in common are read and multiplied once for the whole group, and copies of rows
+ * between pages of a pool (a forked sequence's partial page, a compaction).
+ *
+ * Crane has no counterpart: every sequence holds its own K/V rows
+ * (Attention.kv_cache, qwen3/modeling.rs:173-176), so n requests behind one
+ * system prompt hold and read its rows n times.  crane_pkv.h has the manager
+ * that shares pages and calls these launchers.  Conventions are those of
+ * crane_hip.h: 0 or a CRANE_HIP_E_* status, arguments checked on the host before
+ * anything is enqueued, nothing allocated or synchronised, everything ordered on
+ * `stream`.
+ */
+#ifndef CRANE_SHARED_H
+#define CRANE_SHARED_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Bytes of workspace crane_hip_attn_shared_paged needs for these sizes (the
+ * arguments of the call); 0 where the call would be rejected or has nothing to
+ * do. */
+size_t crane_hip_attn_shared_workspace(int n_groups, int max_group, int64_t max_shared, int64_t max_own, int B, int S,
+                                       int Hq, int Hkv, int D, int dtype);
+
+/* Attention of the last S rows of every sequence over its rows of the pools, the
+ * rows shared by a group read once for the group.
+ *
+ * q        [B, Hq, S, D] (S = 1: a decode step's [B, Hq, D])
+ * k_pool, v_pool, n_pages, page_rows, block_table, table_stride: as in
+ *          crane_hip_attn_decode_paged; a page id outside [0, n_pages) reads as
+ *          zero rows
+ * kv_len   [B] int32, device: rows of every sequence, its S new ones included;
+ *          query i sits at row kv_len[b] - S + i.  kv_len[b] <= max_kv
+ * shared_rows [B] int32, device: sequence b shares its first shared_rows[b] rows
+ *          (0: none) with every member of its group; any number, not only whole
+ *          pages.  NULL when n_groups is 0
+ * group_start [n_groups + 1], group_seq [group_start[n_groups]] int32, device:
+ *          the members of group g are the batch rows group_seq[group_start[g] ..
+ *          group_start[g + 1]), read through the first one's row of the block
+ *          table.  A sequence with shared rows is in exactly one group, whose
+ *          members all have its shared_rows; other sequences are in none.  A
+ *          description that breaks this gives unspecified results for the
+ *          sequences concerned and stays in bounds
+ * max_group, max_shared, max_own: host-side bounds of a group's members, of
+ *          shared_rows, and of kv_len[b] - shared_rows[b]; rows past them need not
+ *          be attended.  max_shared + max_own < 2^31 - 2^14
+ * flags    CRANE_HIP_PREFILL_CAUSAL: query i sees rows [0, kv_len[b] - S + i];
+ *          0: every query sees all kv_len[b] rows.  A query that sees none gets
+ *          zeros.  Rows a query does not see have no influence on it, whatever
+ *          they hold
+ * workspace device scratch of at least crane_hip_attn_shared_workspace(...) bytes,
+ *          16-byte aligned, any contents; calls that overlap in time must not
+ *          share one.  May be NULL when that is 0
+ * out      [B, S, Hq*D]
+ *
+ * The scores, their softmax and all sums are f32 and only the probabilities (bf16
+ * calls) are rounded before the product with V: candle's rounding of every score
+ * to the model dtype, which crane_hip_attn_decode reproduces, is not part of this
+ * call, so the two agree to that rounding and not bit for bit.  The order of the
+ * sums follows the host-side bounds and the group sizes; two runs of one call
+ * give the same bits. */
+int crane_hip_attn_shared_paged(const void* q, const void* k_pool, const void* v_pool, int64_t n_pages, int page_rows,
+                                const int32_t* block_table, int64_t table_stride, const int32_t* kv_len, int64_t max_kv,
+                                const int32_t* shared_rows, const int32_t* group_start, const int32_t* group_seq,
+                                int n_groups, int max_group, int64_t max_shared, int64_t max_own, int B, int S, int Hq,
+                                int Hkv, int D, float scale, int flags, void* workspace, size_t ws_bytes, void* out,
+                                int dtype, void* stream);
+
+/* Copy rows [0, rows[i]) of page src[i] to page dst[i] (all heads), i < n, in
+ * every one of n_pools pools [n_pages, Hkv, page_rows, D] (the K and V pools of
+ * one or of all layers).
+ *
+ * pools, src, dst, rows: HOST arrays, read before the call returns; rows may be
+ *          NULL (whole pages).  pools[i] is device memory, 16-byte aligned, each
+ *          a pool of its own
+ * A page may be the source of several copies; a destination is named once and is
+ * no copy's source (CRANE_HIP_E_INVALID otherwise).  Rows of dst[i] past rows[i]
+ * keep what they hold. */
+int crane_hip_copy_pages(void* const* pools, int n_pools, int64_t n_pages, int page_rows, int Hkv, int D,
+                         const int32_t* src, const int32_t* dst, const int32_t* rows, int n, int dtype, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* CRANE_SHARED_H */

@@ -1,0 +1,498 @@
+"""Attention over pages that sequences share and page copies (include/crane_shared.h).
+
+Crane has no counterpart of either, so the reference is the definition in 64 bits:
+every sequence by itself over its own rows.  Two kinds of inputs:
+
+  exact  q = 0 and V of -1 and 1: every weight is 1, all sums are whole numbers below
+         2^24, and the result is T(f32(sum) / f32(count)) to the last bit.  A key
+         lost, taken twice or taken past a row's limit changes it (by at least
+         1 / count, against values of about count^-1/2 whose rounding is 2^-8 of
+         that).
+  close  normal q, K, V with element-wise bounds (bounds() derives them).
+
+Pool rows that no query may see hold NaN."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+import cases
+
+D = 128
+U32, U16 = 2.0 ** -24, 2.0 ** -8  # half a step of f32 and bf16, relative
+
+
+# ------------------------------------------------------------------ inputs
+
+def layout(seed, lens, groups, rows, P, spare=2):
+    """Tables on shuffled pages: a group's members name the same pages for its first
+    rows[g] rows (up to the page that rows[g] ends in, when they have rows past it in
+    other pages only; else the caller passes whole pages or identical sequences)."""
+    r = cases.rng(seed)
+    B = len(lens)
+    width = max(1, max(math.ceil(n / P) for n in lens)) + 1
+    total = sum(math.ceil(n / P) for n in lens) + sum(math.ceil(x / P) for x in rows) + spare
+    perm = r.permutation(total).astype(np.int32)
+    table = np.full((B, width), -1, np.int32)
+    at = 0
+    for members, n in zip(groups, rows):
+        pages = math.ceil(n / P)
+        for b in members:
+            table[b, :pages] = perm[at:at + pages]
+        at += pages
+    for b, n in enumerate(lens):
+        for i in range(math.ceil(n / P)):
+            if table[b, i] < 0:
+                table[b, i] = perm[at]
+                at += 1
+    for b, n in enumerate(lens):  # entries past a sequence's rows are of no page
+        table[b, math.ceil(n / P):] = -7
+    return table, total
+
+
+def pools(seed, total, Hkv, P, table, lens, exact):
+    """K and V pools: NaN but for the rows some sequence holds."""
+    r = cases.rng(seed)
+    k = np.full((total, Hkv, P, D), np.nan, np.float32)
+    v = np.full_like(k, np.nan)
+    for b, n in enumerate(lens):
+        for i in range(math.ceil(n / P)):
+            m = min(P, n - i * P)
+            page = table[b, i]
+            fresh = np.isnan(k[page, 0, :m, 0])
+            if exact:
+                kk, vv = cases.normal(r, (Hkv, m, D)), r.integers(0, 2, (Hkv, m, D)).astype(np.float32) * 2 - 1
+            else:
+                kk, vv = cases.normal(r, (Hkv, m, D)), cases.normal(r, (Hkv, m, D))
+            k[page][:, :m][:, fresh] = kk[:, fresh]
+            v[page][:, :m][:, fresh] = vv[:, fresh]
+    return k, v
+
+
+def rows_of(pool, table, b, n, P):
+    return np.concatenate([pool[table[b, i], :, :min(P, n - i * P)] for i in range(math.ceil(n / P))], 1) \
+        if n else pool[0, :, :0]
+
+
+def reference(q, k, v, table, lens, P, scale, causal):
+    """(out [B, S, Hq D], sum of w |v| of the same shape, largest sum |q k| scale) in
+    float64."""
+    B, Hq, S, _ = q.shape
+    Hkv = k.shape[1]
+    G = Hq // Hkv
+    out = np.zeros((B, S, Hq, D))
+    mag = np.zeros_like(out)
+    most = 0.0
+    for b, n in enumerate(lens):
+        kb, vb = (rows_of(x, table, b, n, P).astype(np.float64) for x in (k, v))
+        for h in range(Hq):
+            for s in range(S):
+                L = n - S + 1 + s if causal else n
+                if L <= 0:
+                    continue
+                x, kk, vv = q[b, h, s].astype(np.float64), kb[h // G, :L], vb[h // G, :L]
+                sc = kk @ x * scale
+                w = np.exp(sc - sc.max())
+                w /= w.sum()
+                out[b, s, h] = w @ vv
+                mag[b, s, h] = w @ np.abs(vv)
+                most = max(most, float((np.abs(kk) @ np.abs(x)).max()) * scale)
+    return out.reshape(B, S, -1), mag.reshape(B, S, -1), most
+
+
+def bounds(out, mag, most, n, dtype):
+    """|kernel - exact| per element.  With weights w (1 + d), |d| <= e, over their own
+    sum: |o' - o| <= e / (1 - e) (sum w |v| + |o|).  e: bf16 rounds every weight once,
+    2^-8.  f32 arithmetic, for both types: a 128-term product errs by at most 128 half
+    steps of sum |q k| scale, its scaling and the reference's subtraction by 4 more
+    (the exponent's size is at most twice that sum, log2 e < 2), and an exponent's
+    error is the weight's relative one; exp2 2 steps; the sums' order n half steps
+    each, the joins' scalings 16.  The result is rounded once."""
+    e = U32 * (2 * 132 * most + 4 + 2 * n + 16) + (U16 if dtype == "bf16" else 0)
+    last = U16 if dtype == "bf16" else U32
+    return e / (1 - e) * (mag + np.abs(out)) * (1 + last) + last * np.abs(out) + 1e-30
+
+
+def tens(x, dtype, dev):
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(x))
+    return (t.to(torch.bfloat16) if dtype == "bf16" else t).to(dev)
+
+
+def ints(x, dev):
+    import torch
+    return torch.as_tensor(np.asarray(x, np.int32), device=dev)
+
+
+def call(gpu, q, k, v, table, lens, groups, rows, dtype, **kw):
+    from crane_amd import ops
+    B = len(lens)
+    g = ops.prefix_groups(groups, rows, B, gpu)
+    qq = tens(q, dtype, gpu)
+    if kw.pop("flat", q.shape[2] == 1):
+        qq = qq.view(B, q.shape[1], D)
+    return ops.attention_shared_paged(qq, tens(k, dtype, gpu), tens(v, dtype, gpu), ints(table, gpu), ints(lens, gpu),
+                                      max(max(lens), 1), g, **kw)
+
+
+def check_exact(gpu, seed, lens, groups, rows, P, Hq, Hkv, S, dtype, causal=True, **kw):
+    import torch
+    print(f"exact {seed} lens={lens[:6]} groups={len(groups)} rows={rows} P={P} {Hq}/{Hkv} S={S} {dtype} {causal}",
+          flush=True)
+    table, total = layout(seed, lens, groups, rows, P)
+    k, v = pools(seed + 1, total, Hkv, P, table, lens, True)
+    q = np.zeros((len(lens), Hq, S, D), np.float32)
+    got = call(gpu, q, cases.cast(k, dtype), v, table, lens, groups, rows, dtype, causal=causal, **kw)
+    want = np.zeros((len(lens), S, Hkv, Hq // Hkv, D), np.float32)
+    for b, n in enumerate(lens):
+        total_v = np.cumsum(rows_of(v, table, b, n, P).astype(np.float64), 1)
+        for s in range(S):
+            L = n - S + 1 + s if causal else n
+            if L > 0:
+                want[b, s] = (total_v[:, L - 1].astype(np.float32) / np.float32(L))[:, None, :]
+    want = torch.from_numpy(want.reshape(len(lens), S, -1)).to(got.dtype)
+    assert got.shape == want.shape
+    assert torch.equal(got.cpu(), want)
+
+
+def check_close(gpu, seed, lens, groups, rows, P, Hq, Hkv, S, dtype, causal=True, q_scale=1.5, **kw):
+    print(f"close {seed} lens={lens[:6]} groups={len(groups)} rows={rows} P={P} {Hq}/{Hkv} S={S} {dtype} {causal}",
+          flush=True)
+    table, total = layout(seed, lens, groups, rows, P)
+    k, v = pools(seed + 1, total, Hkv, P, table, lens, False)
+    q = cases.normal(cases.rng(seed + 2), (len(lens), Hq, S, D)) * np.float32(q_scale)
+    q, k, v = (cases.cast(x, dtype) for x in (q, k, v))
+    got = call(gpu, q, k, v, table, lens, groups, rows, dtype, causal=causal, **kw).float().cpu().numpy()
+    out, mag, most = reference(q, k, v, table, lens, P, D ** -0.5, causal)
+    tol = bounds(out, mag, most, max(lens), dtype)
+    assert np.isfinite(got).all()
+    worst = float((np.abs(got - out) / tol).max())
+    assert worst <= 1, worst
+    return got
+
+
+# ------------------------------------------------------------------ refusals (CPU)
+
+BASE = dict(q=16, k=16, v=16, n_pages=64, P=256, table=16, stride=8, kv_len=16, max_kv=1024, shared=16, gs=16, gq=16,
+            n_groups=1, max_group=4, max_shared=512, max_own=512, B=4, S=1, Hq=32, Hkv=8, D=128, scale=0.088, flags=1,
+            ws=16, ws_bytes=1 << 40, out=16, dtype=1, stream=None)
+
+
+def shared_call(**kw):
+    from crane_amd import _lib
+    return _lib.lib().crane_hip_attn_shared_paged(*{**BASE, **kw}.values())
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=2), "E_DTYPE"), (dict(D=64), "E_HEAD_DIM"), (dict(Hq=30), "E_GQA"), (dict(Hkv=0), "E_INVALID"),
+    (dict(P=100), "E_INVALID"), (dict(n_pages=0), "E_INVALID"), (dict(table=None), "E_INVALID"),
+    (dict(stride=0), "E_INVALID"), (dict(max_kv=8 * 256 + 1), "E_CAPACITY"), (dict(max_kv=0), "E_INVALID"),
+    (dict(max_shared=1025), "E_CAPACITY"), (dict(max_own=1025), "E_CAPACITY"), (dict(max_own=-1), "E_INVALID"),
+    (dict(max_shared=-1), "E_INVALID"), (dict(n_groups=5), "E_INVALID"), (dict(n_groups=-1), "E_INVALID"),
+    (dict(max_group=5), "E_INVALID"), (dict(max_group=0), "E_INVALID"), (dict(n_groups=0), "E_INVALID"),
+    (dict(flags=2), "E_INVALID"), (dict(flags=3), "E_INVALID"), (dict(scale=0.0), "E_INVALID"),
+    (dict(scale=float("nan")), "E_INVALID"), (dict(scale=float("inf")), "E_INVALID"), (dict(q=None), "E_INVALID"),
+    (dict(out=None), "E_INVALID"), (dict(kv_len=None), "E_INVALID"), (dict(shared=None), "E_INVALID"),
+    (dict(gs=None), "E_INVALID"), (dict(gq=None), "E_INVALID"), (dict(q=8), "E_ALIGN"), (dict(k=24), "E_ALIGN"),
+    (dict(v=8), "E_ALIGN"), (dict(out=8), "E_ALIGN"), (dict(ws=None), "E_WORKSPACE"), (dict(ws=8), "E_WORKSPACE"),
+    (dict(ws_bytes=100), "E_WORKSPACE"), (dict(B=-1), "E_INVALID"), (dict(S=-1), "E_INVALID"),
+    (dict(B=65536), "E_INVALID"), (dict(B=0, n_groups=0, max_group=0, max_shared=0), "OK"), (dict(S=0), "OK"),
+    (dict(S=1 << 30), "E_INVALID"),                                   # more than 2^31 query rows
+    (dict(P=1 << 28, stride=7, n_pages=1, max_kv=7 << 28, max_shared=7 << 28, max_own=7 << 28), "E_INVALID"),
+])
+def test_attention_refusals(kw, code):
+    from crane_amd import _lib
+    assert shared_call(**kw) == getattr(_lib, code)
+
+
+def test_workspace_query():
+    from crane_amd import _lib
+    L = _lib.lib()
+    ws = lambda **kw: L.crane_hip_attn_shared_workspace(*[{**BASE, **kw}[x] for x in (
+        "n_groups", "max_group", "max_shared", "max_own", "B", "S", "Hq", "Hkv", "D", "dtype")])
+    need = ws()
+    assert need > 0 and shared_call(ws_bytes=need - 1) == _lib.E_WORKSPACE
+    assert ws(n_groups=0, max_group=0, max_shared=0, max_own=64) == 0   # one chunk: written directly
+    assert ws(D=64) == 0 and ws(dtype=9) == 0 and ws(B=0) == 0 and ws(S=0) == 0 and ws(max_own=-1) == 0
+
+
+def copy_call(pools=(16, 32), n_pages=8, P=256, Hkv=4, D=128, src=(0,), dst=(1,), rows=None, dtype=1, n=None):
+    from crane_amd import _lib
+    arr = lambda x: None if x is None else (ctypes.c_int32 * max(len(x), 1))(*x)
+    ptr = (ctypes.c_void_p * max(len(pools), 1))(*pools)
+    return _lib.lib().crane_hip_copy_pages(ptr, len(pools), n_pages, P, Hkv, D, arr(src), arr(dst), arr(rows),
+                                           len(src) if n is None else n, dtype, None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(dtype=3), "E_DTYPE"), (dict(D=96), "E_HEAD_DIM"), (dict(Hkv=0), "E_INVALID"), (dict(P=100), "E_INVALID"),
+    (dict(n_pages=0), "E_INVALID"), (dict(n=-1), "E_INVALID"), (dict(pools=(16, None)), "E_INVALID"),
+    (dict(pools=(16, 24)), "E_ALIGN"), (dict(src=(8,)), "E_INVALID"), (dict(src=(-1,)), "E_INVALID"),
+    (dict(dst=(8,)), "E_INVALID"), (dict(dst=(-1,)), "E_INVALID"), (dict(rows=(257,)), "E_INVALID"),
+    (dict(rows=(-1,)), "E_INVALID"), (dict(src=(1,), dst=(1,)), "E_INVALID"),
+    (dict(src=(0, 2), dst=(3, 3)), "E_INVALID"),                      # one destination twice
+    (dict(src=(0, 1), dst=(1, 2)), "E_INVALID"),                      # a destination that is a source
+    (dict(src=(1, 0), dst=(2, 1)), "E_INVALID"),
+    (dict(src=(), dst=()), "OK"),
+    (dict(pools=()), "OK"), (dict(src=(0, 0), dst=(1, 2), rows=(0, 0)), "OK"),
+])
+def test_copy_refusals(kw, code):
+    from crane_amd import _lib
+    assert copy_call(**kw) == getattr(_lib, code)
+
+
+def test_prefix_groups_checks():
+    from crane_amd import ops
+    from crane_amd._lib import CraneHipError
+    g = ops.prefix_groups([[3, 0], [1]], [512, 100], 5, "cpu")
+    assert g.shared_rows.tolist() == [512, 100, 0, 512, 0]
+    assert g.group_start.tolist() == [0, 2, 3] and g.group_seq.tolist() == [3, 0, 1]
+    assert (g.n_groups, g.max_group, g.max_shared, g.min_shared) == (2, 2, 512, 0)
+    g = ops.prefix_groups([], [], 3, "cpu")
+    assert (g.n_groups, g.max_group, g.max_shared, g.min_shared) == (0, 0, 0, 0)
+    for groups, rows in (([[0, 1], [1]], [1, 2]), ([[5]], [1]), ([[-1]], [1]), ([[0, 0]], [4]), ([[]], [1]),
+                         ([[0]], [-1]), ([[0]], [1, 2]), ([[0]], [1 << 31])):
+        with pytest.raises(CraneHipError):
+            ops.prefix_groups(groups, rows, 5, "cpu")
+
+
+def test_host_tensors_are_refused():
+    import torch
+    from crane_amd import ops
+    from crane_amd._lib import CraneHipError
+    pool = torch.zeros(4, 2, 256, D)
+    with pytest.raises(CraneHipError, match="GPU only"):
+        ops.copy_pages([pool, pool], [0], [1])
+    with pytest.raises(CraneHipError, match="GPU only"):
+        ops.attention_shared_paged(torch.zeros(1, 4, D), pool, pool, torch.zeros(1, 2, dtype=torch.int32),
+                                   torch.zeros(1, dtype=torch.int32), 4, ops.prefix_groups([], [], 1, "cpu"))
+
+
+# ------------------------------------------------------------------ GPU: attention
+
+SHAPES = [  # lens, groups, rows, P, Hq, Hkv, S
+    ([257], [], [], 256, 8, 8, 1),
+    ([1], [], [], 256, 4, 1, 1),
+    ([31, 32, 33, 0, 1], [], [], 256, 4, 2, 1),
+    ([513, 530], [[0, 1]], [512], 256, 16, 8, 1),
+    ([256, 256, 256], [[0, 1, 2]], [256], 256, 8, 2, 1),               # nothing of their own
+    ([700, 530, 1025, 512, 90, 2300], [[3, 0, 1], [5, 2]], [512, 1024], 512, 14, 2, 1),
+    ([640] * 9 + [700] * 8, [list(range(0, 17, 2)), list(range(1, 17, 2))], [512, 256], 256, 8, 8, 1),
+    ([2049 + 7 * i for i in range(21)], [list(range(21))], [2048], 256, 28, 4, 1),
+    ([300, 310, 280], [[0, 1, 2]], [256], 256, 8, 2, 5),               # queries inside and past the shared rows
+    ([260, 257, 256], [[0, 1, 2]], [256], 256, 7, 1, 17),
+    ([40, 5, 70, 0], [], [], 256, 4, 2, 40),                           # fewer rows than queries
+    ([1500, 1400], [[0, 1]], [1280], 256, 4, 4, 129),
+    ([900, 3000, 1200], [[1, 2]], [512], 512, 16, 2, 64),
+    ([4100], [[0]], [4096], 256, 8, 1, 3),                             # a group of one
+    ([9000, 9100], [[0, 1]], [8704], 512, 2, 2, 1),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_every_key_once(gpu, case, dtype):
+    lens, groups, rows, P, Hq, Hkv, S = SHAPES[case]
+    check_exact(gpu, 100 + case, lens, groups, rows, P, Hq, Hkv, S, dtype)
+    check_exact(gpu, 200 + case, lens, groups, rows, P, Hq, Hkv, S, dtype, causal=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", [i for i in range(len(SHAPES)) if i not in (11, 12)])
+def test_attention_close(gpu, case, dtype):
+    lens, groups, rows, P, Hq, Hkv, S = SHAPES[case]
+    check_close(gpu, 300 + case, lens, groups, rows, P, Hq, Hkv, S, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 31, 32, 33, 100, 255, 300])
+@pytest.mark.parametrize("S", [1, 4])
+def test_shared_rows_of_any_number(gpu, rows, S):
+    """Rows shared up to the middle of a page or a tile: the sequences are one and the
+    same, described as sharing only their first rows."""
+    import torch
+    from crane_amd import ops
+    for dtype in ("bf16", "f32"):
+        lens, P, Hq, Hkv = [333, 333], 256, 8, 2
+        table, total = layout(50 + rows, lens, [[0, 1]], [333], P)
+        k, v = pools(51 + rows, total, Hkv, P, table, lens, True)
+        q = np.zeros((2, Hq, S, D), np.float32)
+        got = call(gpu, q, cases.cast(k, dtype), v, table, lens, [[1, 0]], [rows], dtype)
+        want = call(gpu, q, cases.cast(k, dtype), v, table, lens, [], [], dtype)
+        assert torch.equal(got, want) and torch.equal(got[0], got[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_large_scores(gpu, dtype):
+    """Scores of many hundreds: the running maximum moves often and most weights
+    vanish."""
+    check_close(gpu, 400, [800, 1100, 777], [[0, 2], [1]], [512, 768], 256, 8, 2, 1, dtype, q_scale=60.0)
+    check_close(gpu, 403, [333, 290], [[0, 1]], [256], 256, 8, 2, 6, dtype, q_scale=60.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_hidden_rows_have_no_influence(gpu, dtype, bad):
+    """A key that a causal query does not see, NaN or infinite in K and in V, has no
+    influence on it; the queries that see it are as the definition says."""
+    lens, groups, rows, P, Hq, Hkv, S = [300, 290], [[0, 1]], [256], 256, 8, 2, 9
+    table, total = layout(61, lens, groups, rows, P)
+    k, v = pools(62, total, Hkv, P, table, lens, False)
+    q = cases.normal(cases.rng(63), (2, Hq, S, D))
+    q, k, v = (cases.cast(x, dtype) for x in (q, k, v))
+    out, mag, most = reference(q, k, v, table, lens, P, D ** -0.5, True)
+    tol = bounds(out, mag, most, 300, dtype)
+    untouched = np.ones(out.shape, bool)
+    for which in ("k", "v"):
+        k2, v2 = k.copy(), v.copy()
+        j = 300 - 4                                # seen by sequence 0's last 4 queries only
+        (k2 if which == "k" else v2)[table[0, j // P], :, j % P, ::3] = bad
+        got = call(gpu, q, k2, v2, table, lens, groups, rows, dtype).float().cpu().numpy()
+        untouched[0, S - 4:] = False
+        if which == "v":                           # the other dims of those queries, too
+            seen = untouched[0, S - 4:].reshape(4, Hq, D)
+            seen[..., np.arange(D) % 3 != 0] = True
+            hit = got[0, S - 4:].reshape(4, Hq, D)[..., ::3]
+            assert np.isnan(hit).all() if math.isnan(bad) else (hit == bad).all()
+        assert (np.abs(got - out)[untouched] <= tol[untouched]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [1, 5])
+def test_members_shorter_than_the_shared_rows(gpu, S):
+    """A member whose length ends inside the group's shared rows sees its own rows
+    only (a page id of its table past its end is not used)."""
+    lens, P = [700, 512, 300, 2, 0], 256
+    for dtype in ("bf16", "f32"):
+        table, total = layout(70, [700, 512, 512, 512, 512], [list(range(5))], [512], P)
+        k, v = pools(71, total, 2, P, table, [700, 512, 512, 512, 512], False)
+        q = cases.cast(cases.normal(cases.rng(72), (5, 8, S, D)), dtype)
+        k, v = cases.cast(k, dtype), cases.cast(v, dtype)
+        got = call(gpu, q, k, v, table, lens, [[0, 1, 2, 3, 4]], [512], dtype).float().cpu().numpy()
+        out, mag, most = reference(q, k, v, table, lens, P, D ** -0.5, True)
+        assert (np.abs(got - out) <= bounds(out, mag, most, 700, dtype)).all()
+        assert (got[4] == 0).all()
+
+
+@pytest.mark.gpu
+def test_pages_outside_the_pool_read_as_zero(gpu):
+    import torch
+    lens, groups, rows, P = [900, 820], [[0, 1]], [512], 256
+    for dtype in ("bf16", "f32"):
+        table, total = layout(80, lens, groups, rows, P)
+        k, v = pools(81, total, 2, P, table, lens, False)
+        q, k, v = (cases.cast(x, dtype) for x in (cases.normal(cases.rng(82), (2, 8, 1, D)), k, v))
+        kz, vz, bad = k.copy(), v.copy(), table.copy()
+        for b, i, x in ((0, 1, 10 ** 6), (1, 1, 10 ** 6), (1, 3, -5)):
+            kz[table[b, i]] = 0
+            vz[table[b, i]] = 0
+            bad[b, i] = x
+        got = call(gpu, q, k, v, bad, lens, groups, rows, dtype)
+        assert torch.equal(got, call(gpu, q, kz, vz, table, lens, groups, rows, dtype))
+
+
+@pytest.mark.gpu
+def test_inconsistent_descriptions_stay_in_bounds(gpu):
+    """Members and starts outside the batch, and lengths past the host's bounds, are
+    not followed; sequences the description gets right keep their results."""
+    import torch
+    from crane_amd import ops
+    lens, P = [600, 700, 300], 256
+    table, total = layout(90, lens, [[0, 1]], [512], P)
+    k, v = pools(91, total, 2, P, table, lens, False)
+    q, k, v = (cases.cast(x, "bf16") for x in (cases.normal(cases.rng(92), (3, 8, 1, D)), k, v))
+    want = call(gpu, q, k, v, table, lens, [[0, 1]], [512], "bf16")
+    g = ops.prefix_groups([[0, 1]], [512], 3, gpu)
+    args = lambda: (tens(q, "bf16", gpu).view(3, 8, D), tens(k, "bf16", gpu), tens(v, "bf16", gpu), ints(table, gpu),
+                    ints(lens, gpu), 700, g)
+    g.group_seq = ints([0, 99], gpu)
+    got = ops.attention_shared_paged(*args())
+    assert torch.equal(got[2], want[2])
+    g.group_start, g.group_seq = ints([-50, 1 << 30], gpu), ints([0, 1, 2], gpu)
+    got = ops.attention_shared_paged(*args())
+    assert torch.equal(got[2], want[2])
+
+
+@pytest.mark.gpu
+def test_replays_and_streams(gpu):
+    """A captured call replayed with other lengths and other eager calls between
+    equals the eager call; another stream and a repeated call give the same bits."""
+    import torch
+    from crane_amd import ops
+    lens, groups, rows, P, Hq, Hkv = [1100, 1300, 1030, 600], [[0, 1, 2]], [1024], 256, 16, 2
+    table, total = layout(95, lens, groups, rows, P)
+    k, v = pools(96, total, Hkv, P, table, lens, False)
+    q = cases.cast(cases.normal(cases.rng(97), (4, Hq, 1, D)), "bf16")
+    t = dict(q=tens(q, "bf16", gpu).view(4, Hq, D), k=tens(k, "bf16", gpu), v=tens(v, "bf16", gpu),
+             table=ints(table, gpu), n=ints(lens, gpu))
+    g = ops.prefix_groups(groups, rows, 4, gpu)
+    run = lambda n: ops.attention_shared_paged(t["q"], t["k"], t["v"], t["table"], n, 1300, g)
+    want = run(t["n"])
+    assert torch.equal(run(t["n"]), want)
+    side = torch.cuda.Stream(gpu)
+    side.wait_stream(torch.cuda.current_stream(gpu))
+    with torch.cuda.stream(side):
+        other = run(t["n"])
+    torch.cuda.current_stream(gpu).wait_stream(side)
+    assert torch.equal(other, want)
+    graphs = []
+    for _ in range(2):  # two graphs of one call, each with its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(t["n"])
+        graphs.append((graph, out))
+    for step in range(4):
+        t["n"].copy_(ints([x - 5 * step for x in lens], gpu))
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize(gpu)
+        want = run(t["n"])
+        for _, out in graphs:
+            assert torch.equal(out, want), step
+
+
+# ------------------------------------------------------------------ GPU: copies
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,P,Hkv,n_pools", [("bf16", 256, 8, 2), ("f32", 512, 3, 2), ("bf16", 256, 1, 74),
+                                                 ("bf16", 256, 2, 131)])
+def test_copy_pages(gpu, dtype, P, Hkv, n_pools):
+    import torch
+    from crane_amd import ops
+    r = cases.rng(500 + n_pools)
+    n_pages = 300 if n_pools == 2 else 12
+    for pairs in ([1, 3, 140] if n_pools == 2 else [5]):  # 140: more than one launch's pairs
+        ids = r.permutation(n_pages)
+        src = [int(ids[i % max(1, min(7, pairs // 2))]) for i in range(pairs)]
+        dst = [int(x) for x in ids[-pairs:]]
+        for rows in (None, [int(x) for x in r.integers(0, P + 1, pairs)]):
+            print(f"copy {dtype} P={P} Hkv={Hkv} pools={n_pools} pairs={pairs} rows={rows and rows[:4]}", flush=True)
+            pools_ = [torch.randn((n_pages, Hkv, P, D), device=gpu).to(torch.bfloat16 if dtype == "bf16" else
+                                                                      torch.float32) for _ in range(n_pools)]
+            want = [p.clone() for p in pools_]
+            ops.copy_pages(pools_, src, dst, rows)
+            for p in want:
+                for i, (a, b) in enumerate(zip(src, dst)):
+                    n = P if rows is None else rows[i]
+                    p[b, :, :n] = p[a, :, :n]
+            assert all(torch.equal(a, b) for a, b in zip(pools_, want))
+
+
+@pytest.mark.gpu
+def test_copy_pages_python_refusals(gpu):
+    import torch
+    from crane_amd import ops
+    from crane_amd._lib import CraneHipError
+    a = torch.zeros((4, 2, 256, D), device=gpu)
+    for args in (([a, a[:3]], [0], [1]), ([a, a.bfloat16()], [0], [1]), ([a], [0, 1], [2]), ([a], [0], [4]),
+                 ([a], [1 << 32], [1]), ([a], [0], [1], [257]), ([a], [0], [1], [1, 2]), ([a], [0, 0], [1, 1]),
+                 ([a.transpose(1, 2)], [0], [1]), ([a[..., :64].contiguous()], [0], [1])):
+        with pytest.raises(CraneHipError):
+            ops.copy_pages(*args)
+    ops.copy_pages([], [0], [1])
+    ops.copy_pages([a], [], [])
