@@ -108,6 +108,7 @@ SIGNATURES = {
     "crane_hip_attn_shared_paged": (
         [_vp, _vp, _vp, _i64, _i, _i32p, _i64, _i32p, _i64, _i32p, _i32p, _i32p, _i, _i, _i64, _i64,
          _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp, _i, _vp], _i),
+    "crane_hip_group_prefixes": ([_i32p, _i64, _i32p, _i, _i32p, _i32p, _i32p, _ip], _i),
     "crane_hip_copy_pages": ([_vpp, _i, _i64, _i, _i, _i, _i32p, _i32p, _i32p, _i, _i, _vp], _i),
     # include/crane_pkv.h
     "crane_pkv_create": ([_i, _i, _i, _i, _i64, _i, _i, _vpp], _i),
@@ -123,6 +124,11 @@ SIGNATURES = {
         [_vp, _vp, _i64, _vp, _vp, _f, _i, _vp, _vp, _i64, _i64, _i32p, _vp, _i, _i, _vp], _i),
     "crane_pkv_decode": ([_vp, _vp, _i, _f, _i, _vp, _sz, _vp, _vp], _i),
     "crane_pkv_prefill": ([_vp, _vp, _i, _i, _f, _i, _vp, _vp], _i),
+    "crane_pkv_fork": ([_vpp, _i, _i, _i64, _i, _ip, _vp], _i),
+    "crane_pkv_truncate": ([_vpp, _i, _i, _i64, _vp], _i),
+    "crane_pkv_compact": ([_vpp, _i, _i64p, _vp], _i),
+    "crane_pkv_shared_workspace": ([_vp, _i, _i], _sz),
+    "crane_pkv_attention_shared": ([_vp, _vp, _i, _i, _f, _i, _vp, _sz, _vp, _vp], _i),
     "crane_pkv_read_seq": ([_vp, _i, _vp, _vp, _vp], _i),
     "crane_pkv_write_seq": ([_vp, _i, _vp, _vp, _i64, _vp], _i),
     "crane_pkv_views": ([_vp, _vpp, _vpp, _vpp, _i64p, _vpp], _i),

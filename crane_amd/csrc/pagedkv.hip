@@ -13,12 +13,24 @@
 // uploads them, and an append that opens new pages patches the device table
 // with a kernel whose arguments carry the new entries (no host buffer, no
 // synchronisation on the decode path).
+//
+// Pages are shared: each counts the sequences that hold it, a fork adds owners to the
+// pages its rows fill and copies the page they end in, and a page returns to the free
+// list with its last owner.  A shared page is full of rows for each of its owners, and
+// every operation keeps it so (fork and truncate copy the page that would be partial,
+// write_seq gives its shared pages up first), so an append only ever writes pages of
+// one owner and needs no check.  set_batch groups the batch by its shared pages for
+// the attention that reads them once.  Calls over several layers' caches plan every
+// cache first and change none unless all can go through; caches that need the same
+// copies get them in one launch.
 #include <algorithm>
 #include <new>
 #include <vector>
 
 #include "common.h"
+#include "page_groups.h"
 #include "../../include/crane_pkv.h"
+#include "../../include/crane_shared.h"
 
 namespace crane {
 namespace {
@@ -99,6 +111,17 @@ struct Seq {
     std::vector<int32_t> pages;
 };
 
+// Page copies of one cache: rows [0, rows[i]) of page src[i] to page dst[i].
+struct Copies {
+    std::vector<int32_t> src, dst, rows;
+    void add(int32_t s, int32_t d, int64_t r) {
+        src.push_back(s);
+        dst.push_back(d);
+        rows.push_back((int32_t)r);
+    }
+    bool operator==(const Copies& o) const { return src == o.src && dst == o.dst && rows == o.rows; }
+};
+
 }  // namespace
 
 class PagedKv {
@@ -116,10 +139,12 @@ class PagedKv {
             hipMalloc(&d_table_, sizeof(int32_t) * (size_t)max_seqs_ * max_pps_) != hipSuccess ||
             hipMalloc(&d_len_, sizeof(int32_t) * (size_t)max_seqs_) != hipSuccess ||
             hipMalloc(&d_start_, sizeof(int32_t) * (size_t)max_seqs_) != hipSuccess ||
-            hipMalloc(&d_one_, sizeof(int32_t) * (size_t)max_pps_) != hipSuccess) {
+            hipMalloc(&d_one_, sizeof(int32_t) * (size_t)max_pps_) != hipSuccess ||
+            hipMalloc(&d_groups_, sizeof(int32_t) * (3 * (size_t)max_seqs_ + 1)) != hipSuccess) {
             release();
             return CRANE_HIP_E_LAUNCH;
         }
+        refs_.assign((size_t)n_pages_, 0);
         free_.reserve((size_t)n_pages_);
         for (int64_t p = n_pages_ - 1; p >= 0; --p) free_.push_back((int32_t)p);
         return CRANE_HIP_OK;
@@ -159,7 +184,7 @@ class PagedKv {
     int seq_free(int id) {
         if (!live(id) || in_batch(id)) return CRANE_HIP_E_INVALID;
         Seq& s = seqs_[id];
-        for (auto it = s.pages.rbegin(); it != s.pages.rend(); ++it) free_.push_back(*it);
+        for (auto it = s.pages.rbegin(); it != s.pages.rend(); ++it) drop(*it);
         s = Seq();
         return CRANE_HIP_OK;
     }
@@ -171,19 +196,37 @@ class PagedKv {
             if (!live(ids[b]) || seen[ids[b]]) return CRANE_HIP_E_INVALID;
             seen[ids[b]] = 1;
         }
-        batch_.assign(ids, ids + B);
-        if (B == 0) return CRANE_HIP_OK;
-        std::vector<int32_t> table((size_t)B * max_pps_, -1), lens((size_t)B);
+        PageGroups groups;
+        std::vector<int32_t> table((size_t)B * max_pps_, -1), lens((size_t)B), shared;
         for (int b = 0; b < B; ++b) {
             const Seq& s = seqs_[ids[b]];
             std::copy(s.pages.begin(), s.pages.end(), table.begin() + (size_t)b * max_pps_);
             lens[b] = (int32_t)s.len;
         }
-        int rc = hip_rc(hipMemcpyAsync(d_table_, table.data(), sizeof(int32_t) * table.size(), hipMemcpyHostToDevice, st));
-        if (!rc) rc = hip_rc(hipMemcpyAsync(d_len_, lens.data(), sizeof(int32_t) * lens.size(), hipMemcpyHostToDevice, st));
+        if (shared_pages_ > 0) {
+            std::vector<PageList> lists((size_t)B);
+            for (int b = 0; b < B; ++b) lists[b] = {seqs_[ids[b]].pages.data(), seqs_[ids[b]].pages.size()};
+            groups = group_pages(lists);
+        }
+        if (groups.count()) {  // shared rows per sequence, then the groups' starts and members
+            for (int32_t pages : groups.shared) shared.push_back(pages * P_);
+            shared.insert(shared.end(), groups.start.begin(), groups.start.end());
+            shared.insert(shared.end(), groups.members.begin(), groups.members.end());
+        }
+        std::vector<int> batch(ids, ids + B);
+        batch_.clear();  // no batch if an upload fails
+        n_groups_ = max_group_ = 0;
+        if (B == 0) return CRANE_HIP_OK;
+        int rc = upload(d_table_, table, st);
+        if (!rc) rc = upload(d_len_, lens, st);
+        if (!rc && !shared.empty()) rc = upload(d_groups_, shared, st);
         if (!rc) rc = hip_rc(hipStreamSynchronize(st));  // the staging vectors go out of scope
-        if (rc) batch_.clear();
-        return rc;
+        if (rc) return rc;
+        batch_.swap(batch);
+        n_groups_ = groups.count();
+        for (int i = 0; i < n_groups_; ++i) max_group_ = std::max(max_group_, groups.start[i + 1] - groups.start[i]);
+        batch_shared_.swap(groups.shared);
+        return CRANE_HIP_OK;
     }
 
     // Pages for S more rows in every batch sequence: checked first, then taken
@@ -207,8 +250,7 @@ class PagedKv {
             const int64_t need = (s.len + S + P_ - 1) / P_;
             while ((int64_t)s.pages.size() < need) {
                 if (added) ++(*added)[b];
-                const int32_t page = free_.back();
-                free_.pop_back();
+                const int32_t page = take();
                 patch.idx[patch.n] = (int32_t)((int64_t)b * max_pps_ + (int64_t)s.pages.size());
                 patch.val[patch.n] = page;
                 ++patch.n;
@@ -230,7 +272,7 @@ class PagedKv {
         for (int b = B() - 1; b >= 0; --b) {
             Seq& s = seqs_[batch_[b]];
             for (int i = 0; i < added[b]; ++i) {
-                free_.push_back(s.pages.back());
+                drop(s.pages.back());
                 s.pages.pop_back();
             }
         }
@@ -314,19 +356,184 @@ class PagedKv {
         Seq& s = seqs_[id];
         const int64_t need = (len + P_ - 1) / P_;
         if (need > max_pps_ || len > 0x7fffffffLL) return CRANE_HIP_E_CAPACITY;
-        if (need - (int64_t)s.pages.size() > (int64_t)free_.size()) return CRANE_HIP_E_CAPACITY;
-        while ((int64_t)s.pages.size() > need) {
-            free_.push_back(s.pages.back());
-            s.pages.pop_back();
+        // A page other sequences hold is not written: it is given up for another.
+        int64_t kept = 0, back = 0;
+        for (int32_t p : s.pages) {
+            if (refs_[p] == 1 && kept < need) ++kept;
+            else if (refs_[p] == 1) ++back;
         }
-        while ((int64_t)s.pages.size() < need) {
-            s.pages.push_back(free_.back());
-            free_.pop_back();
+        if (need - kept > (int64_t)free_.size() + back) return CRANE_HIP_E_CAPACITY;
+        std::vector<int32_t> pages;
+        pages.reserve((size_t)need);
+        for (int32_t p : s.pages)
+            if (refs_[p] == 1 && (int64_t)pages.size() < need) pages.push_back(p);
+        int64_t left = kept;
+        for (size_t i = s.pages.size(); i-- > 0;) {  // from the last: free ids come back in order
+            const int32_t p = s.pages[i];
+            if (left > 0 && p == pages[left - 1]) --left;
+            else drop(p);
         }
+        while ((int64_t)pages.size() < need) pages.push_back(take());
+        s.pages.swap(pages);
         s.len = len;
         if (len == 0) return CRANE_HIP_OK;
         const int rc = upload_one(s.pages, st);
         return rc ? rc : scatter(k, v, one_rows(), nullptr, 1, len, st);
+    }
+
+    // ---- shared pages: plan_* fill a plan and change nothing, commit_* apply it
+
+    struct Fork {
+        std::vector<Seq> children;
+        Copies copies;
+    };
+    int plan_fork(int src, int64_t rows, int count, Fork* f) const {
+        if (!live(src)) return CRANE_HIP_E_INVALID;
+        const Seq& s = seqs_[src];
+        const int64_t n = rows < 0 ? s.len : rows;
+        if (n > s.len) return CRANE_HIP_E_INVALID;
+        const int64_t full = n / P_, part = n % P_;
+        if (count > max_seqs_ || (part && (int64_t)count > free_pages())) return CRANE_HIP_E_CAPACITY;
+        f->children.resize((size_t)count);
+        for (int c = 0; c < count; ++c) {
+            Seq& child = f->children[c];
+            child.live = true;
+            child.len = n;
+            child.pages.assign(s.pages.begin(), s.pages.begin() + full);
+            if (part) {
+                child.pages.push_back(free_[free_.size() - 1 - (size_t)c]);
+                f->copies.add(s.pages[full], child.pages.back(), part);
+            }
+        }
+        return CRANE_HIP_OK;
+    }
+    void commit_fork(Fork& f, const int* ids) {
+        for (size_t c = 0; c < f.children.size(); ++c) {
+            Seq& child = f.children[c];
+            const int64_t full = child.len / P_;
+            for (int64_t i = 0; i < full; ++i) hold(child.pages[i]);
+            if (child.len % P_) take();  // the planned one
+            seqs_[ids[c]] = std::move(child);
+        }
+    }
+
+    struct Cut {
+        int64_t rows = 0;
+        bool copy = false;  // the last page is shared and becomes partial
+        Copies copies;
+    };
+    int plan_truncate(int id, int64_t rows, Cut* c) const {
+        if (!live(id) || in_batch(id) || rows < 0 || rows > seqs_[id].len) return CRANE_HIP_E_INVALID;
+        const Seq& s = seqs_[id];
+        const int64_t need = (rows + P_ - 1) / P_;
+        c->rows = rows;
+        c->copy = rows % P_ && refs_[s.pages[need - 1]] > 1;
+        if (!c->copy) return CRANE_HIP_OK;
+        // The page it takes: the list's last, or else the last page it gives back.
+        int32_t page = free_.empty() ? -1 : free_.back();
+        for (int64_t i = (int64_t)s.pages.size() - 1; i >= need; --i)
+            if (refs_[s.pages[i]] == 1) page = s.pages[i];
+        if (page < 0) return CRANE_HIP_E_CAPACITY;
+        c->copies.add(s.pages[need - 1], page, rows % P_);
+        return CRANE_HIP_OK;
+    }
+    void commit_truncate(int id, const Cut& c) {
+        Seq& s = seqs_[id];
+        const int64_t need = (c.rows + P_ - 1) / P_;
+        while ((int64_t)s.pages.size() > need) {
+            drop(s.pages.back());
+            s.pages.pop_back();
+        }
+        if (c.copy) {
+            drop(s.pages.back());
+            s.pages.back() = take();
+        }
+        s.len = c.rows;
+    }
+
+    struct Move {
+        std::vector<int32_t> to;    // every page's place afterwards
+        std::vector<int32_t> free;  // the free list afterwards
+        Copies copies;
+    };
+    int plan_compact(Move* m) const {
+        const int64_t used = n_pages_ - free_pages();
+        m->to.resize((size_t)n_pages_);
+        m->free.reserve((size_t)n_pages_);
+        int64_t hole = 0;
+        for (int64_t p = 0; p < n_pages_; ++p) {
+            m->to[p] = (int32_t)p;
+            if (p < used || refs_[p] == 0) continue;
+            while (refs_[hole] != 0) ++hole;  // as many free ids lie below `used` as held ones from it on
+            m->to[p] = (int32_t)hole;
+            m->copies.add((int32_t)p, (int32_t)hole, P_);
+            ++hole;
+        }
+        for (int64_t p = n_pages_ - 1; p >= used; --p) m->free.push_back((int32_t)p);
+        return CRANE_HIP_OK;
+    }
+    int commit_compact(Move& m, hipStream_t st) {
+        for (size_t i = 0; i < m.copies.src.size(); ++i) {
+            refs_[m.copies.dst[i]] = refs_[m.copies.src[i]];
+            refs_[m.copies.src[i]] = 0;
+        }
+        free_.swap(m.free);
+        TablePatch patch;
+        patch.n = 0;
+        int rc = CRANE_HIP_OK;
+        for (int b = 0; b < B(); ++b) {
+            const Seq& s = seqs_[batch_[b]];
+            for (size_t i = 0; i < s.pages.size(); ++i) {
+                if (m.to[s.pages[i]] == s.pages[i]) continue;
+                patch.idx[patch.n] = (int32_t)((int64_t)b * max_pps_ + (int64_t)i);
+                patch.val[patch.n] = m.to[s.pages[i]];
+                if (++patch.n < kPatch) continue;
+                rc = rc ? rc : launch_patch(d_table_, patch, st);
+                patch.n = 0;
+            }
+        }
+        for (Seq& s : seqs_)
+            for (int32_t& p : s.pages) p = m.to[p];
+        return rc || !patch.n ? rc : launch_patch(d_table_, patch, st);
+    }
+
+    // Attention of the batch's last S rows, shared pages read once per group.
+    int64_t max_own() const {
+        int64_t m = 0;
+        for (int b = 0; b < B(); ++b) m = std::max(m, seqs_[batch_[b]].len - shared_rows(b));
+        return m;
+    }
+    int64_t max_shared() const {
+        int64_t m = 0;
+        for (int b = 0; b < B(); ++b) m = std::max(m, shared_rows(b));
+        return m;
+    }
+    size_t shared_workspace(int Hq, int S) const {
+        return crane_hip_attn_shared_workspace(n_groups_, max_group_, max_shared(), max_own(), B(), S, Hq, Hkv_, D_,
+                                               dtype_);
+    }
+    int attention_shared(const void* q, int Hq, int S, float scale, int flags, void* ws, size_t ws_bytes, void* out,
+                         hipStream_t st) const {
+        if (S < 0) return CRANE_HIP_E_INVALID;
+        if (batch_.empty() || S == 0) return CRANE_HIP_OK;
+        for (int id : batch_)
+            if (S > 1 && seqs_[id].len < S) return CRANE_HIP_E_INVALID;  // every sequence holds its S new rows
+        if (max_len() == 0) return CRANE_HIP_E_INVALID;
+        const int32_t *shared = d_groups_, *start = shared + B(), *members = start + n_groups_ + 1;
+        return crane_hip_attn_shared_paged(q, k_pool_, v_pool_, n_pages_, P_, d_table_, max_pps_, d_len_, max_len(),
+                                           shared, start, members, n_groups_, max_group_, max_shared(), max_own(), B(),
+                                           S, Hq, Hkv_, D_, scale, flags, ws, ws_bytes, out, dtype_, st);
+    }
+
+    bool same_shape(const PagedKv& o) const {
+        return Hkv_ == o.Hkv_ && D_ == o.D_ && dtype_ == o.dtype_ && P_ == o.P_ && n_pages_ == o.n_pages_;
+    }
+    int max_seqs() const { return max_seqs_; }
+    void* k_pool() const { return k_pool_; }
+    void* v_pool() const { return v_pool_; }
+    int copy_into(std::vector<void*>& pools, const Copies& c, hipStream_t st) const {
+        return crane_hip_copy_pages(pools.data(), (int)pools.size(), n_pages_, P_, Hkv_, D_, c.src.data(), c.dst.data(),
+                                    c.rows.data(), (int)c.src.size(), dtype_, st);
     }
 
     void views(void** k, void** v, const int32_t** table, int64_t* stride, const int32_t** dlen) const {
@@ -338,6 +545,26 @@ class PagedKv {
     }
 
   private:
+    // A page's owners: take one for a first owner, add one, drop one.
+    int32_t take() {
+        const int32_t p = free_.back();
+        free_.pop_back();
+        refs_[p] = 1;
+        return p;
+    }
+    void hold(int32_t p) {
+        if (++refs_[p] == 2) ++shared_pages_;
+    }
+    void drop(int32_t p) {
+        if (refs_[p] == 2) --shared_pages_;
+        if (--refs_[p] == 0) free_.push_back(p);
+    }
+    int64_t shared_rows(int b) const { return n_groups_ ? (int64_t)batch_shared_[b] * P_ : 0; }
+
+    static int upload(int32_t* dst, const std::vector<int32_t>& v, hipStream_t st) {
+        return hip_rc(hipMemcpyAsync(dst, v.data(), sizeof(int32_t) * v.size(), hipMemcpyHostToDevice, st));
+    }
+
     static int launch_patch(int32_t* table, const TablePatch& p, hipStream_t st) {
         hipLaunchKernelGGL(patch_table_kernel, dim3(1), dim3(kPatch), 0, st, table, p);
         return launch_status(hipGetLastError());
@@ -364,10 +591,11 @@ class PagedKv {
     }
 
     void release() {
-        for (void* p : {k_pool_, v_pool_, (void*)d_table_, (void*)d_len_, (void*)d_start_, (void*)d_one_})
+        for (void* p : {k_pool_, v_pool_, (void*)d_table_, (void*)d_len_, (void*)d_start_, (void*)d_one_,
+                        (void*)d_groups_})
             if (p) (void)hipFree(p);
         k_pool_ = v_pool_ = nullptr;
-        d_table_ = d_len_ = d_start_ = d_one_ = nullptr;
+        d_table_ = d_len_ = d_start_ = d_one_ = d_groups_ = nullptr;
     }
 
     int Hkv_, D_, dtype_;
@@ -381,9 +609,14 @@ class PagedKv {
     int32_t* d_len_ = nullptr;    // current batch lengths
     int32_t* d_start_ = nullptr;  // prefill chunk starts
     int32_t* d_one_ = nullptr;    // one sequence's page ids (read_seq / write_seq)
+    int32_t* d_groups_ = nullptr; // current batch: shared rows, group starts, members (when there are groups)
     std::vector<int32_t> free_;
+    std::vector<int32_t> refs_;   // owners of every page
+    int64_t shared_pages_ = 0;    // pages of more than one owner
     std::vector<Seq> seqs_;
     std::vector<int> batch_;
+    std::vector<int32_t> batch_shared_;  // pages each batch sequence shares (when there are groups)
+    int n_groups_ = 0, max_group_ = 0;
 };
 
 }  // namespace crane
@@ -395,6 +628,114 @@ struct crane_pkv {
     crane_pkv(int Hkv, int D, int dtype, int P, int64_t n_pages, int max_seqs, int max_pps)
         : impl(Hkv, D, dtype, P, n_pages, max_seqs, max_pps) {}
 };
+
+namespace {
+
+// The caches of a call over several layers: distinct and non-null.
+int check_caches(crane_pkv* const* caches, int n) {
+    if (n < 0 || (n > 0 && !caches)) return CRANE_HIP_E_INVALID;
+    std::vector<const crane_pkv*> seen(caches, caches + n);
+    std::sort(seen.begin(), seen.end());
+    if (n && (!seen[0] || std::adjacent_find(seen.begin(), seen.end()) != seen.end())) return CRANE_HIP_E_INVALID;
+    return CRANE_HIP_OK;
+}
+
+// Every cache's planned copies, the pools of caches of one shape with the same copies
+// in one launch.
+template <class PLAN>
+int copy_all(crane_pkv* const* caches, const std::vector<PLAN>& plans, hipStream_t st) {
+    std::vector<char> done(plans.size(), 0);
+    for (size_t i = 0; i < plans.size(); ++i) {
+        if (done[i] || plans[i].copies.src.empty()) continue;
+        const PagedKv& first = caches[i]->impl;
+        std::vector<void*> pools;
+        for (size_t j = i; j < plans.size(); ++j) {
+            const PagedKv& c = caches[j]->impl;
+            if (done[j] || !c.same_shape(first) || !(plans[j].copies == plans[i].copies)) continue;
+            done[j] = 1;
+            pools.push_back(c.k_pool());
+            pools.push_back(c.v_pool());
+        }
+        const int rc = first.copy_into(pools, plans[i].copies, st);
+        if (rc) return rc;
+    }
+    return CRANE_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" int crane_pkv_fork(crane_pkv* const* caches, int n, int seq_id, int64_t rows, int count, int* new_ids,
+                              void* stream) {
+    try {
+        int rc = check_caches(caches, n);
+        if (rc) return rc;
+        if (count < 0 || rows < -1 || (count > 0 && !new_ids)) return CRANE_HIP_E_INVALID;
+        if (n == 0 || count == 0) return CRANE_HIP_OK;
+        std::vector<PagedKv::Fork> plans((size_t)n);
+        for (int i = 0; i < n; ++i)
+            if ((rc = caches[i]->impl.plan_fork(seq_id, rows, count, &plans[i]))) return rc;
+        std::vector<int> ids;  // the lowest ids free in every cache
+        for (int id = 0; id < caches[0]->impl.max_seqs() && (int)ids.size() < count; ++id) {
+            bool open = true;
+            for (int i = 0; i < n; ++i) open = open && id < caches[i]->impl.max_seqs() && !caches[i]->impl.live(id);
+            if (open) ids.push_back(id);
+        }
+        if ((int)ids.size() < count) return CRANE_HIP_E_CAPACITY;
+        if ((rc = copy_all(caches, plans, (hipStream_t)stream))) return rc;
+        for (int i = 0; i < n; ++i) caches[i]->impl.commit_fork(plans[i], ids.data());
+        std::copy(ids.begin(), ids.end(), new_ids);
+        return CRANE_HIP_OK;
+    } catch (...) {  // no memory
+        return CRANE_HIP_E_INVALID;
+    }
+}
+
+extern "C" int crane_pkv_truncate(crane_pkv* const* caches, int n, int seq_id, int64_t rows, void* stream) {
+    try {
+        int rc = check_caches(caches, n);
+        if (rc) return rc;
+        std::vector<PagedKv::Cut> plans((size_t)n);
+        for (int i = 0; i < n; ++i)
+            if ((rc = caches[i]->impl.plan_truncate(seq_id, rows, &plans[i]))) return rc;
+        if ((rc = copy_all(caches, plans, (hipStream_t)stream))) return rc;
+        for (int i = 0; i < n; ++i) caches[i]->impl.commit_truncate(seq_id, plans[i]);
+        return CRANE_HIP_OK;
+    } catch (...) {
+        return CRANE_HIP_E_INVALID;
+    }
+}
+
+extern "C" int crane_pkv_compact(crane_pkv* const* caches, int n, int64_t* moved, void* stream) {
+    try {
+        int rc = check_caches(caches, n);
+        if (rc) return rc;
+        std::vector<PagedKv::Move> plans((size_t)n);
+        int64_t total = 0;
+        for (int i = 0; i < n; ++i) {
+            if ((rc = caches[i]->impl.plan_compact(&plans[i]))) return rc;
+            total += (int64_t)plans[i].copies.src.size();
+        }
+        if ((rc = copy_all(caches, plans, (hipStream_t)stream))) return rc;
+        for (int i = 0; i < n; ++i) {
+            const int c = caches[i]->impl.commit_compact(plans[i], (hipStream_t)stream);
+            rc = rc ? rc : c;
+        }
+        if (moved) *moved = total;
+        return rc;
+    } catch (...) {
+        return CRANE_HIP_E_INVALID;
+    }
+}
+
+extern "C" size_t crane_pkv_shared_workspace(const crane_pkv* pkv, int Hq, int S) {
+    return pkv ? pkv->impl.shared_workspace(Hq, S) : 0;
+}
+
+extern "C" int crane_pkv_attention_shared(const crane_pkv* pkv, const void* q, int Hq, int S, float scale, int flags,
+                                          void* workspace, size_t ws_bytes, void* out, void* stream) {
+    return pkv ? pkv->impl.attention_shared(q, Hq, S, scale, flags, workspace, ws_bytes, out, (hipStream_t)stream)
+               : CRANE_HIP_E_INVALID;
+}
 
 extern "C" int crane_pkv_create(int Hkv, int D, int dtype, int page_rows, int64_t n_pages, int max_seqs,
                                 int max_pages_per_seq, crane_pkv** out) {
@@ -436,7 +777,11 @@ extern "C" int64_t crane_pkv_free_pages(const crane_pkv* pkv) { return pkv ? pkv
 extern "C" uint64_t crane_pkv_bytes(const crane_pkv* pkv) { return pkv ? pkv->impl.bytes() : 0; }
 
 extern "C" int crane_pkv_set_batch(crane_pkv* pkv, const int* seq_ids, int B, void* stream) {
-    return pkv ? pkv->impl.set_batch(seq_ids, B, (hipStream_t)stream) : CRANE_HIP_E_INVALID;
+    try {
+        return pkv ? pkv->impl.set_batch(seq_ids, B, (hipStream_t)stream) : CRANE_HIP_E_INVALID;
+    } catch (...) {  // no memory
+        return CRANE_HIP_E_INVALID;
+    }
 }
 
 extern "C" int crane_pkv_update(crane_pkv* pkv, const void* k, const void* v, int S, void* stream) {
@@ -464,12 +809,20 @@ extern "C" int crane_pkv_prefill(crane_pkv* pkv, const void* q, int Hq, int S, f
 }
 
 extern "C" int crane_pkv_read_seq(crane_pkv* pkv, int seq_id, void* k, void* v, void* stream) {
-    return pkv ? pkv->impl.read_seq(seq_id, k, v, (hipStream_t)stream) : CRANE_HIP_E_INVALID;
+    try {
+        return pkv ? pkv->impl.read_seq(seq_id, k, v, (hipStream_t)stream) : CRANE_HIP_E_INVALID;
+    } catch (...) {  // no memory
+        return CRANE_HIP_E_INVALID;
+    }
 }
 
 extern "C" int crane_pkv_write_seq(crane_pkv* pkv, int seq_id, const void* k, const void* v, int64_t len,
                                    void* stream) {
-    return pkv ? pkv->impl.write_seq(seq_id, k, v, len, (hipStream_t)stream) : CRANE_HIP_E_INVALID;
+    try {
+        return pkv ? pkv->impl.write_seq(seq_id, k, v, len, (hipStream_t)stream) : CRANE_HIP_E_INVALID;
+    } catch (...) {  // no memory
+        return CRANE_HIP_E_INVALID;
+    }
 }
 
 extern "C" int crane_pkv_views(const crane_pkv* pkv, void** k_pool, void** v_pool, const int32_t** block_table,

@@ -1,5 +1,6 @@
-// pages.hip -- copies of rows between pages of the K/V pools; the C ABI is
-// crane_hip_copy_pages in include/crane_shared.h.
+// pages.hip -- copies of rows between pages of the K/V pools, and the grouping of
+// sequences by the pages they share; the C ABI is crane_hip_copy_pages and
+// crane_hip_group_prefixes in include/crane_shared.h.
 //
 // A page [Hkv, page_rows, D] of a pool is Hkv runs of page_rows rows, and a copy
 // takes the first rows of each run.  The pairs and the pools' addresses go to the
@@ -9,6 +10,7 @@
 #include <vector>
 
 #include "common.h"
+#include "page_groups.h"
 #include "../../include/crane_shared.h"
 
 namespace crane {
@@ -47,10 +49,145 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a, int blocks,
             *reinterpret_cast<u32x4_v*>(dst + at + i * 4096) = *reinterpret_cast<const u32x4_v*>(src + at + i * 4096);
 }
 
+// The lists sorted form a tree: a node is a run of them with `common` first pages in
+// common, its kids the sub-runs with more.  A node opened as a group takes the lists
+// below it that no deeper open node takes; each is then read as `common` pages fewer,
+// but once:  saved = sum over lists of c(deepest open node above it) - sum over open
+// nodes of c.  best() maximises that over the nodes to open, for every node and every
+// possible open node above it (c = 0: none).
+class Grouping {
+  public:
+    explicit Grouping(const std::vector<PageList>& lists) : lists_(lists), order_(lists.size()) {
+        for (size_t i = 0; i < order_.size(); ++i) order_[i] = (int32_t)i;
+        std::sort(order_.begin(), order_.end(), [&](int32_t a, int32_t b) {
+            const PageList &x = lists_[a], &y = lists_[b];
+            const auto m = std::mismatch(x.ids, x.ids + std::min(x.n, y.n), y.ids);
+            if (m.first != x.ids + std::min(x.n, y.n)) return *m.first < *m.second;
+            return x.n != y.n ? x.n < y.n : a < b;
+        });
+    }
+    PageGroups run() {
+        PageGroups g;
+        g.shared.assign(lists_.size(), 0);
+        if (lists_.size() < 2) return g;
+        Node root = build(0, order_.size(), 0);
+        std::vector<int64_t> above{0};
+        best(root, above);
+        std::vector<std::vector<int32_t>> open(1);
+        std::vector<size_t> c{0};
+        collect(root, 0, 1, open, c, {0});
+        for (size_t i = 1; i < open.size(); ++i) {
+            for (int32_t b : open[i]) {
+                g.members.push_back(b);
+                g.shared[b] = (int32_t)c[i];
+            }
+            g.start.push_back((int32_t)g.members.size());
+        }
+        return g;
+    }
+
+  private:
+    struct Node {
+        size_t lo, hi, common;
+        std::vector<Node> kids;
+        std::vector<char> open;  // by the open node above: whether to open this one
+    };
+    Node build(size_t lo, size_t hi, size_t common) {
+        const PageList &a = lists_[order_[lo]], &b = lists_[order_[hi - 1]];
+        // sorted: what the first and the last share, all share; an id below 0 names no page
+        while (common < a.n && common < b.n && a.ids[common] == b.ids[common] && a.ids[common] >= 0) ++common;
+        Node node{lo, hi, common, {}, {}};
+        for (size_t i = lo; i < hi;) {
+            const PageList& p = lists_[order_[i]];
+            size_t j = i + 1;
+            if (p.n > common && p.ids[common] >= 0)
+                while (j < hi && lists_[order_[j]].n > common && lists_[order_[j]].ids[common] == p.ids[common]) ++j;
+            if (j - i > 1 && j - i < hi - lo) node.kids.push_back(build(i, j, common));
+            i = j;
+        }
+        return node;
+    }
+    // What the lists below `node` add to the sum for every open node above (above[k]
+    // = its c).
+    std::vector<int64_t> best(Node& node, std::vector<int64_t>& above) {
+        const int64_t c = (int64_t)node.common;
+        int64_t singles = (int64_t)(node.hi - node.lo);
+        const size_t n = above.size();
+        above.push_back(c);
+        std::vector<int64_t> kids(n + 1, 0);
+        for (Node& kid : node.kids) {
+            singles -= (int64_t)(kid.hi - kid.lo);
+            const std::vector<int64_t> v = best(kid, above);
+            for (size_t k = 0; k <= n; ++k) kids[k] += v[k];
+        }
+        above.pop_back();
+        std::vector<int64_t> value(n);
+        node.open.resize(n);
+        const int64_t opened = kids[n] + (singles - 1) * c;
+        for (size_t k = 0; k < n; ++k) {
+            const int64_t closed = kids[k] + singles * above[k];
+            node.open[k] = opened > closed;
+            value[k] = std::max(opened, closed);
+        }
+        return value;
+    }
+    // The members of every open node; open[at[k]] is the group the k-th node above
+    // stands for, open[0] the lists of no group.
+    void collect(const Node& node, size_t k, size_t n, std::vector<std::vector<int32_t>>& open, std::vector<size_t>& c,
+                 std::vector<size_t> at) {
+        at.push_back(at[k]);
+        if (node.open[k]) {
+            at[n] = open.size();
+            open.emplace_back();
+            c.push_back(node.common);
+        }
+        const size_t below = node.open[k] ? n : k;
+        size_t i = node.lo;
+        for (const Node& kid : node.kids) {
+            for (; i < kid.lo; ++i) open[at[below]].push_back(order_[i]);
+            collect(kid, below, n + 1, open, c, at);
+            i = kid.hi;
+        }
+        for (; i < node.hi; ++i) open[at[below]].push_back(order_[i]);
+    }
+
+    const std::vector<PageList>& lists_;
+    std::vector<int32_t> order_;
+};
+
 }  // namespace
+
+PageGroups group_pages(const std::vector<PageList>& lists) { return Grouping(lists).run(); }
+
 }  // namespace crane
 
 using namespace crane;
+
+extern "C" int crane_hip_group_prefixes(const int32_t* table, int64_t stride, const int32_t* pages, int B,
+                                        int32_t* shared_pages, int32_t* group_start, int32_t* group_seq,
+                                        int* n_groups) {
+    if (!n_groups || B < 0 || stride < 0) return CRANE_HIP_E_INVALID;
+    *n_groups = 0;
+    if (!group_start) return CRANE_HIP_E_INVALID;
+    group_start[0] = 0;
+    if (B == 0) return CRANE_HIP_OK;
+    if (!pages || !shared_pages || !group_seq || (stride > 0 && !table)) return CRANE_HIP_E_INVALID;
+    try {
+        std::vector<PageList> lists((size_t)B);
+        for (int b = 0; b < B; ++b) {
+            if (pages[b] < 0 || pages[b] > stride) return CRANE_HIP_E_INVALID;
+            lists[b] = {table + b * stride, (size_t)pages[b]};
+        }
+        const PageGroups g = group_pages(lists);
+        std::copy(g.shared.begin(), g.shared.end(), shared_pages);
+        std::copy(g.start.begin(), g.start.end(), group_start);
+        std::copy(g.members.begin(), g.members.end(), group_seq);
+        *n_groups = g.count();
+    } catch (...) {  // no memory
+        return CRANE_HIP_E_INVALID;
+    }
+    return CRANE_HIP_OK;
+}
 
 extern "C" int crane_hip_copy_pages(void* const* pools, int n_pools, int64_t n_pages, int page_rows, int Hkv, int D,
                                     const int32_t* src, const int32_t* dst, const int32_t* rows, int n, int dtype,

@@ -18,7 +18,8 @@ import torch
 
 from . import _lib
 from ._lib import CraneHipError, check
-from .ops import HEAD_DIM, _ORDERS, _dev, _dtype_code, _prefill_flags, _ptr, _rope_inputs, _stream
+from .ops import (HEAD_DIM, PREFILL_CAUSAL, _ORDERS, _dev, _dtype_code, _on_device, _prefill_flags, _ptr,
+                  _rope_inputs, _stream)
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
@@ -260,6 +261,19 @@ class PagedKvCache:
     def free_sequence(self, sid: int) -> None:
         check(_lib.lib().crane_pkv_seq_free(self._h, sid), "crane_pkv_seq_free")
 
+    def fork_sequence(self, sid: int, count: int = 1, rows: Optional[int] = None) -> List[int]:
+        """`count` new sequences that hold sid's first `rows` rows (default: all):
+        whole pages shared, the rows of a partial last page copied."""
+        return fork_sequence([self], sid, count, rows)
+
+    def truncate_sequence(self, sid: int, rows: int) -> None:
+        """Cut a sequence (not in the batch) to its first `rows` rows."""
+        truncate_sequence([self], sid, rows)
+
+    def compact(self) -> int:
+        """Move the pages in use to the lowest ids; the number moved."""
+        return compact([self])
+
     def seq_len(self, sid: int) -> int:
         return int(_lib.lib().crane_pkv_seq_len(self._h, sid))
 
@@ -370,6 +384,28 @@ class PagedKvCache:
                                            _stream(q.device)), "crane_pkv_prefill")
         return out
 
+    def attention_shared(self, q: torch.Tensor, scale: Optional[float] = None, causal: bool = True,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of the batch sequences' last tokens, the pages they share read
+        once for all that share them (ops.attention_shared_paged): q [B, Hq, D] (a
+        decode step) gives [B, 1, Hq*D], q [B, Hq, S, D] gives [B, S, Hq*D]."""
+        _check_q(q, 4 if q.dim() == 4 else 3, len(self._batch), self.dtype, self.device)
+        q = q.contiguous()
+        B, Hq, S = q.shape[0], q.shape[1], q.shape[2] if q.dim() == 4 else 1
+        need = int(_lib.lib().crane_pkv_shared_workspace(self._h, Hq, S))
+        if workspace is not None:
+            _dev(q, workspace)
+        elif need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        out = torch.empty((B, S, Hq * HEAD_DIM), dtype=q.dtype, device=q.device)
+        with _on_device(q.device):
+            check(_lib.lib().crane_pkv_attention_shared(
+                self._h, q.data_ptr(), Hq, S, HEAD_DIM ** -0.5 if scale is None else scale,
+                PREFILL_CAUSAL if causal else 0, _ptr(workspace),
+                workspace.numel() * workspace.element_size() if workspace is not None else 0, out.data_ptr(),
+                _stream(q.device)), "crane_pkv_attention_shared")
+        return out
+
     def read_sequence(self, sid: int):
         """A sequence's rows as contiguous (k, v) [Hkv, len, D] (get_kv_caches)."""
         n = self.seq_len(sid)
@@ -391,3 +427,48 @@ class PagedKvCache:
         n = k.shape[1]
         check(_lib.lib().crane_pkv_write_seq(self._h, sid, k.data_ptr() if n else None, v.data_ptr() if n else None,
                                              n, _stream(self.device)), "crane_pkv_write_seq")
+
+
+# fork, truncate and compact of all layers' caches at once (driven with the same ids):
+# every cache changes or none, and their page copies go in one launch.
+
+def _handles(caches: Sequence[PagedKvCache]):
+    if any(c.device != caches[0].device for c in caches):
+        raise CraneHipError(_lib.E_INVALID, "caches on different devices")
+    return (ctypes.c_void_p * len(caches))(*[c._h.value for c in caches])
+
+
+def fork_sequence(caches: Sequence[PagedKvCache], sid: int, count: int = 1, rows: Optional[int] = None) -> List[int]:
+    """PagedKvCache.fork_sequence in every cache; the new ids, the same in all."""
+    if not caches:
+        raise CraneHipError(_lib.E_INVALID, "no caches")
+    if not 0 <= count <= caches[0].max_seqs or (rows is not None and rows < 0):
+        raise CraneHipError(_lib.E_CAPACITY if count > caches[0].max_seqs else _lib.E_INVALID,
+                            f"{count} forks of {rows} rows")
+    ids = (ctypes.c_int * max(count, 1))()
+    dev = caches[0].device
+    with _on_device(dev):
+        check(_lib.lib().crane_pkv_fork(_handles(caches), len(caches), sid, -1 if rows is None else rows, count, ids,
+                                        _stream(dev)), "crane_pkv_fork")
+    return list(ids[:count])
+
+
+def truncate_sequence(caches: Sequence[PagedKvCache], sid: int, rows: int) -> None:
+    """PagedKvCache.truncate_sequence in every cache."""
+    if not caches:
+        raise CraneHipError(_lib.E_INVALID, "no caches")
+    dev = caches[0].device
+    with _on_device(dev):
+        check(_lib.lib().crane_pkv_truncate(_handles(caches), len(caches), sid, rows, _stream(dev)),
+              "crane_pkv_truncate")
+
+
+def compact(caches: Sequence[PagedKvCache]) -> int:
+    """PagedKvCache.compact of every cache; the pages moved in all."""
+    if not caches:
+        raise CraneHipError(_lib.E_INVALID, "no caches")
+    dev, moved = caches[0].device, ctypes.c_int64()
+    with _on_device(dev):
+        check(_lib.lib().crane_pkv_compact(_handles(caches), len(caches), ctypes.byref(moved), _stream(dev)),
+              "crane_pkv_compact")
+    return moved.value

@@ -505,6 +505,26 @@ def prefix_groups(groups: Sequence[Sequence[int]], rows: Sequence[int], batch: i
                         max(map(len, groups), default=0), max(shared, default=0), min(shared, default=0))
 
 
+def group_prefixes(tables: Sequence[Sequence[int]]):
+    """(groups, pages) of a batch whose sequence b holds the pages tables[b], in
+    order: the batch rows of every group of sequences that share their first pages,
+    and how many.  Where sequences share more with some than with others, the grouping
+    that reads the fewest pages.  With pages times the page's rows, what prefix_groups
+    takes."""
+    B = len(tables)
+    width = max(map(len, tables), default=0)
+    if any(len(t) and not -2 ** 31 <= min(t) <= max(t) < 2 ** 31 for t in tables):
+        raise CraneHipError(_lib.E_INVALID, "page ids are 32-bit")
+    flat = (ctypes.c_int32 * max(B * width, 1))(*[x for t in tables for x in list(t) + [-1] * (width - len(t))])
+    out = [(ctypes.c_int32 * (B + 1))() for _ in range(3)]
+    n = ctypes.c_int()
+    check(_lib.lib().crane_hip_group_prefixes(flat, width, (ctypes.c_int32 * max(B, 1))(*map(len, tables)), B, *out,
+                                              ctypes.byref(n)), "group_prefixes")
+    shared, start, seq = out
+    groups = [list(seq[start[g]:start[g + 1]]) for g in range(n.value)]
+    return groups, [shared[members[0]] for members in groups]
+
+
 def _on_device(dev: torch.device):
     """The device of a launch made current: a default stream's handle does not say
     which device it is on."""

@@ -20,6 +20,11 @@
  *       [Hkv, len, D] buffer.
  *   active_kv_cache_bytes (:912-929): crane_pkv_bytes.
  *
+ * Pages can be shared: crane_pkv_fork makes sequences that hold another's rows
+ * without copying the pages those rows fill, and crane_pkv_attention_shared reads such
+ * pages once for all of the batch's sequences that share them.  Crane copies a whole
+ * cache instead (its sequences share nothing).
+ *
  * Conventions are those of crane_hip.h: 0 or a CRANE_HIP_E_* status, checked
  * on the host before anything is enqueued (a call that fails changes nothing);
  * everything is ordered on `stream`.  crane_pkv_create allocates the pools and
@@ -50,8 +55,8 @@ void crane_pkv_destroy(crane_pkv* pkv);
 
 /* A new, empty sequence; its id is in [0, max_seqs). */
 int crane_pkv_seq_add(crane_pkv* pkv, int* seq_id);
-/* Release a sequence: its pages return to the free list.  It must not be in
- * the current batch. */
+/* Release a sequence: its pages that no other sequence holds return to the free
+ * list.  It must not be in the current batch. */
 int crane_pkv_seq_free(crane_pkv* pkv, int seq_id);
 /* Valid rows of a live sequence, or -1. */
 int64_t crane_pkv_seq_len(const crane_pkv* pkv, int seq_id);
@@ -86,10 +91,44 @@ int crane_pkv_decode(const crane_pkv* pkv, const void* q, int Hq, float scale, i
 int crane_pkv_prefill(crane_pkv* pkv, const void* q, int Hq, int S, float scale, int flags, void* out,
                       void* stream);
 
+/* ---- Sequences that share pages.  fork, truncate and compact take n caches (the
+ * layers of a model, of one device, driven with the same ids): all are changed, their
+ * copies in one launch where they need the same ones, or none (a launch error aside).
+ * They do not synchronise; work queued on other streams that still reads the pages
+ * concerned is the caller's to order. */
+
+/* `count` new sequences that hold the first `rows` rows of seq_id (-1: all of each
+ * cache's), under ids that are free in every cache, the lowest first (new_ids
+ * [count]).  Whole pages are shared, the rows of a last partial page are copied to a
+ * page of each new sequence.  seq_id may be in the current batch.
+ * CRANE_HIP_E_CAPACITY without enough ids or free pages. */
+int crane_pkv_fork(crane_pkv* const* pkvs, int n, int seq_id, int64_t rows, int count, int* new_ids, void* stream);
+
+/* Cut a sequence to its first `rows` rows (at most its length): pages past them are
+ * released, and a shared page that becomes partial is replaced by a copy
+ * (CRANE_HIP_E_CAPACITY without a free page for it).  The sequence must not be in the
+ * current batch. */
+int crane_pkv_truncate(crane_pkv* const* pkvs, int n, int seq_id, int64_t rows, void* stream);
+
+/* Move the pages sequences hold to the lowest ids, so that pages from
+ * n_pages - crane_pkv_free_pages on are free; a shared page moves once.  The current
+ * batch and its block table follow.  *moved (or NULL): pages moved, over all caches. */
+int crane_pkv_compact(crane_pkv* const* pkvs, int n, int64_t* moved, void* stream);
+
+/* Attention of the last S rows of every batch sequence (q [B, Hq, S, D]; S = 1 is a
+ * decode step), pages that batch sequences share read once for them
+ * (crane_hip_attn_shared_paged, where the arguments and results are described; the
+ * groups are those of the last set_batch).  With S > 1 every sequence holds S rows or
+ * more; with S = 1 one without rows gets zeros.
+ * The workspace's size follows the batch and its lengths; 0: none is needed. */
+size_t crane_pkv_shared_workspace(const crane_pkv* pkv, int Hq, int S);
+int crane_pkv_attention_shared(const crane_pkv* pkv, const void* q, int Hq, int S, float scale, int flags,
+                               void* workspace, size_t ws_bytes, void* out, void* stream);
+
 /* Copy a live sequence's len rows into k, v [Hkv, len, D] (contiguous). */
 int crane_pkv_read_seq(crane_pkv* pkv, int seq_id, void* k, void* v, void* stream);
 /* Replace a live sequence's rows by k, v [Hkv, len, D] (contiguous); it must
- * not be in the current batch. */
+ * not be in the current batch.  Pages it shares are given up, not written. */
 int crane_pkv_write_seq(crane_pkv* pkv, int seq_id, const void* k, const void* v, int64_t len, void* stream);
 
 /* Device pointers for custom kernels: the pools, the current batch's block

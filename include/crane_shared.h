@@ -72,6 +72,17 @@ int crane_hip_attn_shared_paged(const void* q, const void* k_pool, const void* v
                                 int Hkv, int D, float scale, int flags, void* workspace, size_t ws_bytes, void* out,
                                 int dtype, void* stream);
 
+/* The groups of a batch whose sequences name the same first pages (host only, no
+ * side effects): row b of `table` (HOST, `stride` ids a row) lists pages[b] page ids.
+ * Writes shared_pages [B] (pages sequence b shares with its group; 0: in none),
+ * group_start [B + 1] and group_seq [B] (as far as *n_groups groups need them).
+ * Where sequences share more with some than with others, the grouping that reads
+ * the fewest pages is taken.  Ids below 0 are shared by none.  shared_pages times the
+ * page's rows are crane_hip_attn_shared_paged's shared_rows where every shared page is
+ * full of rows. */
+int crane_hip_group_prefixes(const int32_t* table, int64_t stride, const int32_t* pages, int B, int32_t* shared_pages,
+                             int32_t* group_start, int32_t* group_seq, int* n_groups);
+
 /* Copy rows [0, rows[i]) of page src[i] to page dst[i] (all heads), i < n, in
  * every one of n_pools pools [n_pages, Hkv, page_rows, D] (the K and V pools of
  * one or of all layers).

@@ -496,3 +496,318 @@ def test_copy_pages_python_refusals(gpu):
             ops.copy_pages(*args)
     ops.copy_pages([], [0], [1])
     ops.copy_pages([a], [], [])
+
+
+# ------------------------------------------------------------------ grouping (CPU)
+
+def partitions(items):
+    if not items:
+        yield []
+        return
+    first, rest = items[0], items[1:]
+    for p in partitions(rest):
+        yield [[first]] + p
+        for i in range(len(p)):
+            yield p[:i] + [[first] + p[i]] + p[i + 1:]
+
+
+def common(tables, members):
+    n = 0
+    while all(len(tables[b]) > n and tables[b][n] == tables[members[0]][n] >= 0 for b in members):
+        n += 1
+    return n
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_group_prefixes_saves_most(seed):
+    """Against every partition of up to six page lists that branch from one another."""
+    from crane_amd import ops
+    r = cases.rng(seed)
+    tables, nxt = [[]], 1
+    for _ in range(int(r.integers(1, 6))):
+        src = tables[int(r.integers(len(tables)))]
+        t = src[:int(r.integers(0, len(src) + 1))] if seed % 4 else list(src)
+        n = int(r.integers(0, 5))
+        t = t + list(range(nxt, nxt + n))
+        nxt += n
+        tables.append(t)
+    if seed % 5 == 0:
+        tables[0] = [-1, 7]
+        tables[-1] = [-1, 7]
+    groups, pages = ops.group_prefixes(tables)
+    assert len(groups) == len(pages)
+    flat = [b for g in groups for b in g]
+    assert len(flat) == len(set(flat))
+    for g, n in zip(groups, pages):
+        assert len(g) > 1 and n == common(tables, g) > 0
+    saved = sum((len(g) - 1) * n for g, n in zip(groups, pages))
+    best = max(sum((len(g) - 1) * common(tables, g) for g in p) for p in partitions(list(range(len(tables)))))
+    assert saved == best
+
+
+def test_group_prefixes_edges():
+    from crane_amd import _lib, ops
+    from crane_amd._lib import CraneHipError
+    assert ops.group_prefixes([]) == ([], [])
+    assert ops.group_prefixes([[], []]) == ([], [])
+    assert ops.group_prefixes([[5, 6], [1], [5, 6]]) == ([[0, 2]], [2])
+    with pytest.raises(CraneHipError):
+        ops.group_prefixes([[0], [1 << 32]])
+    L, n = _lib.lib(), ctypes.c_int()
+    buf = (ctypes.c_int32 * 8)()
+    assert L.crane_hip_group_prefixes(buf, 2, (ctypes.c_int32 * 1)(3), 1, buf, buf, buf, ctypes.byref(n)) == \
+        _lib.E_INVALID                                                  # more pages than the table's stride
+    assert L.crane_hip_group_prefixes(None, 2, (ctypes.c_int32 * 1)(1), 1, buf, buf, buf, ctypes.byref(n)) == \
+        _lib.E_INVALID
+    assert L.crane_hip_group_prefixes(buf, 2, buf, 1, buf, None, buf, ctypes.byref(n)) == _lib.E_INVALID
+    assert L.crane_hip_group_prefixes(buf, 2, buf, -1, buf, buf, buf, ctypes.byref(n)) == _lib.E_INVALID
+
+
+def test_manager_refusals_without_a_cache():
+    from crane_amd import _lib
+    L = _lib.lib()
+    ids, null = (ctypes.c_int * 4)(), (ctypes.c_void_p * 2)(None, None)
+    assert L.crane_pkv_fork(null, 2, 0, -1, 1, ids, None) == _lib.E_INVALID
+    assert L.crane_pkv_fork(None, 1, 0, -1, 1, ids, None) == _lib.E_INVALID
+    assert L.crane_pkv_fork(null, -1, 0, -1, 1, ids, None) == _lib.E_INVALID
+    assert L.crane_pkv_truncate(null, 1, 0, 0, None) == _lib.E_INVALID
+    assert L.crane_pkv_compact(null, 1, None, None) == _lib.E_INVALID
+    assert L.crane_pkv_shared_workspace(None, 8, 1) == 0
+    assert L.crane_pkv_attention_shared(None, 16, 8, 1, 0.1, 1, None, 0, 16, None) == _lib.E_INVALID
+
+
+# ------------------------------------------------------------------ GPU: the manager
+
+class Model:
+    """What the caches should hold: every sequence's rows per layer, and which
+    sequences hold which pages (a page is named by the object that filled it)."""
+
+    def __init__(self, layers, P):
+        self.rows, self.pages, self.P, self.layers, self.made = {}, {}, P, layers, 0
+
+    def new(self):
+        self.made += 1
+        return self.made
+
+    def grow(self, sid):
+        n = self.rows[sid][0][0].shape[1]
+        while len(self.pages[sid]) * self.P < n:
+            self.pages[sid].append(self.new())
+
+    def cut(self, sid, n):
+        need = math.ceil(n / self.P)
+        held = [p for s, ps in self.pages.items() if s != sid for p in ps]
+        self.pages[sid] = self.pages[sid][:need]
+        if n % self.P and self.pages[sid][-1] in held:
+            self.pages[sid][-1] = self.new()
+
+    def used(self):
+        return len({p for ps in self.pages.values() for p in ps})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed,dtype", [(1, "bf16"), (2, "f32"), (3, "bf16")])
+def test_forks_appends_cuts_and_compactions(gpu, seed, dtype):
+    """A random run over two layers' caches: sequences written, forked, appended to in
+    batches, cut, freed and compacted, against rows kept apart; every step's attention
+    against the definition, and the pages in use counted."""
+    import torch
+    from crane_amd import kv
+    from crane_amd._lib import CraneHipError
+    r = cases.rng(900 + seed)
+    Hkv, Hq, P, n_pages = 2, 8, 256, 24
+    td = torch.bfloat16 if dtype == "bf16" else torch.float32
+    caches = [kv.PagedKvCache(Hkv, n_pages, td, P, max_seqs=8, max_pages_per_seq=8, device=gpu) for _ in range(2)]
+    m = Model(2, P)
+    rand = lambda *shape: tens(cases.normal(r, shape), dtype, gpu)
+    batch = []
+
+    def check(sids):
+        for sid in sids:
+            for c, layer in zip(caches, m.rows[sid]):
+                k, v = c.read_sequence(sid)
+                assert torch.equal(k, layer[0]) and torch.equal(v, layer[1]), sid
+        assert all(c.free_pages == n_pages - m.used() for c in caches)
+
+    for step in range(60):
+        what = ["write", "fork", "append", "append", "cut", "free", "compact", "append"][int(r.integers(8))]
+        live = sorted(m.rows)
+        idle = [s for s in live if s not in batch]
+        print(f"step {step}: {what} live={live} used={m.used()}", flush=True)
+        try:
+            if what == "write":
+                n = int(r.integers(0, 3 * P))
+                new = not idle or r.integers(2)
+                sids = [c.add_sequence() for c in caches] if new else [idle[0]] * 2
+                assert sids[0] == sids[1]
+                rows = [[rand(Hkv, n, D), rand(Hkv, n, D)] for _ in caches]
+                if new:
+                    m.rows[sids[0]], m.pages[sids[0]] = [[x[:, :0] for x in l] for l in rows], []
+                for c, (k, v) in zip(caches, rows):
+                    c.write_sequence(sids[0], k, v)
+                held = [p for s, ps in m.pages.items() if s != sids[0] for p in ps]
+                m.pages[sids[0]] = [p for p in m.pages[sids[0]] if p not in held][:math.ceil(n / P)]
+                m.rows[sids[0]] = rows
+                m.grow(sids[0])
+            elif what == "fork" and live:
+                sid, count = live[int(r.integers(len(live)))], int(r.integers(1, 4))
+                full = m.rows[sid][0][0].shape[1]
+                n = None if r.integers(2) else int(r.integers(0, full + 1))
+                ids = kv.fork_sequence(caches, sid, count, n)
+                n = full if n is None else n
+                assert len(set(ids)) == count and not set(ids) & set(live)
+                for i in ids:
+                    m.rows[i] = [[x[:, :n].clone() for x in l] for l in m.rows[sid]]
+                    m.pages[i] = m.pages[sid][:n // P] + ([m.new()] if n % P else [])
+            elif what == "append" and live:
+                batch = [s for s in live if r.integers(4)] or live[:1]
+                for c in caches:
+                    c.set_batch(batch)
+                S = int(r.integers(1, 6)) if r.integers(3) else int(r.integers(100, 300))
+                new = [[rand(len(batch), Hkv, S, D), rand(len(batch), Hkv, S, D)] for _ in caches]
+                for c, (k, v) in zip(caches, new):
+                    c.update_kv_cache(k, v)
+                for i, sid in enumerate(batch):
+                    m.rows[sid] = [[torch.cat([x, y[i]], 1) for x, y in zip(l, nl)] for l, nl in zip(m.rows[sid], new)]
+                    m.grow(sid)
+                Sq = min(S, 3)
+                q = cases.cast(cases.normal(r, (len(batch), Hq, Sq, D)), dtype)
+                for c, layer in zip(caches, range(2)):
+                    got = c.attention_shared(tens(q, dtype, gpu) if Sq > 1 else tens(q, dtype, gpu)[:, :, 0])
+                    for i, sid in enumerate(batch):
+                        k, v = (x.float().cpu().numpy() for x in m.rows[sid][layer])
+                        n = k.shape[1]
+                        t = np.zeros((1, 1), np.int32)
+                        out, mag, most = reference(q[i:i + 1], k[None], v[None], t, [n], n, D ** -0.5, True)
+                        err = np.abs(got[i:i + 1].float().cpu().numpy() - out)
+                        assert (err <= bounds(out, mag, most, n, dtype)).all(), (sid, n)
+            elif what == "cut" and idle:
+                sid = idle[int(r.integers(len(idle)))]
+                n = int(r.integers(0, m.rows[sid][0][0].shape[1] + 1))
+                kv.truncate_sequence(caches, sid, n)
+                m.rows[sid] = [[x[:, :n].clone() for x in l] for l in m.rows[sid]]
+                m.cut(sid, n)
+            elif what == "free" and idle:
+                for c in caches:
+                    c.free_sequence(idle[-1])
+                del m.rows[idle[-1]], m.pages[idle[-1]]
+            elif what == "compact":
+                kv.compact(caches)
+                assert kv.compact(caches) == 0
+                for c in caches:
+                    assert c.block_table().max() < m.used() if batch else True
+        except CraneHipError as e:              # (both layers refuse alike, the first before the second)
+            assert "capacity" in str(e), e      # out of pages or ids: nothing has changed
+        check(m.rows)
+    for c in caches:
+        c.close()
+
+
+@pytest.mark.gpu
+def test_answers_to_one_prompt(gpu):
+    """A prompt prefilled once, forked into answers that decode together, beside copies
+    of it that share nothing: the same appends give the same rows, the attention is
+    the definition's for both, and freeing the answers leaves the prompt."""
+    import torch
+    from crane_amd import kv, ops
+    Hq, Hkv, P, S0, n = 16, 2, 256, 700, 5
+    g = torch.Generator(device=gpu).manual_seed(5)
+    r16 = lambda *s: torch.randn(s, generator=g, device=gpu).to(torch.bfloat16)
+    cos, sin = ops.rope_tables(D, 1e6, 2048, device=gpu, dtype=torch.bfloat16)
+    c = kv.PagedKvCache(Hkv, 40, torch.bfloat16, P, max_seqs=16, max_pages_per_seq=6, device=gpu)
+    first = c.add_sequence()
+    c.set_batch([first])
+    qkv, at = r16(1, S0, (Hq + 2 * Hkv) * D), torch.zeros(1, dtype=torch.int32, device=gpu)
+    q = c.append_qkv(qkv, cos, sin, at, Hq)
+    got = c.attention_shared(q).float().cpu().numpy()   # the prompt itself: one sequence, no groups
+    k, v = c.read_sequence(first)
+    kk, vv = k.float().cpu().numpy(), v.float().cpu().numpy()
+    out, mag, most = reference(q.float().cpu().numpy(), kk[None], vv[None], np.zeros((1, 1), np.int32), [S0], S0,
+                               D ** -0.5, True)
+    assert (np.abs(got - out) <= bounds(out, mag, most, S0, "bf16")).all()
+    used = 40 - c.free_pages
+    answers = c.fork_sequence(first, n)
+    assert 40 - c.free_pages == used + n                # the 188 rows past two whole pages, copied
+    copies = []
+    for _ in range(n):
+        copies.append(c.add_sequence())
+        c.write_sequence(copies[-1], k, v)
+    for step in range(3):
+        tok = r16(n, 1, (Hq + 2 * Hkv) * D)
+        at = torch.full((n,), S0 + step, dtype=torch.int32, device=gpu)
+        outs, rows = [], []
+        for ids in (answers, copies):
+            c.set_batch(ids)
+            q = c.append_qkv(tok, cos, sin, at, Hq)
+            outs.append(c.attention_shared(q.view(n, Hq, D)).float().cpu().numpy())
+            rows.append([c.read_sequence(i) for i in ids])
+        for (ka, va), (kb, vb) in zip(*rows):
+            assert torch.equal(ka, kb) and torch.equal(va, vb)
+        qn = q.float().cpu().numpy()
+        for i, (ka, va) in enumerate(rows[0]):
+            kk, vv = ka.float().cpu().numpy(), va.float().cpu().numpy()
+            out, mag, most = reference(qn[i:i + 1], kk[None], vv[None], np.zeros((1, 1), np.int32), [kk.shape[1]],
+                                       kk.shape[1], D ** -0.5, True)
+            tol = bounds(out, mag, most, kk.shape[1], "bf16")
+            assert (np.abs(outs[0][i] - out[0]) <= tol[0]).all() and (np.abs(outs[1][i] - out[0]) <= tol[0]).all()
+        if step == 1:
+            c.set_batch([])
+            c.free_sequence(copies.pop())
+            copies.append(c.fork_sequence(answers[-1])[0])  # and a fork of a fork in a copy's place
+            moved = c.compact()
+            assert moved >= 0 and c.compact() == 0
+    c.set_batch([])
+    for i in answers + copies:
+        c.free_sequence(i)
+    assert 40 - c.free_pages == used
+    k2, v2 = c.read_sequence(first)
+    assert torch.equal(k, k2) and torch.equal(v, v2)
+    c.close()
+
+
+@pytest.mark.gpu
+def test_manager_refusals(gpu):
+    import torch
+    from crane_amd import _lib, kv
+    from crane_amd._lib import CraneHipError
+    c = kv.PagedKvCache(2, 8, torch.bfloat16, 256, max_seqs=4, max_pages_per_seq=4, device=gpu)
+    a = c.add_sequence()
+    z = torch.zeros((2, 300, D), dtype=torch.bfloat16, device=gpu)
+    c.write_sequence(a, z, z)
+    c.set_batch([a])
+
+    def refused(code, f, *args):
+        with pytest.raises(CraneHipError) as e:
+            f(*args)
+        assert e.value.code == code, e.value
+
+    refused(_lib.E_INVALID, c.fork_sequence, 3)                # not live
+    refused(_lib.E_INVALID, c.fork_sequence, a, 1, 301)        # more rows than it has
+    refused(_lib.E_INVALID, c.fork_sequence, a, 1, -1)
+    refused(_lib.E_INVALID, c.fork_sequence, a, -1)
+    refused(_lib.E_CAPACITY, c.fork_sequence, a, 4)            # 3 ids left
+    refused(_lib.E_INVALID, c.truncate_sequence, a, 10)        # in the batch
+    refused(_lib.E_INVALID, kv.fork_sequence, [c, c], a)       # one cache twice
+    refused(_lib.E_INVALID, kv.compact, [])
+    assert c.fork_sequence(a, 0) == []
+    b, = c.fork_sequence(a, 1, 256)                            # a whole page: nothing copied
+    assert c.seq_len(b) == 256 and c.free_pages == 6
+    refused(_lib.E_INVALID, c.truncate_sequence, b, 257)
+    refused(_lib.E_INVALID, c.truncate_sequence, b, -1)
+    q = torch.zeros((1, 4, D), dtype=torch.bfloat16, device=gpu)
+    refused(_lib.E_INVALID, c.attention_shared, q.expand(2, 4, D))
+    refused(_lib.E_DTYPE, c.attention_shared, q.float())
+    refused(_lib.E_INVALID, c.attention_shared, q.view(1, 4, 1, D).expand(1, 4, 301, D))
+    refused(_lib.E_INVALID, c.attention_shared, q, -1.0)
+    other = kv.PagedKvCache(2, 3, torch.bfloat16, 256, max_seqs=4, max_pages_per_seq=4, device=gpu)
+    other.write_sequence(other.add_sequence(), z[:, :200], z[:, :200])
+    refused(_lib.E_INVALID, kv.fork_sequence, [c, other], a, 1, 256)   # `other` has 200 rows
+    assert c.free_pages == 6 and other.free_pages == 2
+    other.set_batch([])
+    d, = other.fork_sequence(0)
+    e, = other.fork_sequence(0)
+    assert other.free_pages == 0
+    refused(_lib.E_CAPACITY, other.fork_sequence, 0)           # no page for the copied rows
+    assert [other.seq_len(i) for i in (0, d, e, 3)] == [200, 200, 200, -1]
+    c.close()
+    other.close()
