@@ -140,7 +140,7 @@ class PagedKv {
             hipMalloc(&d_len_, sizeof(int32_t) * (size_t)max_seqs_) != hipSuccess ||
             hipMalloc(&d_start_, sizeof(int32_t) * (size_t)max_seqs_) != hipSuccess ||
             hipMalloc(&d_one_, sizeof(int32_t) * (size_t)max_pps_) != hipSuccess ||
-            hipMalloc(&d_groups_, sizeof(int32_t) * (3 * (size_t)max_seqs_ + 1)) != hipSuccess) {
+            hipMalloc(&d_groups_, sizeof(int32_t) * 4 * (size_t)max_seqs_) != hipSuccess) {
             release();
             return CRANE_HIP_E_LAUNCH;
         }
@@ -208,10 +208,13 @@ class PagedKv {
             for (int b = 0; b < B; ++b) lists[b] = {seqs_[ids[b]].pages.data(), seqs_[ids[b]].pages.size()};
             groups = group_pages(lists);
         }
-        if (groups.count()) {  // shared rows per sequence, then the groups' starts and members
-            for (int32_t pages : groups.shared) shared.push_back(pages * P_);
-            shared.insert(shared.end(), groups.start.begin(), groups.start.end());
+        if (groups.count()) {  // crane_hip_attn_shared_paged's groups, members and shared rows
+            for (int i = 0; i < groups.count(); ++i) {
+                const int32_t at = groups.start[i], leader = groups.members[at];
+                for (int32_t x : {at, groups.start[i + 1] - at, leader, groups.shared[leader] * P_}) shared.push_back(x);
+            }
             shared.insert(shared.end(), groups.members.begin(), groups.members.end());
+            for (int32_t pages : groups.shared) shared.push_back(pages * P_);
         }
         std::vector<int> batch(ids, ids + B);
         batch_.clear();  // no batch if an upload fails
@@ -224,6 +227,7 @@ class PagedKv {
         if (rc) return rc;
         batch_.swap(batch);
         n_groups_ = groups.count();
+        n_members_ = (int)groups.members.size();
         for (int i = 0; i < n_groups_; ++i) max_group_ = std::max(max_group_, groups.start[i + 1] - groups.start[i]);
         batch_shared_.swap(groups.shared);
         return CRANE_HIP_OK;
@@ -519,9 +523,9 @@ class PagedKv {
         for (int id : batch_)
             if (S > 1 && seqs_[id].len < S) return CRANE_HIP_E_INVALID;  // every sequence holds its S new rows
         if (max_len() == 0) return CRANE_HIP_E_INVALID;
-        const int32_t *shared = d_groups_, *start = shared + B(), *members = start + n_groups_ + 1;
+        const int32_t *members = d_groups_ + 4 * n_groups_, *shared = members + n_members_;
         return crane_hip_attn_shared_paged(q, k_pool_, v_pool_, n_pages_, P_, d_table_, max_pps_, d_len_, max_len(),
-                                           shared, start, members, n_groups_, max_group_, max_shared(), max_own(), B(),
+                                           shared, d_groups_, members, n_groups_, max_group_, max_shared(), max_own(), B(),
                                            S, Hq, Hkv_, D_, scale, flags, ws, ws_bytes, out, dtype_, st);
     }
 
@@ -609,14 +613,14 @@ class PagedKv {
     int32_t* d_len_ = nullptr;    // current batch lengths
     int32_t* d_start_ = nullptr;  // prefill chunk starts
     int32_t* d_one_ = nullptr;    // one sequence's page ids (read_seq / write_seq)
-    int32_t* d_groups_ = nullptr; // current batch: shared rows, group starts, members (when there are groups)
+    int32_t* d_groups_ = nullptr;  // current batch: groups, their members, shared rows (when there are groups)
     std::vector<int32_t> free_;
     std::vector<int32_t> refs_;   // owners of every page
     int64_t shared_pages_ = 0;    // pages of more than one owner
     std::vector<Seq> seqs_;
     std::vector<int> batch_;
     std::vector<int32_t> batch_shared_;  // pages each batch sequence shares (when there are groups)
-    int n_groups_ = 0, max_group_ = 0;
+    int n_groups_ = 0, n_members_ = 0, max_group_ = 0;
 };
 
 }  // namespace crane

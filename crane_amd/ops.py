@@ -470,12 +470,13 @@ def attention_prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
 
 class PrefixGroups:
     """Which sequences of a batch share their first rows (prefix_groups makes and
-    checks it): per-sequence shared rows and the groups' members on the device, and
-    their host-side bounds.  Kept for as long as the batch and its sharing stay."""
+    checks it): the groups {first member's place, members, batch row, shared rows},
+    their members and every sequence's shared rows on the device, and their host-side
+    bounds.  Kept for as long as the batch and its sharing stay."""
 
-    def __init__(self, batch: int, shared_rows, group_start, group_seq, n_groups: int, max_group: int,
-                 max_shared: int, min_shared: int):
-        self.batch, self.shared_rows, self.group_start, self.group_seq = batch, shared_rows, group_start, group_seq
+    def __init__(self, batch: int, groups, members, shared_rows, n_groups: int, max_group: int, max_shared: int,
+                 min_shared: int):
+        self.batch, self.groups, self.members, self.shared_rows = batch, groups, members, shared_rows
         self.n_groups, self.max_group = n_groups, max_group
         self.max_shared, self.min_shared = max_shared, min_shared
 
@@ -488,20 +489,21 @@ def prefix_groups(groups: Sequence[Sequence[int]], rows: Sequence[int], batch: i
     and waits for them."""
     if len(groups) != len(rows):
         raise CraneHipError(_lib.E_INVALID, f"{len(groups)} groups, {len(rows)} row counts")
-    shared, start, seq, seen = [0] * batch, [0], [], set()
-    for members, n in zip(groups, rows):
-        if n < 0 or n > 0x7fffffff or not len(members):
+    shared, desc, seq, seen = [0] * batch, [], [], set()
+    for of, n in zip(groups, rows):
+        if n < 0 or n > 0x7fffffff or not len(of):
             raise CraneHipError(_lib.E_INVALID, "a group has members and shares 0 or more rows")
-        for b in members:
+        desc += [len(seq), len(of), int(of[0]), int(n)]
+        for b in of:
             if not 0 <= b < batch or b in seen:
                 raise CraneHipError(_lib.E_INVALID, f"sequence {b}: not in a batch of {batch}, or in two groups")
             seen.add(b)
             shared[b] = int(n)
             seq.append(int(b))
-        start.append(len(seq))
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-    flat = torch.tensor(shared + start + seq, dtype=torch.int32).to(dev)
-    return PrefixGroups(batch, flat[:batch], flat[batch:batch + len(start)], flat[batch + len(start):], len(groups),
+    flat = torch.tensor(desc + seq + shared, dtype=torch.int32).to(dev)
+    at = len(desc) + len(seq)
+    return PrefixGroups(batch, flat[:len(desc)].view(-1, 4), flat[len(desc):at], flat[at:], len(groups),
                         max(map(len, groups), default=0), max(shared, default=0), min(shared, default=0))
 
 
@@ -567,8 +569,8 @@ def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     with _on_device(dev):
         rc = _lib.lib().crane_hip_attn_shared_paged(
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, page_rows, block_table.data_ptr(), stride,
-            kv_len.data_ptr(), max_kv, groups.shared_rows.data_ptr(), groups.group_start.data_ptr(),
-            groups.group_seq.data_ptr(), groups.n_groups, groups.max_group, groups.max_shared, max_own, B, S, Hq, Hkv,
+            kv_len.data_ptr(), max_kv, groups.shared_rows.data_ptr(), groups.groups.data_ptr(),
+            groups.members.data_ptr(), groups.n_groups, groups.max_group, groups.max_shared, max_own, B, S, Hq, Hkv,
             HEAD_DIM, scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace),
             workspace.numel() * workspace.element_size() if workspace is not None else 0, out.data_ptr(), dt,
             _stream(dev))

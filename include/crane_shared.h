@@ -40,13 +40,13 @@ size_t crane_hip_attn_shared_workspace(int n_groups, int max_group, int64_t max_
  * shared_rows [B] int32, device: sequence b shares its first shared_rows[b] rows
  *          (0: none) with every member of its group; any number, not only whole
  *          pages.  NULL when n_groups is 0
- * group_start [n_groups + 1], group_seq [group_start[n_groups]] int32, device:
- *          the members of group g are the batch rows group_seq[group_start[g] ..
- *          group_start[g + 1]), read through the first one's row of the block
- *          table.  A sequence with shared rows is in exactly one group, whose
- *          members all have its shared_rows; other sequences are in none.  A
- *          description that breaks this gives unspecified results for the
- *          sequences concerned and stays in bounds
+ * groups   [n_groups, 4] int32, device, 16-byte aligned: {s, n, b, r}: the group's
+ *          members are the batch rows members[s .. s + n), it shares r rows, and they
+ *          are read through row b of the block table (a member's).  A sequence with
+ *          shared rows is in exactly one group, whose r is its shared_rows; other
+ *          sequences are in none.  A description that breaks this gives unspecified
+ *          results for the sequences concerned and stays in bounds
+ * members  int32, device, B entries at most
  * max_group, max_shared, max_own: host-side bounds of a group's members, of
  *          shared_rows, and of kv_len[b] - shared_rows[b]; rows past them need not
  *          be attended.  max_shared + max_own < 2^31 - 2^14
@@ -67,8 +67,8 @@ size_t crane_hip_attn_shared_workspace(int n_groups, int max_group, int64_t max_
  * give the same bits. */
 int crane_hip_attn_shared_paged(const void* q, const void* k_pool, const void* v_pool, int64_t n_pages, int page_rows,
                                 const int32_t* block_table, int64_t table_stride, const int32_t* kv_len, int64_t max_kv,
-                                const int32_t* shared_rows, const int32_t* group_start, const int32_t* group_seq,
-                                int n_groups, int max_group, int64_t max_shared, int64_t max_own, int B, int S, int Hq,
+                                const int32_t* shared_rows, const int32_t* groups, const int32_t* members, int n_groups,
+                                int max_group, int64_t max_shared, int64_t max_own, int B, int S, int Hq,
                                 int Hkv, int D, float scale, int flags, void* workspace, size_t ws_bytes, void* out,
                                 int dtype, void* stream);
 

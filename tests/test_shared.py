@@ -153,7 +153,8 @@ def check_exact(gpu, seed, lens, groups, rows, P, Hq, Hkv, S, dtype, causal=True
                 want[b, s] = (total_v[:, L - 1].astype(np.float32) / np.float32(L))[:, None, :]
     want = torch.from_numpy(want.reshape(len(lens), S, -1)).to(got.dtype)
     assert got.shape == want.shape
-    assert torch.equal(got.cpu(), want)
+    wrong = int((got.cpu() != want).sum())
+    assert wrong == 0, wrong
 
 
 def check_close(gpu, seed, lens, groups, rows, P, Hq, Hkv, S, dtype, causal=True, q_scale=1.5, **kw):
@@ -174,7 +175,7 @@ def check_close(gpu, seed, lens, groups, rows, P, Hq, Hkv, S, dtype, causal=True
 
 # ------------------------------------------------------------------ refusals (CPU)
 
-BASE = dict(q=16, k=16, v=16, n_pages=64, P=256, table=16, stride=8, kv_len=16, max_kv=1024, shared=16, gs=16, gq=16,
+BASE = dict(q=16, k=16, v=16, n_pages=64, P=256, table=16, stride=8, kv_len=16, max_kv=1024, shared=16, groups=16, members=16,
             n_groups=1, max_group=4, max_shared=512, max_own=512, B=4, S=1, Hq=32, Hkv=8, D=128, scale=0.088, flags=1,
             ws=16, ws_bytes=1 << 40, out=16, dtype=1, stream=None)
 
@@ -194,7 +195,7 @@ def shared_call(**kw):
     (dict(flags=2), "E_INVALID"), (dict(flags=3), "E_INVALID"), (dict(scale=0.0), "E_INVALID"),
     (dict(scale=float("nan")), "E_INVALID"), (dict(scale=float("inf")), "E_INVALID"), (dict(q=None), "E_INVALID"),
     (dict(out=None), "E_INVALID"), (dict(kv_len=None), "E_INVALID"), (dict(shared=None), "E_INVALID"),
-    (dict(gs=None), "E_INVALID"), (dict(gq=None), "E_INVALID"), (dict(q=8), "E_ALIGN"), (dict(k=24), "E_ALIGN"),
+    (dict(groups=None), "E_INVALID"), (dict(members=None), "E_INVALID"), (dict(groups=8), "E_ALIGN"), (dict(q=8), "E_ALIGN"), (dict(k=24), "E_ALIGN"),
     (dict(v=8), "E_ALIGN"), (dict(out=8), "E_ALIGN"), (dict(ws=None), "E_WORKSPACE"), (dict(ws=8), "E_WORKSPACE"),
     (dict(ws_bytes=100), "E_WORKSPACE"), (dict(B=-1), "E_INVALID"), (dict(S=-1), "E_INVALID"),
     (dict(B=65536), "E_INVALID"), (dict(B=0, n_groups=0, max_group=0, max_shared=0), "OK"), (dict(S=0), "OK"),
@@ -247,7 +248,7 @@ def test_prefix_groups_checks():
     from crane_amd._lib import CraneHipError
     g = ops.prefix_groups([[3, 0], [1]], [512, 100], 5, "cpu")
     assert g.shared_rows.tolist() == [512, 100, 0, 512, 0]
-    assert g.group_start.tolist() == [0, 2, 3] and g.group_seq.tolist() == [3, 0, 1]
+    assert g.groups.tolist() == [[0, 2, 3, 512], [2, 1, 1, 100]] and g.members.tolist() == [3, 0, 1]
     assert (g.n_groups, g.max_group, g.max_shared, g.min_shared) == (2, 2, 512, 0)
     g = ops.prefix_groups([], [], 3, "cpu")
     assert (g.n_groups, g.max_group, g.max_shared, g.min_shared) == (0, 0, 0, 0)
@@ -410,12 +411,14 @@ def test_inconsistent_descriptions_stay_in_bounds(gpu):
     g = ops.prefix_groups([[0, 1]], [512], 3, gpu)
     args = lambda: (tens(q, "bf16", gpu).view(3, 8, D), tens(k, "bf16", gpu), tens(v, "bf16", gpu), ints(table, gpu),
                     ints(lens, gpu), 700, g)
-    g.group_seq = ints([0, 99], gpu)
-    got = ops.attention_shared_paged(*args())
-    assert torch.equal(got[2], want[2])
-    g.group_start, g.group_seq = ints([-50, 1 << 30], gpu), ints([0, 1, 2], gpu)
-    got = ops.attention_shared_paged(*args())
-    assert torch.equal(got[2], want[2])
+    for groups, members in (([[0, 2, 0, 512]], [0, 99]), ([[0, 2, 0, 512]], [-3, 1]),
+                            ([[-50, 1 << 30, 0, 512]], [0, 1, 2]), ([[0, 2, 99, 512]], [0, 1]),
+                            ([[0, 2, -1, 512]], [0, 1]), ([[0, -4, 0, 512]], [0, 1]),
+                            ([[0, 2, 0, 1 << 30]], [0, 1]), ([[0, 2, 0, -9]], [0, 1]), ([[1 << 30, 2, 0, 512]], [0, 1])):
+        print(groups, members, flush=True)
+        g.groups, g.members = ints(groups, gpu), ints(members + [0] * 3, gpu)
+        got = ops.attention_shared_paged(*args())
+        assert torch.equal(got[2], want[2])
 
 
 @pytest.mark.gpu
