@@ -218,7 +218,7 @@ class PagedKv {
         }
         std::vector<int> batch(ids, ids + B);
         batch_.clear();  // no batch if an upload fails
-        n_groups_ = max_group_ = 0;
+        n_groups_ = 0;
         if (B == 0) return CRANE_HIP_OK;
         int rc = upload(d_table_, table, st);
         if (!rc) rc = upload(d_len_, lens, st);
@@ -228,8 +228,7 @@ class PagedKv {
         batch_.swap(batch);
         n_groups_ = groups.count();
         n_members_ = (int)groups.members.size();
-        for (int i = 0; i < n_groups_; ++i) max_group_ = std::max(max_group_, groups.start[i + 1] - groups.start[i]);
-        batch_shared_.swap(groups.shared);
+        batch_groups_.swap(shared);
         return CRANE_HIP_OK;
     }
 
@@ -504,17 +503,17 @@ class PagedKv {
     // Attention of the batch's last S rows, shared pages read once per group.
     int64_t max_own() const {
         int64_t m = 0;
-        for (int b = 0; b < B(); ++b) m = std::max(m, seqs_[batch_[b]].len - shared_rows(b));
+        for (int b = 0; b < B(); ++b) m = std::max(m, seqs_[batch_[b]].len - batch_shared_rows(b));
         return m;
     }
-    int64_t max_shared() const {
-        int64_t m = 0;
-        for (int b = 0; b < B(); ++b) m = std::max(m, shared_rows(b));
-        return m;
+    int64_t mean_own() const {
+        int64_t sum = 0;
+        for (int b = 0; b < B(); ++b) sum += seqs_[batch_[b]].len - batch_shared_rows(b);
+        return B() ? sum / B() : 0;
     }
     size_t shared_workspace(int Hq, int S) const {
-        return crane_hip_attn_shared_workspace(n_groups_, max_group_, max_shared(), max_own(), B(), S, Hq, Hkv_, D_,
-                                               dtype_);
+        return crane_hip_attn_shared_workspace(batch_groups_.data(), n_groups_, max_own(), mean_own(), B(), S, Hq, Hkv_,
+                                               D_, dtype_);
     }
     int attention_shared(const void* q, int Hq, int S, float scale, int flags, void* ws, size_t ws_bytes, void* out,
                          hipStream_t st) const {
@@ -525,8 +524,8 @@ class PagedKv {
         if (max_len() == 0) return CRANE_HIP_E_INVALID;
         const int32_t *members = d_groups_ + 4 * n_groups_, *shared = members + n_members_;
         return crane_hip_attn_shared_paged(q, k_pool_, v_pool_, n_pages_, P_, d_table_, max_pps_, d_len_, max_len(),
-                                           shared, d_groups_, members, n_groups_, max_group_, max_shared(), max_own(), B(),
-                                           S, Hq, Hkv_, D_, scale, flags, ws, ws_bytes, out, dtype_, st);
+                                           shared, d_groups_, members, batch_groups_.data(), n_groups_, max_own(), mean_own(),
+                                           B(), S, Hq, Hkv_, D_, scale, flags, ws, ws_bytes, out, dtype_, st);
     }
 
     bool same_shape(const PagedKv& o) const {
@@ -563,7 +562,7 @@ class PagedKv {
         if (refs_[p] == 2) --shared_pages_;
         if (--refs_[p] == 0) free_.push_back(p);
     }
-    int64_t shared_rows(int b) const { return n_groups_ ? (int64_t)batch_shared_[b] * P_ : 0; }
+    int64_t batch_shared_rows(int b) const { return n_groups_ ? batch_groups_[(size_t)(4 * n_groups_ + n_members_ + b)] : 0; }
 
     static int upload(int32_t* dst, const std::vector<int32_t>& v, hipStream_t st) {
         return hip_rc(hipMemcpyAsync(dst, v.data(), sizeof(int32_t) * v.size(), hipMemcpyHostToDevice, st));
@@ -619,8 +618,8 @@ class PagedKv {
     int64_t shared_pages_ = 0;    // pages of more than one owner
     std::vector<Seq> seqs_;
     std::vector<int> batch_;
-    std::vector<int32_t> batch_shared_;  // pages each batch sequence shares (when there are groups)
-    int n_groups_ = 0, n_members_ = 0, max_group_ = 0;
+    std::vector<int32_t> batch_groups_;  // what d_groups_ holds
+    int n_groups_ = 0, n_members_ = 0;
 };
 
 }  // namespace crane

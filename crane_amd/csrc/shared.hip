@@ -12,8 +12,8 @@
 // shared chunks, (query, head) of one sequence for its own.  A second kernel joins the
 // chunks.  Two forms, by the rows there are:
 //
-// Stream (up to 16 rows: HBM-bound).  Every wave takes 32-key steps of its own, K and V
-// from memory to registers two steps ahead, and the waves' m, l, o are joined through
+// Stream (16 or 32 rows: HBM-bound).  Every wave takes 32-key steps of its own, K and V
+// from memory to registers ahead of their use, and the waves' m, l, o are joined through
 // LDS at the end.  bf16, v_mfma_f32_16x16x32_bf16: S^T = K Q^T with K rows as A and
 // query rows as B, so lane (i, g) = (lane % 16, lane / 16) holds, for query row i, keys
 // 4 g + r of two 16-key halves.  Those 8 values, rounded to bf16, are the B operand
@@ -23,18 +23,28 @@
 // pairs them into the A operand of eight products, product n giving dims 8 m + n: a
 // lane ends with dims [32 g, 32 g + 32) of its query row.
 //
-// Block (more rows: 128 of bf16, 64 of f32, a share for each wave).  The waves walk the
-// same keys, staged in LDS by buffer_load ... lds one tile ahead, so that K and V are
-// read from memory once for the block.  bf16, v_mfma_f32_32x32x16_bf16: the same
-// products with 32 rows a wave and 64 keys a tile; V^T comes from the row-major tile
-// by transposed LDS reads.
+// f32 runs this layout on v_mfma_f32_16x16x4_f32: a k slot takes one key (or dim) of
+// every lane group, so no pairing is needed.
 //
-// f32 runs the stream's layout on v_mfma_f32_16x16x4_f32 in both forms: a k slot takes
-// one key (or dim) of every lane group, so no pairing is needed.
+// Block (bf16, more rows: 32 for each wave).  The waves walk the same keys, staged in
+// LDS by buffer_load ... lds one tile ahead, so that K and V are read from memory once
+// for the block.  v_mfma_f32_32x32x16_bf16: the same products with 32 rows a wave and
+// 64 keys a tile; V^T comes from the row-major tile by transposed LDS reads.
 //
 // l sums p as computed in f32; only the P operand is rounded (bf16).
+//
+// A row's m is settled by the first keys of its walk (two steps, one tile) and then left
+// alone: exp2(s - m) of f32 or bf16 stays exact to its own rounding however far s passes
+// m, until it overflows.  So the walk takes no maximum and scales nothing (60 of about
+// 150 vector instructions of a step), and looks once, at its end, whether l passed
+// kMostSum or o is not finite.  That is so after a row's scores rose by 2^60 (41 in
+// natural units) over its first keys, or where V holds an infinity or a NaN, even in a
+// key the row does not see (0 x inf).  Then the walk is repeated with m moved at every
+// step and such keys added to the rows that see them only.
 #include <float.h>
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -46,10 +56,10 @@ namespace {
 constexpr int kAlign = 64;         // chunk bounds are multiples of it (whole steps of every form)
 constexpr int kWaves = 4;
 constexpr float kNoMax = -FLT_MAX; // m before the first key (finite: exp2(-inf - m) is 0, not NaN)
+constexpr float kMostSum = 0x1p60f;  // see above
 constexpr int kMaxChunk = 8192;    // rows per chunk: its pages' ids fit one lane each
 constexpr int kMinChunk = 128;
-constexpr int kStreamRows = 16;    // query rows of a workgroup
-template <typename T> constexpr int kBlockRows = sizeof(T) == 2 ? 128 : 64;
+constexpr int kBlockRows = 128;    // query rows of a workgroup's block form
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
@@ -86,6 +96,12 @@ struct Args {
     __device__ __forceinline__ int shared_of(int b) const { return shared ? max(0, min(shared[b], max_shared)) : 0; }
     // Rows query s of sequence b sees.
     __device__ __forceinline__ int limit(int b, int s) const { return causal ? len(b) - S + 1 + s : len(b); }
+    // The row of out [B, S, Hq] that is row `at` of q [B, Hq, S].
+    __device__ __forceinline__ int64_t out_row(int at) const {
+        if (S == 1) return at;
+        const int bh = at / S, s = at - bh * S, b = bh / Hq;
+        return ((int64_t)b * S + s) * Hq + (bh - b * Hq);
+    }
     // First row of own chunk 0: chunk bounds sit on tile bounds.
     __device__ __forceinline__ static int own_base(int shared_rows) { return shared_rows & ~(kAlign - 1); }
 };
@@ -167,20 +183,32 @@ template <typename T> __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsr
     return make_rsrc(reinterpret_cast<const T*>(pool) + t.off, t.bytes);
 }
 
-__device__ __forceinline__ int wave_max_int(int x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x = max(x, __shfl_xor(x, d));
+// Maximum over N = 16 or 32 neighbouring lanes, for values that repeat every N lanes of
+// the wave; uniform.
+template <int CTRL> __device__ __forceinline__ int dpp_int(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, false);
+}
+template <int N> __device__ __forceinline__ int rows_max(int x) {
+    x = max(x, dpp_int<0xB1>(x));   // quad_perm [1,0,3,2]
+    x = max(x, dpp_int<0x4E>(x));   // quad_perm [2,3,0,1]
+    x = max(x, dpp_int<0x124>(x));  // row_ror:4
+    x = max(x, dpp_int<0x128>(x));  // row_ror:8
+    if constexpr (N == 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+        x = max((int)r[0], (int)r[1]);
+    }
     return __builtin_amdgcn_readfirstlane(x);
 }
-__device__ __forceinline__ int wave_min_int(int x) { return -wave_max_int(-x); }
+template <int N> __device__ __forceinline__ int rows_min(int x) { return -rows_max<N>(-x); }
 
-struct StreamShared {
+template <int RT> struct StreamShared {
     static constexpr int kStride = kHeadDim + 4;  // f32 per row: 16 rows at one column hit different banks
-    float m[kWaves][kStreamRows];
-    float l[kWaves][kStreamRows];
-    __attribute__((aligned(16))) float o[kWaves][kStreamRows][kStride];
+    float m[kWaves][16 * RT];
+    float l[kWaves][16 * RT];
+    int place[16 * RT], to[16 * RT];  // Segment::query of every row
+    __attribute__((aligned(16))) float o[kWaves][16 * RT][kStride];
 };
-// Tiles of 16 KiB: 64 keys of bf16, 32 of f32.
+// Tiles of 64 keys.
 constexpr int kTileBytes = 16384;
 struct BlockShared {
     __attribute__((aligned(1024))) uint8_t k[2][kTileBytes];
@@ -312,26 +340,27 @@ __device__ __forceinline__ float groups_max(float x) {
     return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
 
-// p = exp2(s c - m) of the step's scores, with m moved to the largest so far and o, l
-// scaled to it.  Without a branch: one around the scaling makes the compiler copy o
-// on both sides of it, in every step.
-template <typename T, int N> __device__ __forceinline__ void softmax_step(Row<T>& st, float (&s)[N], float c) {
-    float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    if constexpr (N == 8) mx = fmaxf(mx, fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    const float m = fmaxf(st.m, groups_max(mx) * c);
-    const float a = fast_exp2(st.m - m);
-    st.m = m;
+// p = exp2(s c - m) of the step's scores; MOVE: m moved to the largest so far first, and
+// o and l scaled to it.
+template <bool MOVE, typename T, int N> __device__ __forceinline__ void softmax_step(Row<T>& st, float (&s)[N], float c) {
+    if constexpr (MOVE) {
+        float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        if constexpr (N == 8) mx = fmaxf(mx, fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        const float m = fmaxf(st.m, groups_max(mx) * c), a = fast_exp2(st.m - m);
+        st.m = m;
+        st.l *= a;
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st.o[n][r] *= a;
+    }
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        s[e] = fast_exp2(__builtin_fmaf(s[e], c, -m));
+        s[e] = fast_exp2(__builtin_fmaf(s[e], c, -st.m));
         sum += s[e];
     }
-    st.l = __builtin_fmaf(st.l, a, sum);
-#pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) st.o[n][r] *= a;
+    st.l += sum;
 }
 
 // Sum over the four lane groups; every lane gets it.
@@ -343,22 +372,30 @@ __device__ __forceinline__ float groups_sum(float x) {
     return __uint_as_float(t[0]) + __uint_as_float(t[1]);
 }
 
-// o += P V.
-__device__ __forceinline__ void accumulate(Row<bf16_t>& st, const Frag<bf16_t>& f, const float (&p)[8]) {
-    u32x4_v b;
+// o += P V, every V operand for all row tiles.
+template <int RT>
+__device__ __forceinline__ void accumulate(Row<bf16_t> (&st)[RT], const Frag<bf16_t>& f, const float (&p)[RT][8]) {
+    u32x4_v b[RT];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) b[w] = pack_bf16x2(p[2 * w], p[2 * w + 1]);
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) b[t][w] = pack_bf16x2(p[t][2 * w], p[t][2 * w + 1]);
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-        st.o[n] = mfma(v_operand(f, n), b, st.o[n]);
+        const u32x4_v v = v_operand(f, n);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) st[t].o[n] = mfma(v, b[t], st[t].o[n]);
         if (n & 1) __builtin_amdgcn_sched_barrier(0);  // two operands paired ahead, not all eight
     }
 }
-__device__ __forceinline__ void accumulate(Row<float>& st, const Frag<float>& f, const float (&p)[4]) {
+template <int RT>
+__device__ __forceinline__ void accumulate(Row<float> (&st)[RT], const Frag<float>& f, const float (&p)[RT][4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int n = 0; n < 8; ++n) st.o[n] = mfma(v_operand(f, e, n), p[e], st.o[n]);
+        for (int n = 0; n < 8; ++n)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) st[t].o[n] = mfma(v_operand(f, e, n), p[t][e], st[t].o[n]);
 }
 
 // The same where rows do not see every key and V holds an infinity or a NaN: p = 0 times
@@ -407,6 +444,16 @@ __device__ __forceinline__ void accumulate_each(Row<float>& st, const Frag<float
     }
 }
 
+// Whether a walk that did not move m came out well (a row without keys did).
+template <typename T> __device__ __forceinline__ bool sound(const Row<T>& st) {
+    bool ok = st.l <= kMostSum;
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ok = ok && fabsf(st.o[n][r]) < INFINITY;
+    return ok;
+}
+
 // A row sees keys [lo, hi) only: the others' scores vanish.
 template <int N> __device__ __forceinline__ void mask_step(float (&s)[N], int j, int g, int lo, int hi) {
 #pragma unroll
@@ -416,31 +463,42 @@ template <int N> __device__ __forceinline__ void mask_step(float (&s)[N], int j,
     }
 }
 
-// ---- the stream form
+// ---- the stream form: 16 RT query rows
 
-template <typename T, bool SHARED>
-__device__ __forceinline__ void attend_stream(const Args& a, StreamShared& sm, int seg, int kvh, int block, int chunk) {
+template <typename T, int RT, bool SHARED>
+__device__ __forceinline__ void attend_stream(const Args& a, StreamShared<RT>& sm, int seg, int kvh, int block,
+                                              int chunk) {
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: buffer resources are scalar
     constexpr int kKeys = Frag<T>::kKeys, kSlots = Frag<T>::kSlots;
     const Segment<SHARED> sg(a, seg);
-    const int row0 = block * kStreamRows;
+    const int row0 = block * 16 * RT;
     if (row0 >= sg.n_rows) return;
     const int per = SHARED ? a.shared_chunk : a.own_chunk, lo = sg.lo, begin = sg.base() + chunk * per;
     const Pages pages(a, sg.table_row, begin, lane);
 
-    int hi;
-    const int64_t at = sg.query(row0 + i, kvh, hi);
-    QFrag<T> q;
-    q.load(reinterpret_cast<const T*>(a.q) + (at < 0 ? 0 : at) * kHeadDim, g);
-    const int end = min(begin + per, wave_max_int(hi));
-    hi = min(hi, end);  // a step may reach past the chunk's end
-    const int min_hi = wave_min_int(at < 0 ? end : hi);
+    int hi[RT], at[RT], most = 0;
+    QFrag<T> q[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        at[t] = (int)sg.query(row0 + 16 * t + i, kvh, hi[t]);  // fewer than 2^31 query rows
+        q[t].load(reinterpret_cast<const T*>(a.q) + (int64_t)max(at[t], 0) * kHeadDim, g);
+        most = max(most, hi[t]);
+    }
+    const int end = min(begin + per, rows_max<16>(most));
+    int least = end;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        hi[t] = min(hi[t], end);  // a step may reach past the chunk's end
+        least = min(least, at[t] < 0 ? end : hi[t]);
+    }
+    const int min_hi = rows_min<16>(least);
     const bool direct = a.slots() == 1;
     if (begin >= end && !direct) return;  // the join reads no slot past a row's keys
 
-    Row<T> st;
-    st.clear();
+    Row<T> st[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) st[t].clear();
     auto tile_at = [&](int j) __attribute__((always_inline)) { return pages.tile<T>(a, kvh, j, kKeys, end); };
     auto k_tile = [&](Frag<T>& f, const Pages::Tile& t) __attribute__((always_inline)) {
         load_k(f, tile_rsrc<T>(a.k, t), i, g);
@@ -448,128 +506,148 @@ __device__ __forceinline__ void attend_stream(const Args& a, StreamShared& sm, i
     auto v_tile = [&](Frag<T>& f, const Pages::Tile& t) __attribute__((always_inline)) {
         load_v(f, tile_rsrc<T>(a.v, t), i, g);
     };
-    // Two steps' tiles are in flight: a step's K registers are loaded again, for the
-    // step after the next, once its scores are taken, its V registers after its
-    // product.  A step past the end loads nothing and sees no key.
-    constexpr int kStride = kWaves * kKeys;
+    // kAhead steps' tiles are in flight (two for 16 rows, whose registers allow it): a
+    // step's K registers are loaded again, for the step kAhead on, once its scores are
+    // taken, its V registers after its product.  A step past the end loads nothing and
+    // sees no key.
+    constexpr int kAhead = RT == 1 ? 2 : 1, kStride = kWaves * kKeys;
     const int j0 = begin + wave * kKeys;
-    Frag<T> f[2];
-    bool again = false;  // a key some rows do not see has an infinity or a NaN in V
-    auto step = [&](Frag<T>& f, int j) __attribute__((always_inline)) {
-        const Pages::Tile next = tile_at(j + 2 * kStride);
-        float s[kSlots];
-        scores(f, q, s);
+    Frag<T> f[kAhead];
+    auto step = [&](Frag<T>& f, int j, auto move) __attribute__((always_inline)) {
+        const Pages::Tile next = tile_at(j + kAhead * kStride);
+        float s[RT][kSlots];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) scores(f, q[t], s[t]);
         __builtin_amdgcn_sched_barrier(0);  // the loads take the registers just read, not new ones
         k_tile(f, next);
         if (j < lo || j + kKeys > min_hi) {
-            mask_step(s, j, g, lo, hi);
-            if (j < lo || min_hi < min(j + kKeys, end)) again = again || __any(any_nonfinite(f));
+#pragma unroll
+            for (int t = 0; t < RT; ++t) mask_step(s[t], j, g, lo, hi[t]);
         }
-        softmax_step(st, s, a.c);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) softmax_step<decltype(move)::value>(st[t], s[t], a.c);
         accumulate(st, f, s);
         __builtin_amdgcn_sched_barrier(0);
         v_tile(f, next);
     };
-    {
-        // In the steps' own order: the loop's first wait has to hold for both.
-        const Pages::Tile t0 = tile_at(j0), t1 = tile_at(j0 + kStride);
+    // In the steps' own order: the loop's first wait has to hold for both.
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) {
+        const Pages::Tile t = tile_at(j0 + x * kStride);
         __builtin_amdgcn_sched_barrier(0);
-        k_tile(f[0], t0);
+        k_tile(f[x], t);
         __builtin_amdgcn_sched_barrier(0);
-        v_tile(f[0], t0);
-        __builtin_amdgcn_sched_barrier(0);
-        k_tile(f[1], t1);
-        __builtin_amdgcn_sched_barrier(0);
-        v_tile(f[1], t1);
+        v_tile(f[x], t);
         __builtin_amdgcn_sched_barrier(0);
     }
-    for (int j = j0; j < end; j += 2 * kStride) {
-        step(f[0], j);
-        step(f[1], j + kStride);
+    // A row that sees any key of the wave's sees one in its first two steps: lo is less
+    // than kAlign past the chunk's begin.
+    step(f[0], j0, std::true_type());
+    step(f[kAhead - 1], j0 + kStride, std::true_type());
+    for (int j = j0 + 2 * kStride; j < end; j += kAhead * kStride) {
+        step(f[0], j, std::false_type());
+        if constexpr (kAhead == 2) step(f[1], j + kStride, std::false_type());
     }
-    if (again) {  // the wave's keys once more, each added only to the rows that see it
-        st.clear();
+    bool again = false;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) again = again || (at[t] >= 0 && !sound(st[t]));
+    if (__any(again)) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) st[t].clear();
         for (int j = j0; j < end; j += kStride) {
             const Pages::Tile tile = tile_at(j);
             k_tile(f[0], tile);
             v_tile(f[0], tile);
-            float s[kSlots];
-            scores(f[0], q, s);
-            mask_step(s, j, g, lo, hi);
-            softmax_step(st, s, a.c);
-            accumulate_each(st, f[0], s, g, lo - j, hi - j);
+            float s[RT][kSlots];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                scores(f[0], q[t], s[t]);
+                mask_step(s[t], j, g, lo, hi[t]);
+                softmax_step<true>(st[t], s[t], a.c);
+            }
+            if (__any(any_nonfinite(f[0]))) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t) accumulate_each(st[t], f[0], s[t], g, lo - j, hi[t] - j);
+            } else {
+                accumulate(st, f[0], s);
+            }
         }
     }
 
     // Join the waves: m first, then o and l at the common m.
-    const float l = groups_sum(st.l);
-    if (g == 0) sm.m[wave][i] = st.m;
-    __syncthreads();
-    {
-        const float m = fmaxf(fmaxf(sm.m[0][i], sm.m[1][i]), fmaxf(sm.m[2][i], sm.m[3][i]));
-        const float w = fast_exp2(st.m - m);
-        if (g == 0) sm.l[wave][i] = w * l;
+    float l[RT];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+    for (int t = 0; t < RT; ++t) {
+        l[t] = groups_sum(st[t].l);
+        if (g == 0) sm.m[wave][16 * t + i] = st[t].m;
+        if (tid < 16) {
+            sm.place[16 * t + i] = at[t];
+            sm.to[16 * t + i] = hi[t];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int r = 16 * t + i;
+        const float m = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
+        const float w = fast_exp2(st[t].m - m);
+        if (g == 0) sm.l[wave][r] = w * l[t];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
             for (int n0 = 0; n0 < 8; n0 += 4) {
-                const float x[4] = {w * st.o[n0][r], w * st.o[n0 + 1][r], w * st.o[n0 + 2][r], w * st.o[n0 + 3][r]};
-                store4(&sm.o[wave][i][Row<T>::dim(n0, r, g)], x);
+                const f32x4_v* o = st[t].o + n0;
+                const float y[4] = {w * o[0][x], w * o[1][x], w * o[2][x], w * o[3][x]};
+                store4(&sm.o[wave][r][Row<T>::dim(n0, x, g)], y);
             }
     }
     __syncthreads();
     // 16 threads per row, 8 dims each.
-    const int r = tid >> 4, d = 8 * (tid & 15);
-    int to;
-    const int64_t place = sg.query(row0 + r, kvh, to);
-    if (place < 0) return;
-    float x[8];
-    load8(&sm.o[0][r][d], x);
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) {
-        float y[8];
-        load8(&sm.o[w][r][d], y);
+    for (int t = 0; t < RT; ++t) {
+        const int r = 16 * t + (tid >> 4), d = 8 * (tid & 15), place = sm.place[r];
+        if (place < 0) continue;
+        float x[8];
+        load8(&sm.o[0][r][d], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] += y[e];
-    }
-    const float m = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
-    const float sum = (sm.l[0][r] + sm.l[1][r]) + (sm.l[2][r] + sm.l[3][r]);
-    if (direct) {
-        const typename Segment<SHARED>::Row w = sg.row(row0 + r);
+        for (int w = 1; w < kWaves; ++w) {
+            float y[8];
+            load8(&sm.o[w][r][d], y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = to <= lo ? 0.f : x[e] / sum;
-        store8(reinterpret_cast<T*>(a.out) + (((int64_t)w.b * a.S + w.s) * a.Hq + kvh * a.G + w.h) * kHeadDim + d, x);
-    } else {
-        const int64_t slot = place * a.slots() + (SHARED ? 0 : a.shared_splits) + chunk;
-        store8(a.ws_o + slot * kHeadDim + d, x);
-        if (d == 0) a.ws_ml[slot] = make_float2(m, sum);
+            for (int e = 0; e < 8; ++e) x[e] += y[e];
+        }
+        const float m = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
+        const float sum = (sm.l[0][r] + sm.l[1][r]) + (sm.l[2][r] + sm.l[3][r]);
+        if (direct) {
+            const bool none = sm.to[r] <= lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = none ? 0.f : x[e] / sum;
+            store8(reinterpret_cast<T*>(a.out) + a.out_row(place) * kHeadDim + d, x);
+        } else {
+            const int64_t slot = (int64_t)place * a.slots() + (SHARED ? 0 : a.shared_splits) + chunk;
+            store8(a.ws_o + slot * kHeadDim + d, x);
+            if (d == 0) a.ws_ml[slot] = make_float2(m, sum);
+        }
     }
 }
 
 // ---- the block form
 
-// LDS tiles keep the pools' rows with their 16-byte chunks XOR-permuted by the row, so
-// that neither 16 rows read at one chunk (K) nor whole or transposed rows (V) meet in a
-// bank.  bf16 rows of 16 chunks: by the row's two 2-bit halves swapped (transposed
-// reads take 4 rows x 4 chunks); f32 rows of 32 chunks: by the row mod 16.
-template <typename T> __device__ __forceinline__ int swizzle(int row) {
-    return sizeof(T) == 2 ? ((row & 3) << 2) | ((row >> 2) & 3) : row & 15;
-}
-// The byte of a tile's row its 16-byte chunk c sits at.
-template <typename T> __device__ __forceinline__ int chunk_at(int row, int c) {
-    return row * kHeadDim * (int)sizeof(T) + 16 * (c ^ swizzle<T>(row));
-}
+// LDS tiles keep the pools' rows (256 bytes, a full sweep of the banks) with their
+// 16-byte chunks XOR-permuted by the row's two low 2-bit halves swapped, so that neither
+// 16 rows read at one chunk (K) nor 4 rows x 4 chunks (transposed V) meet in a bank.
+constexpr int kRowBytes = kHeadDim * 2;
+__device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+// The byte of a tile its row's 16-byte chunk c sits at.
+__device__ __forceinline__ int chunk_at(int row, int c) { return row * kRowBytes + 16 * (c ^ swizzle(row)); }
 
-// One tile into LDS: a wave copies 4 KiB of K and of V, 1 KiB an instruction, lane l
-// the 16 bytes at 16 l of it.
-template <typename T>
+// One tile into LDS: a wave copies 4 KiB of K and of V, 1 KiB (4 rows) an instruction,
+// lane l the 16 bytes at 16 l of it.
 __device__ __forceinline__ void stage(const Args& a, const Pages::Tile& t, uint8_t* k, uint8_t* v, int wave, int lane) {
-    constexpr int kRow = kHeadDim * (int)sizeof(T);
-    const __amdgpu_buffer_rsrc_t rk = tile_rsrc<T>(a.k, t), rv = tile_rsrc<T>(a.v, t);
+    const __amdgpu_buffer_rsrc_t rk = tile_rsrc<bf16_t>(a.k, t), rv = tile_rsrc<bf16_t>(a.v, t);
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-        const int at = 4096 * wave + 1024 * x + 16 * lane, row = at / kRow;
-        const int from = row * kRow + 16 * (((at % kRow) / 16) ^ swizzle<T>(row));
+        const int row = 16 * wave + 4 * x + (lane >> 4), from = chunk_at(row, lane & 15);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, k + 4096 * wave + 1024 * x, 16, from, 0, 0, 0);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, v + 4096 * wave + 1024 * x, 16, from, 0, 0, 0);
     }
@@ -577,13 +655,18 @@ __device__ __forceinline__ void stage(const Args& a, const Pages::Tile& t, uint8
 // Wait for the wave's own copies (expcnt and lgkmcnt at their maxima).
 __device__ __forceinline__ void wait_copies() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
-__device__ __forceinline__ u32x4_v lds_read16(const uint8_t* p) { return *(const u32x4_v*)p; }
+// LDS reads at byte addresses.
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
+}
+__device__ __forceinline__ u32x4_v lds_read16(uint32_t at) {
+    return *(const __attribute__((address_space(3))) u32x4_v*)(uintptr_t)at;
+}
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_v;
 typedef __attribute__((address_space(3))) s16x4_v lds_s16x4_v;
 // Within 16 lanes, lane x gets column x of the 4 rows x 16 columns of bf16 that the
 // lanes point at (lane x: 4 columns from 4 (x % 4) on of row x / 4).
-__device__ __forceinline__ uint2 lds_read_tr16(const uint8_t* p) {
-    const uint32_t at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
+__device__ __forceinline__ uint2 lds_read_tr16(uint32_t at) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_v*)(uintptr_t)at));
 }
 __device__ __forceinline__ f32x16_v mfma(u32x4_v a, u32x4_v b, f32x16_v c) {
@@ -601,21 +684,29 @@ __device__ __forceinline__ float halves_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// A wave's share of a block: Q, o, m and l of its rows, and one tile's work.
-template <typename T> struct BlockWave;
-
-// bf16: 32 rows; lane (n, h) = (lane % 32, lane / 32) holds, for row n, keys 32 b +
+// A wave's share of a block: Q, o, m and l of its 32 rows, and one tile's work.  Lane (n, h) = (lane % 32, lane / 32) holds, for row n, keys 32 b +
 // 8 (r / 4) + 4 h + r % 4 in register r of score block b, and dims 32 d + 8 (r / 4) +
 // 4 h + r % 4 in register r of o[d].
-template <> struct BlockWave<bf16_t> {
+struct BlockWave {
     static constexpr int kRows = 32, kKeys = 64;
     u32x4_v q[8];
     f32x16_v o[4];
     float m, l;
-    int n, h, vrow, vcol;
-    __device__ __forceinline__ explicit BlockWave(int lane) : n(lane & 31), h(lane >> 5) {
-        vrow = 4 * h + ((lane & 15) >> 2);
-        vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    int n, h;
+    // Byte offsets in a tile, the swizzle of rows 16 apart being the same: ko[t] of row n,
+    // chunk 2 t + h; vo[2 d + e] of row 8 e + 4 h + lane % 16 / 4, where the transposed
+    // reads of dims 32 d + lane % 32 start.
+    uint32_t ko[8], vo[8];
+    __device__ __forceinline__ BlockWave(int lane, const BlockShared& sm) : n(lane & 31), h(lane >> 5) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) ko[t] = lds_at(sm.k) + chunk_at(n, 2 * t + h);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * e + 4 * h + ((lane & 15) >> 2), col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                vo[2 * d + e] = lds_at(sm.v) + chunk_at(row, col >> 3) + 2 * (col & 7);
+            }
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -629,15 +720,24 @@ template <> struct BlockWave<bf16_t> {
 #pragma unroll
         for (int t = 0; t < 8; ++t) q[t] = reinterpret_cast<const u32x4_v*>(row)[2 * t + h];
     }
+    __device__ __forceinline__ bool sound() const {
+        bool ok = l <= kMostSum;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ok = ok && fabsf(o[d][r]) < INFINITY;
+        return ok;
+    }
     // V^T, dims 32 d + lane % 32, of keys 16 s + 8 e + 4 h + (0 .. 3), e = 0, 1.
-    __device__ __forceinline__ u32x4_v v_frag(const uint8_t* v, int s, int d) const {
-        const int r0 = 16 * s + vrow, c = (32 * d + vcol) >> 3, byte = 2 * (vcol & 7);
-        const uint2 x = lds_read_tr16(v + chunk_at<bf16_t>(r0, c) + byte);
-        const uint2 y = lds_read_tr16(v + chunk_at<bf16_t>(r0 + 8, c) + byte);
+    __device__ __forceinline__ u32x4_v v_frag(uint32_t buf, int s, int d) const {
+        const uint2 x = lds_read_tr16(vo[2 * d] + buf + 16 * s * kRowBytes);
+        const uint2 y = lds_read_tr16(vo[2 * d + 1] + buf + 16 * s * kRowBytes);
         return u32x4_v{x.x, x.y, y.x, y.y};
     }
-    template <bool EDGE, bool EACH>
-    __device__ __forceinline__ void tile(const uint8_t* k, const uint8_t* v, int j, int lo, int hi, float c) {
+    // One tile's keys.  MOVE: as in softmax_step.  EACH: as in accumulate_each.
+    // edge: some rows do not see all of the tile's keys.
+    template <bool MOVE, bool EACH>
+    __device__ __forceinline__ void tile(uint32_t buf, int j, bool edge, int lo, int hi, float c) {
         f32x16_v s[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -646,8 +746,8 @@ template <> struct BlockWave<bf16_t> {
 #pragma unroll
         for (int t = 0; t < 8; ++t)
 #pragma unroll
-            for (int b = 0; b < 2; ++b) s[b] = mfma(lds_read16(k + chunk_at<bf16_t>(32 * b + n, 2 * t + h)), q[t], s[b]);
-        if constexpr (EDGE) {
+            for (int b = 0; b < 2; ++b) s[b] = mfma(lds_read16(ko[t] + buf + 32 * b * kRowBytes), q[t], s[b]);
+        if (edge) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -656,14 +756,20 @@ template <> struct BlockWave<bf16_t> {
                     s[b][r] = key >= lo && key < hi ? s[b][r] : -INFINITY;
                 }
         }
-        float mx = s[0][0];
+        if constexpr (MOVE) {
+            float mx = s[0][0];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-        const float next = fmaxf(m, halves_max(mx) * c);
-        const float w = fast_exp2(m - next);
-        m = next;
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+            const float next = fmaxf(m, halves_max(mx) * c), w = fast_exp2(m - next);
+            m = next;
+            l *= w;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= w;
+        }
         float sum = 0.f;
         u32x4_v p[4];
 #pragma unroll
@@ -674,22 +780,18 @@ template <> struct BlockWave<bf16_t> {
                 sum += x + y;
                 p[2 * b + (r >> 3)][(r & 7) >> 1] = pack_bf16x2(x, y);
             }
-        l = __builtin_fmaf(l, w, sum);
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] *= w;
+        l += sum;
         if constexpr (!EACH) {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) o[d] = mfma(v_frag(v, t, d), p[t], o[d]);
+                for (int d = 0; d < 4; ++d) o[d] = mfma(v_frag(buf, t, d), p[t], o[d]);
         } else {  // see accumulate_each; key 16 t + 8 e + 4 h + x is slot 4 e + x of half h in step t
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
-                    const u32x4_v x = v_frag(v, t, d);
+                    const u32x4_v x = v_frag(buf, t, d);
 #pragma unroll 1
                     for (int key = 0; key < 16; ++key) {
                         const int e = 4 * (key >> 3) + (key & 3), at = j + 16 * t + key;
@@ -707,87 +809,28 @@ template <> struct BlockWave<bf16_t> {
                 }
         }
     }
-    __device__ __forceinline__ float sum() const { return halves_sum(l); }
-    template <class F> __device__ __forceinline__ void rows4(F f) const {  // f(dim, four consecutive values)
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const float x[4] = {o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
-                f(32 * d + 2 * r + 4 * h, x);
-            }
-    }
-    static __device__ __forceinline__ int row(int lane) { return lane & 31; }
-    __device__ __forceinline__ bool writes_ml() const { return h == 0; }
 };
-
-// f32: 16 rows, the stream's layout with the fragments from LDS.
-template <> struct BlockWave<float> {
-    static constexpr int kRows = 16, kKeys = 32;
-    QFrag<float> q;
-    Row<float> st;
-    int i, g;
-    __device__ __forceinline__ explicit BlockWave(int lane) : i(lane & 15), g(lane >> 4) {}
-    __device__ __forceinline__ void clear() { st.clear(); }
-    __device__ __forceinline__ void load_q(const float* row) { q.load(row, g); }
-    template <bool EDGE, bool EACH>
-    __device__ __forceinline__ void tile(const uint8_t* k, const uint8_t* v, int j, int lo, int hi, float c) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            Frag<float> f;
-#pragma unroll
-            for (int t = 0; t < 8; ++t) f.k[t] = lds_read16(k + chunk_at<float>(16 * half + i, 4 * t + g));
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int d = 0; d < 2; ++d) f.v[e][d] = lds_read16(v + chunk_at<float>(16 * half + 4 * g + e, 16 * d + i));
-            float s[4];
-            scores(f, q, s);
-            if constexpr (EDGE) mask_step(s, j + 16 * half, g, lo, hi);
-            softmax_step(st, s, c);
-            if constexpr (EACH) accumulate_each(st, f, s, g, lo - j - 16 * half, hi - j - 16 * half);
-            else accumulate(st, f, s);
-        }
-    }
-    __device__ __forceinline__ float sum() const { return groups_sum(st.l); }
-    template <class F> __device__ __forceinline__ void rows4(F f) const {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int n0 = 0; n0 < 8; n0 += 4) {
-                const float x[4] = {st.o[n0][r], st.o[n0 + 1][r], st.o[n0 + 2][r], st.o[n0 + 3][r]};
-                f(Row<float>::dim(n0, r, g), x);
-            }
-    }
-    static __device__ __forceinline__ int row(int lane) { return lane & 15; }
-    __device__ __forceinline__ bool writes_ml() const { return g == 0; }
-};
-template <typename T> __device__ __forceinline__ float wave_m(const BlockWave<T>& w) {
-    if constexpr (sizeof(T) == 2) return w.m;
-    else return w.st.m;
-}
 
 // Whether a V tile holds an infinity or a NaN (the whole tile, by one wave).
-template <typename T> __device__ __forceinline__ bool tile_nonfinite(const uint8_t* v, int lane) {
-    constexpr uint32_t kExp = sizeof(T) == 2 ? 0x7f80u : 0;
+__device__ __forceinline__ bool tile_nonfinite(const uint8_t* v, int lane) {
+    const uint32_t at = lds_at(v) + 16 * lane;
     bool bad = false;
 #pragma unroll 4
     for (int x = 0; x < kTileBytes / 1024; ++x) {
-        const u32x4_v u = lds_read16(v + 1024 * x + 16 * lane);
+        const u32x4_v u = lds_read16(at + 1024 * x);
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-            bad |= (u[y] & 0x7f800000u) == 0x7f800000u || (kExp && (u[y] & kExp) == kExp);
+        for (int y = 0; y < 4; ++y) bad |= (u[y] & 0x7f800000u) == 0x7f800000u || (u[y] & 0x7f80u) == 0x7f80u;
     }
     return __any(bad);
 }
 
-template <typename T, bool SHARED>
+template <bool SHARED>
 __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int seg, int kvh, int block, int chunk) {
-    typedef BlockWave<T> Wave;
+    constexpr int kKeys = BlockWave::kKeys;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Segment<SHARED> sg(a, seg);
-    const int row0 = block * kBlockRows<T>;
+    const int row0 = block * kBlockRows;
     if (row0 >= sg.n_rows) return;
     const int per = SHARED ? a.shared_chunk : a.own_chunk, lo = sg.lo, begin = sg.base() + chunk * per;
     const Pages pages(a, sg.table_row, begin, lane);
@@ -795,71 +838,74 @@ __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int
     // query sees.
     int end = begin + per;
     if constexpr (SHARED) end = min(end, sg.hi);
-    else end = min(end, a.limit(seg, (min(row0 + kBlockRows<T>, sg.n_rows) - 1) / a.G));
+    else end = min(end, a.limit(seg, (min(row0 + kBlockRows, sg.n_rows) - 1) / a.G));
     end = __builtin_amdgcn_readfirstlane(end);
     const bool direct = a.slots() == 1;
     if (begin >= end && !direct) return;
 
-    Wave w(lane);
+    BlockWave w(lane, sm);
     int hi;
-    const int r = row0 + Wave::kRows * wave + Wave::row(lane);
-    const int64_t at = sg.query(r, kvh, hi);
-    w.load_q(reinterpret_cast<const T*>(a.q) + (at < 0 ? 0 : at) * kHeadDim);
+    const int64_t at = sg.query(row0 + BlockWave::kRows * wave + w.n, kvh, hi);
+    w.load_q(reinterpret_cast<const bf16_t*>(a.q) + (at < 0 ? 0 : at) * kHeadDim);
     w.clear();
     hi = min(hi, end);
-    const int max_hi = wave_max_int(hi), min_hi = wave_min_int(at < 0 ? end : hi);
+    const int max_hi = rows_max<32>(hi), min_hi = rows_min<32>(at < 0 ? end : hi);
 
     // Tile t is computed while tile t + 1 comes in: its buffer's last readers passed the
     // barrier before the copies are issued.
-    const int n = max(0, (end - begin + Wave::kKeys - 1) / Wave::kKeys);
+    const int n = max(0, (end - begin + kKeys - 1) / kKeys);
     auto issue = [&](int t) __attribute__((always_inline)) {
-        stage<T>(a, pages.tile<T>(a, kvh, begin + t * Wave::kKeys, Wave::kKeys, end), sm.k[t & 1], sm.v[t & 1], wave, lane);
+        stage(a, pages.tile<bf16_t>(a, kvh, begin + t * kKeys, kKeys, end), sm.k[t & 1], sm.v[t & 1], wave, lane);
     };
-    auto walk = [&](auto each) __attribute__((always_inline)) {
-        constexpr bool kEach = decltype(each)::value;
-        bool bad = false;
-        if (n > 0) issue(0);
-        for (int t = 0; t < n; ++t) {
+    // Every wave passes the barrier of every tile; `work` is a tile of keys its rows see.
+    auto walk = [&](int t, int to, auto work) __attribute__((always_inline)) {
+        for (; t < to; ++t) {
             wait_copies();
             __syncthreads();
             if (t + 1 < n) issue(t + 1);
-            const int j = begin + t * Wave::kKeys;
-            const uint8_t *k = sm.k[t & 1], *v = sm.v[t & 1];
-            if (j >= max_hi) continue;  // none of the wave's rows sees the tile
-            if constexpr (kEach) {
-                w.template tile<true, true>(k, v, j, lo, hi, a.c);
-            } else if (j < lo || j + Wave::kKeys > min_hi) {
-                if (j < lo || min_hi < min(j + Wave::kKeys, end)) bad = bad || tile_nonfinite<T>(v, lane);
-                w.template tile<true, false>(k, v, j, lo, hi, a.c);
+            const int j = begin + t * kKeys;
+            if (j < max_hi) work((t & 1) * kTileBytes, j);
+        }
+    };
+    if (n > 0) issue(0);
+    // A row that sees any key of the chunk sees one in its first tile.
+    walk(0, min(n, 1), [&](uint32_t buf, int j) __attribute__((always_inline)) {
+        w.tile<true, false>(buf, j, true, lo, hi, a.c);
+    });
+    walk(1, n, [&](uint32_t buf, int j) __attribute__((always_inline)) {
+        w.tile<false, false>(buf, j, j + kKeys > min_hi, lo, hi, a.c);
+    });
+    sm.again[wave] = __any(at >= 0 && !w.sound());
+    __syncthreads();
+    if (sm.again[0] | sm.again[1] | sm.again[2] | sm.again[3]) {
+        w.clear();
+        issue(0);
+        walk(0, n, [&](uint32_t buf, int j) __attribute__((always_inline)) {
+            if (tile_nonfinite(sm.v[0] + buf, lane)) w.tile<true, true>(buf, j, true, lo, hi, a.c);
+            else w.tile<true, false>(buf, j, true, lo, hi, a.c);
+        });
+    }
+    const float l = halves_sum(w.l);
+    if (at < 0) return;
+    const int64_t slot = at * a.slots() + (SHARED ? 0 : a.shared_splits) + chunk;
+    bf16_t* out = reinterpret_cast<bf16_t*>(a.out) + a.out_row((int)at) * kHeadDim;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = w.o[d][r + e];
+            const int dim = 32 * d + 2 * r + 4 * w.h;
+            if (direct) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = hi <= lo ? 0.f : x[e] / l;
+                store4(out + dim, x);
             } else {
-                w.template tile<false, false>(k, v, j, lo, hi, a.c);
+                store4(a.ws_o + slot * kHeadDim + dim, x);
             }
         }
-        return bad;
-    };
-    const bool bad = walk(std::false_type());
-    sm.again[wave] = bad;
-    __syncthreads();
-    if (sm.again[0] | sm.again[1] | sm.again[2] | sm.again[3]) {  // once more, keys one by one
-        w.clear();
-        walk(std::true_type());
-    }
-    const float l = w.sum();
-    if (at < 0) return;
-    if (direct) {
-        const typename Segment<SHARED>::Row x = sg.row(r);
-        T* out = reinterpret_cast<T*>(a.out) + (((int64_t)x.b * a.S + x.s) * a.Hq + kvh * a.G + x.h) * kHeadDim;
-        w.rows4([&](int d, const float(&y)[4]) {
-            float z[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = hi <= lo ? 0.f : y[e] / l;
-            store4(out + d, z);
-        });
-    } else {
-        const int64_t slot = at * a.slots() + (SHARED ? 0 : a.shared_splits) + chunk;
-        w.rows4([&](int d, const float(&y)[4]) { store4(a.ws_o + slot * kHeadDim + d, y); });
-        if (w.writes_ml()) a.ws_ml[slot] = make_float2(wave_m(w), l);
-    }
+    if (!direct && w.h == 0) a.ws_ml[slot] = make_float2(w.m, l);
 }
 
 // A role's item x of `units` (segment, kv head, chunk) units with `blocks` row blocks
@@ -880,71 +926,108 @@ struct Item {
     }
 };
 
+// The forms of a role, by its query rows per workgroup.
+template <typename T, int ROWS, bool SHARED, class SM>
+__device__ __forceinline__ void attend(const Args& a, SM& sm, const Item& x) {
+    if constexpr (ROWS == kBlockRows) attend_block<SHARED>(a, sm.block, x.seg, x.kvh, x.block, x.chunk);
+    else if constexpr (ROWS == 32) attend_stream<T, 2, SHARED>(a, sm.stream32, x.seg, x.kvh, x.block, x.chunk);
+    else attend_stream<T, 1, SHARED>(a, sm.stream16, x.seg, x.kvh, x.block, x.chunk);
+}
+
 // grid: the shared role's items, then the own role's.
-template <typename T, bool SHARED_BLOCK, bool OWN_BLOCK>
+template <typename T, int SHARED_ROWS, int OWN_ROWS>
 __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(Args a) {
+    constexpr int kMost = SHARED_ROWS > OWN_ROWS ? SHARED_ROWS : OWN_ROWS;
     __shared__ union {
-        StreamShared stream;
-        typename std::conditional<SHARED_BLOCK || OWN_BLOCK, BlockShared, int>::type block;
+        StreamShared<1> stream16;
+        typename std::conditional<SHARED_ROWS == 32 || OWN_ROWS == 32, StreamShared<2>, int>::type stream32;
+        typename std::conditional<kMost == kBlockRows, BlockShared, int>::type block;
     } sm;
     if ((int)blockIdx.x < a.shared_items) {
         const Item x(blockIdx.x, a.shared_tiles, a.Hkv, a.n_groups, a.shared_splits);
-        if (!x.ok) return;
-        if constexpr (SHARED_BLOCK) attend_block<T, true>(a, sm.block, x.seg, x.kvh, x.block, x.chunk);
-        else attend_stream<T, true>(a, sm.stream, x.seg, x.kvh, x.block, x.chunk);
+        if (x.ok) attend<T, SHARED_ROWS, true>(a, sm, x);
     } else {
         const Item x(blockIdx.x - a.shared_items, a.own_tiles, a.Hkv, a.B, a.own_splits);
-        if (!x.ok) return;
-        if constexpr (OWN_BLOCK) attend_block<T, false>(a, sm.block, x.seg, x.kvh, x.block, x.chunk);
-        else attend_stream<T, false>(a, sm.stream, x.seg, x.kvh, x.block, x.chunk);
+        if (x.ok) attend<T, OWN_ROWS, false>(a, sm, x);
     }
 }
 
-// Join a query row's chunks: one wave per row, lane l owns dims 2 l, 2 l + 1.
-template <typename T> __global__ __launch_bounds__(256) void shared_join_kernel(Args a, int64_t n_rows) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= n_rows) return;
-    const int64_t bh = row / a.S;
-    const int s = (int)(row - bh * a.S);
-    const int b = (int)(bh / a.Hq), h = (int)(bh - (int64_t)b * a.Hq);
-    const int limit = a.limit(b, s), shared = a.shared_of(b);
-    const int seen = min(shared, limit);
+// Join a query row's chunks: P waves per row, lane l owns dims 2 l, 2 l + 1, wave p takes
+// slots p, p + P, ...  Every first load (8 slots a wave, the m and l of 64) is issued
+// before the row's lengths are known, so that up to 8 P slots cost one round trip; slots
+// past the row's keys hold anything and are left out by selects.
+constexpr int kJoinRegs = 8;
+template <typename T, int P>
+__global__ __launch_bounds__(P == 1 ? 256 : 64 * P) void shared_join_kernel(Args a, int n_rows) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = P == 1 ? 0 : wave;
+    const int row = P == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    if (row >= n_rows) return;  // P > 1: the whole workgroup
+    const int slots = a.slots();
+    const float2* ml = a.ws_ml + (int64_t)row * slots;
+    const float2* o = reinterpret_cast<const float2*>(a.ws_o + (int64_t)row * slots * kHeadDim) + lane;
+    float2 x[kJoinRegs];
+#pragma unroll
+    for (int i = 0; i < kJoinRegs; ++i) x[i] = o[(int64_t)min(p + P * i, slots - 1) * (kHeadDim / 2)];
+    const float2 first = ml[min(lane, slots - 1)];
+    const int bh = row / a.S, s = row - bh * a.S, b = bh / a.Hq;
+    const int n = a.len(b), shared = a.shared_of(b);
+#pragma unroll
+    for (int i = 0; i < kJoinRegs; ++i) asm volatile("" ::"v"(x[i].x), "v"(x[i].y));  // loaded above the branches below
+    asm volatile("" ::"v"(first.x), "v"(first.y));
+    const int limit = a.causal ? n - a.S + 1 + s : n;
+    const int seen = min(shared, limit), own = limit - Args::own_base(shared);
     const int n_shared = seen > 0 ? (seen + a.shared_chunk - 1) / a.shared_chunk : 0;
-    const int own = limit - Args::own_base(shared);
-    const int n_own = limit > shared ? min((own + a.own_chunk - 1) / a.own_chunk, a.own_splits) : 0;
-    const int n = n_shared + n_own;
-    const float2* ml = a.ws_ml + row * a.slots();
-    const float2* o = reinterpret_cast<const float2*>(a.ws_o + row * a.slots() * kHeadDim) + lane;
-    // slot of the c-th chunk the row sees
-    auto slot = [&](int c) { return c < n_shared ? c : a.shared_splits + c - n_shared; };
-    float mx = kNoMax;
-    for (int c = lane; c < n; c += 64) mx = fmaxf(mx, ml[slot(c)].x);
+    const int n_own = limit > shared ? (own + a.own_chunk - 1) / a.own_chunk : 0;
+    // the row has keys in the chunk of slot c
+    auto has = [&](int c) __attribute__((always_inline)) {
+        return c < a.shared_splits ? c < n_shared : c < slots && c - a.shared_splits < n_own;
+    };
+    float mx = has(lane) ? first.x : kNoMax;
+    for (int c = lane + 64; c < slots; c += 64) mx = fmaxf(mx, has(c) ? ml[c].x : kNoMax);
     mx = wave_max(mx);
     float den = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int c0 = 0; c0 < n; c0 += 64) {
-        float w = 0.f;
-        if (c0 + lane < n) {
-            const float2 t = ml[slot(c0 + lane)];
-            w = fast_exp2(t.x - mx);
-            den += w * t.y;
-        }
-        for (int c = c0; c < min(n, c0 + 64); ++c) {
+    for (int c0 = 0; c0 < slots; c0 += 64) {
+        const float2 t = c0 == 0 ? first : ml[min(c0 + lane, slots - 1)];
+        const float w = has(c0 + lane) ? fast_exp2(t.x - mx) : 0.f;
+        den += has(c0 + lane) ? w * t.y : 0.f;
+        auto add = [&](int c, float2 y) __attribute__((always_inline)) {
+            if (!has(c)) return;
             const float wc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), c - c0));
-            const float2 t = o[(int64_t)slot(c) * (kHeadDim / 2)];
-            x0 += wc * t.x;
-            x1 += wc * t.y;
+            x0 += wc * y.x;
+            x1 += wc * y.y;
+        };
+        int c = c0 + p;
+        if (c0 == 0) {
+#pragma unroll
+            for (int i = 0; i < kJoinRegs; ++i)
+                if (p + P * i < 64) add(p + P * i, x[i]);
+            c += P * kJoinRegs;
         }
+        for (; c < min(slots, c0 + 64); c += P) add(c, o[(int64_t)c * (kHeadDim / 2)]);
     }
     den = wave_sum(den);
-    T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.S + s) * a.Hq + h) * kHeadDim + 2 * lane;
-    Elem<T>::store(out, n ? x0 / den : 0.f);
-    Elem<T>::store(out + 1, n ? x1 / den : 0.f);
+    if constexpr (P > 1) {
+        __shared__ float2 part[P - 1][64];
+        if (p > 0) part[p - 1][lane] = make_float2(x0, x1);
+        __syncthreads();
+        if (p > 0) return;
+#pragma unroll
+        for (int i = 0; i < P - 1; ++i) {
+            x0 += part[i][lane].x;
+            x1 += part[i][lane].y;
+        }
+    }
+    const bool none = n_shared + n_own == 0;
+    T* out = reinterpret_cast<T*>(a.out) + a.out_row(row) * kHeadDim + 2 * lane;
+    Elem<T>::store(out, none ? 0.f : x0 / den);
+    Elem<T>::store(out + 1, none ? 0.f : x1 / den);
 }
 
 // How a call is cut: the forms, row blocks and key chunks of both roles.
 struct Plan {
-    bool share, shared_block, own_block;
+    bool share;
+    int max_group, max_shared;
+    int shared_rows, own_rows;  // query rows per workgroup
     int shared_tiles, own_tiles, shared_chunk, own_chunk, shared_splits, own_splits;
     int64_t shared_items, own_items;
     size_t ml_off, total;
@@ -952,27 +1035,84 @@ struct Plan {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-bool make_plan(int n_groups, int max_group, int64_t max_shared, int64_t max_own, int B, int S, int Hq, int Hkv, int dtype,
+// Microseconds for 128 keys of a workgroup that has a CU to itself, and of a CU kept busy
+// by two, by the workgroup's query rows (f32: bound by v_mfma_f32_16x16x4_f32 either way).
+struct KeyCost {
+    double alone, busy;
+};
+KeyCost key_cost(bool bf16, int rows) {
+    if (!bf16) return rows == 16 ? KeyCost{2.1, 2.1} : KeyCost{4.2, 4.2};
+    return rows == 16 ? KeyCost{1.06, 0.8} : rows == 32 ? KeyCost{1.5, 1.2} : KeyCost{2.66, 1.85};
+}
+
+// Chunk sizes tried, in units of 128 keys.
+constexpr int kChunks[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 32, 48, 64};
+
+// Groups (HOST): {first member's place, members, block table row, shared rows}.
+bool make_plan(const int32_t* groups, int n_groups, int64_t max_own, int64_t mean_own, int B, int S, int Hq, int Hkv, int dtype,
                Plan* p) {
-    const int64_t R = (int64_t)S * (Hq / Hkv), M = (int64_t)max_group * R;
-    const int block_rows = dtype == CRANE_HIP_F32 ? kBlockRows<float> : kBlockRows<bf16_t>;
+    const bool bf16 = dtype == CRANE_HIP_BF16;
+    const int64_t R = (int64_t)S * (Hq / Hkv);
+    p->max_group = p->max_shared = 0;
+    int64_t all_shared = 0;  // over all sequences
+    for (int g = 0; g < n_groups; ++g) {
+        all_shared += (int64_t)groups[4 * g + 1] * groups[4 * g + 3];
+        p->max_group = std::max(p->max_group, (int)groups[4 * g + 1]);
+        p->max_shared = std::max(p->max_shared, (int)groups[4 * g + 3]);
+    }
+    // Up to 96 rows the 32-row form, whose waves each take keys of their own, is the
+    // faster (5 groups of 35 to 70 rows: 45 us in blocks of 128, 30 in 32s; 128 rows:
+    // 37 in either); a block reads its keys once for more rows.
+    auto rows_for = [&](int64_t rows) { return rows <= 16 ? 16 : !bf16 || rows <= 96 ? 32 : kBlockRows; };
     // A sequence that fills whole row blocks by itself has nothing to gain.
-    p->share = n_groups > 0 && max_shared > 0 && R < block_rows;
-    p->shared_block = M > kStreamRows;
-    p->own_block = R > kStreamRows;
-    const int64_t st = p->share ? ceil_div(M, p->shared_block ? block_rows : kStreamRows) : 0;
-    const int64_t ot = ceil_div(R, p->own_block ? block_rows : kStreamRows);
-    // own chunk 0 starts on a multiple of kAlign
-    const int64_t shared = p->share ? max_shared : 0, own = max_own + (p->share ? kAlign : max_shared);
-    // Rows times keys of all items, spread over 1024 workgroups (4 per CU).
-    const int64_t total = (int64_t)n_groups * Hkv * st * shared + (int64_t)B * Hkv * ot * own;
-    int64_t chunk = ceil_div(ceil_div(total, 1024), kMinChunk) * kMinChunk;
-    chunk = chunk < 2 * kMinChunk ? 2 * kMinChunk : chunk > kMaxChunk ? kMaxChunk : chunk;
-    p->shared_chunk = p->own_chunk = (int)chunk;
-    const int64_t ss = ceil_div(shared, chunk), os = ceil_div(own, chunk);
+    p->share = p->max_group > 0 && p->max_shared > 0 && R < kBlockRows;
+    p->own_rows = rows_for(R);
+    p->shared_rows = p->share ? rows_for(p->max_group * R) : p->own_rows;
+    const int64_t st = p->share ? ceil_div(p->max_group * R, p->shared_rows) : 0, ot = ceil_div(R, p->own_rows);
+    // Own chunk 0 starts on a multiple of kAlign.
+    const int64_t shared = p->share ? p->max_shared : 0, own = max_own + (p->share ? kAlign : p->max_shared);
+    const KeyCost shared_cost = key_cost(bf16, p->shared_rows), own_cost = key_cost(bf16, p->own_rows);
+    const int64_t rows = (int64_t)B * Hq * S;
+    const double mean = std::max(64.0, (double)mean_own + (p->share ? 0.0 : (double)all_shared / B));
+    // What a cut costs: the workgroups' work on 256 CUs (the longest one's at least),
+    // 12 ns a workgroup for its start and end, and the partial rows written and read
+    // (1 KiB each, at 5 TB/s), which a single chunk does not have.
+    auto cost = [&](int64_t sc, int64_t oc) {
+        double work = 0, items = 0;
+        for (int g = 0; p->share && g < n_groups; ++g) {
+            const double tiles = (double)Hkv * ceil_div(groups[4 * g + 1] * R, p->shared_rows);
+            work += tiles * groups[4 * g + 3] * shared_cost.busy / 128;
+            items += tiles * ceil_div(groups[4 * g + 3], sc);
+        }
+        const double per = (double)B * Hkv * ot;
+        work += per * mean * own_cost.busy / 128;
+        items += per * std::max(1.0, mean / oc);
+        const int64_t slots = ceil_div(shared, sc) + ceil_div(own, oc);
+        const double longest = std::max(std::min(shared, sc) * shared_cost.alone, std::min(own, oc) * own_cost.alone) / 128;
+        double t = std::max(longest, work * std::ceil(items / 256) / items) + 0.012 * items;
+        if (slots > 1) t += 3 + (slots > 8) * 0.5 + (slots > 32) * 1.5 + 2.05e-4 * rows * slots;
+        return t;
+    };
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < (int)(sizeof(kChunks) / sizeof(int)); ++i) {
+        const double t = cost(kMinChunk * kChunks[i], kMinChunk * kChunks[i]);
+        if (i == 0 || t < least) {
+            best = kMinChunk * kChunks[i];
+            least = t;
+        }
+    }
+    p->shared_chunk = p->own_chunk = best;
+    for (int k : kChunks) {  // then the shared rows' chunk for itself
+        const double t = p->share ? cost(kMinChunk * k, best) : least;
+        if (t < least) {
+            p->shared_chunk = kMinChunk * k;
+            least = t;
+        }
+    }
+    const int64_t ss = ceil_div(shared, p->shared_chunk), os = ceil_div(own, p->own_chunk);
     p->shared_items = 8 * st * ceil_div((int64_t)n_groups * Hkv * ss, 8);
     p->own_items = 8 * ot * ceil_div((int64_t)B * Hkv * os, 8);
-    const int64_t rows = (int64_t)B * Hq * S;
     if (rows > 0x7fffffffLL || st > 0x7fffffffLL || ot > 0x7fffffffLL || p->shared_items + p->own_items > 0x7fffffffLL)
         return false;
     p->shared_tiles = (int)st;
@@ -988,32 +1128,45 @@ bool make_plan(int n_groups, int max_group, int64_t max_shared, int64_t max_own,
 
 template <typename T> int launch(Args& a, const Plan& p, int64_t n_rows, hipStream_t st) {
     const dim3 grid((unsigned)(p.shared_items + p.own_items)), threads(64 * kWaves);
-    if (p.own_block)
-        hipLaunchKernelGGL((shared_attn_kernel<T, true, true>), grid, threads, 0, st, a);
-    else if (p.share && p.shared_block)
-        hipLaunchKernelGGL((shared_attn_kernel<T, true, false>), grid, threads, 0, st, a);
-    else
-        hipLaunchKernelGGL((shared_attn_kernel<T, false, false>), grid, threads, 0, st, a);
+#define CRANE_SHARED_CASE(s, o)                                                               \
+    if (p.shared_rows == s && p.own_rows == o)                                                \
+        hipLaunchKernelGGL((shared_attn_kernel<T, s, o>), grid, threads, 0, st, a);
+    CRANE_SHARED_CASE(16, 16)
+    CRANE_SHARED_CASE(32, 16)
+    CRANE_SHARED_CASE(32, 32)
+    if constexpr (sizeof(T) == 2) {
+        CRANE_SHARED_CASE(128, 16)
+        CRANE_SHARED_CASE(128, 32)
+        CRANE_SHARED_CASE(128, 128)
+    }
+#undef CRANE_SHARED_CASE
     int rc = launch_status(hipGetLastError());
     if (rc || p.shared_splits + p.own_splits == 1) return rc;
-    hipLaunchKernelGGL((shared_join_kernel<T>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a, n_rows);
+    const int slots = p.shared_splits + p.own_splits;
+    if (slots <= kJoinRegs)
+        hipLaunchKernelGGL((shared_join_kernel<T, 1>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a, (int)n_rows);
+    else if (slots <= 4 * kJoinRegs)
+        hipLaunchKernelGGL((shared_join_kernel<T, 4>), dim3((unsigned)n_rows), dim3(256), 0, st, a, (int)n_rows);
+    else
+        hipLaunchKernelGGL((shared_join_kernel<T, 16>), dim3((unsigned)n_rows), dim3(1024), 0, st, a, (int)n_rows);
     return launch_status(hipGetLastError());
 }
 
 // The checks both entry points make of the sizes.
-int check_sizes(int n_groups, int max_group, int64_t max_shared, int64_t max_own, int B, int S, int Hq, int Hkv, int D,
-                int dtype) {
+int check_sizes(const int32_t* groups, int n_groups, int64_t max_own, int B, int S, int Hq, int Hkv, int D, int dtype) {
     if (dtype != CRANE_HIP_F32 && dtype != CRANE_HIP_BF16) return CRANE_HIP_E_DTYPE;
     if (D != kHeadDim) return CRANE_HIP_E_HEAD_DIM;
     if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0) return CRANE_HIP_E_INVALID;
     if (Hq % Hkv != 0) return CRANE_HIP_E_GQA;
-    if (B > 65535 || n_groups < 0 || n_groups > B || max_group < 0 || max_group > B) return CRANE_HIP_E_INVALID;
+    if (B > 65535 || n_groups < 0 || n_groups > B || (n_groups > 0 && !groups)) return CRANE_HIP_E_INVALID;
     // a chunk's bounds stay within 31 bits
-    if (max_shared < 0 || max_own < 0 || max_shared > 0x7fffffffLL - 2 * kMaxChunk ||
-        max_own > 0x7fffffffLL - 2 * kMaxChunk - max_shared)
-        return CRANE_HIP_E_INVALID;
-    if (n_groups > 0 && max_group == 0) return CRANE_HIP_E_INVALID;
-    if (n_groups == 0 && max_shared > 0) return CRANE_HIP_E_INVALID;
+    const int64_t most = 0x7fffffffLL - 2 * kMaxChunk;
+    if (max_own < 0 || max_own > most) return CRANE_HIP_E_INVALID;
+    for (int g = 0; g < n_groups; ++g) {
+        const int32_t* d = groups + 4 * g;
+        if (d[0] < 0 || d[1] < 0 || (int64_t)d[0] + d[1] > B || d[2] < 0 || d[2] >= B || d[3] < 0 || d[3] > most - max_own)
+            return CRANE_HIP_E_INVALID;
+    }
     return CRANE_HIP_OK;
 }
 
@@ -1022,29 +1175,28 @@ int check_sizes(int n_groups, int max_group, int64_t max_shared, int64_t max_own
 
 using namespace crane;
 
-extern "C" size_t crane_hip_attn_shared_workspace(int n_groups, int max_group, int64_t max_shared, int64_t max_own, int B,
-                                                  int S, int Hq, int Hkv, int D, int dtype) {
-    if (check_sizes(n_groups, max_group, max_shared, max_own, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0) return 0;
+extern "C" size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups, int64_t max_own,
+                                                  int64_t mean_own, int B, int S, int Hq, int Hkv, int D, int dtype) {
+    if (check_sizes(groups_host, n_groups, max_own, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0) return 0;
     Plan p;
-    return make_plan(n_groups, max_group, max_shared, max_own, B, S, Hq, Hkv, dtype, &p) ? p.total : 0;
+    return make_plan(groups_host, n_groups, max_own, mean_own, B, S, Hq, Hkv, dtype, &p) ? p.total : 0;
 }
 
 extern "C" int crane_hip_attn_shared_paged(const void* q, const void* k_pool, const void* v_pool, int64_t n_pages,
                                            int page_rows, const int32_t* block_table, int64_t table_stride,
                                            const int32_t* kv_len, int64_t max_kv, const int32_t* shared_rows,
-                                           const int32_t* groups, const int32_t* members, int n_groups, int max_group,
-                                           int64_t max_shared, int64_t max_own, int B, int S, int Hq, int Hkv, int D,
-                                           float scale, int flags, void* workspace, size_t ws_bytes, void* out,
-                                           int dtype, void* stream) {
-    int rc = check_sizes(n_groups, max_group, max_shared, max_own, B, S, Hq, Hkv, D, dtype);
+                                           const int32_t* groups, const int32_t* members, const int32_t* groups_host,
+                                           int n_groups, int64_t max_own, int64_t mean_own, int B, int S, int Hq,
+                                           int Hkv, int D, float scale, int flags, void* workspace, size_t ws_bytes,
+                                           void* out, int dtype, void* stream) {
+    int rc = check_sizes(groups_host, n_groups, max_own, B, S, Hq, Hkv, D, dtype);
     if (rc) return rc;
     if (flags & ~CRANE_HIP_PREFILL_CAUSAL) return CRANE_HIP_E_INVALID;
     if (!(scale > 0.0f) || !__builtin_isfinite(scale)) return CRANE_HIP_E_INVALID;
     rc = check_paged(n_pages, page_rows, block_table, table_stride, Hkv);
     if (rc) return rc;
     if (max_kv <= 0) return CRANE_HIP_E_INVALID;
-    if (max_kv > table_stride * page_rows) return CRANE_HIP_E_CAPACITY;
-    if (max_shared > max_kv || max_own > max_kv) return CRANE_HIP_E_CAPACITY;
+    if (max_kv > table_stride * page_rows || max_own > max_kv) return CRANE_HIP_E_CAPACITY;
     if (B == 0 || S == 0) return CRANE_HIP_OK;
     if (!q || !k_pool || !v_pool || !kv_len || !out) return CRANE_HIP_E_INVALID;
     if (n_groups > 0 && (!shared_rows || !groups || !members)) return CRANE_HIP_E_INVALID;
@@ -1052,7 +1204,8 @@ extern "C" int crane_hip_attn_shared_paged(const void* q, const void* k_pool, co
         (n_groups > 0 && !aligned16(groups)))
         return CRANE_HIP_E_ALIGN;
     Plan p;
-    if (!make_plan(n_groups, max_group, max_shared, max_own, B, S, Hq, Hkv, dtype, &p)) return CRANE_HIP_E_INVALID;
+    if (!make_plan(groups_host, n_groups, max_own, mean_own, B, S, Hq, Hkv, dtype, &p)) return CRANE_HIP_E_INVALID;
+    if (p.max_shared > max_kv) return CRANE_HIP_E_CAPACITY;
     if (p.total && (!workspace || ws_bytes < p.total || !aligned16(workspace))) return CRANE_HIP_E_WORKSPACE;
     Args a;
     a.q = q;
@@ -1065,8 +1218,8 @@ extern "C" int crane_hip_attn_shared_paged(const void* q, const void* k_pool, co
     a.groups = groups;
     a.members = members;
     a.n_groups = n_groups;
-    a.max_group = max_group;
-    a.max_shared = (int)max_shared;
+    a.max_group = p.max_group;
+    a.max_shared = p.max_shared;
     a.B = B;
     a.S = S;
     a.Hq = Hq;

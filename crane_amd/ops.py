@@ -470,23 +470,24 @@ def attention_prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
 
 class PrefixGroups:
     """Which sequences of a batch share their first rows (prefix_groups makes and
-    checks it): the groups {first member's place, members, batch row, shared rows},
-    their members and every sequence's shared rows on the device, and their host-side
-    bounds.  Kept for as long as the batch and its sharing stay."""
+    checks it): the groups {first member's place, members, batch row, shared rows} on
+    the host and on the device, their members and every sequence's shared rows there.
+    Kept for as long as the batch and its sharing stay."""
 
-    def __init__(self, batch: int, groups, members, shared_rows, n_groups: int, max_group: int, max_shared: int,
-                 min_shared: int):
-        self.batch, self.groups, self.members, self.shared_rows = batch, groups, members, shared_rows
-        self.n_groups, self.max_group = n_groups, max_group
-        self.max_shared, self.min_shared = max_shared, min_shared
+    def __init__(self, batch: int, groups_host, groups: torch.Tensor, members: torch.Tensor, shared_rows: torch.Tensor,
+                 min_shared: int, max_shared: int):
+        self.batch, self.groups_host = batch, groups_host
+        self.min_shared, self.max_shared = min_shared, max_shared
+        self.groups, self.members, self.shared_rows = groups, members, shared_rows
+        self.n_groups = len(groups_host) // 4
 
 
 def prefix_groups(groups: Sequence[Sequence[int]], rows: Sequence[int], batch: int,
                   device: Optional[torch.device] = None) -> PrefixGroups:
     """groups[g]: the batch rows whose first rows[g] cache rows are the same rows
     (their block tables name the same pages there).  A sequence is in one group at
-    most; sequences in none share nothing.  Copies three small arrays to the device
-    and waits for them."""
+    most; sequences in none share nothing.  Copies one small array to the device and
+    waits for it."""
     if len(groups) != len(rows):
         raise CraneHipError(_lib.E_INVALID, f"{len(groups)} groups, {len(rows)} row counts")
     shared, desc, seq, seen = [0] * batch, [], [], set()
@@ -503,8 +504,8 @@ def prefix_groups(groups: Sequence[Sequence[int]], rows: Sequence[int], batch: i
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     flat = torch.tensor(desc + seq + shared, dtype=torch.int32).to(dev)
     at = len(desc) + len(seq)
-    return PrefixGroups(batch, flat[:len(desc)].view(-1, 4), flat[len(desc):at], flat[at:], len(groups),
-                        max(map(len, groups), default=0), max(shared, default=0), min(shared, default=0))
+    return PrefixGroups(batch, (ctypes.c_int32 * len(desc))(*desc), flat[:len(desc)].view(-1, 4), flat[len(desc):at],
+                        flat[at:], min(shared, default=0), max(shared, default=0))
 
 
 def group_prefixes(tables: Sequence[Sequence[int]]):
@@ -535,13 +536,14 @@ def _on_device(dev: torch.device):
 
 def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
                            kv_len: torch.Tensor, max_kv: int, groups: PrefixGroups, scale: Optional[float] = None,
-                           causal: bool = True, max_own: Optional[int] = None,
+                           causal: bool = True, max_own: Optional[int] = None, mean_own: Optional[int] = None,
                            workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of every sequence's last tokens over a paged cache whose sequences
     share their first rows: q [B, Hq, D] (one token each, a decode step) gives
     [B, 1, Hq*D], q [B, Hq, S, D] gives [B, S, Hq*D].  kv_len counts the S new rows;
     with causal query i sees the rows up to its own, else all kv_len.  max_own:
-    host-side bound of kv_len - shared rows (default: what max_kv leaves).
+    host-side bound of kv_len - shared rows (default: what max_kv leaves); mean_own:
+    about its average, which steers how the work is cut (default: a guess).
 
     The shared rows are read once per group.  Scores and softmax stay in f32, where
     attention_decode_paged rounds every score as candle does."""
@@ -559,9 +561,11 @@ def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
         raise CraneHipError(_lib.E_INVALID, f"groups of a batch of {groups.batch}, q of {B}")
     if max_own is None:
         max_own = max(max_kv - groups.min_shared, 0)
+    if mean_own is None:  # the longest sequence is likely one that shares most
+        mean_own = 6 * max(max_kv - groups.max_shared, 0) // 10
     scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-    need = int(_lib.lib().crane_hip_attn_shared_workspace(groups.n_groups, groups.max_group, groups.max_shared, max_own,
-                                                          B, S, Hq, Hkv, HEAD_DIM, dt))
+    need = int(_lib.lib().crane_hip_attn_shared_workspace(groups.groups_host, groups.n_groups, max_own, mean_own, B, S,
+                                                          Hq, Hkv, HEAD_DIM, dt))
     # Allocated per call, not kept per stream: a captured graph keeps its own.
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -570,8 +574,7 @@ def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
         rc = _lib.lib().crane_hip_attn_shared_paged(
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, page_rows, block_table.data_ptr(), stride,
             kv_len.data_ptr(), max_kv, groups.shared_rows.data_ptr(), groups.groups.data_ptr(),
-            groups.members.data_ptr(), groups.n_groups, groups.max_group, groups.max_shared, max_own, B, S, Hq, Hkv,
-            HEAD_DIM, scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace),
+            groups.members.data_ptr(), groups.groups_host, groups.n_groups, max_own, mean_own, B, S, Hq, Hkv, HEAD_DIM, scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace),
             workspace.numel() * workspace.element_size() if workspace is not None else 0, out.data_ptr(), dt,
             _stream(dev))
     check(rc, "attention_shared_paged")

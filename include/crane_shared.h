@@ -25,8 +25,8 @@ extern "C" {
 /* Bytes of workspace crane_hip_attn_shared_paged needs for these sizes (the
  * arguments of the call); 0 where the call would be rejected or has nothing to
  * do. */
-size_t crane_hip_attn_shared_workspace(int n_groups, int max_group, int64_t max_shared, int64_t max_own, int B, int S,
-                                       int Hq, int Hkv, int D, int dtype);
+size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups, int64_t max_own, int64_t mean_own,
+                                       int B, int S, int Hq, int Hkv, int D, int dtype);
 
 /* Attention of the last S rows of every sequence over its rows of the pools, the
  * rows shared by a group read once for the group.
@@ -47,9 +47,13 @@ size_t crane_hip_attn_shared_workspace(int n_groups, int max_group, int64_t max_
  *          sequences are in none.  A description that breaks this gives unspecified
  *          results for the sequences concerned and stays in bounds
  * members  int32, device, B entries at most
- * max_group, max_shared, max_own: host-side bounds of a group's members, of
- *          shared_rows, and of kv_len[b] - shared_rows[b]; rows past them need not
- *          be attended.  max_shared + max_own < 2^31 - 2^14
+ * groups_host the same n_groups descriptions on the HOST, read before the call
+ *          returns: they steer how the work is cut and bound what the device's may
+ *          say (CRANE_HIP_E_INVALID for members or rows outside the batch)
+ * max_own  host-side bound of kv_len[b] - shared_rows[b]; rows past it need not be
+ *          attended.  max_own + a group's rows < 2^31 - 2^14
+ * mean_own about what kv_len[b] - shared_rows[b] is on average: it steers how the
+ *          work is cut, nothing else (negative counts as 0)
  * flags    CRANE_HIP_PREFILL_CAUSAL: query i sees rows [0, kv_len[b] - S + i];
  *          0: every query sees all kv_len[b] rows.  A query that sees none gets
  *          zeros.  Rows a query does not see have no influence on it, whatever
@@ -67,8 +71,8 @@ size_t crane_hip_attn_shared_workspace(int n_groups, int max_group, int64_t max_
  * give the same bits. */
 int crane_hip_attn_shared_paged(const void* q, const void* k_pool, const void* v_pool, int64_t n_pages, int page_rows,
                                 const int32_t* block_table, int64_t table_stride, const int32_t* kv_len, int64_t max_kv,
-                                const int32_t* shared_rows, const int32_t* groups, const int32_t* members, int n_groups,
-                                int max_group, int64_t max_shared, int64_t max_own, int B, int S, int Hq,
+                                const int32_t* shared_rows, const int32_t* groups, const int32_t* members,
+                                const int32_t* groups_host, int n_groups, int64_t max_own, int64_t mean_own, int B, int S, int Hq,
                                 int Hkv, int D, float scale, int flags, void* workspace, size_t ws_bytes, void* out,
                                 int dtype, void* stream);
 

@@ -176,31 +176,42 @@ def check_close(gpu, seed, lens, groups, rows, P, Hq, Hkv, S, dtype, causal=True
 # ------------------------------------------------------------------ refusals (CPU)
 
 BASE = dict(q=16, k=16, v=16, n_pages=64, P=256, table=16, stride=8, kv_len=16, max_kv=1024, shared=16, groups=16, members=16,
-            n_groups=1, max_group=4, max_shared=512, max_own=512, B=4, S=1, Hq=32, Hkv=8, D=128, scale=0.088, flags=1,
+            groups_host=[0, 4, 0, 512], n_groups=1, max_own=512, mean_own=100, B=4, S=1, Hq=32, Hkv=8, D=128, scale=0.088, flags=1,
             ws=16, ws_bytes=1 << 40, out=16, dtype=1, stream=None)
+
+
+def host(groups):
+    return None if groups is None else (ctypes.c_int32 * max(len(groups), 1))(*groups)
 
 
 def shared_call(**kw):
     from crane_amd import _lib
-    return _lib.lib().crane_hip_attn_shared_paged(*{**BASE, **kw}.values())
+    a = {**BASE, **kw}
+    a["groups_host"] = host(a["groups_host"])
+    return _lib.lib().crane_hip_attn_shared_paged(*a.values())
 
 
 @pytest.mark.parametrize("kw,code", [
     (dict(dtype=2), "E_DTYPE"), (dict(D=64), "E_HEAD_DIM"), (dict(Hq=30), "E_GQA"), (dict(Hkv=0), "E_INVALID"),
     (dict(P=100), "E_INVALID"), (dict(n_pages=0), "E_INVALID"), (dict(table=None), "E_INVALID"),
     (dict(stride=0), "E_INVALID"), (dict(max_kv=8 * 256 + 1), "E_CAPACITY"), (dict(max_kv=0), "E_INVALID"),
-    (dict(max_shared=1025), "E_CAPACITY"), (dict(max_own=1025), "E_CAPACITY"), (dict(max_own=-1), "E_INVALID"),
-    (dict(max_shared=-1), "E_INVALID"), (dict(n_groups=5), "E_INVALID"), (dict(n_groups=-1), "E_INVALID"),
-    (dict(max_group=5), "E_INVALID"), (dict(max_group=0), "E_INVALID"), (dict(n_groups=0), "E_INVALID"),
+    (dict(groups_host=[0, 4, 0, 1025]), "E_CAPACITY"), (dict(max_own=1025), "E_CAPACITY"),
+    (dict(max_own=-1), "E_INVALID"), (dict(n_groups=5, groups_host=[0, 0, 0, 0] * 5), "E_INVALID"),
+    (dict(n_groups=-1), "E_INVALID"), (dict(groups_host=None), "E_INVALID"),
+    (dict(groups_host=[0, 5, 0, 512]), "E_INVALID"), (dict(groups_host=[-1, 2, 0, 512]), "E_INVALID"),
+    (dict(groups_host=[0, -1, 0, 512]), "E_INVALID"), (dict(groups_host=[0, 4, 4, 512]), "E_INVALID"),
+    (dict(groups_host=[0, 4, -1, 512]), "E_INVALID"), (dict(groups_host=[0, 4, 0, -1]), "E_INVALID"),
+    (dict(groups_host=[3, 0x7fffffff, 0, 512]), "E_INVALID"), (dict(groups_host=[0, 4, 0, 0x7fffffff]), "E_INVALID"),
     (dict(flags=2), "E_INVALID"), (dict(flags=3), "E_INVALID"), (dict(scale=0.0), "E_INVALID"),
     (dict(scale=float("nan")), "E_INVALID"), (dict(scale=float("inf")), "E_INVALID"), (dict(q=None), "E_INVALID"),
     (dict(out=None), "E_INVALID"), (dict(kv_len=None), "E_INVALID"), (dict(shared=None), "E_INVALID"),
     (dict(groups=None), "E_INVALID"), (dict(members=None), "E_INVALID"), (dict(groups=8), "E_ALIGN"), (dict(q=8), "E_ALIGN"), (dict(k=24), "E_ALIGN"),
     (dict(v=8), "E_ALIGN"), (dict(out=8), "E_ALIGN"), (dict(ws=None), "E_WORKSPACE"), (dict(ws=8), "E_WORKSPACE"),
     (dict(ws_bytes=100), "E_WORKSPACE"), (dict(B=-1), "E_INVALID"), (dict(S=-1), "E_INVALID"),
-    (dict(B=65536), "E_INVALID"), (dict(B=0, n_groups=0, max_group=0, max_shared=0), "OK"), (dict(S=0), "OK"),
+    (dict(B=65536), "E_INVALID"), (dict(B=0, n_groups=0), "OK"), (dict(S=0), "OK"),
     (dict(S=1 << 30), "E_INVALID"),                                   # more than 2^31 query rows
-    (dict(P=1 << 28, stride=7, n_pages=1, max_kv=7 << 28, max_shared=7 << 28, max_own=7 << 28), "E_INVALID"),
+    (dict(P=1 << 28, stride=7, n_pages=1, max_kv=7 << 28, max_own=7 << 28,
+          groups_host=[0, 4, 0, 7 << 28]), "E_INVALID"),
 ])
 def test_attention_refusals(kw, code):
     from crane_amd import _lib
@@ -210,12 +221,17 @@ def test_attention_refusals(kw, code):
 def test_workspace_query():
     from crane_amd import _lib
     L = _lib.lib()
-    ws = lambda **kw: L.crane_hip_attn_shared_workspace(*[{**BASE, **kw}[x] for x in (
-        "n_groups", "max_group", "max_shared", "max_own", "B", "S", "Hq", "Hkv", "D", "dtype")])
+    def ws(**kw):
+        a = {**BASE, **kw}
+        a["groups_host"] = host(a["groups_host"])
+        return L.crane_hip_attn_shared_workspace(*[a[x] for x in ("groups_host", "n_groups", "max_own", "mean_own", "B", "S",
+                                                                  "Hq", "Hkv", "D", "dtype")])
+
     need = ws()
     assert need > 0 and shared_call(ws_bytes=need - 1) == _lib.E_WORKSPACE
-    assert ws(n_groups=0, max_group=0, max_shared=0, max_own=64) == 0   # one chunk: written directly
-    assert ws(D=64) == 0 and ws(dtype=9) == 0 and ws(B=0) == 0 and ws(S=0) == 0 and ws(max_own=-1) == 0
+    assert ws(n_groups=0, max_own=60, mean_own=60) == 0                          # one chunk: written directly
+    assert ws(D=64) == 0 and ws(dtype=9) == 0 and ws(B=0, n_groups=0) == 0 and ws(S=0) == 0 and ws(max_own=-1) == 0
+    assert ws(groups_host=[0, 9, 0, 512]) == 0
 
 
 def copy_call(pools=(16, 32), n_pages=8, P=256, Hkv=4, D=128, src=(0,), dst=(1,), rows=None, dtype=1, n=None):
@@ -249,9 +265,9 @@ def test_prefix_groups_checks():
     g = ops.prefix_groups([[3, 0], [1]], [512, 100], 5, "cpu")
     assert g.shared_rows.tolist() == [512, 100, 0, 512, 0]
     assert g.groups.tolist() == [[0, 2, 3, 512], [2, 1, 1, 100]] and g.members.tolist() == [3, 0, 1]
-    assert (g.n_groups, g.max_group, g.max_shared, g.min_shared) == (2, 2, 512, 0)
+    assert (g.n_groups, g.min_shared, list(g.groups_host)) == (2, 0, g.groups.flatten().tolist())
     g = ops.prefix_groups([], [], 3, "cpu")
-    assert (g.n_groups, g.max_group, g.max_shared, g.min_shared) == (0, 0, 0, 0)
+    assert (g.n_groups, g.min_shared) == (0, 0)
     for groups, rows in (([[0, 1], [1]], [1, 2]), ([[5]], [1]), ([[-1]], [1]), ([[0, 0]], [4]), ([[]], [1]),
                          ([[0]], [-1]), ([[0]], [1, 2]), ([[0]], [1 << 31])):
         with pytest.raises(CraneHipError):
