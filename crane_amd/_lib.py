@@ -104,7 +104,7 @@ SIGNATURES = {
     "crane_few_attn_linear": ([_vp, _vp, _vp, _i64, _vp, _i64, _i, _i, _i, _f, _i, _vp, _sz, _vp, _vp, _vp, _i64, _i, _vp],
                               _i),
     # include/crane_shared.h
-    "crane_hip_attn_shared_workspace": ([_i32p, _i, _i64, _i64, _i, _i, _i, _i, _i, _i], _sz),
+    "crane_hip_attn_shared_workspace": ([_i32p, _i, _i64, _i64, _i64, _i, _i, _i, _i, _i, _i], _sz),
     "crane_hip_attn_shared_paged": (
         [_vp, _vp, _vp, _i64, _i, _i32p, _i64, _i32p, _i64, _i32p, _i32p, _i32p, _i32p, _i, _i64, _i64,
          _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp, _i, _vp], _i),

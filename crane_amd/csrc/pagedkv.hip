@@ -512,7 +512,7 @@ class PagedKv {
         return B() ? sum / B() : 0;
     }
     size_t shared_workspace(int Hq, int S) const {
-        return crane_hip_attn_shared_workspace(batch_groups_.data(), n_groups_, max_own(), mean_own(), B(), S, Hq, Hkv_,
+        return crane_hip_attn_shared_workspace(batch_groups_.data(), n_groups_, max_len(), max_own(), mean_own(), B(), S, Hq, Hkv_,
                                                D_, dtype_);
     }
     int attention_shared(const void* q, int Hq, int S, float scale, int flags, void* ws, size_t ws_bytes, void* out,

@@ -59,6 +59,8 @@ constexpr float kNoMax = -FLT_MAX; // m before the first key (finite: exp2(-inf 
 constexpr float kMostSum = 0x1p60f;  // see above
 constexpr int kMaxChunk = 8192;    // rows per chunk: its pages' ids fit one lane each
 constexpr int kMinChunk = 128;
+constexpr int kCus = 256;
+constexpr size_t kHalfLds = 81920;   // half of a CU's LDS
 constexpr int kBlockRows = 128;    // query rows of a workgroup's block form
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, int bytes) {
@@ -85,7 +87,7 @@ struct Args {
     int B, S, Hq, Hkv, G;     // G = Hq / Hkv heads per kv head
     int max_kv, causal;
     float c;                  // scale log2 e
-    int shared_chunk, own_chunk;    // rows per chunk
+    int chunk;    // rows per chunk
     int shared_splits, own_splits;  // chunks
     int shared_tiles, own_tiles;    // row blocks per (group or sequence, kv head)
     int shared_items;               // workgroups of the shared role, which come first (a multiple of 8)
@@ -474,7 +476,7 @@ __device__ __forceinline__ void attend_stream(const Args& a, StreamShared<RT>& s
     const Segment<SHARED> sg(a, seg);
     const int row0 = block * 16 * RT;
     if (row0 >= sg.n_rows) return;
-    const int per = SHARED ? a.shared_chunk : a.own_chunk, lo = sg.lo, begin = sg.base() + chunk * per;
+    const int per = a.chunk, lo = sg.lo, begin = sg.base() + chunk * per;
     const Pages pages(a, sg.table_row, begin, lane);
 
     int hi[RT], at[RT], most = 0;
@@ -641,19 +643,20 @@ __device__ __forceinline__ int swizzle(int row) { return ((row & 3) << 2) | ((ro
 // The byte of a tile its row's 16-byte chunk c sits at.
 __device__ __forceinline__ int chunk_at(int row, int c) { return row * kRowBytes + 16 * (c ^ swizzle(row)); }
 
-// One tile into LDS: a wave copies 4 KiB of K and of V, 1 KiB (4 rows) an instruction,
-// lane l the 16 bytes at 16 l of it.
-__device__ __forceinline__ void stage(const Args& a, const Pages::Tile& t, uint8_t* k, uint8_t* v, int wave, int lane) {
-    const __amdgpu_buffer_rsrc_t rk = tile_rsrc<bf16_t>(a.k, t), rv = tile_rsrc<bf16_t>(a.v, t);
+// One tile into LDS: a wave copies 4 KiB, 1 KiB (4 rows) an instruction, lane l the 16
+// bytes at 16 l of it.
+__device__ __forceinline__ void stage(__amdgpu_buffer_rsrc_t r, uint8_t* to, int wave, int lane) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-        const int row = 16 * wave + 4 * x + (lane >> 4), from = chunk_at(row, lane & 15);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, k + 4096 * wave + 1024 * x, 16, from, 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, v + 4096 * wave + 1024 * x, 16, from, 0, 0, 0);
+        const int row = 16 * wave + 4 * x + (lane >> 4);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, to + 4096 * wave + 1024 * x, 16, chunk_at(row, lane & 15), 0, 0, 0);
     }
 }
-// Wait for the wave's own copies (expcnt and lgkmcnt at their maxima).
-__device__ __forceinline__ void wait_copies() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+// Wait for the wave's own copies but the last N instructions' (expcnt and lgkmcnt at
+// their maxima).
+template <int N> __device__ __forceinline__ void wait_copies() {
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
 
 // LDS reads at byte addresses.
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
@@ -734,11 +737,8 @@ struct BlockWave {
         const uint2 y = lds_read_tr16(vo[2 * d + 1] + buf + 16 * s * kRowBytes);
         return u32x4_v{x.x, x.y, y.x, y.y};
     }
-    // One tile's keys.  MOVE: as in softmax_step.  EACH: as in accumulate_each.
-    // edge: some rows do not see all of the tile's keys.
-    template <bool MOVE, bool EACH>
-    __device__ __forceinline__ void tile(uint32_t buf, int j, bool edge, int lo, int hi, float c) {
-        f32x16_v s[2];
+    // A tile's raw scores.
+    __device__ __forceinline__ void scores(f32x16_v (&s)[2], uint32_t buf) const {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -747,31 +747,29 @@ struct BlockWave {
         for (int t = 0; t < 8; ++t)
 #pragma unroll
             for (int b = 0; b < 2; ++b) s[b] = mfma(lds_read16(ko[t] + buf + 32 * b * kRowBytes), q[t], s[b]);
-        if (edge) {
+    }
+    // Row n sees keys [lo, hi) only.
+    __device__ __forceinline__ void mask(f32x16_v (&s)[2], int j, int lo, int hi) const {
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int key = j + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
-                    s[b][r] = key >= lo && key < hi ? s[b][r] : -INFINITY;
-                }
-        }
-        if constexpr (MOVE) {
-            float mx = s[0][0];
+            for (int r = 0; r < 16; ++r) {
+                const int key = j + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
+                s[b][r] = key >= lo && key < hi ? s[b][r] : -INFINITY;
+            }
+    }
+    // The largest of m and a row's scores.
+    __device__ __forceinline__ float largest(const f32x16_v (&s)[2], float c) const {
+        float mx = s[0][0];
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-            const float next = fmaxf(m, halves_max(mx) * c), w = fast_exp2(m - next);
-            m = next;
-            l *= w;
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][r] *= w;
-        }
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
+        return fmaxf(m, halves_max(mx) * c);
+    }
+    // p = exp2(s c - m), rounded and paired: p[t] is the B operand of keys 16 t ..; l.
+    __device__ __forceinline__ void weights(const f32x16_v (&s)[2], u32x4_v (&p)[4], float c) {
         float sum = 0.f;
-        u32x4_v p[4];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -781,33 +779,55 @@ struct BlockWave {
                 p[2 * b + (r >> 3)][(r & 7) >> 1] = pack_bf16x2(x, y);
             }
         l += sum;
-        if constexpr (!EACH) {
+    }
+    __device__ __forceinline__ void accumulate(const u32x4_v (&p)[4], uint32_t buf) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) o[d] = mfma(v_frag(buf, t, d), p[t], o[d]);
-        } else {  // see accumulate_each; key 16 t + 8 e + 4 h + x is slot 4 e + x of half h in step t
+            for (int d = 0; d < 4; ++d) o[d] = mfma(v_frag(buf, t, d), p[t], o[d]);
+    }
+    // A step's order: K fragments read four ahead of their MFMAs with the exponentials
+    // between, then V fragments two ahead.
+    template <class MORE> static __device__ __forceinline__ void schedule(MORE) {
+        constexpr int kMfma = 0x8, kRead = 0x100, kValu = 0x2;
+        if constexpr (MORE::value) {
+            __builtin_amdgcn_sched_group_barrier(kRead, 4, 0);
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const u32x4_v x = v_frag(buf, t, d);
-#pragma unroll 1
-                    for (int key = 0; key < 16; ++key) {
-                        const int e = 4 * (key >> 3) + (key & 3), at = j + 16 * t + key;
-                        u32x4_v mask;
-#pragma unroll
-                        for (int y = 0; y < 4; ++y)
-                            mask[y] = h == ((key >> 2) & 1) && y == (e >> 1) ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
-                        f32x16_v z;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) z[r] = 0.f;
-                        z = mfma(x & mask, p[t] & mask, z);
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[d][r] += at >= lo && at < hi ? z[r] : 0.f;
-                    }
-                }
+            for (int x = 0; x < 16; ++x) {
+                __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+                if (x < 12) __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kValu, 7, 0);
+            }
         }
+        __builtin_amdgcn_sched_group_barrier(kRead, 4, 0);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            if (x < 14) __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+        }
+    }
+    // As accumulate_each above; key 16 t + 8 e + 4 h + x is slot 4 e + x of half h in step t.
+    __device__ __forceinline__ void accumulate_each(const u32x4_v (&p)[4], uint32_t buf, int j, int lo, int hi) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const u32x4_v x = v_frag(buf, t, d);
+#pragma unroll 1
+                for (int key = 0; key < 16; ++key) {
+                    const int e = 4 * (key >> 3) + (key & 3), at = j + 16 * t + key;
+                    u32x4_v mask;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        mask[y] = h == ((key >> 2) & 1) && y == (e >> 1) ? (e & 1 ? 0xffff0000u : 0xffffu) : 0u;
+                    f32x16_v z;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+                    z = mfma(x & mask, p[t] & mask, z);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[d][r] += at >= lo && at < hi ? z[r] : 0.f;
+                }
+            }
     }
 };
 
@@ -832,7 +852,7 @@ __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int
     const Segment<SHARED> sg(a, seg);
     const int row0 = block * kBlockRows;
     if (row0 >= sg.n_rows) return;
-    const int per = SHARED ? a.shared_chunk : a.own_chunk, lo = sg.lo, begin = sg.base() + chunk * per;
+    const int per = a.chunk, lo = sg.lo, begin = sg.base() + chunk * per;
     const Pages pages(a, sg.table_row, begin, lane);
     // Keys any row of the block can see: a group's shared rows, or what the block's last
     // query sees.
@@ -851,39 +871,76 @@ __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int
     hi = min(hi, end);
     const int max_hi = rows_max<32>(hi), min_hi = rows_min<32>(at < 0 ? end : hi);
 
-    // Tile t is computed while tile t + 1 comes in: its buffer's last readers passed the
-    // barrier before the copies are issued.
     const int n = max(0, (end - begin + kKeys - 1) / kKeys);
-    auto issue = [&](int t) __attribute__((always_inline)) {
-        stage(a, pages.tile<bf16_t>(a, kvh, begin + t * kKeys, kKeys, end), sm.k[t & 1], sm.v[t & 1], wave, lane);
+    auto tile_at = [&](int t) __attribute__((always_inline)) {
+        return pages.tile<bf16_t>(a, kvh, begin + t * kKeys, kKeys, end);
     };
-    // Every wave passes the barrier of every tile; `work` is a tile of keys its rows see.
-    auto walk = [&](int t, int to, auto work) __attribute__((always_inline)) {
-        for (; t < to; ++t) {
-            wait_copies();
-            __syncthreads();
-            if (t + 1 < n) issue(t + 1);
-            const int j = begin + t * kKeys;
-            if (j < max_hi) work((t & 1) * kTileBytes, j);
-        }
+    auto issue_k = [&](int t) __attribute__((always_inline)) { stage(tile_rsrc<bf16_t>(a.k, tile_at(t)), sm.k[t & 1], wave, lane); };
+    auto issue_v = [&](int t) __attribute__((always_inline)) { stage(tile_rsrc<bf16_t>(a.v, tile_at(t)), sm.v[t & 1], wave, lane); };
+    // Step t takes the weights and the V product of tile t and the scores of tile t + 1,
+    // whose MFMAs run beside the exponentials, while K of tile t + 2 and V of tile t + 1
+    // come in (into the buffers of K(t) and V(t - 1), whose readers passed the barrier).
+    // A tile past `max_hi` is seen by none of the wave's rows.
+    f32x16_v sa[2], sb[2];
+    auto step = [&](int t, f32x16_v(&s)[2], f32x16_v(&next)[2], auto more) __attribute__((always_inline)) {
+        wait_copies<0>();
+        __syncthreads();
+        if (t + 2 < n) issue_k(t + 2);
+        if (t + 1 < n) issue_v(t + 1);
+        const int j = begin + t * kKeys;
+        if (j >= max_hi) return;
+        if (j < lo || j + kKeys > min_hi) w.mask(s, j, lo, hi);
+        u32x4_v p[4];
+        if constexpr (decltype(more)::value) w.scores(next, ((t + 1) & 1) * kTileBytes);
+        w.weights(s, p, a.c);
+        w.accumulate(p, (t & 1) * kTileBytes);
+        BlockWave::schedule(more);
     };
-    if (n > 0) issue(0);
-    // A row that sees any key of the chunk sees one in its first tile.
-    walk(0, min(n, 1), [&](uint32_t buf, int j) __attribute__((always_inline)) {
-        w.tile<true, false>(buf, j, true, lo, hi, a.c);
-    });
-    walk(1, n, [&](uint32_t buf, int j) __attribute__((always_inline)) {
-        w.tile<false, false>(buf, j, j + kKeys > min_hi, lo, hi, a.c);
-    });
+    if (n > 0) {
+        issue_k(0);
+        issue_v(0);
+        if (n > 1) issue_k(1);
+        if (n > 1) wait_copies<8>();
+        else wait_copies<4>();
+        __syncthreads();
+        w.scores(sa, 0);
+        // A row that sees any key of the chunk sees one in its first tile.
+        w.mask(sa, begin, lo, hi);
+        w.m = w.largest(sa, a.c);
+    }
+    int t = 0;
+    for (; t + 2 < n; t += 2) {
+        step(t, sa, sb, std::true_type());
+        step(t + 1, sb, sa, std::true_type());
+    }
+    if (t + 2 == n) step(t, sa, sb, std::true_type()), step(t + 1, sb, sa, std::false_type());
+    else if (t < n) step(t, sa, sb, std::false_type());
     sm.again[wave] = __any(at >= 0 && !w.sound());
     __syncthreads();
     if (sm.again[0] | sm.again[1] | sm.again[2] | sm.again[3]) {
         w.clear();
-        issue(0);
-        walk(0, n, [&](uint32_t buf, int j) __attribute__((always_inline)) {
-            if (tile_nonfinite(sm.v[0] + buf, lane)) w.tile<true, true>(buf, j, true, lo, hi, a.c);
-            else w.tile<true, false>(buf, j, true, lo, hi, a.c);
-        });
+        for (t = 0; t < n; ++t) {
+            __syncthreads();
+            issue_k(t);
+            issue_v(t);
+            wait_copies<0>();
+            __syncthreads();
+            const uint32_t buf = (t & 1) * kTileBytes;
+            const int j = begin + t * kKeys;
+            w.scores(sa, buf);
+            w.mask(sa, j, lo, hi);
+            const float m = w.largest(sa, a.c), x = fast_exp2(w.m - m);
+            w.m = m;
+            w.l *= x;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) w.o[d][r] *= x;
+            u32x4_v p[4];
+            w.weights(sa, p, a.c);
+            if (tile_nonfinite(sm.v[t & 1], lane)) w.accumulate_each(p, buf, j, lo, hi);
+            else w.accumulate(p, buf);
+        }
     }
     const float l = halves_sum(w.l);
     if (at < 0) return;
@@ -934,15 +991,16 @@ __device__ __forceinline__ void attend(const Args& a, SM& sm, const Item& x) {
     else attend_stream<T, 1, SHARED>(a, sm.stream16, x.seg, x.kvh, x.block, x.chunk);
 }
 
+template <int SHARED_ROWS, int OWN_ROWS> union AttnShared {
+    StreamShared<1> stream16;
+    typename std::conditional<SHARED_ROWS == 32 || OWN_ROWS == 32, StreamShared<2>, int>::type stream32;
+    typename std::conditional<SHARED_ROWS == kBlockRows || OWN_ROWS == kBlockRows, BlockShared, int>::type block;
+};
+
 // grid: the shared role's items, then the own role's.
 template <typename T, int SHARED_ROWS, int OWN_ROWS>
 __global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(Args a) {
-    constexpr int kMost = SHARED_ROWS > OWN_ROWS ? SHARED_ROWS : OWN_ROWS;
-    __shared__ union {
-        StreamShared<1> stream16;
-        typename std::conditional<SHARED_ROWS == 32 || OWN_ROWS == 32, StreamShared<2>, int>::type stream32;
-        typename std::conditional<kMost == kBlockRows, BlockShared, int>::type block;
-    } sm;
+    __shared__ AttnShared<SHARED_ROWS, OWN_ROWS> sm;
     if ((int)blockIdx.x < a.shared_items) {
         const Item x(blockIdx.x, a.shared_tiles, a.Hkv, a.n_groups, a.shared_splits);
         if (x.ok) attend<T, SHARED_ROWS, true>(a, sm, x);
@@ -976,8 +1034,8 @@ __global__ __launch_bounds__(P == 1 ? 256 : 64 * P) void shared_join_kernel(Args
     asm volatile("" ::"v"(first.x), "v"(first.y));
     const int limit = a.causal ? n - a.S + 1 + s : n;
     const int seen = min(shared, limit), own = limit - Args::own_base(shared);
-    const int n_shared = seen > 0 ? (seen + a.shared_chunk - 1) / a.shared_chunk : 0;
-    const int n_own = limit > shared ? (own + a.own_chunk - 1) / a.own_chunk : 0;
+    const int n_shared = seen > 0 ? (seen + a.chunk - 1) / a.chunk : 0;
+    const int n_own = limit > shared ? (own + a.chunk - 1) / a.chunk : 0;
     // the row has keys in the chunk of slot c
     auto has = [&](int c) __attribute__((always_inline)) {
         return c < a.shared_splits ? c < n_shared : c < slots && c - a.shared_splits < n_own;
@@ -1023,114 +1081,158 @@ __global__ __launch_bounds__(P == 1 ? 256 : 64 * P) void shared_join_kernel(Args
     Elem<T>::store(out + 1, none ? 0.f : x1 / den);
 }
 
-// How a call is cut: the forms, row blocks and key chunks of both roles.
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How a call is cut: whether sharing is used, and the forms (query rows per workgroup),
+// row blocks and key chunks of both roles.
 struct Plan {
     bool share;
     int max_group, max_shared;
-    int shared_rows, own_rows;  // query rows per workgroup
-    int shared_tiles, own_tiles, shared_chunk, own_chunk, shared_splits, own_splits;
-    int64_t shared_items, own_items;
+    int shared_rows, own_rows;
+    int64_t shared_tiles, own_tiles;
+    int chunk;
+    int64_t shared_splits, own_splits, shared_items, own_items;
+    bool spread;  // one workgroup per CU
     size_t ml_off, total;
 };
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// The sizes a plan is made for; groups (HOST): {first member's place, members, block
+// table row, shared rows}.
+struct Sizes {
+    const int32_t* groups;
+    int n_groups;
+    int64_t max_kv, max_own, mean_own;
+    int B, S, Hq, Hkv;
+    bool bf16;
+    int64_t R() const { return (int64_t)S * (Hq / Hkv); }  // query rows per (sequence, kv head)
+    // the own role's most keys
+    int64_t longest(const Plan& p) const { return p.share ? max_own : std::min(max_kv, max_own + p.max_shared); }
+    int64_t rows() const { return (int64_t)B * Hq * S; }
+};
 
 // Microseconds for 128 keys of a workgroup that has a CU to itself, and of a CU kept busy
-// by two, by the workgroup's query rows (f32: bound by v_mfma_f32_16x16x4_f32 either way).
+// by two, by the workgroup's query rows (f32: bound by v_mfma_f32_16x16x4_f32 either way;
+// bf16 blocks: by their MFMAs and exponentials).
 struct KeyCost {
     double alone, busy;
 };
 KeyCost key_cost(bool bf16, int rows) {
-    if (!bf16) return rows == 16 ? KeyCost{2.1, 2.1} : KeyCost{4.2, 4.2};
-    return rows == 16 ? KeyCost{1.06, 0.8} : rows == 32 ? KeyCost{1.5, 1.2} : KeyCost{2.66, 1.85};
+    if (!bf16) return rows == 16 ? KeyCost{2.2, 2.1} : KeyCost{3.7, 3.5};
+    return rows == 16 ? KeyCost{1.1, 0.8} : rows == 32 ? KeyCost{1.0, 1.0} : KeyCost{2.2, 1.8};
+}
+
+// Up to 96 rows the 32-row form, whose waves each take keys of their own, is the faster
+// (5 groups of 35 to 70 rows: 45 us in blocks of 128, 30 in 32s; 128 rows: 37 in either);
+// a block reads its keys once for more rows.
+int form_rows(int64_t rows, bool bf16) { return rows <= 16 ? 16 : !bf16 || rows <= 96 ? 32 : kBlockRows; }
+
+// What a plan costs in microseconds: the CUs' work (all of it spread evenly, or a role's
+// workgroups in turns of 256), the longest workgroup's, K and V from HBM at 5.5 TB/s and
+// what is read again at 10, whichever is most (as a norm of high order, since near each
+// other they add up); with more workgroups than CUs a part of the longest one as a tail;
+// each workgroup's start and end, also of those that find nothing to do; the shared
+// role's longer start; and what several chunks cost, the second kernel and the partial
+// rows written and read (1 KiB each).
+// The constants are a fit to 165 calls of random sizes, 28 cuts each, with the blocks' and
+// the partial rows' costs held at what they measure: the cut it chooses takes 7% more than
+// the best of the 28 on average, and 10% over 48 calls that took no part in the fit.
+double plan_cost(const Sizes& z, Plan& p) {
+    const KeyCost sc = key_cost(z.bf16, p.shared_rows), oc = key_cost(z.bf16, p.own_rows);
+    double work = 0, items = 0, once = 0, loads = 0, mean = std::max<double>(64, z.mean_own);
+    double longest = std::min<double>(z.longest(p), p.chunk) * oc.alone / 128;
+    auto rounds = [](double n) { return std::ceil(n / kCus); };
+    for (int g = 0; g < z.n_groups; ++g) {
+        const int64_t members = z.groups[4 * g + 1], rows = z.groups[4 * g + 3];
+        once += (double)z.Hkv * rows;
+        if (!p.share) {
+            mean += (double)members * rows / z.B;
+            continue;
+        }
+        const double tiles = (double)z.Hkv * ceil_div(members * z.R(), p.shared_rows);
+        work += tiles * rows * sc.busy / 128;
+        loads += tiles * rows;
+        items += tiles * ceil_div(rows, p.chunk);
+    }
+    double even = 0;  // each role's workgroups in turns of 256 at their chunk's cost
+    if (p.share) {
+        const double keys = std::min(p.max_shared, p.chunk) / 128.0;
+        longest = std::max(longest, keys * sc.alone);
+        even = rounds(items) * keys * sc.busy;
+    }
+    const double own = (double)z.B * z.Hkv * p.own_tiles;
+    once += (double)z.B * z.Hkv * z.mean_own;
+    work += own * mean * oc.busy / 128;
+    loads += own * mean;
+    const double own_items = own * std::max(1.0, mean / p.chunk);
+    items += own_items;
+    even = std::max(even, rounds(own_items) * std::min<double>(mean, p.chunk) / 128 * oc.busy);
+    work = std::max(work / kCus, even);
+    p.spread = items <= 240 || p.shared_items + p.own_items <= kCus;
+    const double memory = (once / 5.5e6 + std::max(0.0, loads - once) / 10e6) * (z.bf16 ? 512 : 1024);
+    auto pow4 = [](double x) { return x * x * x * x; };
+    double t = std::sqrt(std::sqrt(pow4(longest) + pow4(memory) + (items <= kCus ? 0 : pow4(work))));
+    t += (items <= kCus ? 0 : 0.08 * longest) + 0.002 * items + 0.0032 * (p.shared_items + p.own_items) + 0.85 * p.share;
+    const double slots = p.shared_splits + p.own_splits;
+    if (slots > 1) t += 1.1 + (slots > 32) * 1.0 + 2e-4 * z.rows() * slots;
+    return t;
+}
+
+// Cuts the roles' keys into chunks; own chunk 0 starts on a multiple of kAlign.
+void cut(const Sizes& z, int chunk, Plan* p) {
+    p->chunk = chunk;
+    p->shared_splits = p->share ? ceil_div(p->max_shared, chunk) : 0;
+    p->own_splits = ceil_div(z.longest(*p) + (p->share ? kAlign : 0), chunk);
+    p->shared_items = 8 * p->shared_tiles * ceil_div(z.n_groups * z.Hkv * p->shared_splits, 8);
+    p->own_items = 8 * p->own_tiles * ceil_div((int64_t)z.B * z.Hkv * p->own_splits, 8);
 }
 
 // Chunk sizes tried, in units of 128 keys.
 constexpr int kChunks[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 32, 48, 64};
 
-// Groups (HOST): {first member's place, members, block table row, shared rows}.
-bool make_plan(const int32_t* groups, int n_groups, int64_t max_own, int64_t mean_own, int B, int S, int Hq, int Hkv, int dtype,
-               Plan* p) {
-    const bool bf16 = dtype == CRANE_HIP_BF16;
-    const int64_t R = (int64_t)S * (Hq / Hkv);
-    p->max_group = p->max_shared = 0;
-    int64_t all_shared = 0;  // over all sequences
-    for (int g = 0; g < n_groups; ++g) {
-        all_shared += (int64_t)groups[4 * g + 1] * groups[4 * g + 3];
-        p->max_group = std::max(p->max_group, (int)groups[4 * g + 1]);
-        p->max_shared = std::max(p->max_shared, (int)groups[4 * g + 3]);
+bool make_plan(const Sizes& z, Plan* best) {
+    Plan p;
+    p.max_group = p.max_shared = 0;
+    for (int g = 0; g < z.n_groups; ++g) {
+        p.max_group = std::max(p.max_group, (int)z.groups[4 * g + 1]);
+        p.max_shared = std::max(p.max_shared, (int)z.groups[4 * g + 3]);
     }
-    // Up to 96 rows the 32-row form, whose waves each take keys of their own, is the
-    // faster (5 groups of 35 to 70 rows: 45 us in blocks of 128, 30 in 32s; 128 rows:
-    // 37 in either); a block reads its keys once for more rows.
-    auto rows_for = [&](int64_t rows) { return rows <= 16 ? 16 : !bf16 || rows <= 96 ? 32 : kBlockRows; };
-    // A sequence that fills whole row blocks by itself has nothing to gain.
-    p->share = p->max_group > 0 && p->max_shared > 0 && R < kBlockRows;
-    p->own_rows = rows_for(R);
-    p->shared_rows = p->share ? rows_for(p->max_group * R) : p->own_rows;
-    const int64_t st = p->share ? ceil_div(p->max_group * R, p->shared_rows) : 0, ot = ceil_div(R, p->own_rows);
-    // Own chunk 0 starts on a multiple of kAlign.
-    const int64_t shared = p->share ? p->max_shared : 0, own = max_own + (p->share ? kAlign : p->max_shared);
-    const KeyCost shared_cost = key_cost(bf16, p->shared_rows), own_cost = key_cost(bf16, p->own_rows);
-    const int64_t rows = (int64_t)B * Hq * S;
-    const double mean = std::max(64.0, (double)mean_own + (p->share ? 0.0 : (double)all_shared / B));
-    // What a cut costs: the workgroups' work on 256 CUs (the longest one's at least),
-    // 12 ns a workgroup for its start and end, and the partial rows written and read
-    // (1 KiB each, at 5 TB/s), which a single chunk does not have.
-    auto cost = [&](int64_t sc, int64_t oc) {
-        double work = 0, items = 0;
-        for (int g = 0; p->share && g < n_groups; ++g) {
-            const double tiles = (double)Hkv * ceil_div(groups[4 * g + 1] * R, p->shared_rows);
-            work += tiles * groups[4 * g + 3] * shared_cost.busy / 128;
-            items += tiles * ceil_div(groups[4 * g + 3], sc);
-        }
-        const double per = (double)B * Hkv * ot;
-        work += per * mean * own_cost.busy / 128;
-        items += per * std::max(1.0, mean / oc);
-        const int64_t slots = ceil_div(shared, sc) + ceil_div(own, oc);
-        const double longest = std::max(std::min(shared, sc) * shared_cost.alone, std::min(own, oc) * own_cost.alone) / 128;
-        double t = std::max(longest, work * std::ceil(items / 256) / items) + 0.012 * items;
-        if (slots > 1) t += 3 + (slots > 8) * 0.5 + (slots > 32) * 1.5 + 2.05e-4 * rows * slots;
-        return t;
-    };
-    int best = 0;
-    double least = 0;
-    for (int i = 0; i < (int)(sizeof(kChunks) / sizeof(int)); ++i) {
-        const double t = cost(kMinChunk * kChunks[i], kMinChunk * kChunks[i]);
-        if (i == 0 || t < least) {
-            best = kMinChunk * kChunks[i];
-            least = t;
+    const int64_t M = p.max_group * z.R();
+    p.own_rows = form_rows(z.R(), z.bf16);
+    p.own_tiles = ceil_div(z.R(), p.own_rows);
+    double least = INFINITY;
+    // Without sharing (a few short sequences do with one kernel, and one that fills whole
+    // row blocks by itself may gain nothing) and with it.
+    for (int share = 0; share < (M > 0 && p.max_shared > 0 ? 2 : 1); ++share) {
+        p.share = share;
+        p.shared_rows = share ? form_rows(M, z.bf16) : p.own_rows;
+        p.shared_tiles = share ? ceil_div(M, p.shared_rows) : 0;
+        for (int k : kChunks) {
+            cut(z, kMinChunk * k, &p);
+            const double t = plan_cost(z, p);
+            if (t < least) {
+                least = t;
+                *best = p;
+            }
         }
     }
-    p->shared_chunk = p->own_chunk = best;
-    for (int k : kChunks) {  // then the shared rows' chunk for itself
-        const double t = p->share ? cost(kMinChunk * k, best) : least;
-        if (t < least) {
-            p->shared_chunk = kMinChunk * k;
-            least = t;
-        }
-    }
-    const int64_t ss = ceil_div(shared, p->shared_chunk), os = ceil_div(own, p->own_chunk);
-    p->shared_items = 8 * st * ceil_div((int64_t)n_groups * Hkv * ss, 8);
-    p->own_items = 8 * ot * ceil_div((int64_t)B * Hkv * os, 8);
-    if (rows > 0x7fffffffLL || st > 0x7fffffffLL || ot > 0x7fffffffLL || p->shared_items + p->own_items > 0x7fffffffLL)
-        return false;
-    p->shared_tiles = (int)st;
-    p->own_tiles = (int)ot;
-    p->shared_splits = (int)ss;
-    p->own_splits = (int)os;
-    const int64_t slots = ss + os;
-    const size_t up = 255;
-    p->ml_off = ((size_t)rows * slots * kHeadDim * sizeof(float) + up) & ~up;
-    p->total = slots > 1 ? p->ml_off + (size_t)rows * slots * sizeof(float2) : 0;
-    return true;
+    p = *best;
+    const int64_t slots = p.shared_splits + p.own_splits;
+    p.ml_off = ((size_t)z.rows() * slots * kHeadDim * sizeof(float) + 255) & ~(size_t)255;
+    p.total = slots > 1 ? p.ml_off + (size_t)z.rows() * slots * sizeof(float2) : 0;
+    *best = p;
+    return p.shared_items + p.own_items <= 0x7fffffffLL;
 }
 
 template <typename T> int launch(Args& a, const Plan& p, int64_t n_rows, hipStream_t st) {
     const dim3 grid((unsigned)(p.shared_items + p.own_items)), threads(64 * kWaves);
-#define CRANE_SHARED_CASE(s, o)                                                               \
-    if (p.shared_rows == s && p.own_rows == o)                                                \
-        hipLaunchKernelGGL((shared_attn_kernel<T, s, o>), grid, threads, 0, st, a);
+    // About 240 workgroups with work, or 256 in all, get a CU each, by LDS that lets no
+    // second one in: the dispatcher otherwise pairs some and leaves CUs idle (9 sequences,
+    // 5 groups of 20000 rows in chunks of 2560, bf16: 80 us for 46; 27 sequences, 5 groups
+    // of 6656 rows: 33 for 26).
+#define CRANE_SHARED_CASE(s, o)                                                                              \
+    if (p.shared_rows == s && p.own_rows == o)                                                               \
+        hipLaunchKernelGGL((shared_attn_kernel<T, s, o>), grid, threads,                                     \
+                           p.spread ? kHalfLds + 256 - sizeof(AttnShared<s, o>) : 0, st, a);
     CRANE_SHARED_CASE(16, 16)
     CRANE_SHARED_CASE(32, 16)
     CRANE_SHARED_CASE(32, 32)
@@ -1142,7 +1244,7 @@ template <typename T> int launch(Args& a, const Plan& p, int64_t n_rows, hipStre
 #undef CRANE_SHARED_CASE
     int rc = launch_status(hipGetLastError());
     if (rc || p.shared_splits + p.own_splits == 1) return rc;
-    const int slots = p.shared_splits + p.own_splits;
+    const int64_t slots = p.shared_splits + p.own_splits;
     if (slots <= kJoinRegs)
         hipLaunchKernelGGL((shared_join_kernel<T, 1>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a, (int)n_rows);
     else if (slots <= 4 * kJoinRegs)
@@ -1159,6 +1261,7 @@ int check_sizes(const int32_t* groups, int n_groups, int64_t max_own, int B, int
     if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0) return CRANE_HIP_E_INVALID;
     if (Hq % Hkv != 0) return CRANE_HIP_E_GQA;
     if (B > 65535 || n_groups < 0 || n_groups > B || (n_groups > 0 && !groups)) return CRANE_HIP_E_INVALID;
+    if ((int64_t)B * Hq > 0x7fffffffLL || (int64_t)B * Hq * S > 0x7fffffffLL) return CRANE_HIP_E_INVALID;
     // a chunk's bounds stay within 31 bits
     const int64_t most = 0x7fffffffLL - 2 * kMaxChunk;
     if (max_own < 0 || max_own > most) return CRANE_HIP_E_INVALID;
@@ -1175,11 +1278,12 @@ int check_sizes(const int32_t* groups, int n_groups, int64_t max_own, int B, int
 
 using namespace crane;
 
-extern "C" size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups, int64_t max_own,
-                                                  int64_t mean_own, int B, int S, int Hq, int Hkv, int D, int dtype) {
-    if (check_sizes(groups_host, n_groups, max_own, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0) return 0;
+extern "C" size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups, int64_t max_kv,
+                                                  int64_t max_own, int64_t mean_own, int B, int S, int Hq, int Hkv, int D, int dtype) {
+    if (check_sizes(groups_host, n_groups, max_own, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0 || max_kv <= 0) return 0;
     Plan p;
-    return make_plan(groups_host, n_groups, max_own, mean_own, B, S, Hq, Hkv, dtype, &p) ? p.total : 0;
+    const Sizes z{groups_host, n_groups, max_kv, max_own, mean_own, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16};
+    return make_plan(z, &p) ? p.total : 0;
 }
 
 extern "C" int crane_hip_attn_shared_paged(const void* q, const void* k_pool, const void* v_pool, int64_t n_pages,
@@ -1204,7 +1308,8 @@ extern "C" int crane_hip_attn_shared_paged(const void* q, const void* k_pool, co
         (n_groups > 0 && !aligned16(groups)))
         return CRANE_HIP_E_ALIGN;
     Plan p;
-    if (!make_plan(groups_host, n_groups, max_own, mean_own, B, S, Hq, Hkv, dtype, &p)) return CRANE_HIP_E_INVALID;
+    const Sizes z{groups_host, n_groups, max_kv, max_own, mean_own, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16};
+    if (!make_plan(z, &p)) return CRANE_HIP_E_INVALID;
     if (p.max_shared > max_kv) return CRANE_HIP_E_CAPACITY;
     if (p.total && (!workspace || ws_bytes < p.total || !aligned16(workspace))) return CRANE_HIP_E_WORKSPACE;
     Args a;
@@ -1228,12 +1333,11 @@ extern "C" int crane_hip_attn_shared_paged(const void* q, const void* k_pool, co
     a.max_kv = (int)max_kv;
     a.causal = flags & CRANE_HIP_PREFILL_CAUSAL;
     a.c = scale * kLog2e;
-    a.shared_chunk = p.shared_chunk;
-    a.own_chunk = p.own_chunk;
-    a.shared_splits = p.shared_splits;
-    a.own_splits = p.own_splits;
-    a.shared_tiles = p.shared_tiles;
-    a.own_tiles = p.own_tiles;
+    a.chunk = p.chunk;
+    a.shared_splits = (int)p.shared_splits;
+    a.own_splits = (int)p.own_splits;
+    a.shared_tiles = (int)p.shared_tiles;
+    a.own_tiles = (int)p.own_tiles;
     a.shared_items = (int)p.shared_items;
     a.ws_o = (float*)workspace;
     a.ws_ml = (float2*)((char*)workspace + p.ml_off);

@@ -564,8 +564,8 @@ def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     if mean_own is None:  # the longest sequence is likely one that shares most
         mean_own = 6 * max(max_kv - groups.max_shared, 0) // 10
     scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-    need = int(_lib.lib().crane_hip_attn_shared_workspace(groups.groups_host, groups.n_groups, max_own, mean_own, B, S,
-                                                          Hq, Hkv, HEAD_DIM, dt))
+    need = int(_lib.lib().crane_hip_attn_shared_workspace(groups.groups_host, groups.n_groups, max_kv, max_own, mean_own,
+                                                          B, S, Hq, Hkv, HEAD_DIM, dt))
     # Allocated per call, not kept per stream: a captured graph keeps its own.
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)

@@ -25,7 +25,7 @@ extern "C" {
 /* Bytes of workspace crane_hip_attn_shared_paged needs for these sizes (the
  * arguments of the call); 0 where the call would be rejected or has nothing to
  * do. */
-size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups, int64_t max_own, int64_t mean_own,
+size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups, int64_t max_kv, int64_t max_own, int64_t mean_own,
                                        int B, int S, int Hq, int Hkv, int D, int dtype);
 
 /* Attention of the last S rows of every sequence over its rows of the pools, the

@@ -224,7 +224,7 @@ def test_workspace_query():
     def ws(**kw):
         a = {**BASE, **kw}
         a["groups_host"] = host(a["groups_host"])
-        return L.crane_hip_attn_shared_workspace(*[a[x] for x in ("groups_host", "n_groups", "max_own", "mean_own", "B", "S",
+        return L.crane_hip_attn_shared_workspace(*[a[x] for x in ("groups_host", "n_groups", "max_kv", "max_own", "mean_own", "B", "S",
                                                                   "Hq", "Hkv", "D", "dtype")])
 
     need = ws()
