@@ -45,6 +45,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <type_traits>
 
 #include "common.h"
@@ -1108,6 +1109,10 @@ struct Sizes {
     // the own role's most keys
     int64_t longest(const Plan& p) const { return p.share ? max_own : std::min(max_kv, max_own + p.max_shared); }
     int64_t rows() const { return (int64_t)B * Hq * S; }
+    bool same(const Sizes& o) const {  // but for the groups' contents
+        return n_groups == o.n_groups && max_kv == o.max_kv && max_own == o.max_own && mean_own == o.mean_own && B == o.B &&
+               S == o.S && Hq == o.Hq && Hkv == o.Hkv && bf16 == o.bf16;
+    }
 };
 
 // Microseconds for 128 keys of a workgroup that has a CU to itself, and of a CU kept busy
@@ -1138,21 +1143,22 @@ int form_rows(int64_t rows, bool bf16) { return rows <= 16 ? 16 : !bf16 || rows 
 // the best of the 28 on average, and 10% over 48 calls that took no part in the fit.
 double plan_cost(const Sizes& z, Plan& p) {
     const KeyCost sc = key_cost(z.bf16, p.shared_rows), oc = key_cost(z.bf16, p.own_rows);
-    double work = 0, items = 0, once = 0, loads = 0, mean = std::max<double>(64, z.mean_own);
+    double work, items = 0, once = 0, loads = 0, mean = std::max<double>(64, z.mean_own);
     double longest = std::min<double>(z.longest(p), p.chunk) * oc.alone / 128;
     auto rounds = [](double n) { return std::ceil(n / kCus); };
+    const double per_chunk = 1.0 / p.chunk, per_block = 1.0 / p.shared_rows, R = z.R(), per_batch = 1.0 / z.B;
     for (int g = 0; g < z.n_groups; ++g) {
-        const int64_t members = z.groups[4 * g + 1], rows = z.groups[4 * g + 3];
-        once += (double)z.Hkv * rows;
+        const double members = z.groups[4 * g + 1], rows = z.groups[4 * g + 3];
+        once += z.Hkv * rows;
         if (!p.share) {
-            mean += (double)members * rows / z.B;
+            mean += members * rows * per_batch;
             continue;
         }
-        const double tiles = (double)z.Hkv * ceil_div(members * z.R(), p.shared_rows);
-        work += tiles * rows * sc.busy / 128;
+        const double tiles = z.Hkv * std::ceil(members * R * per_block);
         loads += tiles * rows;
-        items += tiles * ceil_div(rows, p.chunk);
+        items += tiles * std::ceil(rows * per_chunk);
     }
+    work = loads * sc.busy / 128;
     double even = 0;  // each role's workgroups in turns of 256 at their chunk's cost
     if (p.share) {
         const double keys = std::min(p.max_shared, p.chunk) / 128.0;
@@ -1189,8 +1195,8 @@ void cut(const Sizes& z, int chunk, Plan* p) {
 // Chunk sizes tried, in units of 128 keys.
 constexpr int kChunks[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 32, 48, 64};
 
-bool make_plan(const Sizes& z, Plan* best) {
-    Plan p;
+Plan plan_for(const Sizes& z) {
+    Plan p, best;
     p.max_group = p.max_shared = 0;
     for (int g = 0; g < z.n_groups; ++g) {
         p.max_group = std::max(p.max_group, (int)z.groups[4 * g + 1]);
@@ -1209,18 +1215,43 @@ bool make_plan(const Sizes& z, Plan* best) {
         for (int k : kChunks) {
             cut(z, kMinChunk * k, &p);
             const double t = plan_cost(z, p);
-            if (t < least) {
+            if (!(t >= least)) {
                 least = t;
-                *best = p;
+                best = p;
             }
         }
     }
-    p = *best;
-    const int64_t slots = p.shared_splits + p.own_splits;
-    p.ml_off = ((size_t)z.rows() * slots * kHeadDim * sizeof(float) + 255) & ~(size_t)255;
-    p.total = slots > 1 ? p.ml_off + (size_t)z.rows() * slots * sizeof(float2) : 0;
-    *best = p;
-    return p.shared_items + p.own_items <= 0x7fffffffLL;
+    const int64_t slots = best.shared_splits + best.own_splits;
+    best.ml_off = ((size_t)z.rows() * slots * kHeadDim * sizeof(float) + 255) & ~(size_t)255;
+    best.total = slots > 1 ? best.ml_off + (size_t)z.rows() * slots * sizeof(float2) : 0;
+    return best;
+}
+
+// The plan for these sizes.  A thread's last one is kept, by the sizes' values (up to 256
+// groups): the workspace query, the call and the next layers' calls all ask for the same
+// (1 group: 3.1 us to make, 0.1 to find).
+bool make_plan(const Sizes& z, Plan* p) {
+    constexpr int kKept = 256;
+    struct Kept {
+        bool any;
+        Sizes z;
+        int32_t groups[4 * kKept];
+        Plan p;
+    };
+    static thread_local Kept kept;
+    const size_t bytes = (size_t)z.n_groups * 4 * sizeof(int32_t);
+    if (!kept.any || !kept.z.same(z) || (bytes && std::memcmp(kept.groups, z.groups, bytes))) {
+        *p = plan_for(z);
+        kept.any = z.n_groups <= kKept;
+        if (kept.any) {
+            kept.z = z;
+            kept.p = *p;
+            if (bytes) std::memcpy(kept.groups, z.groups, bytes);
+        }
+    } else {
+        *p = kept.p;
+    }
+    return p->shared_items + p->own_items <= 0x7fffffffLL;
 }
 
 template <typename T> int launch(Args& a, const Plan& p, int64_t n_rows, hipStream_t st) {

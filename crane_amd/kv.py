@@ -392,18 +392,18 @@ class PagedKvCache:
         _check_q(q, 4 if q.dim() == 4 else 3, len(self._batch), self.dtype, self.device)
         q = q.contiguous()
         B, Hq, S = q.shape[0], q.shape[1], q.shape[2] if q.dim() == 4 else 1
-        need = int(_lib.lib().crane_pkv_shared_workspace(self._h, Hq, S))
+        lib = _lib.lib()
+        need = lib.crane_pkv_shared_workspace(self._h, Hq, S)
         if workspace is not None:
             _dev(q, workspace)
         elif need:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         out = torch.empty((B, S, Hq * HEAD_DIM), dtype=q.dtype, device=q.device)
-        with _on_device(q.device):
-            check(_lib.lib().crane_pkv_attention_shared(
-                self._h, q.data_ptr(), Hq, S, HEAD_DIM ** -0.5 if scale is None else scale,
-                PREFILL_CAUSAL if causal else 0, _ptr(workspace),
-                workspace.numel() * workspace.element_size() if workspace is not None else 0, out.data_ptr(),
-                _stream(q.device)), "crane_pkv_attention_shared")
+        check(_on_device(q.device, lib.crane_pkv_attention_shared, (
+            self._h, q.data_ptr(), Hq, S, HEAD_DIM ** -0.5 if scale is None else scale,
+            PREFILL_CAUSAL if causal else 0, _ptr(workspace),
+            workspace.numel() * workspace.element_size() if workspace is not None else 0, out.data_ptr(),
+            _stream(q.device))), "crane_pkv_attention_shared")
         return out
 
     def read_sequence(self, sid: int):
@@ -447,9 +447,8 @@ def fork_sequence(caches: Sequence[PagedKvCache], sid: int, count: int = 1, rows
                             f"{count} forks of {rows} rows")
     ids = (ctypes.c_int * max(count, 1))()
     dev = caches[0].device
-    with _on_device(dev):
-        check(_lib.lib().crane_pkv_fork(_handles(caches), len(caches), sid, -1 if rows is None else rows, count, ids,
-                                        _stream(dev)), "crane_pkv_fork")
+    check(_on_device(dev, _lib.lib().crane_pkv_fork, (
+        _handles(caches), len(caches), sid, -1 if rows is None else rows, count, ids, _stream(dev))), "crane_pkv_fork")
     return list(ids[:count])
 
 
@@ -458,9 +457,8 @@ def truncate_sequence(caches: Sequence[PagedKvCache], sid: int, rows: int) -> No
     if not caches:
         raise CraneHipError(_lib.E_INVALID, "no caches")
     dev = caches[0].device
-    with _on_device(dev):
-        check(_lib.lib().crane_pkv_truncate(_handles(caches), len(caches), sid, rows, _stream(dev)),
-              "crane_pkv_truncate")
+    check(_on_device(dev, _lib.lib().crane_pkv_truncate, (_handles(caches), len(caches), sid, rows, _stream(dev))),
+          "crane_pkv_truncate")
 
 
 def compact(caches: Sequence[PagedKvCache]) -> int:
@@ -468,7 +466,6 @@ def compact(caches: Sequence[PagedKvCache]) -> int:
     if not caches:
         raise CraneHipError(_lib.E_INVALID, "no caches")
     dev, moved = caches[0].device, ctypes.c_int64()
-    with _on_device(dev):
-        check(_lib.lib().crane_pkv_compact(_handles(caches), len(caches), ctypes.byref(moved), _stream(dev)),
-              "crane_pkv_compact")
+    check(_on_device(dev, _lib.lib().crane_pkv_compact, (_handles(caches), len(caches), ctypes.byref(moved),
+                                                         _stream(dev))), "crane_pkv_compact")
     return moved.value

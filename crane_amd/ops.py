@@ -11,7 +11,6 @@ fallback.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 from typing import Optional, Sequence
@@ -528,10 +527,13 @@ def group_prefixes(tables: Sequence[Sequence[int]]):
     return groups, [shared[members[0]] for members in groups]
 
 
-def _on_device(dev: torch.device):
-    """The device of a launch made current: a default stream's handle does not say
-    which device it is on."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _on_device(dev: torch.device, call, args) -> int:
+    """call(*args) with the device made current: a default stream's handle does not
+    say which device it is on."""
+    if dev.index == torch.cuda.current_device():
+        return call(*args)
+    with torch.cuda.device(dev):
+        return call(*args)
 
 
 def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
@@ -564,19 +566,20 @@ def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     if mean_own is None:  # the longest sequence is likely one that shares most
         mean_own = 6 * max(max_kv - groups.max_shared, 0) // 10
     scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-    need = int(_lib.lib().crane_hip_attn_shared_workspace(groups.groups_host, groups.n_groups, max_kv, max_own, mean_own,
-                                                          B, S, Hq, Hkv, HEAD_DIM, dt))
+    lib = _lib.lib()
+    need = lib.crane_hip_attn_shared_workspace(groups.groups_host, groups.n_groups, max_kv, max_own, mean_own, B, S, Hq,
+                                               Hkv, HEAD_DIM, dt)
     # Allocated per call, not kept per stream: a captured graph keeps its own.
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     out = torch.empty((B, S, Hq * HEAD_DIM), dtype=q.dtype, device=dev)
-    with _on_device(dev):
-        rc = _lib.lib().crane_hip_attn_shared_paged(
-            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, page_rows, block_table.data_ptr(), stride,
+    args = (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, page_rows, block_table.data_ptr(), stride,
             kv_len.data_ptr(), max_kv, groups.shared_rows.data_ptr(), groups.groups.data_ptr(),
-            groups.members.data_ptr(), groups.groups_host, groups.n_groups, max_own, mean_own, B, S, Hq, Hkv, HEAD_DIM, scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace),
-            workspace.numel() * workspace.element_size() if workspace is not None else 0, out.data_ptr(), dt,
-            _stream(dev))
+            groups.members.data_ptr(), groups.groups_host, groups.n_groups, max_own, mean_own, B, S, Hq, Hkv, HEAD_DIM,
+            scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace),
+            workspace.numel() * workspace.element_size() if workspace is not None else 0,
+            out.data_ptr(), dt, _stream(dev))
+    rc = _on_device(dev, lib.crane_hip_attn_shared_paged, args)
     check(rc, "attention_shared_paged")
     return out
 
@@ -607,10 +610,9 @@ def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
             raise CraneHipError(_lib.E_INVALID, f"{n_pages} pages of {page_rows} rows: {list(ids)}")
     ints = lambda x: (ctypes.c_int32 * len(x))(*x)  # noqa: E731
     ptrs = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
-    with _on_device(dev):
-        rc = _lib.lib().crane_hip_copy_pages(ptrs, len(pools), n_pages, page_rows, Hkv, HEAD_DIM, ints(src), ints(dst),
-                                             ints(rows) if rows is not None else None, len(src), _dtype_code(first),
-                                             _stream(dev))
+    rc = _on_device(dev, _lib.lib().crane_hip_copy_pages, (
+        ptrs, len(pools), n_pages, page_rows, Hkv, HEAD_DIM, ints(src), ints(dst), ints(rows) if rows is not None else None,
+        len(src), _dtype_code(first), _stream(dev)))
     check(rc, "copy_pages")
 
 
