@@ -18,7 +18,8 @@ namespace {
 
 constexpr int kPools = 128;      // pools per launch: K and V of 64 layers
 constexpr int kPairs = 128;      // pairs per launch
-constexpr int kBlockBytes = 16384;  // bytes of one head's run per workgroup: 4 loads of 16 bytes per thread
+constexpr int kThreads = 256;
+constexpr int kBlockBytes = 16 * kThreads;  // bytes of one head's run per workgroup
 
 typedef unsigned int u32x4_v __attribute__((ext_vector_type(4)));
 
@@ -27,26 +28,21 @@ struct CopyArgs {
     int32_t src[kPairs], dst[kPairs], rows[kPairs];
 };
 
+// One load and one store a thread.  Bound by HBM: the stores go past the caches, which
+// leaves those to a source that is copied to several pages (72 pools, a page of 201 rows
+// to 8 others, 267 MB in all: 36 us, 65 with plain stores; 97 pages to 97, 407 MB: 59 us
+// for 76), and with 2, 4, 8 or 16 loads issued ahead of the stores the first of these
+// takes 44 to 47 us, the second the same.
 // grid: (heads x blocks of a run, pairs, pools)
-__global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a, int blocks, int Hkv, int64_t run_bytes,
-                                                         int row_bytes) {
+__global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a, int blocks, int Hkv, int64_t run_bytes,
+                                                              int row_bytes) {
     const int head = blockIdx.x / blocks, block = blockIdx.x % blocks;
-    const int64_t bytes = (int64_t)a.rows[blockIdx.y] * row_bytes;
     const int64_t at = (int64_t)block * kBlockBytes + 16 * threadIdx.x;
+    if (at >= (int64_t)a.rows[blockIdx.y] * row_bytes) return;
     uint8_t* pool = a.pool[blockIdx.z];
     const uint8_t* src = pool + ((int64_t)a.src[blockIdx.y] * Hkv + head) * run_bytes;
     uint8_t* dst = pool + ((int64_t)a.dst[blockIdx.y] * Hkv + head) * run_bytes;
-    if ((int64_t)(block + 1) * kBlockBytes <= bytes) {  // all loads issued before the first store
-        u32x4_v x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const u32x4_v*>(src + at + i * 4096);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4_v*>(dst + at + i * 4096) = x[i];
-        return;
-    }
-    for (int i = 0; i < 4; ++i)
-        if (at + i * 4096 < bytes)
-            *reinterpret_cast<u32x4_v*>(dst + at + i * 4096) = *reinterpret_cast<const u32x4_v*>(src + at + i * 4096);
+    __builtin_nontemporal_store(*reinterpret_cast<const u32x4_v*>(src + at), reinterpret_cast<u32x4_v*>(dst + at));
 }
 
 // The lists sorted form a tree: a node is a run of them with `common` first pages in
@@ -54,7 +50,8 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a, int blocks,
 // below it that no deeper open node takes; each is then read as `common` pages fewer,
 // but once:  saved = sum over lists of c(deepest open node above it) - sum over open
 // nodes of c.  best() maximises that over the nodes to open, for every node and every
-// possible open node above it (c = 0: none).
+// possible open node above it (c = 0: none).  Nodes nested deeper than kDepth are left out,
+// which bounds the recursion's stack and best()'s depth^2 sums.
 class Grouping {
   public:
     explicit Grouping(const std::vector<PageList>& lists) : lists_(lists), order_(lists.size()) {
@@ -70,7 +67,7 @@ class Grouping {
         PageGroups g;
         g.shared.assign(lists_.size(), 0);
         if (lists_.size() < 2) return g;
-        Node root = build(0, order_.size(), 0);
+        Node root = build(0, order_.size(), 0, kDepth);
         std::vector<int64_t> above{0};
         best(root, above);
         std::vector<std::vector<int32_t>> open(1);
@@ -87,22 +84,24 @@ class Grouping {
     }
 
   private:
+    static constexpr int kDepth = 512;
     struct Node {
         size_t lo, hi, common;
         std::vector<Node> kids;
         std::vector<char> open;  // by the open node above: whether to open this one
     };
-    Node build(size_t lo, size_t hi, size_t common) {
+    Node build(size_t lo, size_t hi, size_t common, int depth) {
         const PageList &a = lists_[order_[lo]], &b = lists_[order_[hi - 1]];
         // sorted: what the first and the last share, all share; an id below 0 names no page
         while (common < a.n && common < b.n && a.ids[common] == b.ids[common] && a.ids[common] >= 0) ++common;
         Node node{lo, hi, common, {}, {}};
+        if (depth == 0) return node;
         for (size_t i = lo; i < hi;) {
             const PageList& p = lists_[order_[i]];
             size_t j = i + 1;
             if (p.n > common && p.ids[common] >= 0)
                 while (j < hi && lists_[order_[j]].n > common && lists_[order_[j]].ids[common] == p.ids[common]) ++j;
-            if (j - i > 1 && j - i < hi - lo) node.kids.push_back(build(i, j, common));
+            if (j - i > 1 && j - i < hi - lo) node.kids.push_back(build(i, j, common, depth - 1));
             i = j;
         }
         return node;
@@ -224,7 +223,7 @@ extern "C" int crane_hip_copy_pages(void* const* pools, int n_pools, int64_t n_p
     const int row_bytes = kHeadDim * elem_size(dtype);
     const int64_t run = (int64_t)page_rows * row_bytes;
     const int64_t blocks = ((int64_t)max_rows * row_bytes + kBlockBytes - 1) / kBlockBytes;
-    if (blocks * Hkv > 0x7fffffffLL) return CRANE_HIP_E_INVALID;
+    if (blocks * Hkv > 0xffffffffLL / kThreads) return CRANE_HIP_E_INVALID;  // a grid's threads: 32 bits
     CopyArgs a;
     for (int p0 = 0; p0 < n_pools; p0 += kPools) {
         const int np = n_pools - p0 < kPools ? n_pools - p0 : kPools;
@@ -236,8 +235,8 @@ extern "C" int crane_hip_copy_pages(void* const* pools, int n_pools, int64_t n_p
                 a.dst[i] = dst[i0 + i];
                 a.rows[i] = rows ? rows[i0 + i] : page_rows;
             }
-            hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(blocks * Hkv), (unsigned)ni, (unsigned)np), dim3(256),
-                               0, (hipStream_t)stream, a, (int)blocks, Hkv, run, row_bytes);
+            hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(blocks * Hkv), (unsigned)ni, (unsigned)np),
+                               dim3(kThreads), 0, (hipStream_t)stream, a, (int)blocks, Hkv, run, row_bytes);
             rc = launch_status(hipGetLastError());
             if (rc) return rc;
         }

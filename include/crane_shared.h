@@ -81,7 +81,8 @@ int crane_hip_attn_shared_paged(const void* q, const void* k_pool, const void* v
  * Writes shared_pages [B] (pages sequence b shares with its group; 0: in none),
  * group_start [B + 1] and group_seq [B] (as far as *n_groups groups need them).
  * Where sequences share more with some than with others, the grouping that reads
- * the fewest pages is taken.  Ids below 0 are shared by none.  shared_pages times the
+ * the fewest pages is taken (of those whose lists branch up to 512 times on the way
+ * to a group's last shared page).  Ids below 0 are shared by none.  shared_pages times the
  * page's rows are crane_hip_attn_shared_paged's shared_rows where every shared page is
  * full of rows. */
 int crane_hip_group_prefixes(const int32_t* table, int64_t stride, const int32_t* pages, int B, int32_t* shared_pages,

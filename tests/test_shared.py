@@ -582,6 +582,18 @@ def test_group_prefixes_edges():
     assert L.crane_hip_group_prefixes(buf, 2, buf, -1, buf, buf, buf, ctypes.byref(n)) == _lib.E_INVALID
 
 
+def test_group_prefixes_nested_deep():
+    """Lists that each extend the last: the nesting stays within a bound, the groups valid."""
+    from crane_amd import ops
+    tables = [list(range(n)) for n in range(1, 2501)]
+    groups, pages = ops.group_prefixes(tables)
+    flat = [b for g in groups for b in g]
+    assert len(flat) == len(set(flat)) and len(groups) == len(pages) >= 1
+    for g, n in zip(groups, pages):
+        assert len(g) > 1 and 0 < n <= min(len(tables[b]) for b in g)
+    assert sum((len(g) - 1) * n for g, n in zip(groups, pages)) >= 1900 * 500   # one group of the longest does that
+
+
 def test_manager_refusals_without_a_cache():
     from crane_amd import _lib
     L = _lib.lib()
