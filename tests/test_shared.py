@@ -475,6 +475,264 @@ def test_replays_and_streams(gpu):
             assert torch.equal(out, want), step
 
 
+# ------------------------------------------------------------------ GPU: sizes at which sharing pays
+
+SHARED_SHAPES = [  # members, shared rows, own rows from, other sequences, P, Hq, Hkv, S
+    (16, 2048, 40, (100, 0), 256, 2, 2, 1),        # 16 rows a kv head in all
+    (33, 1536, 200, (700,), 256, 4, 2, 1),         # 66
+    (96, 512, 50, (), 512, 8, 4, 1),               # 192
+    (4, 4096, 20, (), 256, 8, 8, 20),              # 80, 20 a sequence
+    (16, 2560, 20, (30, 2), 512, 4, 2, 20),        # 640, 40
+    (16, 4096, 65, (), 256, 2, 1, 65),             # 2080, 130
+    (40, 1024, 0, (), 256, 8, 2, 1),               # little or nothing of their own
+    (24, 1024, 0, (), 256, 8, 4, 5),               # queries inside and past the shared rows
+    (6, 16896, 40, (), 256, 2, 2, 1),              # block table rows of 67 pages
+]
+
+
+def shared_shape(i):
+    n, shared, own, others, P, Hq, Hkv, S = SHARED_SHAPES[i]
+    lens = [shared + own + x % 7 for x in range(n)] + list(others)
+    order = cases.rng(i).permutation(len(lens))    # the members in any order in the batch
+    members = [int(np.where(order == x)[0][0]) for x in range(n)]
+    return [lens[x] for x in order], [members], [shared], P, Hq, Hkv, S
+
+
+def only_first_names(table, members, pages):
+    """The table with the shared pages named by the group's first member only."""
+    t = table.copy()
+    for b in members[1:]:
+        t[b, :pages] = -7
+    return t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(SHARED_SHAPES)))
+def test_shared_rows_are_read_once(gpu, case, dtype):
+    """Exact as above; and the members' own entries for shared pages are not read, which
+    says that these calls share."""
+    import torch
+    lens, groups, rows, P, Hq, Hkv, S = shared_shape(case)
+    for causal in (True, False):
+        check_exact(gpu, 500 + case, lens, groups, rows, P, Hq, Hkv, S, dtype, causal)
+    table, total = layout(520 + case, lens, groups, rows, P)
+    k, v = pools(521 + case, total, Hkv, P, table, lens, False)
+    q = cases.cast(cases.normal(cases.rng(522 + case), (len(lens), Hq, S, D)), dtype)
+    args = (q, cases.cast(k, dtype), cases.cast(v, dtype))
+    want = call(gpu, *args, table, lens, groups, rows, dtype)
+    got = call(gpu, *args, only_first_names(table, groups[0], rows[0] // P), lens, groups, rows, dtype)
+    if (case, dtype) != (4, "bf16"):               # (whole row blocks hold 3 sequences: no gain)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", [0, 1, 2, 3, 6, 7])
+@pytest.mark.parametrize("q_scale", [1.5, 60.0])
+def test_shared_attention_close(gpu, case, dtype, q_scale):
+    lens, groups, rows, P, Hq, Hkv, S = shared_shape(case)
+    check_close(gpu, 540 + case, lens, groups, rows, P, Hq, Hkv, S, dtype, q_scale=q_scale)
+
+
+def one_sequence_for_all(seed, n, Hkv, P):
+    """A table row, K and V of one sequence of n rows."""
+    pages = math.ceil(n / P)
+    table, total = layout(seed, [n], [], [], P)
+    k, v = pools(seed + 1, total, Hkv, P, table, [n], False)
+    return table[:, :pages + 1], k, v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("B,Hq,Hkv,S,n,shared", [
+    (300, 2, 2, 1, 1400, 0), (150, 4, 2, 10, 1400, 0), (60, 4, 1, 33, 1400, 0), (64, 8, 8, 1, 4200, 4096),
+    (256, 8, 8, 1, 2100, 2048), (16, 2, 1, 65, 4200, 4096)])
+def test_rising_scores(gpu, B, Hq, Hkv, S, n, shared, dtype):
+    """Scores that rise by 0.8 (natural units) from key to key: past any fixed maximum of a
+    chunk's first keys by hundreds of powers of two."""
+    P = 256
+    table, k, v = one_sequence_for_all(560, n, Hkv, P)
+    r = cases.rng(562)
+    u = np.sign(cases.normal(r, (D,)))
+    ramp = np.arange(n) * (0.8 * math.sqrt(D) / D)
+    for i in range(math.ceil(n / P)):
+        m = min(P, n - i * P)
+        k[table[0, i], :, :m] = 0.05 * k[table[0, i], :, :m] + ramp[i * P:i * P + m, None] * u
+    q = u + 0.05 * cases.normal(r, (B, Hq, S, D))
+    lens = [n - b % 50 for b in range(B)]
+    q, k, v = (cases.cast(x.astype(np.float32), dtype) for x in (q, k, v))
+    table = np.repeat(table, B, 0)
+    groups, rows = ([list(range(B))], [shared]) if shared else ([], [])
+    got = call(gpu, q, k, v, table, lens, groups, rows, dtype).float().cpu().numpy()
+    some = sorted({0, 1, 49, B - 1} & set(range(B)))   # sequences checked (all differ in q)
+    out, mag, most = reference(q[some], k, v, table[some], [lens[b] for b in some], P, D ** -0.5, True)
+    assert np.isfinite(got).all()
+    assert (np.abs(got[some] - out) <= bounds(out, mag, most, n, dtype)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("B,Hq,Hkv,S,n,shared", [(2, 8, 2, 33, 400, 0), (24, 8, 4, 5, 1024, 1024), (16, 2, 1, 65, 4100, 4096)])
+def test_hidden_rows_in_blocks(gpu, B, Hq, Hkv, S, n, shared, bad, dtype):
+    """As test_hidden_rows_have_no_influence, in blocks of 128 rows and in shared rows: key
+    n - 4 is NaN or infinite in K or in V, and the last 4 queries of the sequences that are
+    n long see it."""
+    P = 256
+    table, k, v = one_sequence_for_all(570, n, Hkv, P)
+    table = np.repeat(table, B, 0)
+    lens = [n - b % 2 * 3 for b in range(B)]
+    q = cases.normal(cases.rng(572), (B, Hq, S, D))
+    q, k, v = (cases.cast(x, dtype) for x in (q, k, v))
+    groups, rows = ([list(range(B))], [shared // P * P]) if shared else ([], [])
+    j = n - 4
+    some = [0, 1, B - 1]
+    out, mag, most = reference(q[some], k, v, table[some], [lens[b] for b in some], P, D ** -0.5, True)
+    tol = bounds(out, mag, most, n, dtype).reshape(3, S, Hq, D)
+    out = out.reshape(3, S, Hq, D)
+    for which in ("k", "v"):
+        k2, v2 = k.copy(), v.copy()
+        (k2 if which == "k" else v2)[table[0, j // P], :, j % P, ::3] = bad
+        got = call(gpu, q, k2, v2, table, lens, groups, rows, dtype).float().cpu().numpy()
+        got = got.reshape(B, S, Hq, D)[some]
+        for x, b in enumerate(some):
+            unseen = np.array([lens[b] - S + 1 + i <= j for i in range(S)])
+            assert (np.abs(got[x] - out[x])[unseen] <= tol[x][unseen]).all()
+            if which == "v":
+                hit = got[x][~unseen][..., ::3]
+                assert np.isnan(hit).all() if math.isnan(bad) else (hit == bad).all()
+                clean = np.arange(D) % 3 != 0
+                assert (np.abs(got[x] - out[x])[~unseen][..., clean] <= tol[x][~unseen][..., clean]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_shared_short_members_and_bad_pages(gpu, dtype):
+    """Members that end inside the shared rows, a page outside the pool among the shared
+    ones, and one among a member's own."""
+    import torch
+    P, B, Hq, Hkv, S = 256, 40, 8, 2, 1
+    full = [1024 + 3 * b for b in range(B)]
+    lens = list(full)
+    lens[3], lens[7], lens[20], lens[39] = 1024, 300, 2, 0
+    table, total = layout(580, full, [list(range(B))], [1024], P)
+    k, v = pools(581, total, Hkv, P, table, full, False)
+    q = cases.cast(cases.normal(cases.rng(582), (B, Hq, S, D)), dtype)
+    k, v = cases.cast(k, dtype), cases.cast(v, dtype)
+    groups, rows = [list(range(B))], [1024]
+    got = call(gpu, q, k, v, table, lens, groups, rows, dtype)
+    out, mag, most = reference(q, k, v, table, lens, P, D ** -0.5, True)
+    assert (np.abs(got.float().cpu().numpy() - out) <= bounds(out, mag, most, max(lens), dtype)).all()
+    assert (got[39] == 0).all()
+    kz, vz, bad = k.copy(), v.copy(), table.copy()
+    for b, i, x in ((0, 2, 10 ** 6), (5, 4, -5)):
+        kz[table[b, i]] = 0
+        vz[table[b, i]] = 0
+        bad[b, i] = x
+    got = call(gpu, q, k, v, only_first_names(bad, groups[0], 4), lens, groups, rows, dtype)
+    assert torch.equal(got, call(gpu, q, kz, vz, table, lens, groups, rows, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [1, 5])
+def test_shared_inconsistent_descriptions(gpu, S):
+    """As test_inconsistent_descriptions_stay_in_bounds, where the call shares."""
+    import torch
+    from crane_amd import ops
+    P, B = 256, 41
+    lens = [1024 + b for b in range(B - 1)] + [300]
+    table, total = layout(590, lens, [list(range(B - 1))], [1024], P)
+    k, v = pools(591, total, 2, P, table, lens, False)
+    q, k, v = (cases.cast(x, "bf16") for x in (cases.normal(cases.rng(592), (B, 8, S, D)), k, v))
+    t = [tens(q, "bf16", gpu), tens(k, "bf16", gpu), tens(v, "bf16", gpu), ints(table, gpu), ints(lens, gpu)]
+    g = ops.prefix_groups([list(range(B - 1))], [1024], B, gpu)
+    want = ops.attention_shared_paged(*t, 1024 + B, g)
+    members = list(range(B - 1))
+    for groups, of in (([[0, 40, 0, 1024]], [99] * 40), ([[0, 40, 0, 1024]], [-3] + members[1:]),
+                       ([[-50, 1 << 30, 0, 1024]], members), ([[0, 40, 99, 1024]], members),
+                       ([[0, 40, -1, 1024]], members), ([[0, -4, 0, 1024]], members),
+                       ([[0, 40, 0, 1 << 30]], members), ([[0, 40, 0, -9]], members),
+                       ([[1 << 30, 40, 0, 1024]], members), ([[0, 40, 0, 1024]], [7] * 20 + [8] * 20)):
+        print(groups, of[:3], flush=True)
+        g.groups, g.members = ints(groups, gpu), ints(of, gpu)
+        got = ops.attention_shared_paged(*t, 1024 + B, g)
+        assert torch.equal(got[B - 1], want[B - 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [1, 8])
+def test_shared_replays_streams_and_threads(gpu, S):
+    """Two captured calls that share, replayed with other lengths and eager calls between;
+    calls of two threads at once on streams of their own."""
+    import threading
+
+    import torch
+    from crane_amd import ops
+    lens, P, B, Hq, Hkv = [1100 + 5 * b for b in range(40)], 256, 40, 8, 2
+    table, total = layout(600, lens, [list(range(B))], [1024], P)
+    k, v = pools(601, total, Hkv, P, table, lens, False)
+    q = cases.cast(cases.normal(cases.rng(602), (B, Hq, S, D)), "bf16")
+    q, k, v, table, n = tens(q, "bf16", gpu), tens(k, "bf16", gpu), tens(v, "bf16", gpu), ints(table, gpu), ints(lens, gpu)
+    g = ops.prefix_groups([list(range(B))], [1024], B, gpu)
+    run = lambda n: ops.attention_shared_paged(q, k, v, table, n, max(lens), g)
+    want = run(n)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(n)
+        graphs.append((graph, out))
+    for step in range(3):
+        n.copy_(ints([x - 5 * step for x in lens], gpu))
+        for graph, _ in graphs:
+            graph.replay()
+        want = run(n)
+        torch.cuda.synchronize(gpu)
+        for _, out in graphs:
+            assert torch.equal(out, want), step
+    results = [None, None]
+    def work(i):
+        stream = torch.cuda.Stream(gpu)
+        with torch.cuda.stream(stream):
+            results[i] = [run(n) for _ in range(20)]
+        stream.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(x, want) for r in results for x in r)
+
+
+@pytest.mark.gpu
+def test_pools_past_31_bits(gpu):
+    """Pages past the first 2^31 elements of a pool: attention over them, and copies."""
+    import torch
+    from crane_amd import ops
+    P, Hq, Hkv, B = 256, 8, 8, 24
+    far = 2 ** 31 // (Hkv * P * D)
+    lens = [1024 + 9 * b for b in range(B)]
+    table, total = layout(610, lens, [list(range(B))], [1024], P)
+    k, v = pools(611, total, Hkv, P, table, lens, True)
+    q = torch.zeros(B, Hq, D, dtype=torch.bfloat16, device=gpu)
+    near = [tens(cases.cast(x, "bf16"), "bf16", gpu) for x in (k, v)]
+    big = [torch.empty(far + total, Hkv, P, D, dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    for x, y in zip(big, near):
+        x[far:] = y
+    for groups, rows in (([list(range(B))], [1024]), ([], [])):
+        g = ops.prefix_groups(groups, rows, B, gpu)
+        want = ops.attention_shared_paged(q, *near, ints(table, gpu), ints(lens, gpu), max(lens), g)
+        got = ops.attention_shared_paged(q, *big, ints(np.where(table < 0, table, table + far), gpu), ints(lens, gpu),
+                                         max(lens), g)
+        assert torch.equal(got, want)
+    ops.copy_pages(big, [far, far + 1, far + 2], [0, 1, far + 5], [P, 77, P])
+    for x, y in zip(big, near):
+        assert torch.equal(x[0].view(torch.int16), y[0].view(torch.int16))
+        assert torch.equal(x[1, :, :77].view(torch.int16), y[1, :, :77].view(torch.int16))
+        assert torch.equal(x[far + 5].view(torch.int16), y[2].view(torch.int16))
+
+
 # ------------------------------------------------------------------ GPU: copies
 
 @pytest.mark.gpu
