@@ -211,7 +211,8 @@ class PagedKv {
         if (groups.count()) {  // crane_hip_attn_shared_paged's groups, members and shared rows
             for (int i = 0; i < groups.count(); ++i) {
                 const int32_t at = groups.start[i], leader = groups.members[at];
-                for (int32_t x : {at, groups.start[i + 1] - at, leader, groups.shared[leader] * P_}) shared.push_back(x);
+                for (int32_t x : {at, groups.start[i + 1] - at, leader, groups.shared[leader] * P_})
+                    shared.push_back(x);
             }
             shared.insert(shared.end(), groups.members.begin(), groups.members.end());
             for (int32_t pages : groups.shared) shared.push_back(pages * P_);
@@ -512,8 +513,8 @@ class PagedKv {
         return B() ? sum / B() : 0;
     }
     size_t shared_workspace(int Hq, int S) const {
-        return crane_hip_attn_shared_workspace(batch_groups_.data(), n_groups_, max_len(), max_own(), mean_own(), B(), S, Hq, Hkv_,
-                                               D_, dtype_);
+        return crane_hip_attn_shared_workspace(batch_groups_.data(), n_groups_, max_len(), max_own(), mean_own(), B(),
+                                               S, Hq, Hkv_, D_, dtype_);
     }
     int attention_shared(const void* q, int Hq, int S, float scale, int flags, void* ws, size_t ws_bytes, void* out,
                          hipStream_t st) const {
@@ -524,8 +525,8 @@ class PagedKv {
         if (max_len() == 0) return CRANE_HIP_E_INVALID;
         const int32_t *members = d_groups_ + 4 * n_groups_, *shared = members + n_members_;
         return crane_hip_attn_shared_paged(q, k_pool_, v_pool_, n_pages_, P_, d_table_, max_pps_, d_len_, max_len(),
-                                           shared, d_groups_, members, batch_groups_.data(), n_groups_, max_own(), mean_own(),
-                                           B(), S, Hq, Hkv_, D_, scale, flags, ws, ws_bytes, out, dtype_, st);
+                                           shared, d_groups_, members, batch_groups_.data(), n_groups_, max_own(),
+                                           mean_own(), B(), S, Hq, Hkv_, D_, scale, flags, ws, ws_bytes, out, dtype_, st);
     }
 
     bool same_shape(const PagedKv& o) const {
@@ -562,7 +563,9 @@ class PagedKv {
         if (refs_[p] == 2) --shared_pages_;
         if (--refs_[p] == 0) free_.push_back(p);
     }
-    int64_t batch_shared_rows(int b) const { return n_groups_ ? batch_groups_[(size_t)(4 * n_groups_ + n_members_ + b)] : 0; }
+    int64_t batch_shared_rows(int b) const {
+        return n_groups_ ? batch_groups_[(size_t)(4 * n_groups_ + n_members_ + b)] : 0;
+    }
 
     static int upload(int32_t* dst, const std::vector<int32_t>& v, hipStream_t st) {
         return hip_rc(hipMemcpyAsync(dst, v.data(), sizeof(int32_t) * v.size(), hipMemcpyHostToDevice, st));

@@ -61,6 +61,7 @@ constexpr float kMostSum = 0x1p60f;  // see above
 constexpr int kMaxChunk = 8192;    // rows per chunk: its pages' ids fit one lane each
 constexpr int kMinChunk = 128;
 constexpr int kCus = 256;
+constexpr int64_t kMostThreads = 0xffffffffLL;  // of a grid
 constexpr size_t kHalfLds = 81920;   // half of a CU's LDS
 constexpr int kBlockRows = 128;    // query rows of a workgroup's block form
 
@@ -72,8 +73,8 @@ __device__ __forceinline__ u32x4_v buf_load16(__amdgpu_buffer_rsrc_t r, int off)
     return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
 }
 __device__ __forceinline__ f32x4_v mfma(u32x4_v a, u32x4_v b, f32x4_v c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c, 0,
-                                                   0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c,
+                                                   0, 0, 0);
 }
 __device__ __forceinline__ f32x4_v mfma(float a, float b, f32x4_v c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -182,7 +183,8 @@ struct Pages {
         return Tile{uniform(off), __builtin_amdgcn_readfirstlane(rows * kHeadDim * (int)sizeof(T))};
     }
 };
-template <typename T> __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* pool, const Pages::Tile& t) {
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* pool, const Pages::Tile& t) {
     return make_rsrc(reinterpret_cast<const T*>(pool) + t.off, t.bytes);
 }
 
@@ -345,7 +347,8 @@ __device__ __forceinline__ float groups_max(float x) {
 
 // p = exp2(s c - m) of the step's scores; MOVE: m moved to the largest so far first, and
 // o and l scaled to it.
-template <bool MOVE, typename T, int N> __device__ __forceinline__ void softmax_step(Row<T>& st, float (&s)[N], float c) {
+template <bool MOVE, typename T, int N>
+__device__ __forceinline__ void softmax_step(Row<T>& st, float (&s)[N], float c) {
     if constexpr (MOVE) {
         float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
         if constexpr (N == 8) mx = fmaxf(mx, fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
@@ -674,8 +677,8 @@ __device__ __forceinline__ uint2 lds_read_tr16(uint32_t at) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_v*)(uintptr_t)at));
 }
 __device__ __forceinline__ f32x16_v mfma(u32x4_v a, u32x4_v b, f32x16_v c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c, 0,
-                                                   0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c,
+                                                   0, 0, 0);
 }
 __device__ __forceinline__ float halves_max(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -688,9 +691,10 @@ __device__ __forceinline__ float halves_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// A wave's share of a block: Q, o, m and l of its 32 rows, and one tile's work.  Lane (n, h) = (lane % 32, lane / 32) holds, for row n, keys 32 b +
-// 8 (r / 4) + 4 h + r % 4 in register r of score block b, and dims 32 d + 8 (r / 4) +
-// 4 h + r % 4 in register r of o[d].
+// A wave's share of a block: Q, o, m and l of its 32 rows, and one tile's work.  Lane
+// (n, h) = (lane % 32, lane / 32) holds, for row n, keys 32 b + 8 (r / 4) + 4 h + r % 4 in
+// register r of score block b, and dims 32 d + 8 (r / 4) + 4 h + r % 4 in register r of
+// o[d].
 struct BlockWave {
     static constexpr int kRows = 32, kKeys = 64;
     u32x4_v q[8];
@@ -708,7 +712,8 @@ struct BlockWave {
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int row = 8 * e + 4 * h + ((lane & 15) >> 2), col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                const int row = 8 * e + 4 * h + ((lane & 15) >> 2);
+                const int col = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
                 vo[2 * d + e] = lds_at(sm.v) + chunk_at(row, col >> 3) + 2 * (col & 7);
             }
     }
@@ -775,7 +780,8 @@ struct BlockWave {
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                const float x = fast_exp2(__builtin_fmaf(s[b][r], c, -m)), y = fast_exp2(__builtin_fmaf(s[b][r + 1], c, -m));
+                const float x = fast_exp2(__builtin_fmaf(s[b][r], c, -m));
+                const float y = fast_exp2(__builtin_fmaf(s[b][r + 1], c, -m));
                 sum += x + y;
                 p[2 * b + (r >> 3)][(r & 7) >> 1] = pack_bf16x2(x, y);
             }
@@ -876,8 +882,12 @@ __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int
     auto tile_at = [&](int t) __attribute__((always_inline)) {
         return pages.tile<bf16_t>(a, kvh, begin + t * kKeys, kKeys, end);
     };
-    auto issue_k = [&](int t) __attribute__((always_inline)) { stage(tile_rsrc<bf16_t>(a.k, tile_at(t)), sm.k[t & 1], wave, lane); };
-    auto issue_v = [&](int t) __attribute__((always_inline)) { stage(tile_rsrc<bf16_t>(a.v, tile_at(t)), sm.v[t & 1], wave, lane); };
+    auto issue_k = [&](int t) __attribute__((always_inline)) {
+        stage(tile_rsrc<bf16_t>(a.k, tile_at(t)), sm.k[t & 1], wave, lane);
+    };
+    auto issue_v = [&](int t) __attribute__((always_inline)) {
+        stage(tile_rsrc<bf16_t>(a.v, tile_at(t)), sm.v[t & 1], wave, lane);
+    };
     // Step t takes the weights and the V product of tile t and the scores of tile t + 1,
     // whose MFMAs run beside the exponentials, while K of tile t + 2 and V of tile t + 1
     // come in (into the buffers of K(t) and V(t - 1), whose readers passed the barrier).
@@ -1110,8 +1120,8 @@ struct Sizes {
     int64_t longest(const Plan& p) const { return p.share ? max_own : std::min(max_kv, max_own + p.max_shared); }
     int64_t rows() const { return (int64_t)B * Hq * S; }
     bool same(const Sizes& o) const {  // but for the groups' contents
-        return n_groups == o.n_groups && max_kv == o.max_kv && max_own == o.max_own && mean_own == o.mean_own && B == o.B &&
-               S == o.S && Hq == o.Hq && Hkv == o.Hkv && bf16 == o.bf16;
+        return n_groups == o.n_groups && max_kv == o.max_kv && max_own == o.max_own && mean_own == o.mean_own &&
+               B == o.B && S == o.S && Hq == o.Hq && Hkv == o.Hkv && bf16 == o.bf16;
     }
 };
 
@@ -1177,7 +1187,8 @@ double plan_cost(const Sizes& z, Plan& p) {
     const double memory = (once / 5.5e6 + std::max(0.0, loads - once) / 10e6) * (z.bf16 ? 512 : 1024);
     auto pow4 = [](double x) { return x * x * x * x; };
     double t = std::sqrt(std::sqrt(pow4(longest) + pow4(memory) + (items <= kCus ? 0 : pow4(work))));
-    t += (items <= kCus ? 0 : 0.08 * longest) + 0.002 * items + 0.0032 * (p.shared_items + p.own_items) + 0.85 * p.share;
+    t += (items <= kCus ? 0 : 0.08 * longest) + 0.85 * p.share;
+    t += 0.002 * items + 0.0032 * (p.shared_items + p.own_items);
     const double slots = p.shared_splits + p.own_splits;
     if (slots > 1) t += 1.1 + (slots > 32) * 1.0 + 2e-4 * z.rows() * slots;
     return t;
@@ -1251,7 +1262,7 @@ bool make_plan(const Sizes& z, Plan* p) {
     } else {
         *p = kept.p;
     }
-    return p->shared_items + p->own_items <= 0x7fffffffLL;
+    return p->shared_items + p->own_items <= kMostThreads / (64 * kWaves);
 }
 
 template <typename T> int launch(Args& a, const Plan& p, int64_t n_rows, hipStream_t st) {
@@ -1261,6 +1272,7 @@ template <typename T> int launch(Args& a, const Plan& p, int64_t n_rows, hipStre
     // 5 groups of 20000 rows in chunks of 2560, bf16: 80 us for 46; 27 sequences, 5 groups
     // of 6656 rows: 33 for 26).
 #define CRANE_SHARED_CASE(s, o)                                                                              \
+    static_assert(sizeof(AttnShared<s, o>) <= kHalfLds);                                                     \
     if (p.shared_rows == s && p.own_rows == o)                                                               \
         hipLaunchKernelGGL((shared_attn_kernel<T, s, o>), grid, threads,                                     \
                            p.spread ? kHalfLds + 256 - sizeof(AttnShared<s, o>) : 0, st, a);
@@ -1276,14 +1288,17 @@ template <typename T> int launch(Args& a, const Plan& p, int64_t n_rows, hipStre
     int rc = launch_status(hipGetLastError());
     if (rc || p.shared_splits + p.own_splits == 1) return rc;
     const int64_t slots = p.shared_splits + p.own_splits;
-    if (slots <= kJoinRegs)
-        hipLaunchKernelGGL((shared_join_kernel<T, 1>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a, (int)n_rows);
-    else if (slots <= 4 * kJoinRegs)
+    if (slots <= kJoinRegs || n_rows > kMostThreads / 256)
+        hipLaunchKernelGGL((shared_join_kernel<T, 1>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a,
+                           (int)n_rows);
+    else if (slots <= 4 * kJoinRegs || n_rows > kMostThreads / 1024)
         hipLaunchKernelGGL((shared_join_kernel<T, 4>), dim3((unsigned)n_rows), dim3(256), 0, st, a, (int)n_rows);
     else
         hipLaunchKernelGGL((shared_join_kernel<T, 16>), dim3((unsigned)n_rows), dim3(1024), 0, st, a, (int)n_rows);
     return launch_status(hipGetLastError());
 }
+
+int64_t mean_of(int64_t mean_own, int64_t max_own) { return std::min(std::max<int64_t>(mean_own, 0), max_own); }
 
 // The checks both entry points make of the sizes.
 int check_sizes(const int32_t* groups, int n_groups, int64_t max_own, int B, int S, int Hq, int Hkv, int D, int dtype) {
@@ -1292,13 +1307,14 @@ int check_sizes(const int32_t* groups, int n_groups, int64_t max_own, int B, int
     if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0) return CRANE_HIP_E_INVALID;
     if (Hq % Hkv != 0) return CRANE_HIP_E_GQA;
     if (B > 65535 || n_groups < 0 || n_groups > B || (n_groups > 0 && !groups)) return CRANE_HIP_E_INVALID;
-    if ((int64_t)B * Hq > 0x7fffffffLL || (int64_t)B * Hq * S > 0x7fffffffLL) return CRANE_HIP_E_INVALID;
+    if ((int64_t)B * Hq > 0x7fffffffLL || (int64_t)B * Hq * S > kMostThreads / 64) return CRANE_HIP_E_INVALID;
     // a chunk's bounds stay within 31 bits
     const int64_t most = 0x7fffffffLL - 2 * kMaxChunk;
     if (max_own < 0 || max_own > most) return CRANE_HIP_E_INVALID;
     for (int g = 0; g < n_groups; ++g) {
         const int32_t* d = groups + 4 * g;
-        if (d[0] < 0 || d[1] < 0 || (int64_t)d[0] + d[1] > B || d[2] < 0 || d[2] >= B || d[3] < 0 || d[3] > most - max_own)
+        if (d[0] < 0 || d[1] < 0 || (int64_t)d[0] + d[1] > B || d[2] < 0 || d[2] >= B || d[3] < 0 ||
+            d[3] > most - max_own)
             return CRANE_HIP_E_INVALID;
     }
     return CRANE_HIP_OK;
@@ -1310,10 +1326,13 @@ int check_sizes(const int32_t* groups, int n_groups, int64_t max_own, int B, int
 using namespace crane;
 
 extern "C" size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups, int64_t max_kv,
-                                                  int64_t max_own, int64_t mean_own, int B, int S, int Hq, int Hkv, int D, int dtype) {
-    if (check_sizes(groups_host, n_groups, max_own, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0 || max_kv <= 0) return 0;
+                                                  int64_t max_own, int64_t mean_own, int B, int S, int Hq, int Hkv,
+                                                  int D, int dtype) {
+    if (check_sizes(groups_host, n_groups, max_own, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0 || max_kv <= 0)
+        return 0;
     Plan p;
-    const Sizes z{groups_host, n_groups, max_kv, max_own, mean_own, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16};
+    const Sizes z{groups_host, n_groups, max_kv, max_own, mean_of(mean_own, max_own), B, S,
+                  Hq, Hkv, dtype == CRANE_HIP_BF16};
     return make_plan(z, &p) ? p.total : 0;
 }
 
@@ -1339,7 +1358,8 @@ extern "C" int crane_hip_attn_shared_paged(const void* q, const void* k_pool, co
         (n_groups > 0 && !aligned16(groups)))
         return CRANE_HIP_E_ALIGN;
     Plan p;
-    const Sizes z{groups_host, n_groups, max_kv, max_own, mean_own, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16};
+    const Sizes z{groups_host, n_groups, max_kv, max_own, mean_of(mean_own, max_own), B, S,
+                  Hq, Hkv, dtype == CRANE_HIP_BF16};
     if (!make_plan(z, &p)) return CRANE_HIP_E_INVALID;
     if (p.max_shared > max_kv) return CRANE_HIP_E_CAPACITY;
     if (p.total && (!workspace || ws_bytes < p.total || !aligned16(workspace))) return CRANE_HIP_E_WORKSPACE;

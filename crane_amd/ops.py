@@ -611,8 +611,8 @@ def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
     ints = lambda x: (ctypes.c_int32 * len(x))(*x)  # noqa: E731
     ptrs = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
     rc = _on_device(dev, _lib.lib().crane_hip_copy_pages, (
-        ptrs, len(pools), n_pages, page_rows, Hkv, HEAD_DIM, ints(src), ints(dst), ints(rows) if rows is not None else None,
-        len(src), _dtype_code(first), _stream(dev)))
+        ptrs, len(pools), n_pages, page_rows, Hkv, HEAD_DIM, ints(src), ints(dst),
+        ints(rows) if rows is not None else None, len(src), _dtype_code(first), _stream(dev)))
     check(rc, "copy_pages")
 
 

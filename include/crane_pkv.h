@@ -119,7 +119,7 @@ int crane_pkv_compact(crane_pkv* const* pkvs, int n, int64_t* moved, void* strea
  * decode step), pages that batch sequences share read once for them
  * (crane_hip_attn_shared_paged, where the arguments and results are described; the
  * groups are those of the last set_batch).  With S > 1 every sequence holds S rows or
- * more; with S = 1 one without rows gets zeros.
+ * more; with S = 1 some sequence has rows, and one without gets zeros.
  * The workspace's size follows the batch and its lengths; 0: none is needed. */
 size_t crane_pkv_shared_workspace(const crane_pkv* pkv, int Hq, int S);
 int crane_pkv_attention_shared(const crane_pkv* pkv, const void* q, int Hq, int S, float scale, int flags,

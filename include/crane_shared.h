@@ -25,13 +25,13 @@ extern "C" {
 /* Bytes of workspace crane_hip_attn_shared_paged needs for these sizes (the
  * arguments of the call); 0 where the call would be rejected or has nothing to
  * do. */
-size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups, int64_t max_kv, int64_t max_own, int64_t mean_own,
-                                       int B, int S, int Hq, int Hkv, int D, int dtype);
+size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups, int64_t max_kv, int64_t max_own,
+                                       int64_t mean_own, int B, int S, int Hq, int Hkv, int D, int dtype);
 
 /* Attention of the last S rows of every sequence over its rows of the pools, the
  * rows shared by a group read once for the group.
  *
- * q        [B, Hq, S, D] (S = 1: a decode step's [B, Hq, D])
+ * q        [B, Hq, S, D] (S = 1: a decode step's [B, Hq, D]); fewer than 2^26 rows
  * k_pool, v_pool, n_pages, page_rows, block_table, table_stride: as in
  *          crane_hip_attn_decode_paged; a page id outside [0, n_pages) reads as
  *          zero rows
@@ -53,7 +53,8 @@ size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups,
  * max_own  host-side bound of kv_len[b] - shared_rows[b]; rows past it need not be
  *          attended.  max_own + a group's rows < 2^31 - 2^14
  * mean_own about what kv_len[b] - shared_rows[b] is on average: it steers how the
- *          work is cut, nothing else (negative counts as 0)
+ *          work is cut, and whether the groups are used at all (their members' own
+ *          table rows name the same rows), nothing else (negative counts as 0)
  * flags    CRANE_HIP_PREFILL_CAUSAL: query i sees rows [0, kv_len[b] - S + i];
  *          0: every query sees all kv_len[b] rows.  A query that sees none gets
  *          zeros.  Rows a query does not see have no influence on it, whatever
@@ -72,9 +73,9 @@ size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups,
 int crane_hip_attn_shared_paged(const void* q, const void* k_pool, const void* v_pool, int64_t n_pages, int page_rows,
                                 const int32_t* block_table, int64_t table_stride, const int32_t* kv_len, int64_t max_kv,
                                 const int32_t* shared_rows, const int32_t* groups, const int32_t* members,
-                                const int32_t* groups_host, int n_groups, int64_t max_own, int64_t mean_own, int B, int S, int Hq,
-                                int Hkv, int D, float scale, int flags, void* workspace, size_t ws_bytes, void* out,
-                                int dtype, void* stream);
+                                const int32_t* groups_host, int n_groups, int64_t max_own, int64_t mean_own, int B,
+                                int S, int Hq, int Hkv, int D, float scale, int flags, void* workspace,
+                                size_t ws_bytes, void* out, int dtype, void* stream);
 
 /* The groups of a batch whose sequences name the same first pages (host only, no
  * side effects): row b of `table` (HOST, `stride` ids a row) lists pages[b] page ids.

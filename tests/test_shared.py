@@ -209,7 +209,7 @@ def shared_call(**kw):
     (dict(v=8), "E_ALIGN"), (dict(out=8), "E_ALIGN"), (dict(ws=None), "E_WORKSPACE"), (dict(ws=8), "E_WORKSPACE"),
     (dict(ws_bytes=100), "E_WORKSPACE"), (dict(B=-1), "E_INVALID"), (dict(S=-1), "E_INVALID"),
     (dict(B=65536), "E_INVALID"), (dict(B=0, n_groups=0), "OK"), (dict(S=0), "OK"),
-    (dict(S=1 << 30), "E_INVALID"),                                   # more than 2^31 query rows
+    (dict(S=1 << 30), "E_INVALID"), (dict(S=1 << 19), "E_INVALID"),    # 2^26 query rows or more
     (dict(P=1 << 28, stride=7, n_pages=1, max_kv=7 << 28, max_own=7 << 28,
           groups_host=[0, 4, 0, 7 << 28]), "E_INVALID"),
 ])
