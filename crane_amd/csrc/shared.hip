@@ -69,8 +69,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, in
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
 }
 typedef unsigned int u32x4_v __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x4_v buf_load16(__amdgpu_buffer_rsrc_t r, int off) {
-    return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+// NT: read once, streamed past the caches.
+template <bool NT = false> __device__ __forceinline__ u32x4_v buf_load16(__amdgpu_buffer_rsrc_t r, int off) {
+    return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? 2 : 0);
 }
 __device__ __forceinline__ f32x4_v mfma(u32x4_v a, u32x4_v b, f32x4_v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c,
@@ -240,19 +241,21 @@ __device__ __forceinline__ void load_k(Frag<bf16_t>& f, __amdgpu_buffer_rsrc_t r
 #pragma unroll
         for (int t = 0; t < 4; ++t) f.k[h][t] = buf_load16(r, (16 * h + i) * 256 + 64 * t + 16 * g);
 }
+template <bool NT>
 __device__ __forceinline__ void load_v(Frag<bf16_t>& f, __amdgpu_buffer_rsrc_t r, int i, int g) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = buf_load16(r, (16 * (e >> 2) + 4 * g + (e & 3)) * 256 + 16 * i);
+    for (int e = 0; e < 8; ++e) f.v[e] = buf_load16<NT>(r, (16 * (e >> 2) + 4 * g + (e & 3)) * 256 + 16 * i);
 }
 __device__ __forceinline__ void load_k(Frag<float>& f, __amdgpu_buffer_rsrc_t r, int i, int g) {
 #pragma unroll
     for (int t = 0; t < 8; ++t) f.k[t] = buf_load16(r, i * 512 + 64 * t + 16 * g);
 }
+template <bool NT>
 __device__ __forceinline__ void load_v(Frag<float>& f, __amdgpu_buffer_rsrc_t r, int i, int g) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int d = 0; d < 2; ++d) f.v[e][d] = buf_load16(r, (4 * g + e) * 512 + 256 * d + 16 * i);
+        for (int d = 0; d < 2; ++d) f.v[e][d] = buf_load16<NT>(r, (4 * g + e) * 512 + 256 * d + 16 * i);
 }
 
 // A query row's fragment: the K fragment's dims.
@@ -471,7 +474,7 @@ template <int N> __device__ __forceinline__ void mask_step(float (&s)[N], int j,
 
 // ---- the stream form: 16 RT query rows
 
-template <typename T, int RT, bool SHARED>
+template <typename T, int RT, bool NT, bool SHARED>
 __device__ __forceinline__ void attend_stream(const Args& a, StreamShared<RT>& sm, int seg, int kvh, int block,
                                               int chunk) {
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4;
@@ -510,17 +513,18 @@ __device__ __forceinline__ void attend_stream(const Args& a, StreamShared<RT>& s
         load_k(f, tile_rsrc<T>(a.k, t), i, g);
     };
     auto v_tile = [&](Frag<T>& f, const Pages::Tile& t) __attribute__((always_inline)) {
-        load_v(f, tile_rsrc<T>(a.v, t), i, g);
+        load_v<NT>(f, tile_rsrc<T>(a.v, t), i, g);
     };
-    // kAhead steps' tiles are in flight (two for 16 rows, whose registers allow it): a
-    // step's K registers are loaded again, for the step kAhead on, once its scores are
-    // taken, its V registers after its product.  A step past the end loads nothing and
-    // sees no key.
-    constexpr int kAhead = RT == 1 ? 2 : 1, kStride = kWaves * kKeys;
+    // One step's tiles are in flight: its K registers are loaded again, for the step on,
+    // once its scores are taken, its V registers after its product (two steps in flight
+    // leave 16 rows two workgroups a CU in place of three: 32 sequences of 512 to 4096 keys
+    // in chunks of 256 76 us for 70, a call of 2 short ones 8.7 for 8.4).  A step past the
+    // end loads nothing and sees no key.
+    constexpr int kStride = kWaves * kKeys;
     const int j0 = begin + wave * kKeys;
-    Frag<T> f[kAhead];
-    auto step = [&](Frag<T>& f, int j, auto move) __attribute__((always_inline)) {
-        const Pages::Tile next = tile_at(j + kAhead * kStride);
+    Frag<T> f;
+    auto step = [&](int j, auto move) __attribute__((always_inline)) {
+        const Pages::Tile next = tile_at(j + kStride);
         float s[RT][kSlots];
 #pragma unroll
         for (int t = 0; t < RT; ++t) scores(f, q[t], s[t]);
@@ -536,24 +540,18 @@ __device__ __forceinline__ void attend_stream(const Args& a, StreamShared<RT>& s
         __builtin_amdgcn_sched_barrier(0);
         v_tile(f, next);
     };
+    const Pages::Tile first = tile_at(j0);
     // In the steps' own order: the loop's first wait has to hold for both.
-#pragma unroll
-    for (int x = 0; x < kAhead; ++x) {
-        const Pages::Tile t = tile_at(j0 + x * kStride);
-        __builtin_amdgcn_sched_barrier(0);
-        k_tile(f[x], t);
-        __builtin_amdgcn_sched_barrier(0);
-        v_tile(f[x], t);
-        __builtin_amdgcn_sched_barrier(0);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    k_tile(f, first);
+    __builtin_amdgcn_sched_barrier(0);
+    v_tile(f, first);
+    __builtin_amdgcn_sched_barrier(0);
     // A row that sees any key of the wave's sees one in its first two steps: lo is less
     // than kAlign past the chunk's begin.
-    step(f[0], j0, std::true_type());
-    step(f[kAhead - 1], j0 + kStride, std::true_type());
-    for (int j = j0 + 2 * kStride; j < end; j += kAhead * kStride) {
-        step(f[0], j, std::false_type());
-        if constexpr (kAhead == 2) step(f[1], j + kStride, std::false_type());
-    }
+    step(j0, std::true_type());
+    step(j0 + kStride, std::true_type());
+    for (int j = j0 + 2 * kStride; j < end; j += kStride) step(j, std::false_type());
     bool again = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) again = again || (at[t] >= 0 && !sound(st[t]));
@@ -562,20 +560,20 @@ __device__ __forceinline__ void attend_stream(const Args& a, StreamShared<RT>& s
         for (int t = 0; t < RT; ++t) st[t].clear();
         for (int j = j0; j < end; j += kStride) {
             const Pages::Tile tile = tile_at(j);
-            k_tile(f[0], tile);
-            v_tile(f[0], tile);
+            k_tile(f, tile);
+            v_tile(f, tile);
             float s[RT][kSlots];
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                scores(f[0], q[t], s[t]);
+                scores(f, q[t], s[t]);
                 mask_step(s[t], j, g, lo, hi[t]);
                 softmax_step<true>(st[t], s[t], a.c);
             }
-            if (__any(any_nonfinite(f[0]))) {
+            if (__any(any_nonfinite(f))) {
 #pragma unroll
-                for (int t = 0; t < RT; ++t) accumulate_each(st[t], f[0], s[t], g, lo - j, hi[t] - j);
+                for (int t = 0; t < RT; ++t) accumulate_each(st[t], f, s[t], g, lo - j, hi[t] - j);
             } else {
-                accumulate(st, f[0], s);
+                accumulate(st, f, s);
             }
         }
     }
@@ -994,12 +992,17 @@ struct Item {
     }
 };
 
-// The forms of a role, by its query rows per workgroup.
-template <typename T, int ROWS, bool SHARED, class SM>
+// The forms of a role, by its query rows per workgroup.  V, whose loads take whole rows,
+// streams past the caches where one workgroup reads it: always for 16 rows (16 sequences
+// of 4000 to 8000 keys, 428 MB: 79 us for 73), and for 32 where they are all there are
+// (11 sequences in 3 groups of 11776 f32 rows: 65 for 60; groups of two blocks 27 for 30
+// the other way).  K's loads take half a line at a time and want the caches (32 sequences
+// of 200 to 1500 keys: 25 us, 29 with K streamed too).
+template <typename T, int ROWS, bool ONCE, bool SHARED, class SM>
 __device__ __forceinline__ void attend(const Args& a, SM& sm, const Item& x) {
     if constexpr (ROWS == kBlockRows) attend_block<SHARED>(a, sm.block, x.seg, x.kvh, x.block, x.chunk);
-    else if constexpr (ROWS == 32) attend_stream<T, 2, SHARED>(a, sm.stream32, x.seg, x.kvh, x.block, x.chunk);
-    else attend_stream<T, 1, SHARED>(a, sm.stream16, x.seg, x.kvh, x.block, x.chunk);
+    else if constexpr (ROWS == 32) attend_stream<T, 2, ONCE, SHARED>(a, sm.stream32, x.seg, x.kvh, x.block, x.chunk);
+    else attend_stream<T, 1, true, SHARED>(a, sm.stream16, x.seg, x.kvh, x.block, x.chunk);
 }
 
 template <int SHARED_ROWS, int OWN_ROWS> union AttnShared {
@@ -1008,16 +1011,17 @@ template <int SHARED_ROWS, int OWN_ROWS> union AttnShared {
     typename std::conditional<SHARED_ROWS == kBlockRows || OWN_ROWS == kBlockRows, BlockShared, int>::type block;
 };
 
+// ONCE: one block of rows covers a group's.
 // grid: the shared role's items, then the own role's.
-template <typename T, int SHARED_ROWS, int OWN_ROWS>
-__global__ __launch_bounds__(64 * kWaves, 2) void shared_attn_kernel(Args a) {
+template <typename T, int SHARED_ROWS, int OWN_ROWS, bool ONCE>
+__global__ __launch_bounds__(64 * kWaves, SHARED_ROWS == 16 ? 3 : 2) void shared_attn_kernel(Args a) {
     __shared__ AttnShared<SHARED_ROWS, OWN_ROWS> sm;
     if ((int)blockIdx.x < a.shared_items) {
         const Item x(blockIdx.x, a.shared_tiles, a.Hkv, a.n_groups, a.shared_splits);
-        if (x.ok) attend<T, SHARED_ROWS, true>(a, sm, x);
+        if (x.ok) attend<T, SHARED_ROWS, ONCE, true>(a, sm, x);
     } else {
         const Item x(blockIdx.x - a.shared_items, a.own_tiles, a.Hkv, a.B, a.own_splits);
-        if (x.ok) attend<T, OWN_ROWS, false>(a, sm, x);
+        if (x.ok) attend<T, OWN_ROWS, false, false>(a, sm, x);
     }
 }
 
@@ -1271,18 +1275,19 @@ template <typename T> int launch(Args& a, const Plan& p, int64_t n_rows, hipStre
     // second one in: the dispatcher otherwise pairs some and leaves CUs idle (9 sequences,
     // 5 groups of 20000 rows in chunks of 2560, bf16: 80 us for 46; 27 sequences, 5 groups
     // of 6656 rows: 33 for 26).
-#define CRANE_SHARED_CASE(s, o)                                                                              \
+#define CRANE_SHARED_CASE(s, o, once)                                                                        \
     static_assert(sizeof(AttnShared<s, o>) <= kHalfLds);                                                     \
-    if (p.shared_rows == s && p.own_rows == o)                                                               \
-        hipLaunchKernelGGL((shared_attn_kernel<T, s, o>), grid, threads,                                     \
+    if (p.shared_rows == s && p.own_rows == o && (s != 32 || o != 16 || once == (p.shared_tiles == 1)))      \
+        hipLaunchKernelGGL((shared_attn_kernel<T, s, o, once>), grid, threads,                               \
                            p.spread ? kHalfLds + 256 - sizeof(AttnShared<s, o>) : 0, st, a);
-    CRANE_SHARED_CASE(16, 16)
-    CRANE_SHARED_CASE(32, 16)
-    CRANE_SHARED_CASE(32, 32)
+    CRANE_SHARED_CASE(16, 16, true)
+    CRANE_SHARED_CASE(32, 16, true)
+    CRANE_SHARED_CASE(32, 16, false)
+    CRANE_SHARED_CASE(32, 32, false)
     if constexpr (sizeof(T) == 2) {
-        CRANE_SHARED_CASE(128, 16)
-        CRANE_SHARED_CASE(128, 32)
-        CRANE_SHARED_CASE(128, 128)
+        CRANE_SHARED_CASE(128, 16, false)
+        CRANE_SHARED_CASE(128, 32, false)
+        CRANE_SHARED_CASE(128, 128, false)
     }
 #undef CRANE_SHARED_CASE
     int rc = launch_status(hipGetLastError());
