@@ -536,6 +536,9 @@ def _on_device(dev: torch.device, call, args) -> int:
         return call(*args)
 
 
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
+
+
 def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
                            kv_len: torch.Tensor, max_kv: int, groups: PrefixGroups, scale: Optional[float] = None,
                            causal: bool = True, max_own: Optional[int] = None, mean_own: Optional[int] = None,
@@ -549,12 +552,16 @@ def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
 
     The shared rows are read once per group.  Scores and softmax stay in f32, where
     attention_decode_paged rounds every score as candle does."""
-    dev = _dev(q, k_pool, v_pool, block_table, kv_len, groups.shared_rows, workspace)
-    if q.dim() not in (3, 4) or q.shape[-1] != HEAD_DIM:
-        raise CraneHipError(_lib.E_HEAD_DIM if q.dim() in (3, 4) else _lib.E_INVALID,
+    index = q.get_device()
+    if index < 0 or not (k_pool.get_device() == v_pool.get_device() == block_table.get_device() ==
+                         kv_len.get_device() == groups.shared_rows.get_device() == index):
+        _dev(q, k_pool, v_pool, block_table, kv_len, groups.shared_rows)
+    shape = q.shape
+    if len(shape) not in (3, 4) or shape[-1] != HEAD_DIM:
+        raise CraneHipError(_lib.E_HEAD_DIM if len(shape) in (3, 4) else _lib.E_INVALID,
                             "q must be [B, Hq, 128] or [B, Hq, S, 128]")
-    B, Hq = q.shape[:2]
-    S = q.shape[2] if q.dim() == 4 else 1
+    B, Hq = shape[0], shape[1]
+    S = shape[2] if len(shape) == 4 else 1
     n_pages, Hkv, page_rows, stride = _paged_args(k_pool, v_pool, block_table, B, q.dtype)
     _contig(q, "q")
     dt = _dtype_code(q)
@@ -565,19 +572,22 @@ def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
         max_own = max(max_kv - groups.min_shared, 0)
     if mean_own is None:  # the longest sequence is likely one that shares most
         mean_own = 6 * max(max_kv - groups.max_shared, 0) // 10
-    scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
-    lib = _lib.lib()
+    lib, dev = _lib.lib(), q.device
     need = lib.crane_hip_attn_shared_workspace(groups.groups_host, groups.n_groups, max_kv, max_own, mean_own, B, S, Hq,
                                                Hkv, HEAD_DIM, dt)
     # Allocated per call, not kept per stream: a captured graph keeps its own.
-    if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    out = torch.empty((B, S, Hq * HEAD_DIM), dtype=q.dtype, device=dev)
+    if workspace is not None:
+        _dev(q, workspace)
+        ws_bytes = workspace.numel() * workspace.element_size()
+    elif need:
+        workspace, ws_bytes = torch.empty(need, dtype=torch.uint8, device=dev), need
+    else:
+        ws_bytes = 0
+    out = q.new_empty((B, S, Hq * HEAD_DIM))
     args = (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), n_pages, page_rows, block_table.data_ptr(), stride,
             kv_len.data_ptr(), max_kv, groups.shared_rows.data_ptr(), groups.groups.data_ptr(),
             groups.members.data_ptr(), groups.groups_host, groups.n_groups, max_own, mean_own, B, S, Hq, Hkv, HEAD_DIM,
-            scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace),
-            workspace.numel() * workspace.element_size() if workspace is not None else 0,
+            _SCALE if scale is None else scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace), ws_bytes,
             out.data_ptr(), dt, _stream(dev))
     rc = _on_device(dev, lib.crane_hip_attn_shared_paged, args)
     check(rc, "attention_shared_paged")
