@@ -11,6 +11,7 @@ fallback.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 from typing import Optional, Sequence
@@ -620,14 +621,18 @@ def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
                 raise CraneHipError(_lib.E_DTYPE, f"pool dtypes {p.dtype} and {dtype}")
         raise CraneHipError(_lib.E_INVALID, "pools must have one shape")
     n_pages, Hkv, page_rows, _ = shape
-    for ids, most in ((src, n_pages - 1), (dst, n_pages - 1), (rows or (), page_rows)):
-        if len(ids) and not 0 <= min(ids) <= max(ids) <= most:
-            raise CraneHipError(_lib.E_INVALID, f"{n_pages} pages of {page_rows} rows: {list(ids)}")
-    ints = lambda x: (ctypes.c_int32 * len(x))(*x)  # noqa: E731
+    try:
+        lists = [array.array("i", x) for x in ((src, dst) if rows is None else (src, dst, rows))]
+    except OverflowError:
+        raise CraneHipError(_lib.E_INVALID, f"pages or rows past 32 bits: {src}, {dst}, {rows}") from None
+    n = len(src)
+    if any([len(x) != n for x in lists]):  # bytes, which an array takes four at a time
+        raise CraneHipError(_lib.E_INVALID, "src, dst and rows must be sequences of integers")
+    at = [x.buffer_info()[0] for x in lists]
     ptrs = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
     rc = _on_device(dev, _lib.lib().crane_hip_copy_pages, (
-        ptrs, len(pools), n_pages, page_rows, Hkv, HEAD_DIM, ints(src), ints(dst),
-        ints(rows) if rows is not None else None, len(src), _dtype_code(first), _stream(dev)))
+        ptrs, len(pools), n_pages, page_rows, Hkv, HEAD_DIM, at[0], at[1], at[2] if rows is not None else None, n,
+        _dtype_code_of(dtype), _stream(dev)))
     check(rc, "copy_pages")
 
 

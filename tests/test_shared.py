@@ -768,7 +768,8 @@ def test_copy_pages_python_refusals(gpu):
     a = torch.zeros((4, 2, 256, D), device=gpu)
     for args in (([a, a[:3]], [0], [1]), ([a, a.bfloat16()], [0], [1]), ([a], [0, 1], [2]), ([a], [0], [4]),
                  ([a], [1 << 32], [1]), ([a], [0], [1], [257]), ([a], [0], [1], [1, 2]), ([a], [0, 0], [1, 1]),
-                 ([a.transpose(1, 2)], [0], [1]), ([a[..., :64].contiguous()], [0], [1])):
+                 ([a.transpose(1, 2)], [0], [1]), ([a[..., :64].contiguous()], [0], [1]),
+                 ([a], bytes(4), bytes([1, 0, 0, 0]))):
         with pytest.raises(CraneHipError):
             ops.copy_pages(*args)
     ops.copy_pages([], [0], [1])
