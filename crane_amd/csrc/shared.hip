@@ -985,7 +985,7 @@ __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int
 // one after the other, and reads their keys through its own L2.  Where a whole number of
 // eights makes one chunk of all segments, a segment's chunks would all run on the same
 // XCDs: the segments take turns then (8 sequences at 2 kv heads, one of 30720 keys, the
-// others of 7: 37 us for 21); with heads in eights every segment is on all XCDs anyway.
+// others of 7: 37 us for 19); with heads in eights every segment is on all XCDs anyway.
 struct Item {
     int block, kvh, seg, chunk;
     bool ok;
