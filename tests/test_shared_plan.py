@@ -1,0 +1,83 @@
+"""How the attention over shared pages is cut (crane_amd/csrc/shared_plan.h, compiled for
+the host alone): the order of a role's workgroups."""
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "crane_amd", "csrc")
+SOURCE = """
+#include "shared_plan.h"
+using namespace crane;
+extern "C" void plan(const int32_t* groups, int n_groups, int64_t max_kv, int64_t max_own, int64_t mean_own, int B,
+                     int S, int Hq, int Hkv, int bf16, int64_t* out) {
+    const Plan p = plan_for(Sizes{groups, n_groups, max_kv, max_own, mean_own, B, S, Hq, Hkv, bf16 != 0});
+    const int64_t r[] = {p.share, p.shared_rows, p.own_rows, p.shared_tiles, p.own_tiles, p.chunk,
+                         p.shared_splits, p.own_splits, p.shared_items, p.own_items};
+    std::copy(r, r + 10, out);
+}
+// Every item of a role: {block, kv head, segment, chunk}, or -1 for none.
+extern "C" void items(int n, int blocks, int Hkv, int segs, int chunks, int32_t* out) {
+    for (int x = 0; x < n; ++x) {
+        const Item i(x, blocks, Hkv, segs, chunks);
+        const int32_t r[] = {i.block, i.kvh, i.seg, i.chunk};
+        for (int e = 0; e < 4; ++e) out[4 * x + e] = i.ok ? r[e] : -1;
+    }
+}
+"""
+FIELDS = ("share", "shared_rows", "own_rows", "shared_tiles", "own_tiles", "chunk", "shared_splits", "own_splits",
+          "shared_items", "own_items")
+_i, _i64 = ctypes.c_int, ctypes.c_int64
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    """The header behind two C functions."""
+    at = tmp_path_factory.mktemp("shared_plan")
+    src, lib = at / "plan.cpp", at / "plan.so"
+    src.write_text(SOURCE)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined",
+                    "-fno-sanitize-recover=undefined", "-shared", "-fPIC", "-D__host__=", "-D__device__=",
+                    "-D__forceinline__=inline", "-I", CSRC, str(src), "-o", str(lib)], check=True)
+    L = ctypes.CDLL(str(lib))
+    L.plan.argtypes = [ctypes.POINTER(ctypes.c_int32), _i, _i64, _i64, _i64, _i, _i, _i, _i, _i, ctypes.POINTER(_i64)]
+    L.items.argtypes = [_i] * 5 + [ctypes.c_void_p]
+    L.plan.restype = L.items.restype = None
+    return L
+
+
+def plan(host, groups, max_kv, max_own, mean_own, B, S, Hq, Hkv, bf16):
+    """The plan of groups [(members, rows)]."""
+    desc, at = [], 0
+    for n, rows in groups:
+        desc += [at, n, at, rows]
+        at += n
+    out = (_i64 * len(FIELDS))()
+    host.plan((ctypes.c_int32 * max(len(desc), 1))(*desc), len(groups), max_kv, max_own, mean_own, B, S, Hq, Hkv, bf16,
+              out)
+    return dict(zip(FIELDS, out))
+
+
+def items(host, blocks, Hkv, segs, chunks):
+    n = 8 * blocks * -(-segs * Hkv * chunks // 8)
+    out = np.zeros((n, 4), np.int32)
+    host.items(n, blocks, Hkv, segs, chunks, out.ctypes.data)
+    return out
+
+
+@pytest.mark.parametrize("blocks", [1, 2, 7])
+@pytest.mark.parametrize("Hkv", [1, 2, 3, 4, 8, 16])
+def test_items_are_each_unit_once(host, Hkv, blocks):
+    """Every (block, kv head, segment, chunk) is one workgroup's, and a unit's blocks are
+    on one XCD (workgroups go to the 8 XCDs in turn)."""
+    for segs in (1, 2, 3, 4, 5, 8, 12, 31):
+        for chunks in (1, 2, 5, 16):
+            got = items(host, blocks, Hkv, segs, chunks)
+            some = got[:, 0] >= 0
+            place = np.ravel_multi_index(got[some].T, (blocks, Hkv, segs, chunks))
+            assert sorted(place) == list(range(blocks * Hkv * segs * chunks))
+            unit, xcd = place % (Hkv * segs * chunks), np.flatnonzero(some) % 8
+            order = np.argsort(unit, kind="stable")
+            assert (xcd[order].reshape(-1, blocks) == xcd[order][::blocks, None]).all()
