@@ -144,11 +144,12 @@ inline double plan_cost(const Sizes& z, Plan& p) {
     return t;
 }
 
-// Cuts the roles' keys into chunks; own chunk 0 starts on a multiple of kAlign.
+// Cuts the roles' keys into chunks; own chunk 0 starts on a multiple of kAlign, and is
+// there without keys, too: its workgroups write the zeros of rows that see none.
 inline void cut(const Sizes& z, int chunk, Plan* p) {
     p->chunk = chunk;
     p->shared_splits = p->share ? ceil_div(p->max_shared, chunk) : 0;
-    p->own_splits = ceil_div(z.longest(*p) + (p->share ? kAlign : 0), chunk);
+    p->own_splits = std::max<int64_t>(1, ceil_div(z.longest(*p) + (p->share ? kAlign : 0), chunk));
     p->shared_items = 8 * p->shared_tiles * ceil_div(z.n_groups * z.Hkv * p->shared_splits, 8);
     p->own_items = 8 * p->own_tiles * ceil_div((int64_t)z.B * z.Hkv * p->own_splits, 8);
 }

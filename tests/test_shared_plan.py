@@ -81,3 +81,40 @@ def test_items_are_each_unit_once(host, Hkv, blocks):
             unit, xcd = place % (Hkv * segs * chunks), np.flatnonzero(some) % 8
             order = np.argsort(unit, kind="stable")
             assert (xcd[order].reshape(-1, blocks) == xcd[order][::blocks, None]).all()
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("S", [1, 40, 300])
+@pytest.mark.parametrize("groups", [[], [(2, 0)], [(3, 0), (1, 0)]])
+def test_no_keys_are_one_chunk(host, groups, S, bf16):
+    """Where the bounds leave no key, the own role's workgroups still write the zeros."""
+    p = plan(host, groups, 256, 0, 0, 4, S, 8, 2, bf16)
+    assert (p["shared_splits"], p["own_splits"], p["shared_items"]) == (0, 1, 0)
+    assert p["own_items"] == 8 * p["own_tiles"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("groups,rows", [([], []), ([[0, 2]], [0])])
+@pytest.mark.parametrize("S", [1, 40, 300])
+def test_sequences_without_rows_get_zeros(gpu, S, groups, rows, dtype):
+    """kv_len 0 everywhere with the tight bound max_own = 0."""
+    import torch
+    from crane_amd import _lib, ops
+    B, Hq, Hkv, P = 4, 8, 2, 256
+    td = torch.bfloat16 if dtype == "bf16" else torch.float32
+    k = torch.full((3, Hkv, P, 128), float("nan"), dtype=td, device=gpu)
+    q = torch.ones((B, Hq, S, 128), dtype=td, device=gpu)
+    table = torch.zeros((B, 2), dtype=torch.int32, device=gpu)
+    n = torch.zeros(B, dtype=torch.int32, device=gpu)
+    g = ops.prefix_groups(groups, rows, B, gpu)
+    for causal in (True, False):
+        got = ops.attention_shared_paged(q, k, k, table, n, P, g, causal=causal, max_own=0)
+        assert got.shape == (B, S, Hq * 128) and (got == 0).all()
+        out = torch.full((B, S, Hq * 128), float("nan"), dtype=td, device=gpu)   # and every element is written
+        rc = _lib.lib().crane_hip_attn_shared_paged(
+            q.data_ptr(), k.data_ptr(), k.data_ptr(), 3, P, table.data_ptr(), 2, n.data_ptr(), P,
+            g.shared_rows.data_ptr(), g.groups.data_ptr(), g.members.data_ptr(), g.groups_host, g.n_groups, 0, 0,
+            B, S, Hq, Hkv, 128, 0.1, int(causal), None, 0, out.data_ptr(), int(dtype == "bf16"),
+            torch.cuda.current_stream(gpu).cuda_stream)
+        assert rc == _lib.OK and (out == 0).all()
