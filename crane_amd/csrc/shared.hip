@@ -85,7 +85,7 @@ struct Args {
     void* out;
     PagedRows rows;
     const int32_t *kv_len, *shared, *groups, *members;
-    int n_groups, max_group, max_shared;
+    int n_groups, n_members, max_group, max_shared;
     int B, S, Hq, Hkv, G;     // G = Hq / Hkv heads per kv head
     int max_kv, causal;
     float c;                  // scale log2 e
@@ -119,12 +119,12 @@ template <bool SHARED> struct Segment {
     __device__ __forceinline__ Segment(const Args& args, int seg) : a(args), R(args.S * args.G) {
         if constexpr (SHARED) {
             const int4 d = reinterpret_cast<const int4*>(a.groups)[seg];
-            first = min(max(d.x, 0), a.B);
-            const int members = min(max(d.y, 0), min(a.max_group, a.B - first));
+            const Members of(d.x, d.y, a.n_members, a.max_group);
+            first = of.first;
             table_row = d.z;
             lo = 0;
             hi = min(d.w, a.max_shared);
-            n_rows = table_row < 0 || table_row >= a.B ? 0 : members * R;
+            n_rows = table_row < 0 || table_row >= a.B ? 0 : of.n * R;
         } else {
             first = 0;
             table_row = seg;
@@ -1221,6 +1221,7 @@ extern "C" int crane_hip_attn_shared_paged(const void* q, const void* k_pool, co
     a.groups = groups;
     a.members = members;
     a.n_groups = n_groups;
+    a.n_members = p.members;
     a.max_group = p.max_group;
     a.max_shared = p.max_shared;
     a.B = B;

@@ -42,6 +42,17 @@ struct Item {
     }
 };
 
+// A group's members as the device describes them, in the array whose entries the host's
+// groups account for: never past those, nor more of them than the launch has rows for.
+struct Members {
+    int first, n;
+    __host__ __device__ __forceinline__ Members(int first_place, int count, int entries, int max_group) {
+        first = first_place < 0 ? 0 : first_place < entries ? first_place : entries;
+        const int most = max_group < entries - first ? max_group : entries - first;
+        n = count < 0 ? 0 : count < most ? count : most;
+    }
+};
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // How a call is cut: whether sharing is used, and the forms (query rows per workgroup),
@@ -49,6 +60,7 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct Plan {
     bool share;
     int max_group, max_shared;
+    int members;  // entries of the members array the groups account for
     int shared_rows, own_rows;
     int64_t shared_tiles, own_tiles;
     int chunk;
@@ -159,10 +171,11 @@ constexpr int kChunks[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 32, 48, 64};
 
 inline Plan plan_for(const Sizes& z) {
     Plan p, best;
-    p.max_group = p.max_shared = 0;
+    p.max_group = p.max_shared = p.members = 0;
     for (int g = 0; g < z.n_groups; ++g) {
         p.max_group = std::max(p.max_group, (int)z.groups[4 * g + 1]);
         p.max_shared = std::max(p.max_shared, (int)z.groups[4 * g + 3]);
+        p.members = std::max(p.members, (int)(z.groups[4 * g] + z.groups[4 * g + 1]));
     }
     const int64_t M = p.max_group * z.R();
     p.own_rows = form_rows(z.R(), z.bf16);

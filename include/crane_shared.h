@@ -46,7 +46,8 @@ size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups,
  *          shared rows is in exactly one group, whose r is its shared_rows; other
  *          sequences are in none.  A description that breaks this gives unspecified
  *          results for the sequences concerned and stays in bounds
- * members  int32, device, B entries at most
+ * members  int32, device, B entries at most: as many as groups_host accounts for (the
+ *          largest s + n of its groups); no entry past those is read
  * groups_host the same n_groups descriptions on the HOST, read before the call
  *          returns: they steer how the work is cut and bound what the device's may
  *          say (CRANE_HIP_E_INVALID for members or rows outside the batch)

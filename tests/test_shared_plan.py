@@ -18,6 +18,14 @@ extern "C" void plan(const int32_t* groups, int n_groups, int64_t max_kv, int64_
                          p.shared_splits, p.own_splits, p.shared_items, p.own_items};
     std::copy(r, r + 10, out);
 }
+// A device group's {first place, members} as the kernel takes them; the entries and the
+// largest group of the host's groups.
+extern "C" void members(const int32_t* groups, int n_groups, int B, int first, int count, int32_t* out) {
+    const Plan p = plan_for(Sizes{groups, n_groups, 1024, 512, 100, B, 1, 8, 2, true});
+    const Members m(first, count, p.members, p.max_group);
+    const int32_t r[] = {m.first, m.n, p.members, p.max_group};
+    std::copy(r, r + 4, out);
+}
 // Every item of a role: {block, kv head, segment, chunk}, or -1 for none.
 extern "C" void items(int n, int blocks, int Hkv, int segs, int chunks, int32_t* out) {
     for (int x = 0; x < n; ++x) {
@@ -44,7 +52,8 @@ def host(tmp_path_factory):
     L = ctypes.CDLL(str(lib))
     L.plan.argtypes = [ctypes.POINTER(ctypes.c_int32), _i, _i64, _i64, _i64, _i, _i, _i, _i, _i, ctypes.POINTER(_i64)]
     L.items.argtypes = [_i] * 5 + [ctypes.c_void_p]
-    L.plan.restype = L.items.restype = None
+    L.members.argtypes = [ctypes.POINTER(ctypes.c_int32), _i, _i, _i, _i, ctypes.POINTER(ctypes.c_int32)]
+    L.plan.restype = L.items.restype = L.members.restype = None
     return L
 
 
@@ -81,6 +90,23 @@ def test_items_are_each_unit_once(host, Hkv, blocks):
             unit, xcd = place % (Hkv * segs * chunks), np.flatnonzero(some) % 8
             order = np.argsort(unit, kind="stable")
             assert (xcd[order].reshape(-1, blocks) == xcd[order][::blocks, None]).all()
+
+
+@pytest.mark.parametrize("host_groups,entries", [([(0, 2)], 2), ([(0, 2), (2, 5)], 7), ([(38, 3)], 41), ([(4, 0)], 4)])
+def test_device_groups_stay_in_the_members_array(host, host_groups, entries):
+    """Whatever a device group says, only entries that the host's groups account for are
+    read: those of a batch of 41 with fewer members, too."""
+    desc = (ctypes.c_int32 * (4 * len(host_groups)))(*[x for s, n in host_groups for x in (s, n, 0, 256)])
+    out = (ctypes.c_int32 * 4)()
+    edges = (-2 ** 31, -50, -1, 0, 1, 2, 3, 6, 7, 8, 38, 40, 41, 42, 1 << 30, 2 ** 31 - 1)
+    for first in edges:
+        for count in edges:
+            host.members(desc, len(host_groups), 41, first, count, out)
+            at, n, total, most = out
+            assert (total, most) == (entries, max(c for _, c in host_groups))
+            assert 0 <= at and 0 <= n <= most and at + n <= entries
+            if 0 <= first and 0 <= count <= most and first + count <= entries:
+                assert (at, n) == (first, count)      # what is consistent is taken as it is
 
 
 @pytest.mark.parametrize("bf16", [0, 1])
