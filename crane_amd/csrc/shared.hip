@@ -1108,7 +1108,7 @@ bool make_plan(const Sizes& z, Plan* p) {
     } else {
         *p = kept.p;
     }
-    return p->shared_items + p->own_items <= kMostThreads / (64 * kWaves);
+    return p->fits;
 }
 
 template <typename T> int launch(Args& a, const Plan& p, int64_t n_rows, hipStream_t st) {

@@ -66,6 +66,7 @@ struct Plan {
     int chunk;
     int64_t shared_splits, own_splits, shared_items, own_items;
     bool spread;  // one workgroup per CU
+    bool fits;    // a grid; else no cut's workgroups do, and nothing but the groups' bounds is set
     size_t ml_off, total;  // of the workspace
 };
 
@@ -170,13 +171,13 @@ inline void cut(const Sizes& z, int chunk, Plan* p) {
 constexpr int kChunks[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 32, 48, 64};
 
 inline Plan plan_for(const Sizes& z) {
-    Plan p, best;
-    p.max_group = p.max_shared = p.members = 0;
+    Plan p{}, best;
     for (int g = 0; g < z.n_groups; ++g) {
         p.max_group = std::max(p.max_group, (int)z.groups[4 * g + 1]);
         p.max_shared = std::max(p.max_shared, (int)z.groups[4 * g + 3]);
         p.members = std::max(p.members, (int)(z.groups[4 * g] + z.groups[4 * g + 1]));
     }
+    best = p;
     const int64_t M = p.max_group * z.R();
     p.own_rows = form_rows(z.R(), z.bf16);
     p.own_tiles = ceil_div(z.R(), p.own_rows);
@@ -189,6 +190,8 @@ inline Plan plan_for(const Sizes& z) {
         p.shared_tiles = share ? ceil_div(M, p.shared_rows) : 0;
         for (int k : kChunks) {
             cut(z, kMinChunk * k, &p);
+            p.fits = p.shared_items + p.own_items <= kMostThreads / (64 * kWaves);
+            if (!p.fits) continue;
             const double t = plan_cost(z, p);
             if (!(t >= least)) {
                 least = t;

@@ -65,6 +65,10 @@ size_t crane_hip_attn_shared_workspace(const int32_t* groups_host, int n_groups,
  *          share one.  May be NULL when that is 0
  * out      [B, S, Hq*D]
  *
+ * CRANE_HIP_E_INVALID also where no cut of the work, into at least 128 and at most 8192
+ * keys a workgroup, fits a grid of fewer than 2^24 workgroups (about 16 to 128 query rows
+ * of a kv head each, every sequence counted with max_own keys).
+ *
  * The scores, their softmax and all sums are f32 and only the probabilities (bf16
  * calls) are rounded before the product with V: candle's rounding of every score
  * to the model dtype, which crane_hip_attn_decode reproduces, is not part of this

@@ -15,8 +15,8 @@ extern "C" void plan(const int32_t* groups, int n_groups, int64_t max_kv, int64_
                      int S, int Hq, int Hkv, int bf16, int64_t* out) {
     const Plan p = plan_for(Sizes{groups, n_groups, max_kv, max_own, mean_own, B, S, Hq, Hkv, bf16 != 0});
     const int64_t r[] = {p.share, p.shared_rows, p.own_rows, p.shared_tiles, p.own_tiles, p.chunk,
-                         p.shared_splits, p.own_splits, p.shared_items, p.own_items};
-    std::copy(r, r + 10, out);
+                         p.shared_splits, p.own_splits, p.shared_items, p.own_items, p.fits};
+    std::copy(r, r + 11, out);
 }
 // A device group's {first place, members} as the kernel takes them; the entries and the
 // largest group of the host's groups.
@@ -36,7 +36,7 @@ extern "C" void items(int n, int blocks, int Hkv, int segs, int chunks, int32_t*
 }
 """
 FIELDS = ("share", "shared_rows", "own_rows", "shared_tiles", "own_tiles", "chunk", "shared_splits", "own_splits",
-          "shared_items", "own_items")
+          "shared_items", "own_items", "fits")
 _i, _i64 = ctypes.c_int, ctypes.c_int64
 
 
@@ -117,6 +117,21 @@ def test_no_keys_are_one_chunk(host, groups, S, bf16):
     p = plan(host, groups, 256, 0, 0, 4, S, 8, 2, bf16)
     assert (p["shared_splits"], p["own_splits"], p["shared_items"]) == (0, 1, 0)
     assert p["own_items"] == 8 * p["own_tiles"]
+
+
+@pytest.mark.parametrize("groups,max_own,B,Hq,Hkv,bf16,share", [
+    ([(1, 446_000_000)] + [(1, 61_000_000)] * 75 + [(73, 61_000_000)], 29_000, 149, 16, 2, 1, 0),
+                                                                # sharing is cheaper, not sharing fits
+    ([(60, 100_000)] + [(1, 30_000)] * 7, 3_500_000, 67, 16, 4, 1, 1),         # what is chosen fits
+    ([], 45_000, 65535, 64, 64, 1, None),                                     # nothing does
+    ([(268, 2_000_000)], 300_000_000, 268, 8, 2, 0, None),
+])
+def test_a_cut_that_fits_the_grid_is_taken(host, groups, max_own, B, Hq, Hkv, bf16, share):
+    """A grid has fewer than 2^32 threads: cuts into more workgroups are passed over."""
+    p = plan(host, groups, max_own + max((r for _, r in groups), default=0), max_own, max_own, B, 1, Hq, Hkv, bf16)
+    assert bool(p["fits"]) == (share is not None)
+    if share is not None:
+        assert p["share"] == share and p["shared_items"] + p["own_items"] <= (2 ** 32 - 1) // 256
 
 
 @pytest.mark.gpu
