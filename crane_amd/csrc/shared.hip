@@ -85,7 +85,7 @@ struct Args {
     void* out;
     PagedRows rows;
     const int32_t *kv_len, *shared, *groups, *members;
-    int n_groups, n_members, max_group, max_shared;
+    int n_groups, n_members, max_shared;
     int B, S, Hq, Hkv, G;     // G = Hq / Hkv heads per kv head
     int max_kv, causal;
     float c;                  // scale log2 e
@@ -119,7 +119,7 @@ template <bool SHARED> struct Segment {
     __device__ __forceinline__ Segment(const Args& args, int seg) : a(args), R(args.S * args.G) {
         if constexpr (SHARED) {
             const int4 d = reinterpret_cast<const int4*>(a.groups)[seg];
-            const Members of(d.x, d.y, a.n_members, a.max_group);
+            const Members of(d.x, d.y, a.n_members);
             first = of.first;
             table_row = d.z;
             lo = 0;
@@ -1222,7 +1222,6 @@ extern "C" int crane_hip_attn_shared_paged(const void* q, const void* k_pool, co
     a.members = members;
     a.n_groups = n_groups;
     a.n_members = p.members;
-    a.max_group = p.max_group;
     a.max_shared = p.max_shared;
     a.B = B;
     a.S = S;

@@ -43,13 +43,13 @@ struct Item {
 };
 
 // A group's members as the device describes them, in the array whose entries the host's
-// groups account for: never past those, nor more of them than the launch has rows for.
+// groups account for: never past those.  (More of them than the host's largest group are
+// past the row blocks that are launched.)
 struct Members {
     int first, n;
-    __host__ __device__ __forceinline__ Members(int first_place, int count, int entries, int max_group) {
-        first = first_place < 0 ? 0 : first_place < entries ? first_place : entries;
-        const int most = max_group < entries - first ? max_group : entries - first;
-        n = count < 0 ? 0 : count < most ? count : most;
+    __host__ __device__ __forceinline__ Members(int first_place, int count, int entries) {
+        first = std::min(std::max(first_place, 0), entries);
+        n = std::min(std::max(count, 0), entries - first);
     }
 };
 

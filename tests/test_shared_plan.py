@@ -18,13 +18,13 @@ extern "C" void plan(const int32_t* groups, int n_groups, int64_t max_kv, int64_
                          p.shared_splits, p.own_splits, p.shared_items, p.own_items, p.fits};
     std::copy(r, r + 11, out);
 }
-// A device group's {first place, members} as the kernel takes them; the entries and the
-// largest group of the host's groups.
+// A device group's {first place, members} as the kernel takes them, and the entries of
+// the host's groups.
 extern "C" void members(const int32_t* groups, int n_groups, int B, int first, int count, int32_t* out) {
     const Plan p = plan_for(Sizes{groups, n_groups, 1024, 512, 100, B, 1, 8, 2, true});
-    const Members m(first, count, p.members, p.max_group);
-    const int32_t r[] = {m.first, m.n, p.members, p.max_group};
-    std::copy(r, r + 4, out);
+    const Members m(first, count, p.members);
+    const int32_t r[] = {m.first, m.n, p.members};
+    std::copy(r, r + 3, out);
 }
 // Every item of a role: {block, kv head, segment, chunk}, or -1 for none.
 extern "C" void items(int n, int blocks, int Hkv, int segs, int chunks, int32_t* out) {
@@ -97,15 +97,15 @@ def test_device_groups_stay_in_the_members_array(host, host_groups, entries):
     """Whatever a device group says, only entries that the host's groups account for are
     read: those of a batch of 41 with fewer members, too."""
     desc = (ctypes.c_int32 * (4 * len(host_groups)))(*[x for s, n in host_groups for x in (s, n, 0, 256)])
-    out = (ctypes.c_int32 * 4)()
+    out = (ctypes.c_int32 * 3)()
     edges = (-2 ** 31, -50, -1, 0, 1, 2, 3, 6, 7, 8, 38, 40, 41, 42, 1 << 30, 2 ** 31 - 1)
     for first in edges:
         for count in edges:
             host.members(desc, len(host_groups), 41, first, count, out)
-            at, n, total, most = out
-            assert (total, most) == (entries, max(c for _, c in host_groups))
-            assert 0 <= at and 0 <= n <= most and at + n <= entries
-            if 0 <= first and 0 <= count <= most and first + count <= entries:
+            at, n, total = out
+            assert total == entries
+            assert 0 <= at and 0 <= n and at + n <= entries
+            if 0 <= first and 0 <= count and first + count <= entries:
                 assert (at, n) == (first, count)      # what is consistent is taken as it is
 
 
