@@ -40,7 +40,11 @@
 // kMostSum or o is not finite.  That is so after a row's scores rose by 2^60 (41 in
 // natural units) over its first keys, or where V holds an infinity or a NaN, even in a
 // key the row does not see (0 x inf).  Then the walk is repeated with m moved at every
-// step and such keys added to the rows that see them only.
+// step and such keys added to the rows that see them only.  So it is where m itself is past
+// kMostMax: s scale log2 e - m is one product with one rounding, which leaves every weight of
+// the row the factor exp2(the rounding of m); o / l takes that out again, but it overflows or
+// vanishes once half a step of m passes a hundred.  The repeated walk keeps the maximum as
+// the scores are, too, and takes (s - max) scale log2 e for such rows, 0 for the largest.
 //
 // Measured (both kernels, HIP graph): 2 sequences, 512 shared rows, 16 / 8 heads 8.3 us;
 // 32 sequences of 32 / 8 heads and 200 to 1500 rows behind 4096 33 us, 140 MB; 64 behind
@@ -62,6 +66,7 @@ namespace {
 
 constexpr float kNoMax = -FLT_MAX; // m before the first key (finite: exp2(-inf - m) is 0, not NaN)
 constexpr float kMostSum = 0x1p60f;  // see above
+constexpr float kMostMax = 0x1p26f;  // see above: half a step of m is 2 at most
 constexpr size_t kHalfLds = 81920;   // half of a CU's LDS
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, int bytes) {
@@ -371,6 +376,47 @@ __device__ __forceinline__ void softmax_step(Row<T>& st, float (&s)[N], float c)
     st.l += sum;
 }
 
+// The largest score so far as it is and as an m (finite; of no score: none), and p's
+// exponent for rows of any m.
+struct Largest {
+    float raw = kNoMax, m = kNoMax;
+    bool big = true;
+    // Takes a step's largest score; o's and l's factor.
+    __device__ __forceinline__ float move(float score, float c) {
+        const float r = fmaxf(raw, score), x = fminf(fmaxf(r * c, kNoMax), FLT_MAX);
+        big = fabsf(x) > kMostMax;
+        const float a = fast_exp2(big ? (raw - r) * c : m - x);
+        raw = r;
+        m = x;
+        return a;
+    }
+    __device__ __forceinline__ float exponent(float s, float c) const {
+        return big ? (s - raw) * c : __builtin_fmaf(s, c, -m);
+    }
+};
+
+// softmax_step<true> for rows of any m.
+template <typename T, int N>
+__device__ __forceinline__ void softmax_step(Row<T>& st, Largest& top, float (&s)[N], float c) {
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) mx = fmaxf(mx, s[e]);
+    const float a = top.move(groups_max(mx), c);
+    st.m = top.m;
+    st.l *= a;
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st.o[n][r] *= a;
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        s[e] = fast_exp2(top.exponent(s[e], c));
+        sum += s[e];
+    }
+    st.l += sum;
+}
+
 // Sum over the four lane groups; every lane gets it.
 __device__ __forceinline__ float groups_sum(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -453,8 +499,11 @@ __device__ __forceinline__ void accumulate_each(Row<float>& st, const Frag<float
 }
 
 // Whether a walk that did not move m came out well (a row without keys did).
+__device__ __forceinline__ bool sound_sums(float l, float m) {
+    return (l <= kMostSum) & ((fabsf(m) <= kMostMax) | (m == kNoMax));
+}
 template <typename T> __device__ __forceinline__ bool sound(const Row<T>& st) {
-    bool ok = st.l <= kMostSum;
+    bool ok = sound_sums(st.l, st.m);
 #pragma unroll
     for (int n = 0; n < 8; ++n)
 #pragma unroll
@@ -557,6 +606,7 @@ __device__ __forceinline__ void attend_stream(const Args& a, StreamShared<RT>& s
     if (__any(again)) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) st[t].clear();
+        Largest top[RT];
         for (int j = j0; j < end; j += kStride) {
             const Pages::Tile tile = tile_at(j);
             k_tile(f, tile);
@@ -566,7 +616,7 @@ __device__ __forceinline__ void attend_stream(const Args& a, StreamShared<RT>& s
             for (int t = 0; t < RT; ++t) {
                 scores(f, q[t], s[t]);
                 mask_step(s[t], j, g, lo, hi[t]);
-                softmax_step<true>(st[t], s[t], a.c);
+                softmax_step(st[t], top[t], s[t], a.c);
             }
             if (__any(any_nonfinite(f))) {
 #pragma unroll
@@ -727,7 +777,7 @@ struct BlockWave {
         for (int t = 0; t < 8; ++t) q[t] = reinterpret_cast<const u32x4_v*>(row)[2 * t + h];
     }
     __device__ __forceinline__ bool sound() const {
-        bool ok = l <= kMostSum;
+        bool ok = sound_sums(l, m);
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -761,24 +811,24 @@ struct BlockWave {
                 s[b][r] = key >= lo && key < hi ? s[b][r] : -INFINITY;
             }
     }
-    // The largest of m and a row's scores.
-    __device__ __forceinline__ float largest(const f32x16_v (&s)[2], float c) const {
+    // A row's largest score.
+    __device__ __forceinline__ float largest(const f32x16_v (&s)[2]) const {
         float mx = s[0][0];
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-        return fmaxf(m, halves_max(mx) * c);
+        return halves_max(mx);
     }
-    // p = exp2(s c - m), rounded and paired: p[t] is the B operand of keys 16 t ..; l.
-    __device__ __forceinline__ void weights(const f32x16_v (&s)[2], u32x4_v (&p)[4], float c) {
+    // p = exp2(exponent of s), rounded and paired: p[t] is the B operand of keys 16 t ..; l.
+    template <class EXPONENT>
+    __device__ __forceinline__ void weights(const f32x16_v (&s)[2], u32x4_v (&p)[4], EXPONENT exponent) {
         float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                const float x = fast_exp2(__builtin_fmaf(s[b][r], c, -m));
-                const float y = fast_exp2(__builtin_fmaf(s[b][r + 1], c, -m));
+                const float x = fast_exp2(exponent(s[b][r])), y = fast_exp2(exponent(s[b][r + 1]));
                 sum += x + y;
                 p[2 * b + (r >> 3)][(r & 7) >> 1] = pack_bf16x2(x, y);
             }
@@ -900,7 +950,7 @@ __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int
         if (j < lo || j + kKeys > min_hi) w.mask(s, j, lo, hi);
         u32x4_v p[4];
         if constexpr (decltype(more)::value) w.scores(next, ((t + 1) & 1) * kTileBytes);
-        w.weights(s, p, a.c);
+        w.weights(s, p, [&](float x) __attribute__((always_inline)) { return __builtin_fmaf(x, a.c, -w.m); });
         w.accumulate(p, (t & 1) * kTileBytes);
         BlockWave::schedule(more);
     };
@@ -914,7 +964,7 @@ __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int
         w.scores(sa, 0);
         // A row that sees any key of the chunk sees one in its first tile.
         w.mask(sa, begin, lo, hi);
-        w.m = w.largest(sa, a.c);
+        w.m = fmaxf(w.m, w.largest(sa) * a.c);
     }
     int t = 0;
     for (; t + 2 < n; t += 2) {
@@ -927,6 +977,7 @@ __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int
     __syncthreads();
     if (sm.again[0] | sm.again[1] | sm.again[2] | sm.again[3]) {
         w.clear();
+        Largest top;
         for (t = 0; t < n; ++t) {
             __syncthreads();
             issue_k(t);
@@ -937,15 +988,15 @@ __device__ __forceinline__ void attend_block(const Args& a, BlockShared& sm, int
             const int j = begin + t * kKeys;
             w.scores(sa, buf);
             w.mask(sa, j, lo, hi);
-            const float m = w.largest(sa, a.c), x = fast_exp2(w.m - m);
-            w.m = m;
+            const float x = top.move(w.largest(sa), a.c);
+            w.m = top.m;
             w.l *= x;
 #pragma unroll
             for (int d = 0; d < 4; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) w.o[d][r] *= x;
             u32x4_v p[4];
-            w.weights(sa, p, a.c);
+            w.weights(sa, p, [&](float x) __attribute__((always_inline)) { return top.exponent(x, a.c); });
             if (tile_nonfinite(sm.v[t & 1], lane)) w.accumulate_each(p, buf, j, lo, hi);
             else w.accumulate(p, buf);
         }
