@@ -251,3 +251,73 @@ def test_replays_of_several_tokens_that_share(gpu, dtype, S):
         torch.cuda.synchronize(gpu)
         for _, out in graphs:
             assert torch.equal(out, want), step
+
+
+# ------------------------------------------------------------------ the manager
+
+def manager_lens(step):
+    """Lengths of the batch of test_manager_batches_that_share: 24 forks of a prompt of
+    3000 rows (11 pages shared), 9 of another of 2304 (9 pages), one alone, in this order."""
+    return [3000 + step + b % 3 for b in range(24)] + [2304 + step + b % 2 for b in range(9)] + [70 + step]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_manager_batches_share(host, dtype):  # noqa: F811
+    for step, S in ((1, 1), (4, 3)):
+        lens = manager_lens(step)
+        own = [n - (11 * 256 if b < 24 else 9 * 256 if b < 33 else 0) for b, n in enumerate(lens)]
+        p = plan(host, [(24, 11 * 256), (9, 9 * 256)], max(lens), max(own), sum(own) // len(own), len(lens), S, 8, 2,
+                 dtype == "bf16")
+        assert p["share"], (step, S, p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_manager_batches_that_share(gpu, dtype):
+    """Two forked prompts and a sequence of its own in one batch, in a shuffled order:
+    the cache's own groups steer calls that share, of one and of three tokens, before and
+    after a compaction that moves the shared pages."""
+    import torch
+    from crane_amd import kv
+    td = torch.bfloat16 if dtype == "bf16" else torch.float32
+    r = cases.rng(930)
+    Hkv, Hq, P = 2, 8, 256
+    c = kv.PagedKvCache(Hkv, 140, td, P, max_seqs=40, max_pages_per_seq=16, device=gpu)
+    rand = lambda *shape: ts.tens(cases.normal(r, shape), dtype, gpu)
+    filler = c.add_sequence()
+    c.write_sequence(filler, rand(Hkv, 2000, D), rand(Hkv, 2000, D))
+    ids = []
+    for n, count in ((3000, 24), (2304, 9)):
+        sid = c.add_sequence()
+        c.write_sequence(sid, rand(Hkv, n, D), rand(Hkv, n, D))
+        ids += [sid] + c.fork_sequence(sid, count - 1)
+    ids.append(c.add_sequence())
+    c.write_sequence(ids[-1], rand(Hkv, 70, D), rand(Hkv, 70, D))
+    start = manager_lens(0)
+    for b, sid in enumerate(ids):                                # lengths apart by up to 2 rows
+        extra = start[b] - c.seq_len(sid)
+        if extra:
+            c.set_batch([sid])
+            c.update_kv_cache(rand(1, Hkv, extra, D), rand(1, Hkv, extra, D))
+    order = [int(x) for x in r.permutation(len(ids))]
+    batch = [ids[x] for x in order]
+    c.set_batch(batch)
+    step = 0
+    for S, compacted in ((1, False), (3, False), (1, True), (3, True)):
+        if compacted and S == 1:
+            c.free_sequence(filler)
+            assert c.compact() > 0                               # the batch and its table follow
+        c.update_kv_cache(rand(len(ids), Hkv, S, D), rand(len(ids), Hkv, S, D))
+        step += S
+        assert c.lengths == [manager_lens(step)[x] for x in order]
+        q = cases.cast(cases.normal(r, (len(ids), Hq, S, D)), dtype)
+        qq = ts.tens(q, dtype, gpu)
+        got = c.attention_shared(qq if S > 1 else qq.view(len(ids), Hq, D))
+        for x in (0, 7, 23, 24, 32, 33):
+            b = order.index(x)
+            kk, vv = (y.float().cpu().numpy() for y in c.read_sequence(batch[b]))
+            n = kk.shape[1]
+            out, mag, most = ts.reference(q[b:b + 1], kk[None], vv[None], np.zeros((1, 1), np.int32), [n], n,
+                                          D ** -0.5, True)
+            check(got[b:b + 1], out, ts.bounds(out, mag, most, n, dtype))
+    c.close()
