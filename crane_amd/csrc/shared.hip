@@ -1134,9 +1134,10 @@ void size_workspace(const Sizes& z, Plan* p) {
     p->total = slots > 1 ? p->ml_off + (size_t)z.rows() * slots * sizeof(float2) : 0;
 }
 
-// The plan for these sizes.  A thread's last one is kept, by the sizes' values (up to 256
-// groups): the workspace query, the call and the next layers' calls all ask for the same
-// (1 group: 3.1 us to make, 0.1 to find).
+// The plan for these sizes.  A thread's last one is kept, by the sizes' values: the
+// workspace query, the call and the next layers' calls all ask for the same (1 group: 3.1 us
+// to make, 0.1 to find).  Up to 256 groups, which bounds what a thread holds: past them
+// every question makes it (257 groups: 44 us, 512: 84, where 256 take 3 to compare).
 bool make_plan(const Sizes& z, Plan* p) {
     constexpr int kKept = 256;
     struct Kept {

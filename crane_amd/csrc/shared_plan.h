@@ -22,10 +22,12 @@ constexpr int kBlockRows = 128;    // query rows of a workgroup's block form
 
 // A role's item x of `units` (segment, kv head, chunk) units with `blocks` row blocks
 // each: ids that are equal mod 8 run on one XCD, which so gets the blocks of a unit,
-// one after the other, and reads their keys through its own L2.  Where a whole number of
-// eights makes one chunk of all segments, a segment's chunks would all run on the same
-// XCDs: the segments take turns then (8 sequences at 2 kv heads, one of 30720 keys, the
-// others of 7: 37 us for 19); with heads in eights every segment is on all XCDs anyway.
+// one after the other, and reads their keys through its own L2.  A segment's chunks are
+// segs Hkv units apart: on 8 / gcd(8, segs Hkv) XCDs for each kv head, up to all 8.  Where
+// that is a multiple of 8 they would stay on the XCDs of the heads, and the segments take
+// turns (8 sequences at 2 kv heads, one of 30720 keys, the others of 7: 37 us for 19);
+// with heads in eights every segment is on all XCDs anyway.  Where it is a multiple of 2 or
+// 4 only, they do not: 2 sequences at 2 kv heads are on 4 XCDs each, 4 at one head on 2.
 struct Item {
     int block, kvh, seg, chunk;
     bool ok;

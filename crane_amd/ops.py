@@ -549,7 +549,9 @@ def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
     [B, 1, Hq*D], q [B, Hq, S, D] gives [B, S, Hq*D].  kv_len counts the S new rows;
     with causal query i sees the rows up to its own, else all kv_len.  max_own:
     host-side bound of kv_len - shared rows (default: what max_kv leaves); mean_own:
-    about its average, which steers how the work is cut (default: a guess).
+    about its average, which steers how the work is cut (default: a guess).  Where the
+    host knows the lengths, both can be passed: over 67 calls of random sizes the true
+    values take 1.8% less time, single calls between 28% less and 39% more.
 
     The shared rows are read once per group.  Scores and softmax stay in f32, where
     attention_decode_paged rounds every score as candle does."""
@@ -571,7 +573,11 @@ def attention_shared_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
         raise CraneHipError(_lib.E_INVALID, f"groups of a batch of {groups.batch}, q of {B}")
     if max_own is None:
         max_own = max(max_kv - groups.min_shared, 0)
-    if mean_own is None:  # the longest sequence is likely one that shares most
+    if mean_own is None:
+        # The longest sequence is likely one that shares most; of what it has besides, 0.6.
+        # Over 67 calls of random sizes: 0.3 takes 2.3% more time (decode_groups, 27 sequences
+        # behind 5 prompts: 32.5 us for 25.9), all of it 0.1% more (a batch of 32 behind 4096
+        # rows: 39.0 for 33.2), the true mean 0.9% less.
         mean_own = 6 * max(max_kv - groups.max_shared, 0) // 10
     lib, dev = _lib.lib(), q.device
     need = lib.crane_hip_attn_shared_workspace(groups.groups_host, groups.n_groups, max_kv, max_own, mean_own, B, S, Hq,
