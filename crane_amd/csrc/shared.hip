@@ -46,7 +46,7 @@
 // vanishes once half a step of m passes a hundred.  The repeated walk keeps the maximum as
 // the scores are, too, and takes (s - max) scale log2 e for such rows, 0 for the largest.
 //
-// Measured (both kernels, HIP graph): 2 sequences, 512 shared rows, 16 / 8 heads 8.3 us;
+// Measured (both kernels, HIP graph): 2 sequences, 512 shared rows, 16 / 8 heads 8.7 us;
 // 32 sequences of 32 / 8 heads and 200 to 1500 rows behind 4096 33 us, 140 MB; 64 behind
 // 32768 rows 98 us, 69 GFLOP (0.83 PFLOP/s in the block form, bound by MFMAs and
 // exponentials in turn); 32 sequences of 200 to 1500 rows that share nothing 25 us, 119 MB
