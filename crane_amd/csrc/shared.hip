@@ -376,8 +376,8 @@ __device__ __forceinline__ void softmax_step(Row<T>& st, float (&s)[N], float c)
     st.l += sum;
 }
 
-// The largest score so far as it is and as an m (finite; of no score: none), and p's
-// exponent for rows of any m.
+// The largest score so far as it is and as an m (finite; of no score: no larger than any
+// score's), and p's exponent for rows of any m.
 struct Largest {
     float raw = kNoMax, m = kNoMax;
     bool big = true;
