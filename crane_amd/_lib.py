@@ -3,7 +3,8 @@
 layer's row kernels), include/crane_gemm.h (the QKV / o_proj projections), include/crane_sampling.h
 (argmax, top-k), include/crane_few.h (a decode step's projections at one
 sequence), include/crane_shared.h (attention over pages that sequences share,
-page copies), include/crane_kv.h (host-side KV-cache manager) and
+page copies), include/crane_f8.h (the paged cache in 8 bits),
+include/crane_kv.h (host-side KV-cache manager) and
 include/crane_pkv.h (paged KV-cache manager).
 
 The library is the only compute path: there is no CPU fallback.  Loading
@@ -110,6 +111,16 @@ SIGNATURES = {
          _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp, _i, _vp], _i),
     "crane_hip_group_prefixes": ([_i32p, _i64, _i32p, _i, _i32p, _i32p, _i32p, _ip], _i),
     "crane_hip_copy_pages": ([_vpp, _i, _i64, _i, _i, _i, _i32p, _i32p, _i32p, _i, _i, _vp], _i),
+    # include/crane_f8.h
+    "crane_hip_qknorm_rope_append_paged_f8": (
+        [_vp, _i64, _vp, _vp, _f, _i, _vp, _vp, _i64, _i64, _i32p, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i32p, _i64,
+         _i32p, _i, _i, _i, _i, _i, _i, _vp], _i),
+    "crane_hip_attn_paged_f8_workspace": ([_i64, _i, _i, _i, _i, _i, _i], _sz),
+    "crane_hip_attn_paged_f8": (
+        [_vp, _vp, _vp, _vp, _vp, _i64, _i, _i32p, _i64, _i32p, _i64, _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp, _i,
+         _vp], _i),
+    "crane_hip_read_paged_f8": (
+        [_vp, _vp, _vp, _vp, _i64, _i, _i32p, _i64, _i32p, _i64, _i, _i, _i, _vp, _vp, _i, _vp], _i),
     # include/crane_pkv.h
     "crane_pkv_create": ([_i, _i, _i, _i, _i64, _i, _i, _vpp], _i),
     "crane_pkv_destroy": ([_vp], None),

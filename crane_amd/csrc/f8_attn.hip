@@ -1,0 +1,664 @@
+// f8_attn.hip -- attention over the paged KV cache in 8 bits (gfx950); the C ABI and the
+// cache's format are include/crane_f8.h's.
+//
+// Query i of sequence b sees rows [0, L), L = kv_len[b] - S + 1 + i (causal) or kv_len[b].
+// With s_j = scale q . k_j over any set of keys,
+//     m = max s_j,  l = sum exp(s_j - m),  o = sum exp(s_j - m) v_j,
+// and disjoint sets join as o = sum w o' / sum w l', w = exp(m' - max m).  The rows of a
+// workgroup are (query, head of the GQA group) of one sequence and kv head, which share
+// every key they read.
+//
+// A code times its power-of-two scale has 4 significant bits, so bf16 holds it exactly,
+// and one v_cvt_scalef32_pk_bf16_fp8 makes two of them, scale included.  The products run
+// on bf16 MFMAs, whose sums are f32's: 8-bit MFMAs would take K and V as they are at twice
+// the rate, but q and the probabilities would need two 8-bit parts each (the same time),
+// and they align the products of a sum to its largest and cut them at about 2^-13 of
+// it (measured: 64 products of mixed magnitudes off by up to 2^-12 of the largest, bf16
+// 2^-22).  bf16 calls round the probabilities to bf16; f32 calls split q and the
+// probabilities into three bf16 parts, 24 bits in all, and take three products.
+#include <float.h>
+
+#include <algorithm>
+
+#include "f8.h"
+#include "shared_plan.h"
+
+namespace crane {
+namespace {
+
+constexpr float kNoMax = -FLT_MAX;  // m before the first key (finite: exp2(-inf - m) is 0, not NaN)
+constexpr int kTile = 64;           // keys of a tile: two blocks, within one page
+constexpr int kRow = kHeadDim;      // bytes of a row of codes
+constexpr int kTileBytes = kTile * kRow;
+
+typedef unsigned int u32x4_v __attribute__((ext_vector_type(4)));
+
+struct Args8 {
+    const void* q;
+    const uint8_t *k, *v, *k_scale, *v_scale;
+    void* out;
+    PagedRows rows;
+    const int32_t* kv_len;
+    int B, S, Hq, Hkv, G;  // G = Hq / Hkv heads per kv head
+    int max_kv, causal;
+    float c;               // scale log2 e
+    int chunk, splits, tiles;  // keys per chunk, chunks, row tiles per (sequence, kv head)
+    float* ws_o;           // [B Hq S, splits, D], unnormalised
+    float2* ws_ml;         // [B Hq S, splits] (m, l)
+    __device__ __forceinline__ int len(int b) const { return max(0, min(kv_len[b], max_kv)); }
+    // Rows query s of a sequence of n rows sees.
+    __device__ __forceinline__ int limit(int n, int s) const { return causal ? n - S + 1 + s : n; }
+    // The row of out [B, S, Hq] that is row `at` of q [B, Hq, S].
+    __device__ __forceinline__ int64_t out_row(int at) const {
+        if (S == 1) return at;
+        const int bh = at / S, s = at - bh * S, b = bh / Hq;
+        return ((int64_t)b * S + s) * Hq + (bh - b * Hq);
+    }
+};
+
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// A chunk's pages, one id per lane: those from the chunk's first on, or the whole table
+// row where it fits (then the load waits for nothing).
+struct Pages8 {
+    int ids, page0, P;
+    __device__ __forceinline__ Pages8(const Args8& a, int b, int begin, int lane) : ids(-1), P(a.rows.page_rows) {
+        page0 = a.rows.stride <= 64 ? 0 : begin / P;
+        if (page0 + lane < a.rows.stride) ids = a.rows.table[(int64_t)b * a.rows.stride + page0 + lane];
+    }
+    // The tile of keys [j, j + 64) of a kv head: its offset in a pool, the bytes of its rows
+    // before `end` (0 for a page outside the pool: its rows read as zero), and the byte
+    // of its first block's scale.
+    struct Tile {
+        int64_t off;
+        int bytes;
+    };
+    __device__ __forceinline__ Tile tile(const Args8& a, int kvh, int j, int end) const {
+        const int p = j / P;
+        const int id = __builtin_amdgcn_readlane(ids, (p - page0) & 63);
+        const bool ok = (unsigned)id < (unsigned)a.rows.n_pages;
+        const int rows = ok ? max(0, min(kTile, end - j)) : 0;
+        const int64_t off = (((int64_t)(ok ? id : 0) * a.Hkv + kvh) * P + (j - p * P)) * kRow;
+        return Tile{uniform(off), __builtin_amdgcn_readfirstlane(rows * kRow)};
+    }
+};
+
+// The scales of a tile's two blocks, as f32 (read through the constant address space: one
+// scalar load).  A byte of a block without rows may be anything; 254 keeps 0 times it 0.
+struct Scales {
+    float of[2];
+    __device__ __forceinline__ void load(const uint8_t* pool, int64_t tile_off) {
+        const int64_t at = tile_off / (kRow * kBlockRows8);  // even
+        typedef const __attribute__((address_space(4))) uint32_t* words_t;
+        const uint32_t w = ((words_t)(uintptr_t)pool)[at >> 2] >> (8 * (at & 2));
+        of[0] = scale_of(min(w & 255u, 254u));
+        of[1] = scale_of(min((w >> 8) & 255u, 254u));
+    }
+};
+
+// Eight codes to bf16, times a scale.
+__device__ __forceinline__ u32x4_v widen(uint32_t lo, uint32_t hi, float scale) {
+    u32x4_v r;
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    return r;
+}
+// Not 0 where one of four codes is a NaN.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+__device__ __forceinline__ f32x4_v mfma(u32x4_v a, u32x4_v b, f32x4_v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c,
+                                                   0, 0, 0);
+}
+
+// Eight values as an MFMA operand: bf16 calls round them once, f32 calls carry them in
+// three parts, each the rounding of what the ones before leave.
+template <typename T> struct Parts;
+template <> struct Parts<bf16_t> {
+    static constexpr int kN = 1;
+    u32x4_v part[1];
+    __device__ __forceinline__ void set(const float* x) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) part[0][w] = pack_bf16x2(x[2 * w], x[2 * w + 1]);
+    }
+    __device__ __forceinline__ void load(const bf16_t* p) { part[0] = *reinterpret_cast<const u32x4_v*>(p); }
+};
+template <> struct Parts<float> {
+    static constexpr int kN = 3;
+    u32x4_v part[3];  // the smallest last
+    __device__ __forceinline__ void set(const float* x) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            float a = x[2 * w], b = x[2 * w + 1];
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+                const uint32_t u = pack_bf16x2(a, b);
+                part[n][w] = u;
+                // an infinity leaves a NaN, which the products would make of it anyway
+                a -= bf16_lo(u);
+                b -= bf16_hi(u);
+            }
+        }
+    }
+    __device__ __forceinline__ void load(const float* p) {
+        float x[8];
+        load8(p, x);
+        set(x);
+    }
+};
+// c += a b, the smallest parts first.
+template <typename T, typename C> __device__ __forceinline__ C product(u32x4_v a, const Parts<T>& b, C c) {
+#pragma unroll
+    for (int n = Parts<T>::kN - 1; n >= 0; --n) c = mfma(a, b.part[n], c);
+    return c;
+}
+
+// Maximum and sum over the four lane groups of a query row; every lane gets them.  (A row
+// swap of a value with itself leaves each row's value in one result and its neighbour's
+// in the other.)
+__device__ __forceinline__ float groups_max(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+    const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+__device__ __forceinline__ float groups_sum(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
+
+// LDS byte addresses, and reads at them.
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
+}
+__device__ __forceinline__ u32x4_v lds_read16(uint32_t at) {
+    return *(const __attribute__((address_space(3))) u32x4_v*)(uintptr_t)at;
+}
+typedef int i32x2_v __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2_v lds_i32x2_v;
+// Within 16 lanes, lane x gets column x of the 8 rows x 16 columns of bytes that the lanes
+// point at (lane x: 8 columns from 8 (x % 2) on of row x / 2).
+__device__ __forceinline__ uint2 lds_read_tr8(uint32_t at) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_v*)(uintptr_t)at));
+}
+
+// Wait for the wave's vector memory (or LDS) operations; the other counters at their
+// maxima.
+__device__ __forceinline__ void wait_memory() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
+// ---- the stream form: 16 RT query rows a wave, every wave walking tiles of its own
+//
+// A wave copies its next tile of K and V (8 KiB each) into LDS of its own while it works
+// on the one in its registers: the copies are asynchronous, take whole 128-byte rows, and
+// hold no registers, which the reads could not do for the layouts the products want.
+// LDS keeps the rows (128 bytes, half a sweep of the banks) with their 16-byte chunks
+// XOR-permuted by f(row) below, so that neither the 16 rows of a K read nor the 16 rows of
+// two lane groups' transposed V reads meet in a bank.
+//
+// v_mfma_f32_16x16x32_bf16, S^T = K Q^T with K rows as A: lane (i, g) = (lane % 16, lane /
+// 16) holds, for query row i, rows 4 g + r of the product.  A's row x of product (u, b) is
+// key 32 u + 8 (x / 4) + 4 b + x % 4, so that over b the lane holds keys 32 u + 8 g + (0 ..
+// 7): as P^T, the B operand of O^T = V^T P^T as they stand, with V's bytes of those keys
+// from one transposed read.
+
+// The chunk permutation of a tile's row.
+__device__ __forceinline__ int permute8(int row) {
+    return ((row >> 1) & 1) | ((row >> 2) & 2) | ((((row >> 4) ^ (row >> 2)) & 1) << 2);
+}
+
+template <typename T, int RT> struct Stream {
+    const int lane, i, g;
+    uint32_t k_lds, v_lds;  // the wave's tiles in LDS
+    int from[4];            // byte of a tile that instruction x (mod 4) copies for this lane
+    uint32_t k_at, v_at;    // where this lane's reads start
+    u32x4_v k[4][2];        // [2 u + b][half]: the key's dims 64 half + 16 g ..
+    uint2 v[2][8];          // [u][n]: keys 32 u + 8 g .. of dim 16 n + i
+    Scales ks, vs;
+    Parts<T> q[RT][4];      // dims 16 g .., 16 g + 8 .., 64 + 16 g .., 64 + 16 g + 8 ..
+    f32x4_v o[RT][8];       // dims 16 n + 4 g + r of row i
+    float m[RT], l[RT];     // l: over the lane's own keys
+
+    __device__ __forceinline__ Stream(int ln, uint8_t* lds) : lane(ln), i(ln & 15), g(ln >> 4) {
+        k_lds = lds_at(lds);
+        v_lds = k_lds + kTileBytes;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int row = 8 * x + (lane >> 3);
+            from[x] = row * kRow + 16 * ((lane & 7) ^ permute8(row));
+        }
+        const int k_row = 8 * (i >> 2) + (i & 3);
+        k_at = k_lds + k_row * kRow + 16 * (g ^ permute8(k_row));
+        const int v_row = 8 * g + (i >> 1);
+        v_at = v_lds + v_row * kRow + 16 * permute8(v_row) + 8 * (i & 1);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[t][n][r] = 0.f;
+            m[t] = kNoMax;
+            l[t] = 0.f;
+        }
+    }
+    // Start the copies of a tile.
+    __device__ __forceinline__ void copy(const Args8& a, const Pages8::Tile& t, uint8_t* lds) const {
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.k) + t.off, (short)0, t.bytes, 0x00020000);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.v) + t.off, (short)0, t.bytes, 0x00020000);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lds + 1024 * x, 16, from[x & 3] + 4096 * (x >> 2), 0, 0, 2);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, lds + kTileBytes + 1024 * x, 16, from[x & 3] + 4096 * (x >> 2),
+                                                     0, 0, 2);
+    }
+    // The copied tile into registers.
+    __device__ __forceinline__ void take() {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)  // rows 4 on and chunks 4 on: bit 2 of the chunk flips
+                    k[2 * u + b][half] = lds_read16((k_at ^ ((b ^ half) << 6)) + 32 * u * kRow + 4 * b * kRow);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) v[u][n] = lds_read_tr8((v_at ^ (16 * n)) + 32 * u * kRow);
+        }
+    }
+    // s[t][8 u + e]: the raw score of key 32 u + 8 g + e.
+    __device__ __forceinline__ void scores(float (&s)[RT][16]) const {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+            f32x4_v acc[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[t][r] = 0.f;
+#pragma unroll
+            for (int step = 0; step < 4; ++step) {
+                const u32x4_v& w = k[kt][step >> 1];
+                const u32x4_v x = widen(w[2 * (step & 1)], w[2 * (step & 1) + 1], ks.of[kt >> 1]);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[t] = product(x, q[t][step], acc[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[t][4 * kt + r] = acc[t][r];
+        }
+    }
+    // Weights p = exp2((s - m) c) in place of the scores.  m moves, and o and l are scaled,
+    // only where a score passes it by kSlack (as a power of two): f32 and bf16 hold larger
+    // weights as exactly.  m is kept as a raw score, so that a product with c that has no
+    // bits left below 1 costs nothing.
+    static constexpr float kSlack = 16.f;
+    __device__ __forceinline__ void weights(float (&s)[RT][16], float c) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            float mx = s[t][0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
+            if (__any((mx - m[t]) * c > kSlack)) {
+                const float to = fmaxf(m[t], groups_max(mx)), f = fast_exp2((m[t] - to) * c);
+                m[t] = to;
+                l[t] *= f;
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[t][n][r] *= f;
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[t][e] = fast_exp2((s[t][e] - m[t]) * c);
+                sum += s[t][e];
+            }
+            l[t] += sum;
+        }
+    }
+    __device__ __forceinline__ void accumulate(const float (&p)[RT][16]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            Parts<T> w[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) w[t].set(&p[t][8 * u]);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const u32x4_v x = widen(v[u][n].x, v[u][n].y, vs.of[u]);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) o[t][n] = product(x, w[t], o[t][n]);
+            }
+        }
+    }
+    // Where V holds NaN codes and some rows do not see their keys, 0 times them would reach those
+    // rows: the codes become 0, and the dims that held one become NaN for the rows that see
+    // the first such key, key j + 32 u + 8 g + e those with a limit past it.
+    __device__ __forceinline__ void settle_nan(int j, const int (&hi)[RT]) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) bad |= nan_codes(v[u][n].x) | nan_codes(v[u][n].y);
+        if (!__any(bad != 0)) return;
+        constexpr int kNone = 0x7fffffff;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            int first = kNone;  // of dim 16 n + i
+#pragma unroll
+            for (int u = 1; u >= 0; --u) {
+                const uint32_t x = nan_codes(v[u][n].x), y = nan_codes(v[u][n].y);
+                const int key = j + 32 * u + 8 * g;
+                if (y) first = key + 4 + (__builtin_ctz(y) >> 3);
+                if (x) first = key + (__builtin_ctz(x) >> 3);
+                v[u][n].x &= ~((x >> 7) * 255u);
+                v[u][n].y &= ~((y >> 7) * 255u);
+            }
+            first = min(first, __shfl_xor(first, 16));
+            first = min(first, __shfl_xor(first, 32));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int f = __shfl(first, 4 * g + r);
+#pragma unroll
+                for (int t = 0; t < RT; ++t) o[t][n][r] = f < hi[t] ? __builtin_nanf("") : o[t][n][r];
+            }
+        }
+    }
+};
+
+// The LDS of a workgroup of W waves: their tiles, then (W > 1) their results.
+template <int RT, int W> union StreamLds {
+    static constexpr int kStride = kHeadDim + 4;  // f32 per row: 16 rows at one column hit different banks
+    __attribute__((aligned(1024))) uint8_t tile[W][2 * kTileBytes];
+    struct {
+        float o[W > 1 ? W : 1][16 * RT][W > 1 ? kStride : 1];
+        float m[W][16 * RT], l[W][16 * RT];
+    } join;
+};
+
+template <typename T, int RT, int W>
+__global__ __launch_bounds__(64 * W, RT == 1 ? 2 : 1) void f8_stream_kernel(Args8 a) {
+    __shared__ StreamLds<RT, W> sm;
+    const Item x(blockIdx.x, a.tiles, a.Hkv, a.B, a.splits);
+    if (!x.ok) return;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int b = x.seg, R = a.S * a.G, row0 = x.block * 16 * RT, begin = x.chunk * a.chunk;
+    const int n = a.len(b);
+    // What the tile's first and last queries see; the last sees most.
+    const int last = (min(row0 + 16 * RT, R) - 1) / a.G;
+    const int min_hi = a.limit(n, row0 / a.G);
+    const int end = min(begin + a.chunk, a.limit(n, last));
+    const bool direct = a.splits == 1;
+    if (begin >= end && !direct) return;  // the join reads no chunk past a row's keys
+
+    const Pages8 pages(a, b, begin, lane);
+    Stream<T, RT> st(lane, sm.tile[wave]);
+    int at[RT], hi[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int r = row0 + 16 * t + st.i, s = min(r, R - 1) / a.G, h = min(r, R - 1) - s * a.G;
+        at[t] = r < R ? (int)(((int64_t)b * a.Hq + x.kvh * a.G + h) * a.S + s) : -1;  // fewer than 2^31 query rows
+        hi[t] = min(a.limit(n, s), end);
+        const T* row = reinterpret_cast<const T*>(a.q) + (int64_t)max(at[t], 0) * kHeadDim;
+#pragma unroll
+        for (int step = 0; step < 4; ++step) st.q[t][step].load(row + 64 * (step >> 1) + 16 * st.g + 8 * (step & 1));
+    }
+    constexpr int kStride = W * kTile;
+    int j = begin + wave * kTile;
+    if (j < end) {
+        Pages8::Tile tile = pages.tile(a, x.kvh, j, end);
+        st.copy(a, tile, sm.tile[wave]);
+        for (; j < end; j += kStride) {
+            st.ks.load(a.k_scale, tile.off);
+            st.vs.load(a.v_scale, tile.off);
+            wait_memory();
+            __builtin_amdgcn_sched_barrier(0);
+            st.take();
+            if (j + kStride < end) {
+                tile = pages.tile(a, x.kvh, j + kStride, end);
+                wait_lds();  // the tile is in registers: its LDS is free
+                __builtin_amdgcn_sched_barrier(0);
+                st.copy(a, tile, sm.tile[wave]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            float s[RT][16];
+            st.scores(s);
+            const bool masked = j + kTile > min(min_hi, end);
+            if (masked) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        s[t][e] = j + 32 * (e >> 3) + 8 * st.g + (e & 7) < hi[t] ? s[t][e] : -INFINITY;
+            }
+            st.weights(s, a.c);
+            if (masked && min_hi < end) st.settle_nan(j, hi);
+            st.accumulate(s);
+        }
+    }
+
+    T* out = reinterpret_cast<T*>(a.out);
+    if constexpr (W == 1) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const float l = groups_sum(st.l[t]);
+            if (at[t] < 0) continue;
+            const int64_t slot = (int64_t)at[t] * a.splits + x.chunk;
+            T* to = out + a.out_row(at[t]) * kHeadDim + 4 * st.g;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                float y[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = !direct ? st.o[t][d][r] : hi[t] <= 0 ? 0.f : st.o[t][d][r] / l;
+                if (direct) store4(to + 16 * d, y);
+                else store4(a.ws_o + slot * kHeadDim + 16 * d + 4 * st.g, y);
+            }
+            if (!direct && st.g == 0) a.ws_ml[slot] = make_float2(st.m[t], l);
+        }
+    } else {
+        __syncthreads();  // every wave's tiles are read
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const float l = groups_sum(st.l[t]);
+            if (st.g == 0) {
+                sm.join.m[wave][16 * t + st.i] = st.m[t];
+                sm.join.l[wave][16 * t + st.i] = l;
+            }
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                float y[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = st.o[t][d][r];
+                store4(&sm.join.o[wave][16 * t + st.i][16 * d + 4 * st.g], y);
+            }
+        }
+        __syncthreads();
+        // 16 threads per row, 8 dims each.
+        for (int r = tid >> 4; r < 16 * RT && row0 + r < R; r += 4 * W) {
+            const int s = (row0 + r) / a.G, h = row0 + r - s * a.G, d = 8 * (tid & 15);
+            const int place = (int)(((int64_t)b * a.Hq + x.kvh * a.G + h) * a.S + s);
+            float top = sm.join.m[0][r];
+#pragma unroll
+            for (int w = 1; w < W; ++w) top = fmaxf(top, sm.join.m[w][r]);
+            float l = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float f = fast_exp2((sm.join.m[w][r] - top) * a.c);
+                float z[8];
+                load8(&sm.join.o[w][r][d], z);
+                l += f * sm.join.l[w][r];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] += f * z[e];
+            }
+            if (direct) {
+                const bool none = min(a.limit(n, s), end) <= 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = none ? 0.f : y[e] / l;
+                store8(out + a.out_row(place) * kHeadDim + d, y);
+            } else {
+                const int64_t slot = (int64_t)place * a.splits + x.chunk;
+                store8(a.ws_o + slot * kHeadDim + d, y);
+                if (d == 0) a.ws_ml[slot] = make_float2(top, l);
+            }
+        }
+    }
+}
+
+// Join a query row's chunks: P waves per row, lane x owns dims 2 x, 2 x + 1, wave p takes
+// chunks p, p + P, ...
+template <typename T, int P>
+__global__ __launch_bounds__(P == 1 ? 256 : 64 * P) void f8_join_kernel(Args8 a, int n_rows) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = P == 1 ? 0 : wave;
+    const int row = P == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    if (row >= n_rows) return;  // P > 1: the whole workgroup
+    const int bh = row / a.S, s = row - bh * a.S, b = bh / a.Hq;
+    const int keys = a.limit(a.len(b), s);
+    const int n = keys > 0 ? (keys + a.chunk - 1) / a.chunk : 0;
+    const float2* ml = a.ws_ml + (int64_t)row * a.splits;
+    const float2* o = reinterpret_cast<const float2*>(a.ws_o + (int64_t)row * a.splits * kHeadDim) + lane;
+    float top = kNoMax;
+    for (int c = lane; c < n; c += 64) top = fmaxf(top, ml[c].x);
+    top = wave_max(top);
+    float den = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int c0 = 0; c0 < n; c0 += 64) {
+        const float2 t = c0 + lane < n ? ml[c0 + lane] : make_float2(kNoMax, 0.f);
+        const float w = c0 + lane < n ? fast_exp2((t.x - top) * a.c) : 0.f;
+        den += w * t.y;
+        for (int c = c0 + p; c < min(n, c0 + 64); c += P) {
+            const float wc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), c - c0));
+            const float2 y = o[(int64_t)c * (kHeadDim / 2)];
+            x0 += wc * y.x;
+            x1 += wc * y.y;
+        }
+    }
+    den = wave_sum(den);
+    if constexpr (P > 1) {
+        __shared__ float2 part[P - 1][64];
+        if (p > 0) part[p - 1][lane] = make_float2(x0, x1);
+        __syncthreads();
+        if (p > 0) return;
+#pragma unroll
+        for (int i = 0; i < P - 1; ++i) {
+            x0 += part[i][lane].x;
+            x1 += part[i][lane].y;
+        }
+    }
+    T* out = reinterpret_cast<T*>(a.out) + a.out_row(row) * kHeadDim + 2 * lane;
+    Elem<T>::store(out, n == 0 ? 0.f : x0 / den);
+    Elem<T>::store(out + 1, n == 0 ? 0.f : x1 / den);
+}
+
+// How a call is cut: the rows of a workgroup, its waves, and the chunks of keys.
+struct Plan8 {
+    int rows, waves;
+    int64_t tiles, splits, items;
+    int chunk;
+    size_t ml_off, total;
+};
+
+constexpr int kMostChunk = 8192;  // its pages' ids fit one lane each
+
+Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv) {
+    Plan8 p{};
+    const int64_t R = (int64_t)S * (Hq / Hkv);
+    p.rows = R <= 16 ? 16 : 32;
+    p.tiles = ceil_div(R, p.rows);
+    p.waves = 4;
+    // two workgroups a CU, where every sequence is as long as the longest
+    const int64_t steps = ceil_div(max_kv, 4 * kTile) * ((int64_t)B * Hkv * p.tiles);
+    p.chunk = 4 * kTile * (int)std::max<int64_t>(1, std::min<int64_t>(kMostChunk / (4 * kTile), ceil_div(steps, 2 * kCus)));
+    p.splits = std::max<int64_t>(1, ceil_div(max_kv, p.chunk));
+    p.items = 8 * p.tiles * ceil_div((int64_t)B * Hkv * p.splits, 8);
+    const int64_t rows = (int64_t)B * Hq * S;
+    p.ml_off = (size_t)rows * p.splits * kHeadDim * sizeof(float);
+    p.total = p.splits > 1 ? p.ml_off + (size_t)rows * p.splits * sizeof(float2) : 0;
+    return p;
+}
+
+template <typename T> int launch8(const Args8& a, const Plan8& p, int64_t n_rows, hipStream_t st) {
+    const dim3 grid((unsigned)p.items), threads(64 * p.waves);
+    if (p.rows == 16) hipLaunchKernelGGL((f8_stream_kernel<T, 1, 4>), grid, threads, 0, st, a);
+    else hipLaunchKernelGGL((f8_stream_kernel<T, 2, 4>), grid, threads, 0, st, a);
+    int rc = launch_status(hipGetLastError());
+    if (rc || p.splits == 1) return rc;
+    hipLaunchKernelGGL((f8_join_kernel<T, 1>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a, (int)n_rows);
+    return launch_status(hipGetLastError());
+}
+
+int check_sizes8(int64_t max_kv, int B, int S, int Hq, int Hkv, int D, int dtype) {
+    if (dtype != CRANE_HIP_F32 && dtype != CRANE_HIP_BF16) return CRANE_HIP_E_DTYPE;
+    if (D != kHeadDim) return CRANE_HIP_E_HEAD_DIM;
+    if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0) return CRANE_HIP_E_INVALID;
+    if (Hq % Hkv != 0) return CRANE_HIP_E_GQA;
+    if (B > 65535 || (int64_t)B * Hq > 0x7fffffffLL) return CRANE_HIP_E_INVALID;
+    if ((int64_t)B * Hq * S > kMostThreads / 64) return CRANE_HIP_E_INVALID;  // a wave each in the join
+    if (max_kv > 0x7fffffffLL - 2 * kMostChunk) return CRANE_HIP_E_INVALID;   // a chunk's bounds stay within 31 bits
+    return CRANE_HIP_OK;
+}
+
+}  // namespace
+}  // namespace crane
+
+using namespace crane;
+
+extern "C" size_t crane_hip_attn_paged_f8_workspace(int64_t max_kv, int B, int S, int Hq, int Hkv, int D, int dtype) {
+    if (check_sizes8(max_kv, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0 || max_kv <= 0) return 0;
+    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv);
+    return p.items <= kMostThreads / (64 * p.waves) ? p.total : 0;
+}
+
+extern "C" int crane_hip_attn_paged_f8(const void* q, const void* k_pool, const void* v_pool, const void* k_scale,
+                                       const void* v_scale, int64_t n_pages, int page_rows,
+                                       const int32_t* block_table, int64_t table_stride, const int32_t* kv_len,
+                                       int64_t max_kv, int B, int S, int Hq, int Hkv, int D, float scale, int flags,
+                                       void* workspace, size_t ws_bytes, void* out, int dtype, void* stream) {
+    int rc = check_sizes8(max_kv, B, S, Hq, Hkv, D, dtype);
+    if (rc) return rc;
+    if (flags & ~CRANE_HIP_PREFILL_CAUSAL) return CRANE_HIP_E_INVALID;
+    if (!(scale > 0.0f) || !__builtin_isfinite(scale)) return CRANE_HIP_E_INVALID;
+    if ((rc = check_paged(n_pages, page_rows, block_table, table_stride, Hkv))) return rc;
+    if (max_kv <= 0) return CRANE_HIP_E_INVALID;
+    if (max_kv > table_stride * page_rows) return CRANE_HIP_E_CAPACITY;
+    if (B == 0 || S == 0) return CRANE_HIP_OK;
+    if (!q || !kv_len || !out) return CRANE_HIP_E_INVALID;
+    if ((rc = check_pools8(k_pool, v_pool, k_scale, v_scale))) return rc;
+    if (!aligned16(q) || !aligned16(out)) return CRANE_HIP_E_ALIGN;
+    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv);
+    if (p.items > kMostThreads / (64 * p.waves)) return CRANE_HIP_E_INVALID;
+    if (p.total && (!workspace || ws_bytes < p.total || !aligned16(workspace))) return CRANE_HIP_E_WORKSPACE;
+    Args8 a;
+    a.q = q;
+    a.k = (const uint8_t*)k_pool;
+    a.v = (const uint8_t*)v_pool;
+    a.k_scale = (const uint8_t*)k_scale;
+    a.v_scale = (const uint8_t*)v_scale;
+    a.out = out;
+    a.rows = PagedRows{block_table, table_stride, n_pages, page_rows};
+    a.kv_len = kv_len;
+    a.B = B;
+    a.S = S;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.G = Hq / Hkv;
+    a.max_kv = (int)max_kv;
+    a.causal = flags & CRANE_HIP_PREFILL_CAUSAL;
+    a.c = scale * kLog2e;
+    a.chunk = p.chunk;
+    a.splits = (int)p.splits;
+    a.tiles = (int)p.tiles;
+    a.ws_o = (float*)workspace;
+    a.ws_ml = (float2*)((char*)workspace + p.ml_off);
+    const int64_t n_rows = (int64_t)B * Hq * S;
+    const hipStream_t st = (hipStream_t)stream;
+    return dtype == CRANE_HIP_F32 ? launch8<float>(a, p, n_rows, st) : launch8<bf16_t>(a, p, n_rows, st);
+}

@@ -1,0 +1,368 @@
+// f8_cache.hip -- rows into and out of the paged KV cache in 8 bits (gfx950): the fused
+// per-head QK-RMSNorm + RoPE append that quantises k and v as it writes them, and the
+// read that gives values back.  The C ABI and the format are include/crane_f8.h's.
+//
+// The append is append.hip's pass over the merged qkv rows with 8 lanes to a head row
+// (lane l holds dims [8l, 8l + 8) and [64 + 8l, + 8): the rotation is lane-local), in f32
+// from the row to its one rounding.  q heads are independent items.  k and v need the
+// largest magnitude of all new rows of a 32-row block before any of them can be written:
+// a workgroup takes one block of one head, its 32 lane groups a row each, and holds the
+// rows in registers between the maximum and the codes, so every row is read once and
+// written once.  With one new token a block has one new row, and its lane group needs
+// nobody: those items are independent again.
+//
+// A scale is a power of two.  Codes are floating point: scaling by 2^k moves their
+// exponent and rounds nothing while they stay normal, so a block's common scale costs
+// no precision (a value keeps its 4 significant bits down to 2^-14 of the block's
+// largest), and a block whose scale grows later has its older codes moved exactly
+// (subnormal ones aside).
+#include "f8.h"
+
+namespace crane {
+namespace {
+
+constexpr int kItems = 32;  // head rows of a 256-thread workgroup
+
+// Sum and maximum over the 8 lanes of a row; every lane gets them.
+__device__ __forceinline__ float group8_sum(float x) {
+    x += dpp<0xB1>(x);   // quad_perm [1,0,3,2]
+    x += dpp<0x4E>(x);   // quad_perm [2,3,0,1]
+    x += dpp<0x141>(x);  // row_half_mirror
+    return x;
+}
+__device__ __forceinline__ float group8_max(float x) {
+    x = fmaxf(x, dpp<0xB1>(x));
+    x = fmaxf(x, dpp<0x4E>(x));
+    x = fmaxf(x, dpp<0x141>(x));
+    return x;
+}
+
+template <typename T> struct Append {
+    const T* qkv;
+    int64_t row_stride;
+    const T *qw, *kw;
+    float eps;
+    int order;
+    const T *cos, *sin;
+    int64_t cs_stride, table_rows;
+    const int32_t* positions;
+    T* q_out;
+    uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
+    PagedRows rows;
+    const int32_t* cache_len;
+    int S, Hq, Hkv;
+    int64_t q_items, q_blocks;  // q head rows, and the workgroups that take them
+    int64_t units;              // blocks mode: (sequence, block, k or v head)
+    int blocks;                 // blocks mode: blocks a sequence's S rows can touch
+};
+
+// A lane's 16 values of a head row, normed and rotated in f32.
+struct RowValues {
+    float a[8], b[8];  // dims 8l .., 64 + 8l ..
+};
+
+template <typename T> __device__ __forceinline__ void norm(RowValues& x, const float (&w1)[8], const float (&w2)[8], float eps) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        ss = __builtin_fmaf(x.a[i], x.a[i], ss);
+        ss = __builtin_fmaf(x.b[i], x.b[i], ss);
+    }
+    const float r = 1.0f / sqrtf(group8_sum(ss) * (1.0f / kHeadDim) + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x.a[i] = x.a[i] * r * w1[i];
+        x.b[i] = x.b[i] * r * w2[i];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void norm_rope(RowValues& x, const Append<T>& p, const T* w, int64_t pos, int l) {
+    float c[8], s[8], w1[8], w2[8];
+    load8(p.cos + pos * p.cs_stride + 8 * l, c);
+    load8(p.sin + pos * p.cs_stride + 8 * l, s);
+    if (w) {
+        load8(w + 8 * l, w1);
+        load8(w + 64 + 8 * l, w2);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w1[i] = w2[i] = 1.f;
+    }
+    if (p.order == CRANE_HIP_NORM_THEN_ROPE) norm<T>(x, w1, w2, p.eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float u = x.a[i], v = x.b[i];
+        x.a[i] = u * c[i] - v * s[i];
+        x.b[i] = u * s[i] + v * c[i];
+    }
+    if (p.order == CRANE_HIP_ROPE_THEN_NORM) norm<T>(x, w1, w2, p.eps);
+}
+
+template <typename T> __device__ __forceinline__ void load_row(RowValues& x, const Append<T>& p, int64_t tok, int head, int l) {
+    const T* src = p.qkv + tok * p.row_stride + (int64_t)head * kHeadDim;
+    load8(src + 8 * l, x.a);
+    load8(src + 64 + 8 * l, x.b);
+}
+
+// The largest finite magnitude of a lane's values, 0 or more.
+__device__ __forceinline__ float largest(const RowValues& x) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(x.a[i]), b = fabsf(x.b[i]);
+        m = fmaxf(m, fmaxf(a < INFINITY ? a : 0.f, b < INFINITY ? b : 0.f));
+    }
+    return m;
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* row, const RowValues& x, int byte, int l) {
+    const float inv = scale_of(254 - byte);
+    *reinterpret_cast<uint2*>(row + 8 * l) = codes8(x.a, inv);
+    *reinterpret_cast<uint2*>(row + 64 + 8 * l) = codes8(x.b, inv);
+}
+
+template <typename T> __device__ __forceinline__ void q_item(const Append<T>& p, int64_t item, int l) {
+    if (item >= p.q_items) return;  // whole 8-lane groups leave together
+    const int head = (int)(item % p.Hq);
+    const int64_t tok = item / p.Hq;
+    const int s = (int)(tok % p.S), b = (int)(tok / p.S);
+    const int64_t pos = (int64_t)p.positions[b] + s;
+    RowValues x;
+    load_row(x, p, tok, head, l);
+    if (pos < 0 || pos >= p.table_rows) return;
+    norm_rope(x, p, p.qw, pos, l);
+    T* dst = p.q_out + (((int64_t)b * p.Hq + head) * p.S + s) * kHeadDim;
+    store8(dst + 8 * l, x.a);
+    store8(dst + 64 + 8 * l, x.b);
+}
+
+// S = 1: every head row is an item of 8 lanes.  grid: q items, then k and v items.
+template <typename T> __global__ __launch_bounds__(256) void f8_append_token_kernel(Append<T> p) {
+    const int l = threadIdx.x & 7;
+    if ((int64_t)blockIdx.x < p.q_blocks) return q_item(p, (int64_t)blockIdx.x * kItems + (threadIdx.x >> 3), l);
+    const int64_t item = ((int64_t)blockIdx.x - p.q_blocks) * kItems + (threadIdx.x >> 3);
+    if (item >= p.units) return;
+    const int hh = (int)(item % (2 * p.Hkv)), b = (int)(item / (2 * p.Hkv));
+    const bool is_v = hh >= p.Hkv;
+    const int h = is_v ? hh - p.Hkv : hh;
+    const int64_t j = p.cache_len[b], pos = p.positions[b];
+    RowValues x;
+    load_row(x, p, b, p.Hq + hh, l);
+    const int64_t off = p.rows.offset(b, p.Hkv, h, j);
+    if (off < 0) return;
+    if (!is_v) {
+        if (pos < 0 || pos >= p.table_rows) return;
+        norm_rope(x, p, p.kw, pos, l);
+    }
+    const int64_t at = off / kHeadDim / kBlockRows8;
+    uint8_t* scale = (is_v ? p.v_scale : p.k_scale) + at;
+    uint8_t* block = (is_v ? p.v_pool : p.k_pool) + at * kBlockRows8 * kHeadDim;
+    const int held = (int)(j % kBlockRows8), need = scale_byte(group8_max(largest(x)));
+    const int had = held ? *scale : 0, byte = max(need, had);
+    if (byte > had && held) {
+        const float down = scale_of(max(127 + had - byte, 0));
+        uint4* old = reinterpret_cast<uint4*>(block) + l;
+#pragma unroll 4
+        for (int r = 0; r < held; ++r) {
+            uint4 w = old[8 * r];
+            w = make_uint4(recode4(w.x, down), recode4(w.y, down), recode4(w.z, down), recode4(w.w, down));
+            old[8 * r] = w;
+        }
+    }
+    store_codes(block + held * kHeadDim, x, byte, l);
+    if (l == 0 && byte != had) *scale = (uint8_t)byte;
+}
+
+// Any S.  grid: q items, then one workgroup per (sequence, block, k or v head).
+template <typename T> __global__ __launch_bounds__(256) void f8_append_blocks_kernel(Append<T> p) {
+    const int l = threadIdx.x & 7, r = threadIdx.x >> 3;
+    if ((int64_t)blockIdx.x < p.q_blocks) return q_item(p, (int64_t)blockIdx.x * kItems + r, l);
+    const int64_t unit = (int64_t)blockIdx.x - p.q_blocks;
+    const int hh = (int)(unit % (2 * p.Hkv));
+    const int64_t x0 = unit / (2 * p.Hkv);
+    const int b = (int)(x0 / p.blocks);
+    const bool is_v = hh >= p.Hkv;
+    const int h = is_v ? hh - p.Hkv : hh;
+    const int64_t len = p.cache_len[b];
+    const int64_t first = (len & ~(int64_t)(kBlockRows8 - 1)) + (x0 % p.blocks) * kBlockRows8;
+    if (first >= len + p.S) return;  // the sequence's rows end before
+    const int64_t off = p.rows.offset(b, p.Hkv, h, first);
+    if (off < 0) return;
+    const int64_t s = first + r - len;
+    const bool old = s < 0;
+    bool fresh = !old && s < p.S;
+    RowValues x;
+    if (fresh) {
+        load_row(x, p, (int64_t)b * p.S + s, p.Hq + hh, l);
+        if (!is_v) {
+            const int64_t pos = (int64_t)p.positions[b] + s;
+            fresh = pos >= 0 && pos < p.table_rows;
+            if (fresh) norm_rope(x, p, p.kw, pos, l);
+        }
+    }
+    __shared__ float most[4];
+    const float m = wave_max(fresh ? largest(x) : -1.f);
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+    __syncthreads();
+    const float amax = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    if (amax < 0.f) return;  // no row is written
+    const int64_t at = off / kHeadDim / kBlockRows8;
+    uint8_t* scale = (is_v ? p.v_scale : p.k_scale) + at;
+    uint8_t* row = (is_v ? p.v_pool : p.k_pool) + off + r * kHeadDim;
+    const int had = first < len ? *scale : 0, byte = max(scale_byte(amax), had);
+    if (fresh) store_codes(row, x, byte, l);
+    if (old && byte > had) {
+        const float down = scale_of(max(127 + had - byte, 0));
+        uint4* w = reinterpret_cast<uint4*>(row) + l;
+        const uint4 c = *w;
+        *w = make_uint4(recode4(c.x, down), recode4(c.y, down), recode4(c.z, down), recode4(c.w, down));
+    }
+    __syncthreads();  // every wave has read the old scale
+    if (threadIdx.x == 0) *scale = (uint8_t)byte;
+}
+
+template <typename T> int launch_append(Append<T> p, int B, hipStream_t st) {
+    p.q_items = (int64_t)B * p.S * p.Hq;
+    p.q_blocks = (p.q_items + kItems - 1) / kItems;
+    // S rows from any row of a block on touch at most this many blocks
+    p.blocks = (int)(((int64_t)p.S + 2 * kBlockRows8 - 2) / kBlockRows8);
+    p.units = (int64_t)B * 2 * p.Hkv * (p.S == 1 ? 1 : p.blocks);
+    const int64_t grid = p.q_blocks + (p.S == 1 ? (p.units + kItems - 1) / kItems : p.units);
+    if (grid > 0xffffffffLL / 256) return CRANE_HIP_E_INVALID;  // a grid's threads: 32 bits
+    if (p.S == 1)
+        hipLaunchKernelGGL(f8_append_token_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL(f8_append_blocks_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, p);
+    return launch_status(hipGetLastError());
+}
+
+// Codes to values: a thread takes 16 codes of a row.
+// grid: (chunks of 16 codes of all rows / 256, k and v)
+template <typename T>
+__global__ __launch_bounds__(256) void f8_read_kernel(const uint8_t* __restrict__ k_pool,
+                                                      const uint8_t* __restrict__ v_pool,
+                                                      const uint8_t* __restrict__ k_scale,
+                                                      const uint8_t* __restrict__ v_scale, PagedRows rows,
+                                                      const int32_t* __restrict__ kv_len, int64_t max_kv, int Hkv,
+                                                      T* __restrict__ k_out, T* __restrict__ v_out, int64_t n) {
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= n) return;
+    const int c = (int)(t % 8);
+    const int64_t row = t / 8, bh = row / max_kv, j = row - bh * max_kv;
+    const int b = (int)(bh / Hkv), h = (int)(bh - (int64_t)b * Hkv);
+    const int64_t off = j < kv_len[b] ? rows.offset(b, Hkv, h, j) : -1;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    if (off >= 0) {
+        const uint4 w = *reinterpret_cast<const uint4*>((blockIdx.y ? v_pool : k_pool) + off + 16 * c);
+        const float scale = scale_of((blockIdx.y ? v_scale : k_scale)[off / kHeadDim / kBlockRows8]);
+        values4(w.x, x);
+        values4(w.y, x + 4);
+        values4(w.z, x + 8);
+        values4(w.w, x + 12);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= scale;
+    }
+    T* out = (blockIdx.y ? v_out : k_out) + row * kHeadDim + 16 * c;
+    float y[8];
+#pragma unroll
+    for (int h8 = 0; h8 < 16; h8 += 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[h8 + i];
+        store8(out + h8, y);
+    }
+}
+
+}  // namespace
+}  // namespace crane
+
+using namespace crane;
+
+extern "C" int crane_hip_qknorm_rope_append_paged_f8(const void* qkv, int64_t qkv_row_stride, const void* q_norm_w,
+                                                     const void* k_norm_w, float eps, int order, const void* cos,
+                                                     const void* sin, int64_t cs_stride, int64_t table_rows,
+                                                     const int32_t* positions, void* q_out, void* k_pool, void* v_pool,
+                                                     void* k_scale, void* v_scale, int64_t n_pages, int page_rows,
+                                                     const int32_t* block_table, int64_t table_stride,
+                                                     const int32_t* cache_len, int B, int S, int Hq, int Hkv, int D,
+                                                     int dtype, void* stream) {
+    if (dtype != CRANE_HIP_F32 && dtype != CRANE_HIP_BF16) return CRANE_HIP_E_DTYPE;
+    if (D != kHeadDim) return CRANE_HIP_E_HEAD_DIM;
+    if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0) return CRANE_HIP_E_INVALID;
+    if (Hq % Hkv != 0) return CRANE_HIP_E_GQA;
+    if (order < CRANE_HIP_NORM_THEN_ROPE || order > CRANE_HIP_ROPE_ONLY) return CRANE_HIP_E_INVALID;
+    if (!(eps >= 0.0f)) return CRANE_HIP_E_INVALID;
+    int rc = check_paged(n_pages, page_rows, block_table, table_stride, Hkv);
+    if (rc) return rc;
+    if ((int64_t)S > table_stride * page_rows) return CRANE_HIP_E_CAPACITY;
+    if (B == 0 || S == 0) return CRANE_HIP_OK;
+    if (!qkv || !cos || !sin || !positions || !q_out || !cache_len) return CRANE_HIP_E_INVALID;
+    if ((rc = check_pools8(k_pool, v_pool, k_scale, v_scale))) return rc;
+    if (cs_stride < D / 2 || table_rows <= 0) return CRANE_HIP_E_INVALID;
+    if (qkv_row_stride < ((int64_t)Hq + 2 * (int64_t)Hkv) * D) return CRANE_HIP_E_INVALID;
+    const int64_t per16 = dtype == CRANE_HIP_BF16 ? 8 : 4;  // elements per 16 bytes
+    if (qkv_row_stride % per16 != 0 || cs_stride % per16 != 0) return CRANE_HIP_E_ALIGN;
+    if (!aligned16(qkv) || !aligned16(cos) || !aligned16(sin) || !aligned16(q_out) ||
+        (q_norm_w && !aligned16(q_norm_w)) || (k_norm_w && !aligned16(k_norm_w)))
+        return CRANE_HIP_E_ALIGN;
+    auto go = [&](auto zero) {
+        typedef decltype(zero) T;
+        Append<T> p{};
+        p.qkv = (const T*)qkv;
+        p.row_stride = qkv_row_stride;
+        p.qw = (const T*)q_norm_w;
+        p.kw = (const T*)k_norm_w;
+        p.eps = eps;
+        p.order = order;
+        p.cos = (const T*)cos;
+        p.sin = (const T*)sin;
+        p.cs_stride = cs_stride;
+        p.table_rows = table_rows;
+        p.positions = positions;
+        p.q_out = (T*)q_out;
+        p.k_pool = (uint8_t*)k_pool;
+        p.v_pool = (uint8_t*)v_pool;
+        p.k_scale = (uint8_t*)k_scale;
+        p.v_scale = (uint8_t*)v_scale;
+        p.rows = PagedRows{block_table, table_stride, n_pages, page_rows};
+        p.cache_len = cache_len;
+        p.S = S;
+        p.Hq = Hq;
+        p.Hkv = Hkv;
+        return launch_append(p, B, (hipStream_t)stream);
+    };
+    return dtype == CRANE_HIP_F32 ? go(float()) : go(bf16_t());
+}
+
+extern "C" int crane_hip_read_paged_f8(const void* k_pool, const void* v_pool, const void* k_scale,
+                                       const void* v_scale, int64_t n_pages, int page_rows,
+                                       const int32_t* block_table, int64_t table_stride, const int32_t* kv_len,
+                                       int64_t max_kv, int B, int Hkv, int D, void* k_out, void* v_out, int dtype,
+                                       void* stream) {
+    if (dtype != CRANE_HIP_F32 && dtype != CRANE_HIP_BF16) return CRANE_HIP_E_DTYPE;
+    if (D != kHeadDim) return CRANE_HIP_E_HEAD_DIM;
+    if (B < 0 || Hkv <= 0 || max_kv < 0) return CRANE_HIP_E_INVALID;
+    int rc = check_paged(n_pages, page_rows, block_table, table_stride, Hkv);
+    if (rc) return rc;
+    if (max_kv > table_stride * page_rows) return CRANE_HIP_E_CAPACITY;
+    if (B == 0 || max_kv == 0) return CRANE_HIP_OK;
+    if (!kv_len || !k_out || !v_out) return CRANE_HIP_E_INVALID;
+    if ((rc = check_pools8(k_pool, v_pool, k_scale, v_scale))) return rc;
+    if (!aligned16(k_out) || !aligned16(v_out)) return CRANE_HIP_E_ALIGN;
+    const int64_t heads = (int64_t)B * Hkv;
+    if (heads > 0xffffffffLL / 16 || max_kv > 0xffffffffLL / 16 / heads) return CRANE_HIP_E_INVALID;  // threads of a grid
+    const int64_t n = heads * max_kv * 8;
+    const dim3 grid((unsigned)((n + 255) / 256), 2);
+    const PagedRows rows{block_table, table_stride, n_pages, page_rows};
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == CRANE_HIP_F32)
+        hipLaunchKernelGGL(f8_read_kernel<float>, grid, dim3(256), 0, st, (const uint8_t*)k_pool,
+                           (const uint8_t*)v_pool, (const uint8_t*)k_scale, (const uint8_t*)v_scale, rows, kv_len,
+                           max_kv, Hkv, (float*)k_out, (float*)v_out, n);
+    else
+        hipLaunchKernelGGL(f8_read_kernel<bf16_t>, grid, dim3(256), 0, st, (const uint8_t*)k_pool,
+                           (const uint8_t*)v_pool, (const uint8_t*)k_scale, (const uint8_t*)v_scale, rows, kv_len,
+                           max_kv, Hkv, (bf16_t*)k_out, (bf16_t*)v_out, n);
+    return launch_status(hipGetLastError());
+}

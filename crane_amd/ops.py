@@ -642,6 +642,144 @@ def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
     check(rc, "copy_pages")
 
 
+# ------------------------------------------------------------- paged layout, 8 bits
+# include/crane_f8.h: K and V pools [n_pages, Hkv, page_rows, D] of torch.float8_e4m3fn codes
+# and their scales [n_pages, Hkv, page_rows / 32] of torch.float8_e8m0fnu, a power of two for
+# 32 rows of a head.  `pools` is (K codes, V codes, K scales, V scales).
+
+F8_BLOCK_ROWS = 32
+
+
+def f8_pools(n_pages: int, num_kv_heads: int, page_rows: int = PAGE_ALIGN, device: torch.device | str = "cuda"):
+    """Pools of a paged cache in 8 bits, as the operators below take them: codes 0 and
+    scales 1."""
+    shape = (n_pages, num_kv_heads, page_rows)
+    codes = [torch.zeros(shape + (HEAD_DIM,), dtype=torch.uint8, device=device) for _ in "kv"]
+    scales = [torch.full(shape[:2] + (page_rows // F8_BLOCK_ROWS,), 127, dtype=torch.uint8, device=device) for _ in "kv"]
+    return tuple([t.view(torch.float8_e4m3fn) for t in codes] + [t.view(torch.float8_e8m0fnu) for t in scales])
+
+
+def _f8_args(pools: Sequence[torch.Tensor], block_table: torch.Tensor, B: int, index: int):
+    """Checks of the pools and the block table; (n_pages, Hkv, page_rows, stride)."""
+    if len(pools) != 4:
+        raise CraneHipError(_lib.E_INVALID, "pools must be (K codes, V codes, K scales, V scales)")
+    k, v, ks, vs = pools
+    shape = k.shape
+    if not (k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == block_table.get_device() ==
+            index >= 0):
+        _dev(k, v, ks, vs, block_table)
+        raise CraneHipError(_lib.E_INVALID, "tensors on different devices")
+    if not (k.dtype == v.dtype == torch.float8_e4m3fn and ks.dtype == vs.dtype == torch.float8_e8m0fnu):
+        raise CraneHipError(_lib.E_DTYPE, "pools must be float8_e4m3fn, scales float8_e8m0fnu")
+    if len(shape) != 4 or shape[3] != HEAD_DIM or v.shape != shape or shape[2] % F8_BLOCK_ROWS:
+        raise CraneHipError(_lib.E_INVALID, "pools must be [n_pages, Hkv, page_rows, D]")
+    if not ks.shape == vs.shape == (shape[0], shape[1], shape[2] // F8_BLOCK_ROWS):
+        raise CraneHipError(_lib.E_INVALID, "scales must be [n_pages, Hkv, page_rows / 32]")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise CraneHipError(_lib.E_INVALID, "pools and scales must be contiguous")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or \
+            not block_table.is_contiguous():
+        raise CraneHipError(_lib.E_INVALID, "block_table must be a contiguous int32 [B, max_pages] tensor")
+    return shape[0], shape[1], shape[2], block_table.shape[1]
+
+
+def qk_norm_rope_append_paged_f8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                                 pools: Sequence[torch.Tensor], block_table: torch.Tensor, cache_len: torch.Tensor,
+                                 num_heads: int, q_norm_w: Optional[torch.Tensor] = None,
+                                 k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                                 order: str = "norm_then_rope") -> torch.Tensor:
+    """qk_norm_rope_append_paged into a cache in 8 bits: k and v are quantised as they are
+    written, token s of sequence b into row cache_len[b]+s.  Returns q [B, Hq, S, D].
+
+    f32 throughout and rounded once, q to qkv's dtype and k and v to their codes.  A
+    block of 32 rows takes the smallest scale that holds its new rows, or keeps its own
+    where that is larger; where it grows, the codes it held are rounded to it."""
+    if qkv.dim() != 3:
+        raise CraneHipError(_lib.E_INVALID, "qkv must be [B, S, (Hq+2Hkv)*D]")
+    n_pages, Hkv, page_rows, stride = _f8_args(pools, block_table, qkv.shape[0], qkv.get_device())
+    dev, B, S = _rope_inputs(qkv, (num_heads + 2 * Hkv) * HEAD_DIM, cos, sin, positions, q_norm_w, k_norm_w, order)
+    _dev(qkv, cache_len)
+    dt = _dtype_code(qkv)
+    _i32(cache_len, B, "cache_len")
+    q_out = torch.empty((B, num_heads, S, HEAD_DIM), dtype=qkv.dtype, device=dev)
+    if B == 0:  # an empty block table has no address
+        return q_out
+    args = (qkv.data_ptr(), qkv.stride(1), _ptr(q_norm_w), _ptr(k_norm_w), eps, _ORDERS[order], cos.data_ptr(),
+            sin.data_ptr(), cos.stride(0), cos.shape[0], positions.data_ptr(), q_out.data_ptr(),
+            *[t.data_ptr() for t in pools], n_pages, page_rows, block_table.data_ptr(), stride, cache_len.data_ptr(), B,
+            S, num_heads, Hkv, HEAD_DIM, dt, _stream(dev))
+    check(_on_device(dev, _lib.lib().crane_hip_qknorm_rope_append_paged_f8, args), "qk_norm_rope_append_paged_f8")
+    return q_out
+
+
+def attention_paged_f8(q: torch.Tensor, pools: Sequence[torch.Tensor], block_table: torch.Tensor,
+                       kv_len: torch.Tensor, max_kv: int, scale: Optional[float] = None, causal: bool = True,
+                       workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of every sequence's last tokens over a paged cache in 8 bits: q [B, Hq, D]
+    (one token each, a decode step) gives [B, 1, Hq*D], q [B, Hq, S, D] gives
+    [B, S, Hq*D].  kv_len counts the S new rows; with causal query i sees the rows up to
+    its own, else all kv_len; a query that sees none gets zeros.  max_kv: host-side bound
+    of kv_len.
+
+    Scores, softmax and sums are f32 (attention_decode_paged rounds every score as
+    candle does)."""
+    index = q.get_device()
+    if index < 0 or kv_len.get_device() != index:
+        _dev(q, kv_len)
+    shape = q.shape
+    if len(shape) not in (3, 4) or shape[-1] != HEAD_DIM:
+        raise CraneHipError(_lib.E_HEAD_DIM if len(shape) in (3, 4) else _lib.E_INVALID,
+                            "q must be [B, Hq, 128] or [B, Hq, S, 128]")
+    B, Hq = shape[0], shape[1]
+    S = shape[2] if len(shape) == 4 else 1
+    n_pages, Hkv, page_rows, stride = _f8_args(pools, block_table, B, index)
+    _contig(q, "q")
+    dt = _dtype_code(q)
+    _i32(kv_len, B, "kv_len")
+    lib, dev = _lib.lib(), q.device
+    out = q.new_empty((B, S, Hq * HEAD_DIM))
+    if B == 0:
+        return out
+    need = lib.crane_hip_attn_paged_f8_workspace(max_kv, B, S, Hq, Hkv, HEAD_DIM, dt)
+    # Allocated per call, not kept per stream: a captured graph keeps its own.
+    if workspace is not None:
+        _dev(q, workspace)
+        ws_bytes = workspace.numel() * workspace.element_size()
+    elif need:
+        workspace, ws_bytes = torch.empty(need, dtype=torch.uint8, device=dev), need
+    else:
+        ws_bytes = 0
+    k, v, ks, vs = pools
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), n_pages, page_rows,
+            block_table.data_ptr(), stride, kv_len.data_ptr(), max_kv, B, S, Hq, Hkv, HEAD_DIM,
+            _SCALE if scale is None else scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace), ws_bytes,
+            out.data_ptr(), dt, _stream(dev))
+    check(_on_device(dev, lib.crane_hip_attn_paged_f8, args), "attention_paged_f8")
+    return out
+
+
+def read_paged_f8(pools: Sequence[torch.Tensor], block_table: torch.Tensor, kv_len: torch.Tensor, max_kv: int,
+                  dtype: torch.dtype = torch.bfloat16):
+    """The rows of every sequence of a paged cache in 8 bits as values: (k, v)
+    [B, Hkv, max_kv, D] in `dtype` (exact in bf16 too), zeros from kv_len on."""
+    if block_table.dim() != 2:
+        raise CraneHipError(_lib.E_INVALID, "block_table must be a contiguous int32 [B, max_pages] tensor")
+    B = block_table.shape[0]
+    n_pages, Hkv, page_rows, stride = _f8_args(pools, block_table, B, block_table.get_device())
+    dev = _dev(block_table, kv_len)
+    dt = _dtype_code_of(dtype)
+    _i32(kv_len, B, "kv_len")
+    if max_kv < 0:
+        raise CraneHipError(_lib.E_INVALID, f"max_kv {max_kv}")
+    k, v = (torch.empty((B, Hkv, max_kv, HEAD_DIM), dtype=dtype, device=dev) for _ in "kv")
+    if B == 0:
+        return k, v
+    args = (*[t.data_ptr() for t in pools], n_pages, page_rows, block_table.data_ptr(), stride, kv_len.data_ptr(),
+            max_kv, B, Hkv, HEAD_DIM, k.data_ptr(), v.data_ptr(), dt, _stream(dev))
+    check(_on_device(dev, _lib.lib().crane_hip_read_paged_f8, args), "read_paged_f8")
+    return k, v
+
+
 # ------------------------------------------------------- decoder-layer rows
 # The row kernels either side of the attention block (include/crane_layer.h):
 # RmsNorm, residual add + RmsNorm, SiLU(gate) * up, residual add
