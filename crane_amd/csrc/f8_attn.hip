@@ -42,12 +42,19 @@ struct Args8 {
     int B, S, Hq, Hkv, G;  // G = Hq / Hkv heads per kv head
     int max_kv, causal;
     float c;               // scale log2 e
-    int chunk, splits, tiles;  // keys per chunk, chunks, row tiles per (sequence, kv head)
-    float* ws_o;           // [B Hq S, splits, D], unnormalised
-    float2* ws_ml;         // [B Hq S, splits] (m, l)
+    int tiles;             // row tiles of a (sequence, kv head)
+    int pairs;             // (sequence, chunk) pairs there may be; 0: every sequence is one chunk
+    int tile_rows;         // query rows of a tile
+    float* ws_o;           // [pairs, Hkv, tiles, tile_rows, D], unnormalised
+    float2* ws_ml;         // [pairs, Hkv, tiles, tile_rows] (m, l)
+    int4* ws_cut;          // [B] a sequence's chunks, the pair of its second one, rows of a chunk
     __device__ __forceinline__ int len(int b) const { return max(0, min(kv_len[b], max_kv)); }
     // Rows query s of a sequence of n rows sees.
     __device__ __forceinline__ int limit(int n, int s) const { return causal ? n - S + 1 + s : n; }
+    // Where the partial results of a tile's row are (in rows of ws_o).
+    __device__ __forceinline__ int64_t slot(int pair, int kvh, int tile, int row) const {
+        return (((int64_t)pair * Hkv + kvh) * tiles + tile) * tile_rows + row;
+    }
     // The row of out [B, S, Hq] that is row `at` of q [B, Hq, S].
     __device__ __forceinline__ int64_t out_row(int at) const {
         if (S == 1) return at;
@@ -61,24 +68,119 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// A chunk's pages, one id per lane: those from the chunk's first on, or the whole table
-// row where it fits (then the load waits for nothing).
-struct Pages8 {
-    int ids, page0, P;
-    __device__ __forceinline__ Pages8(const Args8& a, int b, int begin, int lane) : ids(-1), P(a.rows.page_rows) {
-        page0 = a.rows.stride <= 64 ? 0 : begin / P;
-        if (page0 + lane < a.rows.stride) ids = a.rows.table[(int64_t)b * a.rows.stride + page0 + lane];
+// The sequences' chunks.  All are cut into chunks of the same number of tiles, few enough
+// of them that there are no more than `pairs` in all: as many workgroups as the device
+// holds at once, whatever the lengths (and however far above them max_kv is, as in a
+// captured graph).  Every wave works it out from kv_len, lane x holding sequences x, 64 +
+// x, ...  Pair b < B is the first chunk of sequence b, which needs nothing of this to start;
+// the others follow, sequence by sequence.
+struct Cut {
+    int b, chunk;  // a pair's; b = -1 past the last
+    int n, rest;   // the sequence's chunks, and the pair of its second one
+    int tiles;     // tiles of a chunk
+    int len;       // the sequence's rows
+    __device__ __forceinline__ int pair(int c) const { return c == 0 ? b : rest + c - 1; }
+};
+constexpr int kMostCut = 256;   // sequences of a batch that is cut
+constexpr int kLeastChunk = 4;  // tiles: every wave of a workgroup has one
+// Inclusive sums over the wave's lanes.
+__device__ __forceinline__ float wave_scan(float x) {
+    x += dpp<0x111>(x);  // row_shr:1
+    x += dpp<0x112>(x);
+    x += dpp<0x114>(x);
+    x += dpp<0x118>(x);
+    x += dpp_rows<0x142, 0xa>(x, 0.f);  // row_bcast:15 into rows 1, 3
+    x += dpp_rows<0x143, 0xc>(x, 0.f);  // row_bcast:31 into rows 2, 3
+    return x;
+}
+__device__ __forceinline__ float lane_value(float x, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+}
+// ceil(x / d) for x < 2^26 and a quotient below 2^20, r about 1 / d.
+__device__ __forceinline__ int ceil_by(int x, int d, float r) {
+    int q = (int)((float)x * r);
+    q -= q * d > x ? 1 : 0;
+    q += (q + 1) * d <= x ? 1 : 0;
+    return q + (q * d < x ? 1 : 0);
+}
+struct Lengths {
+    static constexpr int kN = kMostCut / 64;
+    int of[kN];
+    __device__ __forceinline__ void load(const Args8& a, int lane) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) of[i] = 64 * i + lane < a.B ? a.kv_len[64 * i + lane] : 0;
     }
-    // The tile of keys [j, j + 64) of a kv head: its offset in a pool, the bytes of its rows
-    // before `end` (0 for a page outside the pool: its rows read as zero), and the byte
-    // of its first block's scale.
+};
+__device__ __forceinline__ Cut cut_at(const Args8& a, const Lengths& raw, int pair, int lane) {
+    constexpr int kN = Lengths::kN;
+    int len[kN], t[kN];
+    float total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        len[i] = max(0, min(raw.of[i], a.max_kv));
+        t[i] = 64 * i + lane < a.B ? max(1, (len[i] + kTile - 1) / kTile) : 0;
+        total += (float)t[i];
+    }
+    total = wave_sum(total);
+    // About half a chunk of every sequence is not filled: start there, and go on until all fit,
+    // which is so at the longest sequence's tiles, at the latest.
+    const float pairs = (float)a.pairs;
+    int c = max(kLeastChunk, (int)(total * __builtin_amdgcn_rcpf(pairs - 0.5f * (float)a.B)));
+    float r;
+    for (;;) {
+        r = __builtin_amdgcn_rcpf((float)c);
+        float f = 0.f;
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (64 * i < a.B) f += (float)ceil_by(t[i], c, r);
+        f = wave_sum(f);
+        if (f <= pairs) break;
+        c = max(c + 1, (int)((float)c * f * __builtin_amdgcn_rcpf(pairs)));
+    }
+    Cut x{-1, 0, 0, 0, c, 0};
+    float before = (float)a.B;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        if (64 * i >= a.B || x.b >= 0) continue;
+        const float n = (float)ceil_by(t[i], c, r), upto = before + wave_scan(n - (64 * i + lane < a.B ? 1.f : 0.f));
+        const uint64_t mine = __ballot(pair < a.B ? 64 * i + lane == pair : (float)pair < upto);
+        if (mine) {
+            const int at = __builtin_ctzll(mine);
+            x.b = 64 * i + at;
+            x.n = (int)lane_value(n, at);
+            x.rest = (int)lane_value(upto, at) - (x.n - 1);
+            x.chunk = pair < a.B ? 0 : pair - x.rest + 1;
+            x.len = __builtin_amdgcn_readlane(len[i], at);
+        }
+        before = lane_value(upto, 63);
+    }
+    return x;
+}
+
+// Pages of a sequence, one id per lane: 64 from `page0` on (all of the table's row where it
+// has no more: then the first load waits for nothing).
+struct Pages8 {
+    const int32_t* row;
+    int stride, ids, page0, P, lane;
+    __device__ __forceinline__ Pages8(const Args8& a, int ln) : stride((int)a.rows.stride), P(a.rows.page_rows), lane(ln) {}
+    __device__ __forceinline__ void open(const Args8& a, int b, int begin) {
+        row = a.rows.table + (int64_t)b * a.rows.stride;
+        load(stride <= 64 ? 0 : begin / P);
+    }
+    __device__ __forceinline__ void load(int from) {
+        page0 = from;
+        ids = page0 + lane < stride ? row[page0 + lane] : -1;
+    }
+    // The tile of keys [j, j + 64) of a kv head: its offset in a pool and the bytes of its rows
+    // before `end` (0 for a page outside the pool: its rows read as zero).  j never falls.
     struct Tile {
         int64_t off;
         int bytes;
     };
-    __device__ __forceinline__ Tile tile(const Args8& a, int kvh, int j, int end) const {
+    __device__ __forceinline__ Tile tile(const Args8& a, int kvh, int j, int end) {
         const int p = j / P;
-        const int id = __builtin_amdgcn_readlane(ids, (p - page0) & 63);
+        if (p - page0 >= 64) load(p);
+        const int id = __builtin_amdgcn_readlane(ids, p - page0);
         const bool ok = (unsigned)id < (unsigned)a.rows.n_pages;
         const int rows = ok ? max(0, min(kTile, end - j)) : 0;
         const int64_t off = (((int64_t)(ok ? id : 0) * a.Hkv + kvh) * P + (j - p * P)) * kRow;
@@ -375,34 +477,75 @@ template <typename T, int RT> struct Stream {
     }
 };
 
-// The LDS of a workgroup of W waves: their tiles, then (W > 1) their results.
+// The LDS of a workgroup of W waves: their tiles, then their results.
 template <int RT, int W> union StreamLds {
     static constexpr int kStride = kHeadDim + 4;  // f32 per row: 16 rows at one column hit different banks
     __attribute__((aligned(1024))) uint8_t tile[W][2 * kTileBytes];
     struct {
-        float o[W > 1 ? W : 1][16 * RT][W > 1 ? kStride : 1];
+        float o[W][16 * RT][kStride];
         float m[W][16 * RT], l[W][16 * RT];
     } join;
 };
 
-template <typename T, int RT, int W>
-__global__ __launch_bounds__(64 * W, RT == 1 ? 2 : 1) void f8_stream_kernel(Args8 a) {
-    __shared__ StreamLds<RT, W> sm;
-    const Item x(blockIdx.x, a.tiles, a.Hkv, a.B, a.splits);
-    if (!x.ok) return;
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int b = x.seg, R = a.S * a.G, row0 = x.block * 16 * RT, begin = x.chunk * a.chunk;
-    const int n = a.len(b);
-    // What the tile's first and last queries see; the last sees most.
-    const int last = (min(row0 + 16 * RT, R) - 1) / a.G;
-    const int min_hi = a.limit(n, row0 / a.G);
-    const int end = min(begin + a.chunk, a.limit(n, last));
-    const bool direct = a.splits == 1;
-    if (begin >= end && !direct) return;  // the join reads no chunk past a row's keys
+// Workgroup x's item: ids that are equal mod 8 run on one XCD, which so gets the row tiles
+// of a (pair, kv head), one after the other, and reads their keys through its own L2.
+struct Item8 {
+    int block, kvh, pair;
+    __device__ __forceinline__ Item8(int x, int tiles, int Hkv) {
+        const int c = x / (8 * tiles), rem = x - c * 8 * tiles;
+        block = rem >> 3;
+        const int unit = 8 * c + (rem & 7);
+        pair = unit / Hkv;
+        kvh = unit - pair * Hkv;
+    }
+};
 
-    const Pages8 pages(a, b, begin, lane);
+template <typename T, int RT, int W>
+__global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1) void f8_stream_kernel(Args8 a) {
+    __shared__ StreamLds<RT, W> sm;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Item8 x(blockIdx.x, a.tiles, a.Hkv);
+    const int R = a.S * a.G, row0 = x.block * 16 * RT;
+    // The tile's first and last queries; the last sees most.
+    const int first = row0 / a.G, last = (min(row0 + 16 * RT, R) - 1) / a.G;
+    Pages8 pages(a, lane);
+    Pages8::Tile tile;
     Stream<T, RT> st(lane, sm.tile[wave]);
+    int b = x.pair, n = 0, begin = 0, end = 0, j = wave * kTile;
+    Lengths lengths;
+    if (a.pairs) lengths.load(a, lane);
+    if (b < a.B) {  // a first chunk: its waves' first tiles are in it however the sequence is cut
+        n = a.len(b);
+        end = a.limit(n, last);
+        pages.open(a, b, 0);
+        if (j < end) st.copy(a, tile = pages.tile(a, x.kvh, j, end), sm.tile[wave]);
+    } else if (!a.pairs) {
+        return;
+    }
+    bool direct = true;
+    if (a.pairs) {
+        const Cut cut = cut_at(a, lengths, x.pair, lane);
+        if (cut.b < 0) return;
+        direct = __builtin_amdgcn_readfirstlane(cut.n) == 1;
+        const int per = __builtin_amdgcn_readfirstlane(cut.tiles) * kTile;
+        begin = __builtin_amdgcn_readfirstlane(cut.chunk) * per;
+        if (begin > 0) {
+            b = __builtin_amdgcn_readfirstlane(cut.b);
+            n = __builtin_amdgcn_readfirstlane(cut.len);
+            end = min(begin + per, a.limit(n, last));
+            if (begin >= end) return;  // the join reads no chunk past a row's keys
+            pages.open(a, b, begin);
+            j = begin + wave * kTile;
+            if (j < end) st.copy(a, tile = pages.tile(a, x.kvh, j, end), sm.tile[wave]);
+        } else if (!direct) {
+            end = min(per, end);
+            if (x.kvh == 0 && x.block == 0 && tid == 0) a.ws_cut[b] = make_int4(cut.n, cut.rest, per, 0);
+        }
+        if (direct && x.kvh == 0 && x.block == 0 && tid == 0) a.ws_cut[b] = make_int4(1, 0, 0, 0);
+    }
+    const int min_hi = a.limit(n, first);
+
     int at[RT], hi[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -414,132 +557,127 @@ __global__ __launch_bounds__(64 * W, RT == 1 ? 2 : 1) void f8_stream_kernel(Args
         for (int step = 0; step < 4; ++step) st.q[t][step].load(row + 64 * (step >> 1) + 16 * st.g + 8 * (step & 1));
     }
     constexpr int kStride = W * kTile;
-    int j = begin + wave * kTile;
-    if (j < end) {
-        Pages8::Tile tile = pages.tile(a, x.kvh, j, end);
-        st.copy(a, tile, sm.tile[wave]);
-        for (; j < end; j += kStride) {
-            st.ks.load(a.k_scale, tile.off);
-            st.vs.load(a.v_scale, tile.off);
-            wait_memory();
+    for (; j < end; j += kStride) {
+        st.ks.load(a.k_scale, tile.off);
+        st.vs.load(a.v_scale, tile.off);
+        wait_memory();
+        __builtin_amdgcn_sched_barrier(0);
+        st.take();
+        if (j + kStride < end) {
+            tile = pages.tile(a, x.kvh, j + kStride, end);
+            wait_lds();  // the tile is in registers: its LDS is free
             __builtin_amdgcn_sched_barrier(0);
-            st.take();
-            if (j + kStride < end) {
-                tile = pages.tile(a, x.kvh, j + kStride, end);
-                wait_lds();  // the tile is in registers: its LDS is free
-                __builtin_amdgcn_sched_barrier(0);
-                st.copy(a, tile, sm.tile[wave]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            float s[RT][16];
-            st.scores(s);
-            const bool masked = j + kTile > min(min_hi, end);
-            if (masked) {
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        s[t][e] = j + 32 * (e >> 3) + 8 * st.g + (e & 7) < hi[t] ? s[t][e] : -INFINITY;
-            }
-            st.weights(s, a.c);
-            if (masked && min_hi < end) st.settle_nan(j, hi);
-            st.accumulate(s);
+            st.copy(a, tile, sm.tile[wave]);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        float s[RT][16];
+        st.scores(s);
+        const bool masked = j + kTile > min(min_hi, end);
+        if (masked) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    s[t][e] = j + 32 * (e >> 3) + 8 * st.g + (e & 7) < hi[t] ? s[t][e] : -INFINITY;
+        }
+        st.weights(s, a.c);
+        if (masked && min_hi < end) st.settle_nan(j, hi);
+        st.accumulate(s);
     }
 
     T* out = reinterpret_cast<T*>(a.out);
-    if constexpr (W == 1) {
+    __syncthreads();  // every wave's tiles are read
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const float l = groups_sum(st.l[t]);
-            if (at[t] < 0) continue;
-            const int64_t slot = (int64_t)at[t] * a.splits + x.chunk;
-            T* to = out + a.out_row(at[t]) * kHeadDim + 4 * st.g;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                float y[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = !direct ? st.o[t][d][r] : hi[t] <= 0 ? 0.f : st.o[t][d][r] / l;
-                if (direct) store4(to + 16 * d, y);
-                else store4(a.ws_o + slot * kHeadDim + 16 * d + 4 * st.g, y);
-            }
-            if (!direct && st.g == 0) a.ws_ml[slot] = make_float2(st.m[t], l);
+    for (int t = 0; t < RT; ++t) {
+        const float l = groups_sum(st.l[t]);
+        if (st.g == 0) {
+            sm.join.m[wave][16 * t + st.i] = st.m[t];
+            sm.join.l[wave][16 * t + st.i] = l;
         }
-    } else {
-        __syncthreads();  // every wave's tiles are read
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const float l = groups_sum(st.l[t]);
-            if (st.g == 0) {
-                sm.join.m[wave][16 * t + st.i] = st.m[t];
-                sm.join.l[wave][16 * t + st.i] = l;
-            }
+        for (int d = 0; d < 8; ++d) {
+            float y[4];
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                float y[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = st.o[t][d][r];
-                store4(&sm.join.o[wave][16 * t + st.i][16 * d + 4 * st.g], y);
-            }
+            for (int r = 0; r < 4; ++r) y[r] = st.o[t][d][r];
+            store4(&sm.join.o[wave][16 * t + st.i][16 * d + 4 * st.g], y);
         }
-        __syncthreads();
-        // 16 threads per row, 8 dims each.
-        for (int r = tid >> 4; r < 16 * RT && row0 + r < R; r += 4 * W) {
-            const int s = (row0 + r) / a.G, h = row0 + r - s * a.G, d = 8 * (tid & 15);
-            const int place = (int)(((int64_t)b * a.Hq + x.kvh * a.G + h) * a.S + s);
-            float top = sm.join.m[0][r];
+    }
+    __syncthreads();
+    // 16 threads per row, 8 dims each.
+    for (int r = tid >> 4; r < 16 * RT && row0 + r < R; r += 4 * W) {
+        const int s = (row0 + r) / a.G, h = row0 + r - s * a.G, d = 8 * (tid & 15);
+        const int place = (int)(((int64_t)b * a.Hq + x.kvh * a.G + h) * a.S + s);
+        float top = sm.join.m[0][r];
 #pragma unroll
-            for (int w = 1; w < W; ++w) top = fmaxf(top, sm.join.m[w][r]);
-            float l = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int w = 1; w < W; ++w) top = fmaxf(top, sm.join.m[w][r]);
+        float l = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float f = fast_exp2((sm.join.m[w][r] - top) * a.c);
-                float z[8];
-                load8(&sm.join.o[w][r][d], z);
-                l += f * sm.join.l[w][r];
+        for (int w = 0; w < W; ++w) {
+            const float f = fast_exp2((sm.join.m[w][r] - top) * a.c);
+            float z[8];
+            load8(&sm.join.o[w][r][d], z);
+            l += f * sm.join.l[w][r];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] += f * z[e];
-            }
-            if (direct) {
-                const bool none = min(a.limit(n, s), end) <= 0;
+            for (int e = 0; e < 8; ++e) y[e] += f * z[e];
+        }
+        if (direct) {
+            const bool none = min(a.limit(n, s), end) <= 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = none ? 0.f : y[e] / l;
-                store8(out + a.out_row(place) * kHeadDim + d, y);
-            } else {
-                const int64_t slot = (int64_t)place * a.splits + x.chunk;
-                store8(a.ws_o + slot * kHeadDim + d, y);
-                if (d == 0) a.ws_ml[slot] = make_float2(top, l);
-            }
+            for (int e = 0; e < 8; ++e) y[e] = none ? 0.f : y[e] / l;
+            store8(out + a.out_row(place) * kHeadDim + d, y);
+        } else {
+            const int64_t slot = a.slot(x.pair, x.kvh, x.block, r);
+            store8(a.ws_o + slot * kHeadDim + d, y);
+            if (d == 0) a.ws_ml[slot] = make_float2(top, l);
         }
     }
 }
 
 // Join a query row's chunks: P waves per row, lane x owns dims 2 x, 2 x + 1, wave p takes
-// chunks p, p + P, ...
+// chunks p, p + P, ...  The first loads (kJoinRegs chunks a wave, m and l of 64) are
+// issued at once.
+constexpr int kJoinRegs = 8;
 template <typename T, int P>
 __global__ __launch_bounds__(P == 1 ? 256 : 64 * P) void f8_join_kernel(Args8 a, int n_rows) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p = P == 1 ? 0 : wave;
-    const int row = P == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    const int row = __builtin_amdgcn_readfirstlane(P == 1 ? blockIdx.x * 4 + wave : blockIdx.x);
     if (row >= n_rows) return;  // P > 1: the whole workgroup
-    const int bh = row / a.S, s = row - bh * a.S, b = bh / a.Hq;
-    const int keys = a.limit(a.len(b), s);
-    const int n = keys > 0 ? (keys + a.chunk - 1) / a.chunk : 0;
-    const float2* ml = a.ws_ml + (int64_t)row * a.splits;
-    const float2* o = reinterpret_cast<const float2*>(a.ws_o + (int64_t)row * a.splits * kHeadDim) + lane;
-    float top = kNoMax;
-    for (int c = lane; c < n; c += 64) top = fmaxf(top, ml[c].x);
+    const int bh = row / a.S, s = row - bh * a.S, b = bh / a.Hq, head = bh - b * a.Hq, kvh = head / a.G;
+    const int4 cut = a.ws_cut[b];
+    if (cut.x == 1) return;  // written by the workgroup that had the sequence
+    const int keys = a.limit(a.len(b), s), n = keys > 0 ? (keys + cut.z - 1) / cut.z : 0;
+    const int r = s * a.G + head - kvh * a.G, tile = r / a.tile_rows;
+    // chunk c's results
+    const int64_t at = a.slot(0, kvh, tile, r - tile * a.tile_rows), next = (int64_t)a.Hkv * a.tiles * a.tile_rows;
+    auto ml = [&](int c) __attribute__((always_inline)) { return a.ws_ml[at + (c == 0 ? b : cut.y + c - 1) * next]; };
+    auto o = [&](int c) __attribute__((always_inline)) {
+        return reinterpret_cast<const float2*>(a.ws_o + (at + (c == 0 ? b : cut.y + c - 1) * next) * kHeadDim)[lane];
+    };
+    float2 x[kJoinRegs];
+#pragma unroll
+    for (int i = 0; i < kJoinRegs; ++i) x[i] = o(min(p + P * i, max(n - 1, 0)));
+    const float2 mine = ml(min(lane, max(n - 1, 0)));
+    float top = lane < n ? mine.x : kNoMax;
+    for (int c = lane + 64; c < n; c += 64) top = fmaxf(top, ml(c).x);
     top = wave_max(top);
     float den = 0.f, x0 = 0.f, x1 = 0.f;
     for (int c0 = 0; c0 < n; c0 += 64) {
-        const float2 t = c0 + lane < n ? ml[c0 + lane] : make_float2(kNoMax, 0.f);
+        const float2 t = c0 == 0 ? mine : ml(min(c0 + lane, n - 1));
         const float w = c0 + lane < n ? fast_exp2((t.x - top) * a.c) : 0.f;
-        den += w * t.y;
-        for (int c = c0 + p; c < min(n, c0 + 64); c += P) {
+        den += c0 + lane < n ? w * t.y : 0.f;
+        auto add = [&](int c, float2 y) __attribute__((always_inline)) {
             const float wc = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), c - c0));
-            const float2 y = o[(int64_t)c * (kHeadDim / 2)];
             x0 += wc * y.x;
             x1 += wc * y.y;
+        };
+        int c = c0 + p;
+        if (c0 == 0) {
+#pragma unroll
+            for (int i = 0; i < kJoinRegs; ++i)
+                if (p + P * i < min(n, 64)) add(p + P * i, x[i]);
+            c += P * kJoinRegs;
         }
+        for (; c < min(n, c0 + 64); c += P) add(c, o(c));
     }
     den = wave_sum(den);
     if constexpr (P > 1) {
@@ -558,40 +696,47 @@ __global__ __launch_bounds__(P == 1 ? 256 : 64 * P) void f8_join_kernel(Args8 a,
     Elem<T>::store(out + 1, n == 0 ? 0.f : x1 / den);
 }
 
-// How a call is cut: the rows of a workgroup, its waves, and the chunks of keys.
+// How a call is launched: the rows of a workgroup, its waves, and whether and into how
+// many chunks at most the sequences are cut.
 struct Plan8 {
     int rows, waves;
-    int64_t tiles, splits, items;
-    int chunk;
-    size_t ml_off, total;
+    int64_t tiles, pairs, items;
+    size_t ml_off, cut_off, total;
 };
-
-constexpr int kMostChunk = 8192;  // its pages' ids fit one lane each
 
 Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv) {
     Plan8 p{};
     const int64_t R = (int64_t)S * (Hq / Hkv);
     p.rows = R <= 16 ? 16 : 32;
     p.tiles = ceil_div(R, p.rows);
-    p.waves = 4;
-    // two workgroups a CU, where every sequence is as long as the longest
-    const int64_t steps = ceil_div(max_kv, 4 * kTile) * ((int64_t)B * Hkv * p.tiles);
-    p.chunk = 4 * kTile * (int)std::max<int64_t>(1, std::min<int64_t>(kMostChunk / (4 * kTile), ceil_div(steps, 2 * kCus)));
-    p.splits = std::max<int64_t>(1, ceil_div(max_kv, p.chunk));
-    p.items = 8 * p.tiles * ceil_div((int64_t)B * Hkv * p.splits, 8);
-    const int64_t rows = (int64_t)B * Hq * S;
-    p.ml_off = (size_t)rows * p.splits * kHeadDim * sizeof(float);
-    p.total = p.splits > 1 ? p.ml_off + (size_t)rows * p.splits * sizeof(float2) : 0;
+    const int64_t heads = Hkv * p.tiles, slots = 2 * kCus;
+    if (B <= kMostCut && B * heads < slots && max_kv > 512) p.pairs = slots / heads;
+    p.waves = !p.pairs && B * heads <= kCus ? 8 : 4;
+    p.items = 8 * p.tiles * ceil_div((p.pairs ? p.pairs : B) * Hkv, 8);
+    const size_t rows = (size_t)(p.pairs * heads * p.rows);
+    p.ml_off = rows * kHeadDim * sizeof(float);
+    p.cut_off = p.ml_off + rows * sizeof(float2);
+    p.total = p.pairs ? p.cut_off + B * sizeof(int4) : 0;
     return p;
 }
 
 template <typename T> int launch8(const Args8& a, const Plan8& p, int64_t n_rows, hipStream_t st) {
     const dim3 grid((unsigned)p.items), threads(64 * p.waves);
-    if (p.rows == 16) hipLaunchKernelGGL((f8_stream_kernel<T, 1, 4>), grid, threads, 0, st, a);
-    else hipLaunchKernelGGL((f8_stream_kernel<T, 2, 4>), grid, threads, 0, st, a);
+#define CRANE_F8_CASE(rt, w) \
+    if (p.rows == 16 * rt && p.waves == w) hipLaunchKernelGGL((f8_stream_kernel<T, rt, w>), grid, threads, 0, st, a);
+    CRANE_F8_CASE(1, 4)
+    CRANE_F8_CASE(1, 8)
+    CRANE_F8_CASE(2, 4)
+    CRANE_F8_CASE(2, 8)
+#undef CRANE_F8_CASE
     int rc = launch_status(hipGetLastError());
-    if (rc || p.splits == 1) return rc;
-    hipLaunchKernelGGL((f8_join_kernel<T, 1>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a, (int)n_rows);
+    if (rc || !p.pairs) return rc;
+    if (p.pairs <= kJoinRegs * a.B)
+        hipLaunchKernelGGL((f8_join_kernel<T, 1>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a, (int)n_rows);
+    else if (p.pairs <= 4 * kJoinRegs * a.B)
+        hipLaunchKernelGGL((f8_join_kernel<T, 4>), dim3((unsigned)n_rows), dim3(256), 0, st, a, (int)n_rows);
+    else
+        hipLaunchKernelGGL((f8_join_kernel<T, 16>), dim3((unsigned)n_rows), dim3(1024), 0, st, a, (int)n_rows);
     return launch_status(hipGetLastError());
 }
 
@@ -602,7 +747,7 @@ int check_sizes8(int64_t max_kv, int B, int S, int Hq, int Hkv, int D, int dtype
     if (Hq % Hkv != 0) return CRANE_HIP_E_GQA;
     if (B > 65535 || (int64_t)B * Hq > 0x7fffffffLL) return CRANE_HIP_E_INVALID;
     if ((int64_t)B * Hq * S > kMostThreads / 64) return CRANE_HIP_E_INVALID;  // a wave each in the join
-    if (max_kv > 0x7fffffffLL - 2 * kMostChunk) return CRANE_HIP_E_INVALID;   // a chunk's bounds stay within 31 bits
+    if (max_kv > 0x7fffffffLL - (1 << 20)) return CRANE_HIP_E_INVALID;  // a tile's bounds stay within 31 bits
     return CRANE_HIP_OK;
 }
 
@@ -653,11 +798,12 @@ extern "C" int crane_hip_attn_paged_f8(const void* q, const void* k_pool, const 
     a.max_kv = (int)max_kv;
     a.causal = flags & CRANE_HIP_PREFILL_CAUSAL;
     a.c = scale * kLog2e;
-    a.chunk = p.chunk;
-    a.splits = (int)p.splits;
     a.tiles = (int)p.tiles;
+    a.pairs = (int)p.pairs;
+    a.tile_rows = p.rows;
     a.ws_o = (float*)workspace;
     a.ws_ml = (float2*)((char*)workspace + p.ml_off);
+    a.ws_cut = (int4*)((char*)workspace + p.cut_off);
     const int64_t n_rows = (int64_t)B * Hq * S;
     const hipStream_t st = (hipStream_t)stream;
     return dtype == CRANE_HIP_F32 ? launch8<float>(a, p, n_rows, st) : launch8<bf16_t>(a, p, n_rows, st);
