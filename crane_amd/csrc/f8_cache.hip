@@ -37,6 +37,17 @@ __device__ __forceinline__ float group8_max(float x) {
     return x;
 }
 
+// 16 bytes past the caches.
+typedef unsigned int u32x4_v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void store_streamed(float* p, const float (&x)[4]) {
+    const u32x4_v w = {__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4_v*>(p));
+}
+__device__ __forceinline__ void store_streamed(bf16_t* p, const float (&x)[8]) {
+    const u32x4_v w = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4_v*>(p));
+}
+
 template <typename T> struct Append {
     const T* qkv;
     int64_t row_stride;
@@ -236,41 +247,52 @@ template <typename T> int launch_append(Append<T> p, int B, hipStream_t st) {
     return launch_status(hipGetLastError());
 }
 
-// Codes to values: a thread takes 16 codes of a row.
-// grid: (chunks of 16 codes of all rows / 256, k and v)
+// Codes to values.  A workgroup takes 64 rows of a head (two blocks, within one page), a
+// thread 16 bytes of values at a time, so that a wave's stores are whole lines side by
+// side; all its loads are issued before the first store.  The stores go past the caches.
+// grid: (row tiles of all heads, k and v)
+constexpr int kReadRows = 2 * kBlockRows8;
 template <typename T>
 __global__ __launch_bounds__(256) void f8_read_kernel(const uint8_t* __restrict__ k_pool,
                                                       const uint8_t* __restrict__ v_pool,
                                                       const uint8_t* __restrict__ k_scale,
                                                       const uint8_t* __restrict__ v_scale, PagedRows rows,
                                                       const int32_t* __restrict__ kv_len, int64_t max_kv, int Hkv,
-                                                      T* __restrict__ k_out, T* __restrict__ v_out, int64_t n) {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= n) return;
-    const int c = (int)(t % 8);
-    const int64_t row = t / 8, bh = row / max_kv, j = row - bh * max_kv;
-    const int b = (int)(bh / Hkv), h = (int)(bh - (int64_t)b * Hkv);
-    const int64_t off = j < kv_len[b] ? rows.offset(b, Hkv, h, j) : -1;
-    float x[16];
+                                                      T* __restrict__ k_out, T* __restrict__ v_out, int tiles) {
+    constexpr int kN = 16 / sizeof(T);                         // codes of a load
+    constexpr int kPerRow = kHeadDim / kN, kLoads = kReadRows * kPerRow / 256;
+    constexpr int kStep = 256 / kPerRow;                       // rows between a thread's loads
+    const int bh = blockIdx.x / tiles, j0 = (blockIdx.x - bh * tiles) * kReadRows;
+    const int b = bh / Hkv, h = bh - b * Hkv;
+    const int r0 = threadIdx.x / kPerRow, c = kN * (threadIdx.x % kPerRow);
+    const uint8_t *pool = blockIdx.y ? v_pool : k_pool, *scales = blockIdx.y ? v_scale : k_scale;
+    const int64_t len = kv_len[b], off = j0 < len ? rows.offset(b, Hkv, h, j0) : -1;
+    const int n = off < 0 ? 0 : (int)min((int64_t)kReadRows, len - j0);  // rows of the tile that have values
+    const int out_rows = (int)min((int64_t)kReadRows, max_kv - j0);
+    uint32_t w[kLoads][kN / 4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = 0.f;
-    if (off >= 0) {
-        const uint4 w = *reinterpret_cast<const uint4*>((blockIdx.y ? v_pool : k_pool) + off + 16 * c);
-        const float scale = scale_of((blockIdx.y ? v_scale : k_scale)[off / kHeadDim / kBlockRows8]);
-        values4(w.x, x);
-        values4(w.y, x + 4);
-        values4(w.z, x + 8);
-        values4(w.w, x + 12);
+    for (int i = 0; i < kLoads; ++i) {
+        const int r = r0 + kStep * i;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= scale;
+        for (int x = 0; x < kN / 4; ++x)
+            w[i][x] = r < n ? reinterpret_cast<const uint32_t*>(pool + off + r * kHeadDim + c)[x] : 0u;
     }
-    T* out = (blockIdx.y ? v_out : k_out) + row * kHeadDim + 16 * c;
-    float y[8];
+    float scale[2] = {0.f, 0.f};
+    if (n > 0) {
+        const uint8_t* s = scales + off / (kHeadDim * kBlockRows8);
+        scale[0] = scale_of(s[0]);
+        scale[1] = n > kBlockRows8 ? scale_of(s[1]) : 0.f;
+    }
+    T* out = (blockIdx.y ? v_out : k_out) + ((int64_t)bh * max_kv + j0) * kHeadDim + c;
 #pragma unroll
-    for (int h8 = 0; h8 < 16; h8 += 8) {
+    for (int i = 0; i < kLoads; ++i) {
+        const int r = r0 + kStep * i;
+        float x[kN];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[h8 + i];
-        store8(out + h8, y);
+        for (int y = 0; y < kN / 4; ++y) values4(w[i][y], x + 4 * y);
+#pragma unroll
+        for (int y = 0; y < kN; ++y) x[y] *= scale[r / kBlockRows8];
+        if (r < out_rows) store_streamed(out + r * kHeadDim, x);
     }
 }
 
@@ -350,19 +372,18 @@ extern "C" int crane_hip_read_paged_f8(const void* k_pool, const void* v_pool, c
     if (!kv_len || !k_out || !v_out) return CRANE_HIP_E_INVALID;
     if ((rc = check_pools8(k_pool, v_pool, k_scale, v_scale))) return rc;
     if (!aligned16(k_out) || !aligned16(v_out)) return CRANE_HIP_E_ALIGN;
-    const int64_t heads = (int64_t)B * Hkv;
-    if (heads > 0xffffffffLL / 16 || max_kv > 0xffffffffLL / 16 / heads) return CRANE_HIP_E_INVALID;  // threads of a grid
-    const int64_t n = heads * max_kv * 8;
-    const dim3 grid((unsigned)((n + 255) / 256), 2);
+    const int64_t heads = (int64_t)B * Hkv, tiles = (max_kv + kReadRows - 1) / kReadRows;
+    if (heads > 0xffffffLL || tiles > 0xffffffLL / heads) return CRANE_HIP_E_INVALID;  // a grid's threads: 32 bits
+    const dim3 grid((unsigned)(heads * tiles), 2);
     const PagedRows rows{block_table, table_stride, n_pages, page_rows};
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == CRANE_HIP_F32)
         hipLaunchKernelGGL(f8_read_kernel<float>, grid, dim3(256), 0, st, (const uint8_t*)k_pool,
                            (const uint8_t*)v_pool, (const uint8_t*)k_scale, (const uint8_t*)v_scale, rows, kv_len,
-                           max_kv, Hkv, (float*)k_out, (float*)v_out, n);
+                           max_kv, Hkv, (float*)k_out, (float*)v_out, (int)tiles);
     else
         hipLaunchKernelGGL(f8_read_kernel<bf16_t>, grid, dim3(256), 0, st, (const uint8_t*)k_pool,
                            (const uint8_t*)v_pool, (const uint8_t*)k_scale, (const uint8_t*)v_scale, rows, kv_len,
-                           max_kv, Hkv, (bf16_t*)k_out, (bf16_t*)v_out, n);
+                           max_kv, Hkv, (bf16_t*)k_out, (bf16_t*)v_out, (int)tiles);
     return launch_status(hipGetLastError());
 }

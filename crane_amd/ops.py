@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import functools
 import math
 from typing import Optional, Sequence
 
@@ -659,15 +660,34 @@ def f8_pools(n_pages: int, num_kv_heads: int, page_rows: int = PAGE_ALIGN, devic
     return tuple([t.view(torch.float8_e4m3fn) for t in codes] + [t.view(torch.float8_e8m0fnu) for t in scales])
 
 
-def _f8_args(pools: Sequence[torch.Tensor], block_table: torch.Tensor, B: int, index: int):
-    """Checks of the pools and the block table; (n_pages, Hkv, page_rows, stride)."""
-    if len(pools) != 4:
-        raise CraneHipError(_lib.E_INVALID, "pools must be (K codes, V codes, K scales, V scales)")
-    k, v, ks, vs = pools
-    shape = k.shape
-    if not (k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == block_table.get_device() ==
-            index >= 0):
-        _dev(k, v, ks, vs, block_table)
+def _f8_call(index: int, call, *args) -> int:
+    """call(*args, stream) with the device `index` current and its current stream (_on_device and
+    _stream, for callers that have the index and no device object)."""
+    if torch._C._cuda_getDevice() == index:
+        return call(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return call(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _f8_args(pools: Sequence[torch.Tensor], block_table: torch.Tensor, kv_len: torch.Tensor, B: int, index: int):
+    """Checks of the pools, the block table and the lengths [B] on the device `index`: (K codes,
+    V codes, K scales, V scales, the pools' shape)."""
+    try:
+        k, v, ks, vs = pools
+    except ValueError:
+        raise CraneHipError(_lib.E_INVALID, "pools must be (K codes, V codes, K scales, V scales)") from None
+    shape, tb = k.shape, block_table.shape
+    # One expression for what every call passes; the cases that fail it are told apart below.
+    if index == k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == block_table.get_device() == \
+            kv_len.get_device() and index >= 0 and \
+            len(shape) == 4 and shape[3] == HEAD_DIM and v.shape == shape and shape[2] % F8_BLOCK_ROWS == 0 and \
+            ks.shape == vs.shape == (shape[0], shape[1], shape[2] // F8_BLOCK_ROWS) and \
+            k.dtype is v.dtype is torch.float8_e4m3fn and ks.dtype is vs.dtype is torch.float8_e8m0fnu and \
+            block_table.dtype is kv_len.dtype is torch.int32 and len(tb) == 2 and tb[0] == B == kv_len.numel() and \
+            k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and \
+            block_table.is_contiguous() and kv_len.is_contiguous():
+        return k, v, ks, vs, shape
+    if _dev(k, v, ks, vs, block_table, kv_len).index != index:
         raise CraneHipError(_lib.E_INVALID, "tensors on different devices")
     if not (k.dtype == v.dtype == torch.float8_e4m3fn and ks.dtype == vs.dtype == torch.float8_e8m0fnu):
         raise CraneHipError(_lib.E_DTYPE, "pools must be float8_e4m3fn, scales float8_e8m0fnu")
@@ -675,12 +695,10 @@ def _f8_args(pools: Sequence[torch.Tensor], block_table: torch.Tensor, B: int, i
         raise CraneHipError(_lib.E_INVALID, "pools must be [n_pages, Hkv, page_rows, D]")
     if not ks.shape == vs.shape == (shape[0], shape[1], shape[2] // F8_BLOCK_ROWS):
         raise CraneHipError(_lib.E_INVALID, "scales must be [n_pages, Hkv, page_rows / 32]")
-    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
-        raise CraneHipError(_lib.E_INVALID, "pools and scales must be contiguous")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or \
-            not block_table.is_contiguous():
-        raise CraneHipError(_lib.E_INVALID, "block_table must be a contiguous int32 [B, max_pages] tensor")
-    return shape[0], shape[1], shape[2], block_table.shape[1]
+    for t, name in ((k, "K codes"), (v, "V codes"), (ks, "K scales"), (vs, "V scales")):
+        _contig(t, name)
+    _i32(kv_len, B, "kv_len" if kv_len.dim() else "lengths")
+    raise CraneHipError(_lib.E_INVALID, "block_table must be a contiguous int32 [B, max_pages] tensor")
 
 
 def qk_norm_rope_append_paged_f8(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
@@ -694,22 +712,44 @@ def qk_norm_rope_append_paged_f8(qkv: torch.Tensor, cos: torch.Tensor, sin: torc
     f32 throughout and rounded once, q to qkv's dtype and k and v to their codes.  A
     block of 32 rows takes the smallest scale that holds its new rows, or keeps its own
     where that is larger; where it grows, the codes it held are rounded to it."""
-    if qkv.dim() != 3:
+    shape, dtype = qkv.shape, qkv.dtype
+    if len(shape) != 3:
         raise CraneHipError(_lib.E_INVALID, "qkv must be [B, S, (Hq+2Hkv)*D]")
-    n_pages, Hkv, page_rows, stride = _f8_args(pools, block_table, qkv.shape[0], qkv.get_device())
-    dev, B, S = _rope_inputs(qkv, (num_heads + 2 * Hkv) * HEAD_DIM, cos, sin, positions, q_norm_w, k_norm_w, order)
-    _dev(qkv, cache_len)
-    dt = _dtype_code(qkv)
-    _i32(cache_len, B, "cache_len")
-    q_out = torch.empty((B, num_heads, S, HEAD_DIM), dtype=qkv.dtype, device=dev)
+    B, S, width = shape
+    index = qkv.get_device()
+    k, v, ks, vs, pshape = _f8_args(pools, block_table, cache_len, B, index)
+    n_pages, Hkv, page_rows, _ = pshape
+    dt, table = _dtype_code_of(dtype), cos.shape
+    # What _rope_inputs checks, in one expression where the rows are contiguous.
+    if (positions is cache_len or (positions.dtype is torch.int32 and positions.numel() == B and
+                                   positions.is_contiguous() and positions.get_device() == index)) and \
+            qkv.is_contiguous() and width == (num_heads + 2 * Hkv) * HEAD_DIM and \
+            index == cos.get_device() == sin.get_device() and cos.dtype is sin.dtype is dtype and \
+            len(table) == 2 and table[1] == HEAD_DIM // 2 and sin.shape == table and cos.is_contiguous() and \
+            sin.is_contiguous() and order in _ORDERS and all([
+                w is None or (w.dtype is dtype and w.numel() == HEAD_DIM and w.get_device() == index and w.is_contiguous())
+                for w in (q_norm_w, k_norm_w)]):
+        row_stride = width
+    else:
+        _rope_inputs(qkv, (num_heads + 2 * Hkv) * HEAD_DIM, cos, sin, positions, q_norm_w, k_norm_w, order)
+        row_stride = qkv.stride(1)
+    q_out = qkv.new_empty((B, num_heads, S, HEAD_DIM))
     if B == 0:  # an empty block table has no address
         return q_out
-    args = (qkv.data_ptr(), qkv.stride(1), _ptr(q_norm_w), _ptr(k_norm_w), eps, _ORDERS[order], cos.data_ptr(),
-            sin.data_ptr(), cos.stride(0), cos.shape[0], positions.data_ptr(), q_out.data_ptr(),
-            *[t.data_ptr() for t in pools], n_pages, page_rows, block_table.data_ptr(), stride, cache_len.data_ptr(), B,
-            S, num_heads, Hkv, HEAD_DIM, dt, _stream(dev))
-    check(_on_device(dev, _lib.lib().crane_hip_qknorm_rope_append_paged_f8, args), "qk_norm_rope_append_paged_f8")
+    rc = _f8_call(index, _lib.lib().crane_hip_qknorm_rope_append_paged_f8, qkv.data_ptr(), row_stride, _ptr(q_norm_w),
+                  _ptr(k_norm_w), eps, _ORDERS[order], cos.data_ptr(), sin.data_ptr(), HEAD_DIM // 2, table[0],
+                  positions.data_ptr(), q_out.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+                  n_pages, page_rows, block_table.data_ptr(), block_table.shape[1], cache_len.data_ptr(), B, S,
+                  num_heads, Hkv, HEAD_DIM, dt)
+    if rc:
+        check(rc, "qk_norm_rope_append_paged_f8")
     return q_out
+
+
+@functools.lru_cache(maxsize=256)
+def _f8_workspace(max_kv: int, B: int, S: int, Hq: int, Hkv: int, dt: int) -> int:
+    """The workspace's bytes for these sizes (a step's layers all ask for the same)."""
+    return _lib.lib().crane_hip_attn_paged_f8_workspace(max_kv, B, S, Hq, Hkv, HEAD_DIM, dt)
 
 
 def attention_paged_f8(q: torch.Tensor, pools: Sequence[torch.Tensor], block_table: torch.Tensor,
@@ -723,38 +763,40 @@ def attention_paged_f8(q: torch.Tensor, pools: Sequence[torch.Tensor], block_tab
 
     Scores, softmax and sums are f32 (attention_decode_paged rounds every score as
     candle does)."""
-    index = q.get_device()
-    if index < 0 or kv_len.get_device() != index:
-        _dev(q, kv_len)
     shape = q.shape
-    if len(shape) not in (3, 4) or shape[-1] != HEAD_DIM:
-        raise CraneHipError(_lib.E_HEAD_DIM if len(shape) in (3, 4) else _lib.E_INVALID,
-                            "q must be [B, Hq, 128] or [B, Hq, S, 128]")
-    B, Hq = shape[0], shape[1]
-    S = shape[2] if len(shape) == 4 else 1
-    n_pages, Hkv, page_rows, stride = _f8_args(pools, block_table, B, index)
-    _contig(q, "q")
-    dt = _dtype_code(q)
-    _i32(kv_len, B, "kv_len")
-    lib, dev = _lib.lib(), q.device
+    if len(shape) == 3:
+        B, Hq, D = shape
+        S = 1
+    elif len(shape) == 4:
+        B, Hq, S, D = shape
+    else:
+        raise CraneHipError(_lib.E_INVALID, "q must be [B, Hq, 128] or [B, Hq, S, 128]")
+    if D != HEAD_DIM:
+        raise CraneHipError(_lib.E_HEAD_DIM, "q must be [B, Hq, 128] or [B, Hq, S, 128]")
+    index = q.get_device()
+    k, v, ks, vs, pshape = _f8_args(pools, block_table, kv_len, B, index)
+    n_pages, Hkv, page_rows, _ = pshape
+    if not q.is_contiguous():
+        _contig(q, "q")
+    dt = _dtype_code_of(q.dtype)
     out = q.new_empty((B, S, Hq * HEAD_DIM))
-    if B == 0:
+    if B == 0:  # an empty block table has no address
         return out
-    need = lib.crane_hip_attn_paged_f8_workspace(max_kv, B, S, Hq, Hkv, HEAD_DIM, dt)
+    need = _f8_workspace(max_kv, B, S, Hq, Hkv, dt)
     # Allocated per call, not kept per stream: a captured graph keeps its own.
+    ws = None
     if workspace is not None:
         _dev(q, workspace)
-        ws_bytes = workspace.numel() * workspace.element_size()
+        need, ws = workspace.numel() * workspace.element_size(), workspace.data_ptr()
     elif need:
-        workspace, ws_bytes = torch.empty(need, dtype=torch.uint8, device=dev), need
-    else:
-        ws_bytes = 0
-    k, v, ks, vs = pools
-    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), n_pages, page_rows,
-            block_table.data_ptr(), stride, kv_len.data_ptr(), max_kv, B, S, Hq, Hkv, HEAD_DIM,
-            _SCALE if scale is None else scale, PREFILL_CAUSAL if causal else 0, _ptr(workspace), ws_bytes,
-            out.data_ptr(), dt, _stream(dev))
-    check(_on_device(dev, lib.crane_hip_attn_paged_f8, args), "attention_paged_f8")
+        workspace = q.new_empty(need // q.element_size())  # need is a multiple of 16
+        ws = workspace.data_ptr()
+    rc = _f8_call(index, _lib.lib().crane_hip_attn_paged_f8, q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
+                  vs.data_ptr(), n_pages, page_rows, block_table.data_ptr(), block_table.shape[1], kv_len.data_ptr(),
+                  max_kv, B, S, Hq, Hkv, HEAD_DIM, _SCALE if scale is None else scale,
+                  PREFILL_CAUSAL if causal else 0, ws, need, out.data_ptr(), dt)
+    if rc:
+        check(rc, "attention_paged_f8")
     return out
 
 
@@ -762,22 +804,23 @@ def read_paged_f8(pools: Sequence[torch.Tensor], block_table: torch.Tensor, kv_l
                   dtype: torch.dtype = torch.bfloat16):
     """The rows of every sequence of a paged cache in 8 bits as values: (k, v)
     [B, Hkv, max_kv, D] in `dtype` (exact in bf16 too), zeros from kv_len on."""
-    if block_table.dim() != 2:
-        raise CraneHipError(_lib.E_INVALID, "block_table must be a contiguous int32 [B, max_pages] tensor")
-    B = block_table.shape[0]
-    n_pages, Hkv, page_rows, stride = _f8_args(pools, block_table, B, block_table.get_device())
-    dev = _dev(block_table, kv_len)
+    B = block_table.shape[0] if block_table.dim() else 0
+    index = block_table.get_device()
+    k, v, ks, vs, pshape = _f8_args(pools, block_table, kv_len, B, index)
+    n_pages, Hkv, page_rows, _ = pshape
     dt = _dtype_code_of(dtype)
-    _i32(kv_len, B, "kv_len")
     if max_kv < 0:
         raise CraneHipError(_lib.E_INVALID, f"max_kv {max_kv}")
-    k, v = (torch.empty((B, Hkv, max_kv, HEAD_DIM), dtype=dtype, device=dev) for _ in "kv")
-    if B == 0:
-        return k, v
-    args = (*[t.data_ptr() for t in pools], n_pages, page_rows, block_table.data_ptr(), stride, kv_len.data_ptr(),
-            max_kv, B, Hkv, HEAD_DIM, k.data_ptr(), v.data_ptr(), dt, _stream(dev))
-    check(_on_device(dev, _lib.lib().crane_hip_read_paged_f8, args), "read_paged_f8")
-    return k, v
+    k_out = torch.empty((B, Hkv, max_kv, HEAD_DIM), dtype=dtype, device=block_table.device)
+    v_out = torch.empty_like(k_out)
+    if B == 0:  # an empty block table has no address
+        return k_out, v_out
+    rc = _f8_call(index, _lib.lib().crane_hip_read_paged_f8, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+                  n_pages, page_rows, block_table.data_ptr(), block_table.shape[1], kv_len.data_ptr(), max_kv, B, Hkv,
+                  HEAD_DIM, k_out.data_ptr(), v_out.data_ptr(), dt)
+    if rc:
+        check(rc, "read_paged_f8")
+    return k_out, v_out
 
 
 # ------------------------------------------------------- decoder-layer rows

@@ -682,7 +682,7 @@ def test_attention_wants_its_workspace():
 
 @pytest.mark.parametrize("kw,code", SHARED + [
     (dict(max_kv=-1), 1), (dict(max_kv=513), 5), (dict(B=1, ko=None), 1), (dict(B=1, vo=None), 1), (dict(B=1, ko=8), 8),
-    (dict(B=1, vo=8), 8), (dict(B=2 ** 30, Hkv=8), 1), (dict(B=2 ** 20, max_kv=512), 1), (dict(), 0), (dict(B=1, max_kv=0), 0)])
+    (dict(B=1, vo=8), 8), (dict(B=2 ** 30, Hkv=8), 1), (dict(B=2 ** 22, max_kv=512), 1), (dict(), 0), (dict(B=1, max_kv=0), 0)])
 def test_read_refuses(kw, code):
     assert _read(**kw) == code
 
