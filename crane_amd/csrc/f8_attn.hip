@@ -260,9 +260,9 @@ template <typename T, typename C> __device__ __forceinline__ C product(u32x4_v a
     return c;
 }
 
-// Maximum and sum over the four lane groups of a query row; every lane gets them.  (A row
-// swap of a value with itself leaves each row's value in one result and its neighbour's
-// in the other.)
+// Maximum over the four lane groups of a query row; every lane gets it.  (A row swap of a
+// value with itself leaves each row's value in one result and its neighbour's in the
+// other.)
 __device__ __forceinline__ float groups_max(float x) {
     const uint32_t u = __float_as_uint(x);
     const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
@@ -270,14 +270,6 @@ __device__ __forceinline__ float groups_max(float x) {
     const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
-__device__ __forceinline__ float groups_sum(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t v = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-    const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
-}
-
 // LDS byte addresses, and reads at them.
 __device__ __forceinline__ uint32_t lds_at(const void* p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
@@ -328,7 +320,10 @@ template <typename T, int RT> struct Stream {
     Scales ks, vs;
     Parts<T> q[RT][4];      // dims 16 g .., 16 g + 8 .., 64 + 16 g .., 64 + 16 g + 8 ..
     f32x4_v o[RT][8];       // dims 16 n + 4 g + r of row i
-    float m[RT], l[RT];     // l: over the lane's own keys
+    f32x4_v l[RT];          // the sum over all keys, in all four
+    float m[RT], mc[RT];    // the raw score p's exponent counts from, and m c (0 before the first key)
+    float limit[RT];        // a score past this moves m
+    bool big;               // some m c has lost bits below 1: its row's exponents are (s - m) c
 
     __device__ __forceinline__ Stream(int ln, uint8_t* lds) : lane(ln), i(ln & 15), g(ln >> 4) {
         k_lds = lds_at(lds);
@@ -348,9 +343,12 @@ template <typename T, int RT> struct Stream {
             for (int n = 0; n < 8; ++n)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[t][n][r] = 0.f;
-            m[t] = kNoMax;
-            l[t] = 0.f;
+            m[t] = limit[t] = kNoMax;
+            mc[t] = 0.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) l[t][r] = 0.f;
         }
+        big = false;
     }
     // Start the copies of a tile.
     __device__ __forceinline__ void copy(const Args8& a, const Pages8::Tile& t, uint8_t* lds) const {
@@ -401,39 +399,54 @@ template <typename T, int RT> struct Stream {
     }
     // Weights p = exp2((s - m) c) in place of the scores.  m moves, and o and l are scaled,
     // only where a score passes it by kSlack (as a power of two): f32 and bf16 hold larger
-    // weights as exactly.  m is kept as a raw score, so that a product with c that has no
-    // bits left below 1 costs nothing.
-    static constexpr float kSlack = 16.f;
+    // weights as exactly.  s c - m c is one product with one rounding, which leaves every
+    // weight of the row the factor exp2(the rounding of m c); o / l takes that out again,
+    // but it overflows or vanishes where half a step of m c passes a hundred: past
+    // kMostMax the difference is taken first.
+    static constexpr float kSlack = 16.f, kMostMax = 0x1p26f;
     __device__ __forceinline__ void weights(float (&s)[RT][16], float c) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             float mx = s[t][0];
 #pragma unroll
             for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
-            if (__any((mx - m[t]) * c > kSlack)) {
+            if (__any(mx > limit[t])) {
                 const float to = fmaxf(m[t], groups_max(mx)), f = fast_exp2((m[t] - to) * c);
                 m[t] = to;
-                l[t] *= f;
+                mc[t] = to == kNoMax ? 0.f : to * c;
+                limit[t] = to == kNoMax ? kNoMax : to + kSlack / c;
+                big = __any(big || !(fabsf(mc[t]) <= kMostMax));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) l[t][r] *= f;
 #pragma unroll
                 for (int n = 0; n < 8; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[t][n][r] *= f;
             }
-            float sum = 0.f;
+        }
+        if (big) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[t][e] = fast_exp2((s[t][e] - m[t]) * c);
-                sum += s[t][e];
-            }
-            l[t] += sum;
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[t][e] = fast_exp2((s[t][e] - m[t]) * c);
+        } else {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[t][e] = fast_exp2(__builtin_fmaf(s[t][e], c, -mc[t]));
         }
     }
+    // o += P V, and l with it: a product of ones sums the weights as they are rounded.
     __device__ __forceinline__ void accumulate(const float (&p)[RT][16]) {
+        const u32x4_v ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             Parts<T> w[RT];
 #pragma unroll
-            for (int t = 0; t < RT; ++t) w[t].set(&p[t][8 * u]);
+            for (int t = 0; t < RT; ++t) {
+                w[t].set(&p[t][8 * u]);
+                l[t] = product(ones, w[t], l[t]);
+            }
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 const u32x4_v x = widen(v[u][n].x, v[u][n].y, vs.of[u]);
@@ -589,10 +602,9 @@ __global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1
     __syncthreads();  // every wave's tiles are read
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        const float l = groups_sum(st.l[t]);
         if (st.g == 0) {
             sm.join.m[wave][16 * t + st.i] = st.m[t];
-            sm.join.l[wave][16 * t + st.i] = l;
+            sm.join.l[wave][16 * t + st.i] = st.l[t][0];
         }
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
