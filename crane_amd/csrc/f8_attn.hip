@@ -27,6 +27,7 @@ namespace crane {
 namespace {
 
 constexpr float kNoMax = -FLT_MAX;  // m before the first key (finite: exp2(-inf - m) is 0, not NaN)
+constexpr float kSlack = 16.f, kMostMax = 0x1p26f;  // see Rows8
 constexpr int kTile = 64;           // keys of a tile: two blocks, within one page
 constexpr int kRow = kHeadDim;      // bytes of a row of codes
 constexpr int kTileBytes = kTile * kRow;
@@ -188,6 +189,10 @@ struct Pages8 {
     }
 };
 
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint8_t* pool, const Pages8::Tile& t) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(pool) + t.off, (short)0, t.bytes, 0x00020000);
+}
+
 // The scales of a tile's two blocks, as f32 (read through the constant address space: one
 // scalar load).  A byte of a block without rows may be anything; 254 keeps 0 times it 0.
 struct Scales {
@@ -215,6 +220,11 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7
 
 __device__ __forceinline__ f32x4_v mfma(u32x4_v a, u32x4_v b, f32x4_v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c,
+                                                   0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16_v mfma(u32x4_v a, u32x4_v b, f32x16_v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c,
                                                    0, 0, 0);
 }
 
@@ -290,93 +300,82 @@ __device__ __forceinline__ uint2 lds_read_tr8(uint32_t at) {
 __device__ __forceinline__ void wait_memory() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
-// ---- the stream form: 16 RT query rows a wave, every wave walking tiles of its own
-//
-// A wave copies its next tile of K and V (8 KiB each) into LDS of its own while it works
-// on the one in its registers: the copies are asynchronous, take whole 128-byte rows, and
-// hold no registers, which the reads could not do for the layouts the products want.
-// LDS keeps the rows (128 bytes, half a sweep of the banks) with their 16-byte chunks
-// XOR-permuted by f(row) below, so that neither the 16 rows of a K read nor the 16 rows of
-// two lane groups' transposed V reads meet in a bank.
+// A tile of K or V in LDS keeps the pools' rows (128 bytes, half a sweep of the banks) with
+// their 16-byte chunks XOR-permuted by permute8(row), so that neither the 16 rows of a K
+// read nor the 16 rows of two lane groups' transposed V reads meet in a bank.
 //
 // v_mfma_f32_16x16x32_bf16, S^T = K Q^T with K rows as A: lane (i, g) = (lane % 16, lane /
 // 16) holds, for query row i, rows 4 g + r of the product.  A's row x of product (u, b) is
 // key 32 u + 8 (x / 4) + 4 b + x % 4, so that over b the lane holds keys 32 u + 8 g + (0 ..
 // 7): as P^T, the B operand of O^T = V^T P^T as they stand, with V's bytes of those keys
 // from one transposed read.
-
-// The chunk permutation of a tile's row.
 __device__ __forceinline__ int permute8(int row) {
     return ((row >> 1) & 1) | ((row >> 2) & 2) | ((((row >> 4) ^ (row >> 2)) & 1) << 2);
 }
+// The byte of a tile that instruction x of its copy (1 KiB, 8 rows) takes for a lane.
+__device__ __forceinline__ int copy_from(int x, int lane) {
+    const int row = 8 * x + (lane >> 3);
+    return row * kRow + 16 * ((lane & 7) ^ permute8(row));
+}
+// A lane's reads of tiles that start at k and v.
+struct TileReads {
+    uint32_t k, v;
+    __device__ __forceinline__ TileReads(uint32_t k_lds, uint32_t v_lds, int lane) {
+        const int i = lane & 15, g = lane >> 4, k_row = 8 * (i >> 2) + (i & 3), v_row = 8 * g + (i >> 1);
+        k = k_lds + k_row * kRow + 16 * (g ^ permute8(k_row));
+        v = v_lds + v_row * kRow + 16 * permute8(v_row) + 8 * (i & 1);
+    }
+    // Dims 64 half + 16 g .. of the key that is row i of product kt = 2 u + b (4 rows on, or 4
+    // chunks, bit 2 of the chunk flips).
+    __device__ __forceinline__ u32x4_v key(int kt, int half, uint32_t buf) const {
+        return lds_read16((k ^ (((kt & 1) ^ half) << 6)) + buf + 32 * (kt >> 1) * kRow + 4 * (kt & 1) * kRow);
+    }
+    // Keys 32 u + 8 g .. of dim 16 n + i.
+    __device__ __forceinline__ uint2 value(int u, int n, uint32_t buf) const {
+        return lds_read_tr8((v ^ (16 * n)) + buf + 32 * u * kRow);
+    }
+};
 
-template <typename T, int RT> struct Stream {
-    const int lane, i, g;
-    uint32_t k_lds, v_lds;  // the wave's tiles in LDS
-    int from[4];            // byte of a tile that instruction x (mod 4) copies for this lane
-    uint32_t k_at, v_at;    // where this lane's reads start
-    u32x4_v k[4][2];        // [2 u + b][half]: the key's dims 64 half + 16 g ..
-    uint2 v[2][8];          // [u][n]: keys 32 u + 8 g .. of dim 16 n + i
-    Scales ks, vs;
-    Parts<T> q[RT][4];      // dims 16 g .., 16 g + 8 .., 64 + 16 g .., 64 + 16 g + 8 ..
-    f32x4_v o[RT][8];       // dims 16 n + 4 g + r of row i
-    f32x4_v l[RT];          // the sum over all keys, in all four
-    float m[RT], mc[RT];    // the raw score p's exponent counts from, and m c (0 before the first key)
-    float limit[RT];        // a score past this moves m
-    bool big;               // some m c has lost bits below 1: its row's exponents are (s - m) c
+// A wave's 16 RT query rows: their q and their running results.
+template <typename T, int RT> struct Rows8 {
+    const int i, g;
+    Parts<T> q[RT][4];    // dims 16 g .., 16 g + 8 .., 64 + 16 g .., 64 + 16 g + 8 ..
+    f32x4_v o[RT][8];     // dims 16 n + 4 g + r of row i
+    f32x4_v l[RT];        // the sum over all keys, in all four
+    float m[RT], mc[RT];  // the raw score p's exponent counts from, and m c (0 before the first key)
+    float limit[RT];      // a score past this moves m
+    bool big;             // some m c has lost bits below 1: its row's exponents are (s - m) c
 
-    __device__ __forceinline__ Stream(int ln, uint8_t* lds) : lane(ln), i(ln & 15), g(ln >> 4) {
-        k_lds = lds_at(lds);
-        v_lds = k_lds + kTileBytes;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int row = 8 * x + (lane >> 3);
-            from[x] = row * kRow + 16 * ((lane & 7) ^ permute8(row));
-        }
-        const int k_row = 8 * (i >> 2) + (i & 3);
-        k_at = k_lds + k_row * kRow + 16 * (g ^ permute8(k_row));
-        const int v_row = 8 * g + (i >> 1);
-        v_at = v_lds + v_row * kRow + 16 * permute8(v_row) + 8 * (i & 1);
+    __device__ __forceinline__ explicit Rows8(int lane) : i(lane & 15), g(lane >> 4), big(false) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
 #pragma unroll
             for (int n = 0; n < 8; ++n)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[t][n][r] = 0.f;
-            m[t] = limit[t] = kNoMax;
-            mc[t] = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) l[t][r] = 0.f;
-        }
-        big = false;
-    }
-    // Start the copies of a tile.
-    __device__ __forceinline__ void copy(const Args8& a, const Pages8::Tile& t, uint8_t* lds) const {
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.k) + t.off, (short)0, t.bytes, 0x00020000);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.v) + t.off, (short)0, t.bytes, 0x00020000);
-#pragma unroll
-        for (int x = 0; x < 8; ++x)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lds + 1024 * x, 16, from[x & 3] + 4096 * (x >> 2), 0, 0, 2);
-#pragma unroll
-        for (int x = 0; x < 8; ++x)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, lds + kTileBytes + 1024 * x, 16, from[x & 3] + 4096 * (x >> 2),
-                                                     0, 0, 2);
-    }
-    // The copied tile into registers.
-    __device__ __forceinline__ void take() {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int half = 0; half < 2; ++half)  // rows 4 on and chunks 4 on: bit 2 of the chunk flips
-                    k[2 * u + b][half] = lds_read16((k_at ^ ((b ^ half) << 6)) + 32 * u * kRow + 4 * b * kRow);
-#pragma unroll
-            for (int n = 0; n < 8; ++n) v[u][n] = lds_read_tr8((v_at ^ (16 * n)) + 32 * u * kRow);
+            m[t] = limit[t] = kNoMax;
+            mc[t] = 0.f;
         }
     }
-    // s[t][8 u + e]: the raw score of key 32 u + 8 g + e.
-    __device__ __forceinline__ void scores(float (&s)[RT][16]) const {
+    // This lane's rows of those from row0 on: their places in q [B, Hq, S] (-1: none), the keys
+    // they see (up to `end`), and q.
+    __device__ __forceinline__ void open(const Args8& a, int b, int kvh, int row0, int n, int end, int (&at)[RT],
+                                         int (&hi)[RT]) {
+        const int R = a.S * a.G;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int r = row0 + 16 * t + i, s = min(r, R - 1) / a.G, h = min(r, R - 1) - s * a.G;
+            at[t] = r < R ? (int)(((int64_t)b * a.Hq + kvh * a.G + h) * a.S + s) : -1;  // fewer than 2^31 query rows
+            hi[t] = min(a.limit(n, s), end);
+            const T* row = reinterpret_cast<const T*>(a.q) + (int64_t)max(at[t], 0) * kHeadDim;
+#pragma unroll
+            for (int step = 0; step < 4; ++step) q[t][step].load(row + 64 * (step >> 1) + 16 * g + 8 * (step & 1));
+        }
+    }
+    // s[t][8 u + e]: the raw score of key 32 u + 8 g + e; key(kt, half) as TileReads::key.
+    template <class KEY> __device__ __forceinline__ void scores(float (&s)[RT][16], const Scales& ks, KEY key) const {
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             f32x4_v acc[RT];
@@ -385,11 +384,14 @@ template <typename T, int RT> struct Stream {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[t][r] = 0.f;
 #pragma unroll
-            for (int step = 0; step < 4; ++step) {
-                const u32x4_v& w = k[kt][step >> 1];
-                const u32x4_v x = widen(w[2 * (step & 1)], w[2 * (step & 1) + 1], ks.of[kt >> 1]);
+            for (int half = 0; half < 2; ++half) {
+                const u32x4_v w = key(kt, half);
 #pragma unroll
-                for (int t = 0; t < RT; ++t) acc[t] = product(x, q[t][step], acc[t]);
+                for (int x = 0; x < 2; ++x) {
+                    const u32x4_v y = widen(w[2 * x], w[2 * x + 1], ks.of[kt >> 1]);
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) acc[t] = product(y, q[t][2 * half + x], acc[t]);
+                }
             }
 #pragma unroll
             for (int t = 0; t < RT; ++t)
@@ -397,14 +399,17 @@ template <typename T, int RT> struct Stream {
                 for (int r = 0; r < 4; ++r) s[t][4 * kt + r] = acc[t][r];
         }
     }
-    // Weights p = exp2((s - m) c) in place of the scores.  m moves, and o and l are scaled,
-    // only where a score passes it by kSlack (as a power of two): f32 and bf16 hold larger
-    // weights as exactly.  s c - m c is one product with one rounding, which leaves every
-    // weight of the row the factor exp2(the rounding of m c); o / l takes that out again,
-    // but it overflows or vanishes where half a step of m c passes a hundred: past
-    // kMostMax the difference is taken first.
-    static constexpr float kSlack = 16.f, kMostMax = 0x1p26f;
-    __device__ __forceinline__ void weights(float (&s)[RT][16], float c) {
+    // The scores, of keys from j on, that a row does not see vanish.
+    __device__ __forceinline__ void mask(float (&s)[RT][16], int j, const int (&hi)[RT]) const {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                s[t][e] = j + 32 * (e >> 3) + 8 * g + (e & 7) < hi[t] ? s[t][e] : -INFINITY;
+    }
+    // m for these scores.  It moves, and o and l are scaled, only where a score passes it by
+    // kSlack (as a power of two): f32 and bf16 hold larger weights as exactly.
+    __device__ __forceinline__ void settle(const float (&s)[RT][16], float c) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
             float mx = s[t][0];
@@ -424,20 +429,22 @@ template <typename T, int RT> struct Stream {
                     for (int r = 0; r < 4; ++r) o[t][n][r] *= f;
             }
         }
-        if (big) {
+    }
+    // Weights p = exp2((s - m) c) in place of the scores.  s c - m c is one product with one
+    // rounding, which leaves every weight of the row the factor exp2(the rounding of m c); o / l
+    // takes that out again, but it overflows or vanishes where half a step of m c passes a
+    // hundred: past kMostMax (`big`) the difference is taken first.
+    template <bool BIG> __device__ __forceinline__ void weights(float (&s)[RT][16], float c) const {
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
+        for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[t][e] = fast_exp2((s[t][e] - m[t]) * c);
-        } else {
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[t][e] = fast_exp2(__builtin_fmaf(s[t][e], c, -mc[t]));
-        }
+            for (int e = 0; e < 16; ++e)
+                s[t][e] = fast_exp2(BIG ? (s[t][e] - m[t]) * c : __builtin_fmaf(s[t][e], c, -mc[t]));
     }
     // o += P V, and l with it: a product of ones sums the weights as they are rounded.
-    __device__ __forceinline__ void accumulate(const float (&p)[RT][16]) {
+    // value(u, n) as TileReads::value.
+    template <class VALUE>
+    __device__ __forceinline__ void accumulate(const float (&p)[RT][16], const Scales& vs, VALUE value) {
         const u32x4_v ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -449,7 +456,8 @@ template <typename T, int RT> struct Stream {
             }
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
-                const u32x4_v x = widen(v[u][n].x, v[u][n].y, vs.of[u]);
+                const uint2 y = value(u, n);
+                const u32x4_v x = widen(y.x, y.y, vs.of[u]);
 #pragma unroll
                 for (int t = 0; t < RT; ++t) o[t][n] = product(x, w[t], o[t][n]);
             }
@@ -458,7 +466,7 @@ template <typename T, int RT> struct Stream {
     // Where V holds NaN codes and some rows do not see their keys, 0 times them would reach those
     // rows: the codes become 0, and the dims that held one become NaN for the rows that see
     // the first such key, key j + 32 u + 8 g + e those with a limit past it.
-    __device__ __forceinline__ void settle_nan(int j, const int (&hi)[RT]) {
+    __device__ __forceinline__ void settle_nan(uint2 (&v)[2][8], int j, const int (&hi)[RT]) {
         uint32_t bad = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -490,6 +498,59 @@ template <typename T, int RT> struct Stream {
     }
 };
 
+// ---- the stream form: 16 RT query rows a wave, every wave walking tiles of its own
+//
+// A wave copies its next tile of K and V (8 KiB each) into LDS of its own while it works
+// on the one in its registers: the copies are asynchronous, take whole 128-byte rows, and
+// hold no registers, which the reads could not do for the layouts the products want.
+template <typename T, int RT> struct Stream : Rows8<T, RT> {
+    typedef Rows8<T, RT> Base;
+    TileReads reads;
+    int from[4];      // copy_from() of instructions x (mod 4)
+    u32x4_v k[4][2];  // TileReads::key and value of the tile
+    uint2 v[2][8];
+    Scales ks, vs;
+    __device__ __forceinline__ Stream(int lane, uint8_t* lds)
+        : Base(lane), reads(lds_at(lds), lds_at(lds) + kTileBytes, lane) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) from[x] = copy_from(x, lane);
+    }
+    // Start the copies of a tile.
+    __device__ __forceinline__ void copy(const Args8& a, const Pages8::Tile& t, uint8_t* lds) const {
+        const auto rk = tile_rsrc(a.k, t), rv = tile_rsrc(a.v, t);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, lds + 1024 * x, 16, from[x & 3] + 4096 * (x >> 2), 0, 0, 2);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, lds + kTileBytes + 1024 * x, 16, from[x & 3] + 4096 * (x >> 2),
+                                                     0, 0, 2);
+    }
+    // The copied tile into registers.
+    __device__ __forceinline__ void take() {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) k[kt][half] = reads.key(kt, half, 0);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) v[u][n] = reads.value(u, n, 0);
+    }
+    // The tile in registers, of keys from j on.  Every row sees the keys before min_hi.
+    __device__ __forceinline__ void step(const Args8& a, int j, const int (&hi)[RT], int min_hi, int end) {
+        float s[RT][16];
+        this->scores(s, ks, [&](int kt, int half) __attribute__((always_inline)) { return k[kt][half]; });
+        const bool masked = j + kTile > min(min_hi, end);
+        if (masked) this->mask(s, j, hi);
+        this->settle(s, a.c);
+        if (this->big) this->template weights<true>(s, a.c);
+        else this->template weights<false>(s, a.c);
+        if (masked && min_hi < end) this->settle_nan(v, j, hi);
+        this->accumulate(s, vs, [&](int u, int n) __attribute__((always_inline)) { return v[u][n]; });
+    }
+};
+
 // The LDS of a workgroup of W waves: their tiles, then their results.
 template <int RT, int W> union StreamLds {
     static constexpr int kStride = kHeadDim + 4;  // f32 per row: 16 rows at one column hit different banks
@@ -500,16 +561,23 @@ template <int RT, int W> union StreamLds {
     } join;
 };
 
-// Workgroup x's item: ids that are equal mod 8 run on one XCD, which so gets the row tiles
-// of a (pair, kv head), one after the other, and reads their keys through its own L2.
+// Workgroup x's item of `units` (pair, kv head) units with `tiles` row tiles each.  Ids that
+// are equal mod 8 run on one XCD: where the units come in eights it gets all tiles of a
+// unit, one after the other, and reads their keys through its own L2.  Otherwise a unit's
+// tiles are on all XCDs (4 units of 66 tiles, 6000 keys: on 4 XCDs 88 us, on all 52).
 struct Item8 {
     int block, kvh, pair;
-    __device__ __forceinline__ Item8(int x, int tiles, int Hkv) {
-        const int c = x / (8 * tiles), rem = x - c * 8 * tiles;
-        block = rem >> 3;
-        const int unit = 8 * c + (rem & 7);
-        pair = unit / Hkv;
-        kvh = unit - pair * Hkv;
+    __device__ __forceinline__ Item8(const Args8& a, int x) {
+        const int units = (a.pairs ? a.pairs : a.B) * a.Hkv;
+        int unit = x / a.tiles;
+        block = x - unit * a.tiles;
+        if (units % 8 == 0) {
+            const int c = x / (8 * a.tiles), rem = x - c * 8 * a.tiles;
+            block = rem >> 3;
+            unit = 8 * c + (rem & 7);
+        }
+        pair = unit / a.Hkv;
+        kvh = unit - pair * a.Hkv;
     }
 };
 
@@ -518,7 +586,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1
     __shared__ StreamLds<RT, W> sm;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Item8 x(blockIdx.x, a.tiles, a.Hkv);
+    const Item8 x(a, blockIdx.x);
     const int R = a.S * a.G, row0 = x.block * 16 * RT;
     // The tile's first and last queries; the last sees most.
     const int first = row0 / a.G, last = (min(row0 + 16 * RT, R) - 1) / a.G;
@@ -560,15 +628,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1
     const int min_hi = a.limit(n, first);
 
     int at[RT], hi[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const int r = row0 + 16 * t + st.i, s = min(r, R - 1) / a.G, h = min(r, R - 1) - s * a.G;
-        at[t] = r < R ? (int)(((int64_t)b * a.Hq + x.kvh * a.G + h) * a.S + s) : -1;  // fewer than 2^31 query rows
-        hi[t] = min(a.limit(n, s), end);
-        const T* row = reinterpret_cast<const T*>(a.q) + (int64_t)max(at[t], 0) * kHeadDim;
-#pragma unroll
-        for (int step = 0; step < 4; ++step) st.q[t][step].load(row + 64 * (step >> 1) + 16 * st.g + 8 * (step & 1));
-    }
+    st.open(a, b, x.kvh, row0, n, end, at, hi);
     constexpr int kStride = W * kTile;
     for (; j < end; j += kStride) {
         st.ks.load(a.k_scale, tile.off);
@@ -583,19 +643,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1
             st.copy(a, tile, sm.tile[wave]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        float s[RT][16];
-        st.scores(s);
-        const bool masked = j + kTile > min(min_hi, end);
-        if (masked) {
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    s[t][e] = j + 32 * (e >> 3) + 8 * st.g + (e & 7) < hi[t] ? s[t][e] : -INFINITY;
-        }
-        st.weights(s, a.c);
-        if (masked && min_hi < end) st.settle_nan(j, hi);
-        st.accumulate(s);
+        st.step(a, j, hi, min_hi, end);
     }
 
     T* out = reinterpret_cast<T*>(a.out);
@@ -643,6 +691,240 @@ __global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1
             if (d == 0) a.ws_ml[slot] = make_float2(top, l);
         }
     }
+}
+
+// ---- the block form: 128 query rows a workgroup, a tile of keys shared by its waves
+//
+// 32 rows to a wave and every wave on the same tile: the workgroup reads K and V once for
+// 128 rows.  Tiles are copied one ahead into the other of two buffers, a quarter of each by
+// every wave.  v_mfma_f32_32x32x16_bf16 (half the instructions and operand reads of the
+// 16-row product for the same work): lane (i, h) = (lane % 32, lane / 32) holds, for query
+// row i, rows 8 a + 4 h + c of a product (register 4 a + c).  A's row x is key 16 (x / 16)
+// + 8 (x / 4 % 2) + 4 (x / 8 % 2) + x % 4 of 32, so that the lane holds keys 16 s + 8 h +
+// (0 .. 7), s = 0, 1: P^T of two products with V^T, whose bytes are one transposed read
+// each.
+struct BlockLds {
+    __attribute__((aligned(1024))) uint8_t k[2][kTileBytes];
+    __attribute__((aligned(1024))) uint8_t v[2][kTileBytes];
+};
+// The chunk permutation of these tiles: 16 rows of a K read, and 8 rows x 2 chunks of a V
+// read, do not meet in a bank.
+__device__ __forceinline__ int permute8_block(int row) { return ((row >> 3) & 1) | (row & 6); }
+
+__device__ __forceinline__ float halves_max(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <typename T> struct BlockRows {
+    const int i, h;
+    uint32_t k_at, v_at;  // where this lane's reads of the first tiles start
+    Parts<T> q[8];        // [2 x + y]: dims 32 x + 16 h + 8 y ..
+    f32x16_v o[4];        // dims 32 d + 8 a + 4 h + c of row i
+    float l, m, mc, limit;  // as Rows8, l over the lane's own keys
+    bool big;
+    __device__ __forceinline__ BlockRows(int lane, const BlockLds& sm)
+        : i(lane & 31), h(lane >> 5), l(0.f), m(kNoMax), mc(0.f), limit(kNoMax), big(false) {
+        const int k_row = (i & 16) | ((i & 4) << 1) | ((i & 8) >> 1) | (i & 3), v_row = 8 * h + ((lane & 15) >> 1);
+        k_at = lds_at(sm.k) + k_row * kRow + 16 * (h ^ permute8_block(k_row));
+        v_at = lds_at(sm.v) + v_row * kRow + 16 * (((lane >> 4) & 1) ^ permute8_block(v_row)) + 8 * (lane & 1);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    }
+    // Chunk 2 x + h of key block u's row i.
+    __device__ __forceinline__ u32x4_v key(int u, int x, uint32_t buf) const {
+        return lds_read16((k_at ^ (32 * x)) + buf + 32 * u * kRow);
+    }
+    // Keys 32 u + 16 s + 8 h .. of dim 32 d + i.
+    __device__ __forceinline__ uint2 value(int u, int s, int d, uint32_t buf) const {
+        return lds_read_tr8((v_at ^ (32 * d)) + buf + (32 * u + 16 * s) * kRow);
+    }
+    // s[u][8 t + e]: the raw score of key 32 u + 16 t + 8 h + e.
+    __device__ __forceinline__ void scores(f32x16_v (&s)[2], const Scales& ks, uint32_t buf) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const u32x4_v w = key(u, x, buf);
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                    s[u] = product(widen(w[2 * y], w[2 * y + 1], ks.of[u]), q[2 * x + y], s[u]);
+            }
+        }
+    }
+    __device__ __forceinline__ void mask(f32x16_v (&s)[2], int j, int hi) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[u][r] = j + 32 * u + 16 * (r >> 3) + 8 * h + (r & 7) < hi ? s[u][r] : -INFINITY;
+    }
+    __device__ __forceinline__ void settle(const f32x16_v (&s)[2], float c) {
+        float mx = s[0][0];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
+        if (__any(mx > limit)) {
+            const float to = fmaxf(m, halves_max(mx)), f = fast_exp2((m - to) * c);
+            m = to;
+            mc = to == kNoMax ? 0.f : to * c;
+            limit = to == kNoMax ? kNoMax : to + kSlack / c;
+            big = __any(big || !(fabsf(mc) <= kMostMax));
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= f;
+        }
+    }
+    template <bool BIG> __device__ __forceinline__ void weights(f32x16_v (&s)[2], float c) {
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[u][r] = fast_exp2(BIG ? (s[u][r] - m) * c : __builtin_fmaf(s[u][r], c, -mc));
+                sum += s[u][r];
+            }
+        l += sum;
+    }
+    template <class VALUE> __device__ __forceinline__ void accumulate(const f32x16_v (&p)[2], const Scales& vs, VALUE value) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = p[u][8 * t + e];
+                Parts<T> w;
+                w.set(x);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint2 y = value(u, t, d);
+                    o[d] = product(widen(y.x, y.y, vs.of[u]), w, o[d]);
+                }
+            }
+    }
+    // As Rows8::settle_nan; key j + 32 u + 16 t + 8 h + e.
+    __device__ __forceinline__ void settle_nan(uint2 (&v)[2][2][4], int j, int hi) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) bad |= nan_codes(v[x >> 3][(x >> 2) & 1][x & 3].x) | nan_codes(v[x >> 3][(x >> 2) & 1][x & 3].y);
+        if (!__any(bad != 0)) return;
+        constexpr int kNone = 0x7fffffff;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            int first = kNone;  // of dim 32 d + i
+#pragma unroll
+            for (int z = 3; z >= 0; --z) {
+                uint2& c = v[z >> 1][z & 1][d];
+                const uint32_t x = nan_codes(c.x), y = nan_codes(c.y);
+                const int key = j + 16 * z + 8 * h;
+                if (y) first = key + 4 + (__builtin_ctz(y) >> 3);
+                if (x) first = key + (__builtin_ctz(x) >> 3);
+                c.x &= ~((x >> 7) * 255u);
+                c.y &= ~((y >> 7) * 255u);
+            }
+            first = min(first, __shfl_xor(first, 32));
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int f = __shfl(first, 8 * (r >> 2) + 4 * h + (r & 3));
+                o[d][r] = f < hi ? __builtin_nanf("") : o[d][r];
+            }
+        }
+    }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256, 2) void f8_block_kernel(Args8 a) {
+    __shared__ BlockLds sm;
+    constexpr int kRows = 128;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Item8 x(a, blockIdx.x);
+    const int R = a.S * a.G, block0 = x.block * kRows, row0 = block0 + 32 * wave;
+    const int b = x.pair, n = a.len(b);
+    // What the block's last row and this wave's first and last rows see.
+    auto seen = [&](int r) __attribute__((always_inline)) { return a.limit(n, min(r, R - 1) / a.G); };
+    const int end = seen(block0 + kRows - 1), min_hi = seen(row0), max_hi = row0 < R ? seen(row0 + 31) : 0;
+
+    Pages8 pages(a, lane);
+    pages.open(a, b, 0);
+    BlockRows<T> st(lane, sm);
+    int from[2];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        const int row = 16 * wave + 8 * y + (lane >> 3);
+        from[y] = row * kRow + 16 * ((lane & 7) ^ permute8_block(row));
+    }
+    auto tile_at = [&](int j) __attribute__((always_inline)) { return pages.tile(a, x.kvh, j, end); };
+    auto copy = [&](const Pages8::Tile& t, int buf) __attribute__((always_inline)) {
+        const auto rk = tile_rsrc(a.k, t), rv = tile_rsrc(a.v, t);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, sm.k[buf] + 1024 * (2 * wave + y), 16, from[y], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, sm.v[buf] + 1024 * (2 * wave + y), 16, from[y], 0, 0, 0);
+        }
+    };
+    Pages8::Tile tile{0, 0};
+    if (end > 0) copy(tile = tile_at(0), 0);
+    const int r = row0 + st.i, s_of = min(r, R - 1) / a.G, head = min(r, R - 1) - s_of * a.G;
+    const int at = r < R ? (int)(((int64_t)b * a.Hq + x.kvh * a.G + head) * a.S + s_of) : -1;
+    const int hi = min(a.limit(n, s_of), end);
+#pragma unroll
+    for (int y = 0; y < 8; ++y)
+        st.q[y].load(reinterpret_cast<const T*>(a.q) + (int64_t)max(at, 0) * kHeadDim + 32 * (y >> 1) + 16 * st.h + 8 * (y & 1));
+    for (int j = 0, half = 0; j < end; j += kTile, half ^= 1) {
+        const uint32_t buf = half * kTileBytes;
+        Scales ks, vs;
+        ks.load(a.k_scale, tile.off);
+        vs.load(a.v_scale, tile.off);
+        wait_memory();
+        __syncthreads();  // the tile is there, and the one before it is used
+        if (j + kTile < end) copy(tile = tile_at(j + kTile), half ^ 1);
+        if (j >= max_hi) continue;  // none of the wave's rows
+        f32x16_v s[2];
+        st.scores(s, ks, buf);
+        const bool masked = j + kTile > min(min_hi, end);
+        if (masked) st.mask(s, j, hi);
+        st.settle(s, a.c);
+        if (st.big) st.template weights<true>(s, a.c);
+        else st.template weights<false>(s, a.c);
+        auto value = [&](int u, int t2, int d) __attribute__((always_inline)) { return st.value(u, t2, d, buf); };
+        if (masked && min_hi < end) {
+            uint2 v[2][2][4];
+#pragma unroll
+            for (int z = 0; z < 16; ++z) v[z >> 3][(z >> 2) & 1][z & 3] = value(z >> 3, (z >> 2) & 1, z & 3);
+            st.settle_nan(v, j, hi);
+            st.accumulate(s, vs, [&](int u, int t2, int d) __attribute__((always_inline)) { return v[u][t2][d]; });
+        } else {
+            st.accumulate(s, vs, value);
+        }
+    }
+
+    const float l = halves_sum(st.l);
+    if (at < 0) return;
+    T* out = reinterpret_cast<T*>(a.out) + a.out_row(at) * kHeadDim + 4 * st.h;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float y[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) y[c] = hi <= 0 ? 0.f : st.o[d][4 * e + c] / l;
+            store4(out + 32 * d + 8 * e, y);
+        }
 }
 
 // Join a query row's chunks: P waves per row, lane x owns dims 2 x, 2 x + 1, wave p takes
@@ -708,23 +990,33 @@ __global__ __launch_bounds__(P == 1 ? 256 : 64 * P) void f8_join_kernel(Args8 a,
     Elem<T>::store(out + 1, n == 0 ? 0.f : x1 / den);
 }
 
-// How a call is launched: the rows of a workgroup, its waves, and whether and into how
-// many chunks at most the sequences are cut.
+// How a call is launched: its form, the rows of a workgroup, its waves, and whether and into
+// how many chunks at most the sequences are cut.
 struct Plan8 {
+    bool block;
     int rows, waves;
     int64_t tiles, pairs, items;
     size_t ml_off, cut_off, total;
 };
 
-Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv) {
+Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv, bool bf16) {
     Plan8 p{};
-    const int64_t R = (int64_t)S * (Hq / Hkv);
-    p.rows = R <= 16 ? 16 : 32;
+    const int64_t R = (int64_t)S * (Hq / Hkv), slots = 2 * kCus;  // two workgroups a CU, of any form
+    // The block form where its workgroups, whose waves all walk all keys, fill the device several
+    // times over.  8 prompts of 2048 tokens at 28 / 4 heads (3584 of them) 338 us, 402 in the
+    // stream form; 1024 tokens of 12 prompts of 9000 (2688) 1331 for 1368, of 4 (896) 494 for 441.
+    // f32: 16 times 256 tokens (1024 of them) 459 for 496, 4 times (256) 165 for 155.
+    const int64_t blocks = B * Hkv * ceil_div(R, 128);
+    p.block = blocks >= (bf16 ? 3 : 2) * slots;
+    p.rows = p.block ? 128 : R <= 16 ? 16 : 32;
     p.tiles = ceil_div(R, p.rows);
-    const int64_t heads = Hkv * p.tiles, slots = 2 * kCus;
-    if (B <= kMostCut && B * heads < slots && max_kv > 512) p.pairs = slots / heads;
-    p.waves = !p.pairs && B * heads <= kCus ? 8 : 4;
-    p.items = 8 * p.tiles * ceil_div((p.pairs ? p.pairs : B) * Hkv, 8);
+    const int64_t heads = Hkv * p.tiles;
+    // Cut where the sequences are fewer than the device holds and longer than the second kernel is
+    // worth (1 sequence of 1000 rows at 32 / 8 heads: 8.3 us whole, 9.4 cut; 4 of 2000: 14.7 and
+    // 10.1); whole ones up to one a CU have 8 waves.
+    if (!p.block && B <= kMostCut && B * heads < slots && max_kv > 1024) p.pairs = slots / heads;
+    p.waves = !p.block && !p.pairs && (bf16 || p.rows == 16) && B * heads <= kCus ? 8 : 4;
+    p.items = (p.pairs ? p.pairs : B) * heads;
     const size_t rows = (size_t)(p.pairs * heads * p.rows);
     p.ml_off = rows * kHeadDim * sizeof(float);
     p.cut_off = p.ml_off + rows * sizeof(float2);
@@ -734,13 +1026,17 @@ Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv) {
 
 template <typename T> int launch8(const Args8& a, const Plan8& p, int64_t n_rows, hipStream_t st) {
     const dim3 grid((unsigned)p.items), threads(64 * p.waves);
-#define CRANE_F8_CASE(rt, w) \
-    if (p.rows == 16 * rt && p.waves == w) hipLaunchKernelGGL((f8_stream_kernel<T, rt, w>), grid, threads, 0, st, a);
+#define CRANE_F8_CASE(rt, w)                                           \
+    if (!p.block && p.rows == 16 * rt && p.waves == w)                 \
+        hipLaunchKernelGGL((f8_stream_kernel<T, rt, w>), grid, threads, 0, st, a);
     CRANE_F8_CASE(1, 4)
     CRANE_F8_CASE(1, 8)
     CRANE_F8_CASE(2, 4)
-    CRANE_F8_CASE(2, 8)
+    if constexpr (sizeof(T) == 2) {
+        CRANE_F8_CASE(2, 8)
+    }
 #undef CRANE_F8_CASE
+    if (p.block) hipLaunchKernelGGL(f8_block_kernel<T>, grid, threads, 0, st, a);
     int rc = launch_status(hipGetLastError());
     if (rc || !p.pairs) return rc;
     if (p.pairs <= kJoinRegs * a.B)
@@ -770,7 +1066,7 @@ using namespace crane;
 
 extern "C" size_t crane_hip_attn_paged_f8_workspace(int64_t max_kv, int B, int S, int Hq, int Hkv, int D, int dtype) {
     if (check_sizes8(max_kv, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0 || max_kv <= 0) return 0;
-    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv);
+    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16);
     return p.items <= kMostThreads / (64 * p.waves) ? p.total : 0;
 }
 
@@ -790,7 +1086,7 @@ extern "C" int crane_hip_attn_paged_f8(const void* q, const void* k_pool, const 
     if (!q || !kv_len || !out) return CRANE_HIP_E_INVALID;
     if ((rc = check_pools8(k_pool, v_pool, k_scale, v_scale))) return rc;
     if (!aligned16(q) || !aligned16(out)) return CRANE_HIP_E_ALIGN;
-    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv);
+    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16);
     if (p.items > kMostThreads / (64 * p.waves)) return CRANE_HIP_E_INVALID;
     if (p.total && (!workspace || ws_bytes < p.total || !aligned16(workspace))) return CRANE_HIP_E_WORKSPACE;
     Args8 a;

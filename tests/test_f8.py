@@ -282,20 +282,18 @@ def reference(c, q, lens, scale, causal):
     slack = torch.zeros((B, S, Hq, 1), dtype=torch.float64)
     for b, n in enumerate(lens):
         k, v = c.rows(0, b, n), c.rows(1, b, n)
+        limit = torch.arange(n - S + 1, n + 1) if causal else torch.full((S,), n)
+        hidden = torch.arange(n)[None, :] >= limit[:, None]
         for h in range(Hq if n else 0):
             x, kk, vv = q[b, h].double(), k[h // G], v[h // G]
-            limit = torch.arange(n - S + 1, n + 1) if causal else torch.full((S,), n)
-            for s in range(S):
-                m = int(limit[s])
-                if m <= 0:
-                    continue
-                w = torch.softmax(scale * (kk[:m] @ x[s]), 0)
-                out[b, s, h], mag[b, s, h] = w @ vv[:m], w @ vv[:m].abs()
-                # a score's sum of 128 products, its difference to the largest and its product with
-                # log2 e are off by 132 half steps of f32 of the size of their terms at most, and so
-                # is the largest; the sums over n keys by n
-                most = scale * float((kk[:m].abs() @ x[s].abs()).max())
-                slack[b, s, h] = 2 * 132 * 2.0 ** -24 * most + (m + 64) * 2.0 ** -24
+            logits = (scale * (x @ kk.T)).masked_fill(hidden, -math.inf)
+            w = torch.nan_to_num(torch.softmax(logits, 1))  # a row of nothing: zeros
+            out[b, :, h], mag[b, :, h] = w @ vv, w @ vv.abs()
+            # a score's sum of 128 products, its difference to the largest and its product with
+            # log2 e are off by 132 half steps of f32 of the size of their terms at most, and so
+            # is the largest; the sums over n keys by n
+            most = scale * (x.abs() @ kk.abs().T).masked_fill(hidden, 0.0).amax(1)
+            slack[b, :, h, 0] = 2 * 132 * 2.0 ** -24 * most + (n + 64) * 2.0 ** -24
     return out.view(B, S, Hq * D), mag.view(B, S, Hq * D), slack.expand(B, S, Hq, D).reshape(B, S, Hq * D)
 
 
@@ -344,16 +342,49 @@ def test_chunk(gpu, dtype, causal, lens, S, Hq, Hkv):
     check_attention(gpu, dtype, lens, S, Hq, Hkv, causal=causal, seed=S)
 
 
+def spread_lengths(B, longest, seed):
+    """Lengths from 0 to `longest`, most of them short."""
+    g = torch.Generator().manual_seed(seed)
+    lens = (longest ** torch.rand(B, generator=g)).long().tolist()
+    return [0, longest] + [0 if b % 7 == 3 else n for b, n in enumerate(lens)][2:]
+
+
 @gpu_test
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("S", [1, 12, 150])
-def test_scores_far_apart(gpu, dtype, S):
+@pytest.mark.parametrize("lens,S,Hq,Hkv,max_kv", [
+    (spread_lengths(70, 2500, 1), 1, 4, 1, None), (spread_lengths(200, 1500, 2), 1, 6, 2, None),
+    (spread_lengths(256, 1300, 3), 1, 1, 1, None), (spread_lengths(257, 1300, 4), 1, 1, 1, None),
+    ([9000] + [10] * 40, 1, 8, 4, None), ([5000, 0, 17, 4999], 5, 8, 2, None), ([3000, 39, 1500], 40, 4, 1, None),
+    ([1100] * 16, 1, 16, 8, None), ([300, 20], 1, 4, 2, 60000), ([70, 1300], 3, 20, 2, 30000), ([0, 0], 1, 4, 2, 2000)])
+def test_sequences_cut_into_chunks(gpu, dtype, lens, S, Hq, Hkv, max_kv):
+    """Batches whose sequences are cut, by their lengths, into as many chunks as fill the device:
+    very different lengths, more sequences than a wave's lanes, bounds far above the lengths."""
+    c = Cache(len(lens), lens, Hkv, 512)
+    if max_kv:
+        c.table = torch.cat((c.table, torch.full((c.B, max_kv // 512 + 1), -7, dtype=torch.int32)), 1)
+    check_attention(gpu, dtype, lens, S, Hq, Hkv, 512, c=c, max_kv=max_kv, seed=len(lens))
+
+
+@gpu_test
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,B,S,Hq,Hkv,P", [("bf16", 13, 260, 56, 8, 256), ("bf16", 50, 129, 32, 8, 512),
+                                                 ("f32", 9, 260, 56, 8, 256), ("f32", 70, 40, 32, 8, 256)])
+def test_chunk_of_many(gpu, dtype, B, S, Hq, Hkv, P, causal):
+    """As many query rows as run in blocks of 128 that share their keys."""
+    lens = [0, S // 2, S, S + 1] + [S + 37 * b % 300 for b in range(4, B)]
+    check_attention(gpu, dtype, lens, S, Hq, Hkv, P, causal=causal, seed=B)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("S,Hq", [(1, 1), (12, 1), (150, 1), (700, 300)])
+def test_scores_far_apart(gpu, dtype, S, Hq):
     """Keys sorted by score, both ways: the running maximum moves at every tile, or never; scores
     from -3000 to 3000, and one scale of 2^-30 the softmax is flat at."""
     lens = [700]
     for way in (1, -1):
         c = Cache(3, lens, 1)
-        q = torch.zeros((1, 1, S, D))
+        q = torch.zeros((1, Hq, S, D))
         q[..., 0] = 256.0
         k = way * torch.linspace(-240, 240, 700, dtype=torch.float64)
         for j in range(0, 700, BLOCK):
@@ -362,14 +393,14 @@ def test_scores_far_apart(gpu, dtype, S):
             c.scales[0, page, :, block] = 127
             c.codes[0, page, :, j % 256:j % 256 + m, 0] = encode(k[j:j + m].float().to(E4M3).double(),
                                                                  torch.tensor(127))
-        check_attention(gpu, dtype, lens, S, 1, 1, c=c, q=q.to(DTYPES[dtype]), scale=0.05)
-        check_attention(gpu, dtype, lens, S, 1, 1, c=c, q=q.to(DTYPES[dtype]), scale=2.0 ** -30)
+        check_attention(gpu, dtype, lens, S, Hq, 1, c=c, q=q.to(DTYPES[dtype]), scale=0.05)
+        check_attention(gpu, dtype, lens, S, Hq, 1, c=c, q=q.to(DTYPES[dtype]), scale=2.0 ** -30)
 
 
 @gpu_test
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("S", [6, 140])
-def test_hidden_nan_reaches_nobody(gpu, dtype, S):
+@pytest.mark.parametrize("S,G", [(6, 3), (140, 3), (500, 400)])
+def test_hidden_nan_reaches_nobody(gpu, dtype, S, G):
     """A token whose k and v are NaN: earlier queries of the chunk are what they are without
     it, it and the later ones get NaN (v's only in the dims that hold one)."""
     from crane_amd import ops
@@ -377,7 +408,7 @@ def test_hidden_nan_reaches_nobody(gpu, dtype, S):
     for which in (0, 1):
         c = Cache(8, [n], 1)
         page, row = (int(y) for y in c.at(0, bad))
-        q = torch.randn((1, 3, S, D), generator=torch.Generator().manual_seed(1)).to(DTYPES[dtype])
+        q = torch.randn((1, G, S, D), generator=torch.Generator().manual_seed(1)).to(DTYPES[dtype])
         args = (ints([n], gpu), n)
         pools, table = c.to(gpu)
         clean = ops.attention_paged_f8(q.to(gpu), pools, table, *args)
@@ -386,16 +417,13 @@ def test_hidden_nan_reaches_nobody(gpu, dtype, S):
         got = ops.attention_paged_f8(q.to(gpu), pools, table, *args)
         last = S - 3  # the query at the row `bad`
         assert torch.equal(got[:, :last], clean[:, :last])
-        nan = torch.isnan(got[:, last:].view(1, -1, 3, D))
+        nan = torch.isnan(got[:, last:].view(1, -1, G, D))
         if which == 0:
             assert nan.all()
         else:
             assert nan[..., 5:9].all() and not nan[..., :5].any() and not nan[..., 9:].any()
-            # the other dims: whichever way they were summed
-            keep = torch.ones(D, dtype=torch.bool, device=gpu)
-            keep[5:9] = False
-            a, b = (x[:, last:].view(1, -1, 3, D)[..., keep].double() for x in (got, clean))
-            assert ((a - b).abs() <= 2 * HALF[dtype] * b.abs() + 600 * 2.0 ** -24 * 4).all()
+            a, b = (x[:, last:].view(1, -1, G, D) for x in (got, clean))  # the other dims: the same bits
+            assert torch.equal(a[..., :5], b[..., :5]) and torch.equal(a[..., 9:], b[..., 9:])
 
 
 @gpu_test
@@ -424,12 +452,12 @@ def test_values_a_scale_holds(gpu):
 
 
 @gpu_test
-@pytest.mark.parametrize("S", [1, 9, 150])
-def test_pages_outside_the_pool_count_as_zeros(gpu, S):
+@pytest.mark.parametrize("S,Hq", [(1, 2), (9, 2), (150, 2), (250, 400)])
+def test_pages_outside_the_pool_count_as_zeros(gpu, S, Hq):
     for bad in (-1, 1 << 30, 2 ** 31 - 1):
         c = Cache(2, [600, 300], 1)
         c.table[0, 1] = bad
-        check_attention(gpu, "bf16", [600, 300], S, 2, 1, c=c, causal=False)
+        check_attention(gpu, "bf16", [600, 300], S, Hq, 1, c=c, causal=False)
 
 
 @gpu_test
