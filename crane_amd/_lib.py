@@ -123,6 +123,7 @@ SIGNATURES = {
         [_vp, _vp, _vp, _vp, _i64, _i, _i32p, _i64, _i32p, _i64, _i, _i, _i, _vp, _vp, _i, _vp], _i),
     # include/crane_pkv.h
     "crane_pkv_create": ([_i, _i, _i, _i, _i64, _i, _i, _vpp], _i),
+    "crane_pkv_create_f8": ([_i, _i, _i, _i, _i64, _i, _i, _vpp], _i),
     "crane_pkv_destroy": ([_vp], None),
     "crane_pkv_seq_add": ([_vp, _ip], _i),
     "crane_pkv_seq_free": ([_vp, _i], _i),
@@ -140,6 +141,9 @@ SIGNATURES = {
     "crane_pkv_compact": ([_vpp, _i, _i64p, _vp], _i),
     "crane_pkv_shared_workspace": ([_vp, _i, _i], _sz),
     "crane_pkv_attention_shared": ([_vp, _vp, _i, _i, _f, _i, _vp, _sz, _vp, _vp], _i),
+    "crane_pkv_attention_f8_workspace": ([_vp, _i, _i], _sz),
+    "crane_pkv_attention_f8": ([_vp, _vp, _i, _i, _f, _i, _vp, _sz, _vp, _vp], _i),
+    "crane_pkv_scales_f8": ([_vp, _vpp, _vpp], _i),
     "crane_pkv_read_seq": ([_vp, _i, _vp, _vp, _vp], _i),
     "crane_pkv_write_seq": ([_vp, _i, _vp, _vp, _i64, _vp], _i),
     "crane_pkv_views": ([_vp, _vpp, _vpp, _vpp, _i64p, _vpp], _i),

@@ -51,10 +51,22 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float down) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * down, x[3] * down, r, true);
 }
 
-}  // namespace crane
+// ---- host
+// Quantise rows k, v [B, Hkv, S, D] of `dtype` into rows start[b] .. (start null: 0 ..) of the
+// pages, as the append does (f8_cache.hip; for the cache manager, which has checked its
+// arguments).
+int f8_write_rows(const void* k, const void* v, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
+                  const PagedRows& rows, const int32_t* start, int B, int64_t S, int Hkv, int dtype, hipStream_t st);
 
-// Host checks the launchers share: the pools' addresses, then the paging.
-namespace crane {
+// A grid's threads are 32 bits and a workgroup is 256 of them.
+constexpr int64_t kMostUnits8 = 0xffffff;
+// The workgroups of f8_write_rows: a block, of k or of v, of a head, for wherever in its first
+// block a sequence's S rows begin.
+inline int64_t f8_rows_units(int B, int64_t S, int Hkv) {
+    return (int64_t)B * 2 * Hkv * ((S + 2 * kBlockRows8 - 2) / kBlockRows8);
+}
+
+// A check the launchers share: the pools' addresses.
 inline int check_pools8(const void* k_pool, const void* v_pool, const void* k_scale, const void* v_scale) {
     if (!k_pool || !v_pool || !k_scale || !v_scale) return CRANE_HIP_E_INVALID;
     return aligned16(k_pool) && aligned16(v_pool) && aligned16(k_scale) && aligned16(v_scale) ? CRANE_HIP_OK

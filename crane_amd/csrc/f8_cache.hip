@@ -90,7 +90,8 @@ template <typename T> struct Append {
     T* q_out;
     uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
     PagedRows rows;
-    const int32_t* cache_len;
+    const int32_t* cache_len;   // null: 0 for every sequence
+    const T *k_rows, *v_rows;   // [B, Hkv, S, D] as they are to be quantised, in place of qkv
     int S, Hq, Hkv;
     int64_t q_items, q_blocks;  // q head rows, and the workgroups that take them
     int64_t units;              // blocks mode: (sequence, block, k or v head)
@@ -215,9 +216,9 @@ template <typename T> __global__ __launch_bounds__(256) void f8_append_token_ker
     if (l == 0 && byte != had) *scale = (uint8_t)byte;
 }
 
-// Any S.  The rows and q, each touched once, go past the caches (8 prompts of 4096 tokens: 105
-// us to 99).  grid: q items, then one workgroup per (sequence, block, k or v head).
-template <typename T> __global__ __launch_bounds__(256) void f8_append_blocks_kernel(Append<T> p) {
+// Any S.  ROWS: k_rows and v_rows in place of qkv's.  The rows and q, each touched once, go
+// past the caches (8 prompts of 4096 tokens: 105 us to 99).  grid: q items, then one workgroup per (sequence, block, k or v head).
+template <typename T, bool ROWS> __global__ __launch_bounds__(256) void f8_append_blocks_kernel(Append<T> p) {
     const int l = threadIdx.x & 7, r = threadIdx.x >> 3;
     if ((int64_t)blockIdx.x < p.q_blocks) return q_item<true>(p, (int64_t)blockIdx.x * kItems + r, l);
     const int64_t unit = (int64_t)blockIdx.x - p.q_blocks;
@@ -226,7 +227,7 @@ template <typename T> __global__ __launch_bounds__(256) void f8_append_blocks_ke
     const int b = (int)(x0 / p.blocks);
     const bool is_v = hh >= p.Hkv;
     const int h = is_v ? hh - p.Hkv : hh;
-    const int64_t len = p.cache_len[b];
+    const int64_t len = ROWS && !p.cache_len ? 0 : p.cache_len[b];
     const int64_t first = (len & ~(int64_t)(kBlockRows8 - 1)) + (x0 % p.blocks) * kBlockRows8;
     if (first >= len + p.S) return;  // the sequence's rows end before
     const int64_t off = p.rows.offset(b, p.Hkv, h, first);
@@ -235,7 +236,11 @@ template <typename T> __global__ __launch_bounds__(256) void f8_append_blocks_ke
     const bool old = s < 0;
     bool fresh = !old && s < p.S;
     RowValues x;
-    if (fresh) {
+    if (ROWS && fresh) {
+        const T* src = (is_v ? p.v_rows : p.k_rows) + (((int64_t)b * p.Hkv + h) * p.S + s) * kHeadDim;
+        take8<true>(src + 8 * l, x.a);
+        take8<true>(src + 64 + 8 * l, x.b);
+    } else if (fresh) {
         load_row<true>(x, p, (int64_t)b * p.S + s, p.Hq + hh, l);
         if (!is_v) {
             const int64_t pos = (int64_t)p.positions[b] + s;
@@ -275,7 +280,14 @@ template <typename T> int launch_append(Append<T> p, int B, hipStream_t st) {
     if (p.S == 1)
         hipLaunchKernelGGL(f8_append_token_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, p);
     else
-        hipLaunchKernelGGL(f8_append_blocks_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((f8_append_blocks_kernel<T, false>), dim3((unsigned)grid), dim3(256), 0, st, p);
+    return launch_status(hipGetLastError());
+}
+
+template <typename T> int launch_rows(Append<T> p, int B, hipStream_t st) {
+    p.units = f8_rows_units(B, p.S, p.Hkv);
+    p.blocks = (int)(p.units / ((int64_t)B * 2 * p.Hkv));
+    hipLaunchKernelGGL((f8_append_blocks_kernel<T, true>), dim3((unsigned)p.units), dim3(256), 0, st, p);
     return launch_status(hipGetLastError());
 }
 
@@ -329,6 +341,28 @@ __global__ __launch_bounds__(256) void f8_read_kernel(const uint8_t* __restrict_
 }
 
 }  // namespace
+
+int f8_write_rows(const void* k, const void* v, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
+                  const PagedRows& rows, const int32_t* start, int B, int64_t S, int Hkv, int dtype, hipStream_t st) {
+    if (S > 0x7fffffffLL || f8_rows_units(B, S, Hkv) > kMostUnits8) return CRANE_HIP_E_INVALID;
+    auto go = [&](auto zero) {
+        typedef decltype(zero) T;
+        Append<T> p{};
+        p.k_rows = (const T*)k;
+        p.v_rows = (const T*)v;
+        p.k_pool = (uint8_t*)k_pool;
+        p.v_pool = (uint8_t*)v_pool;
+        p.k_scale = (uint8_t*)k_scale;
+        p.v_scale = (uint8_t*)v_scale;
+        p.rows = rows;
+        p.cache_len = start;
+        p.S = (int)S;
+        p.Hkv = Hkv;
+        return launch_rows(p, B, st);
+    };
+    return dtype == CRANE_HIP_F32 ? go(float()) : go(bf16_t());
+}
+
 }  // namespace crane
 
 using namespace crane;

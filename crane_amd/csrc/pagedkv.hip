@@ -23,11 +23,17 @@
 // the attention that reads them once.  Calls over several layers' caches plan every
 // cache first and change none unless all can go through; caches that need the same
 // copies get them in one launch.
+//
+// A cache in 8 bits (include/crane_f8.h) has pools of one-byte codes and pools of scales
+// beside them; its pages, lists and batches are the same.  A page copy takes the rows'
+// codes and all of the page's scales: those behind the rows are of blocks that an append
+// begins anew.
 #include <algorithm>
-#include <new>
+#include <memory>
 #include <vector>
 
-#include "common.h"
+#include "f8.h"
+#include "page_copies.h"
 #include "page_groups.h"
 #include "../../include/crane_pkv.h"
 #include "../../include/crane_shared.h"
@@ -126,9 +132,9 @@ struct Copies {
 
 class PagedKv {
   public:
-    PagedKv(int Hkv, int D, int dtype, int P, int64_t n_pages, int max_seqs, int max_pps)
-        : Hkv_(Hkv), D_(D), dtype_(dtype), es_(elem_size(dtype)), P_(P), n_pages_(n_pages), max_seqs_(max_seqs),
-          max_pps_(max_pps), seqs_(max_seqs) {}
+    PagedKv(int Hkv, int D, int dtype, bool f8, int P, int64_t n_pages, int max_seqs, int max_pps)
+        : Hkv_(Hkv), D_(D), dtype_(dtype), f8_(f8), es_(f8 ? 1 : elem_size(dtype)), P_(P), n_pages_(n_pages),
+          max_seqs_(max_seqs), max_pps_(max_pps), seqs_(max_seqs) {}
     ~PagedKv() { release(); }
     PagedKv(const PagedKv&) = delete;
     PagedKv& operator=(const PagedKv&) = delete;
@@ -136,10 +142,12 @@ class PagedKv {
     int init() {
         const size_t pool = pool_bytes();
         if (hipMalloc(&k_pool_, pool) != hipSuccess || hipMalloc(&v_pool_, pool) != hipSuccess ||
+            (f8_ && (hipMalloc(&k_scale_, scale_bytes()) != hipSuccess ||
+                     hipMalloc(&v_scale_, scale_bytes()) != hipSuccess)) ||
             hipMalloc(&d_table_, sizeof(int32_t) * (size_t)max_seqs_ * max_pps_) != hipSuccess ||
             hipMalloc(&d_len_, sizeof(int32_t) * (size_t)max_seqs_) != hipSuccess ||
             hipMalloc(&d_start_, sizeof(int32_t) * (size_t)max_seqs_) != hipSuccess ||
-            hipMalloc(&d_one_, sizeof(int32_t) * (size_t)max_pps_) != hipSuccess ||
+            hipMalloc(&d_one_, sizeof(int32_t) * ((size_t)max_pps_ + 1)) != hipSuccess ||
             hipMalloc(&d_groups_, sizeof(int32_t) * 4 * (size_t)max_seqs_) != hipSuccess) {
             release();
             return CRANE_HIP_E_LAUNCH;
@@ -152,12 +160,15 @@ class PagedKv {
 
     size_t row_bytes() const { return (size_t)D_ * es_; }
     size_t pool_bytes() const { return (size_t)n_pages_ * Hkv_ * P_ * row_bytes(); }
-    uint64_t bytes() const { return 2ull * pool_bytes(); }
+    size_t page_scales() const { return f8_ ? (size_t)Hkv_ * P_ / kBlockRows8 : 0; }
+    size_t scale_bytes() const { return (size_t)n_pages_ * page_scales(); }
+    uint64_t bytes() const { return 2ull * (pool_bytes() + scale_bytes()); }
     int64_t free_pages() const { return (int64_t)free_.size(); }
     int B() const { return (int)batch_.size(); }
     int Hkv() const { return Hkv_; }
     int D() const { return D_; }
     int dtype() const { return dtype_; }
+    bool f8() const { return f8_; }
 
     bool live(int id) const { return id >= 0 && id < max_seqs_ && seqs_[id].live; }
     bool in_batch(int id) const { return std::find(batch_.begin(), batch_.end(), id) != batch_.end(); }
@@ -293,6 +304,7 @@ class PagedKv {
         if (S < 0) return CRANE_HIP_E_INVALID;
         if (S == 0 || batch_.empty()) return CRANE_HIP_OK;
         if (!k || !v || !aligned16(k) || !aligned16(v)) return !k || !v ? CRANE_HIP_E_INVALID : CRANE_HIP_E_ALIGN;
+        if (!rows_fit(B(), S)) return CRANE_HIP_E_INVALID;
         int rc = reserve(S, st);
         if (rc) return rc;
         rc = scatter(k, v, batch_rows(), d_len_, B(), S, st);
@@ -307,9 +319,14 @@ class PagedKv {
         std::vector<int> added;
         int rc = reserve(S, st, &added);
         if (rc) return rc;
-        rc = crane_hip_qknorm_rope_append_paged(qkv, qkv_row_stride, q_norm_w, k_norm_w, eps, order, cos, sin,
-                                                cs_stride, table_rows, positions, q_out, k_pool_, v_pool_, n_pages_,
-                                                P_, d_table_, max_pps_, d_len_, B(), S, Hq, Hkv_, D_, dtype_, st);
+        rc = f8_ ? crane_hip_qknorm_rope_append_paged_f8(
+                       qkv, qkv_row_stride, q_norm_w, k_norm_w, eps, order, cos, sin, cs_stride, table_rows, positions,
+                       q_out, k_pool_, v_pool_, k_scale_, v_scale_, n_pages_, P_, d_table_, max_pps_, d_len_, B(), S,
+                       Hq, Hkv_, D_, dtype_, st)
+                 : crane_hip_qknorm_rope_append_paged(qkv, qkv_row_stride, q_norm_w, k_norm_w, eps, order, cos, sin,
+                                                      cs_stride, table_rows, positions, q_out, k_pool_, v_pool_,
+                                                      n_pages_, P_, d_table_, max_pps_, d_len_, B(), S, Hq, Hkv_, D_,
+                                                      dtype_, st);
         if (rc) {  // rejected arguments: nothing ran, the pages go back
             unreserve(added);
             return rc;
@@ -319,6 +336,7 @@ class PagedKv {
 
     int decode(const void* q, int Hq, float scale, int score_mode, void* ws, size_t ws_bytes, void* out,
                hipStream_t st) const {
+        if (f8_) return CRANE_HIP_E_DTYPE;
         if (batch_.empty()) return CRANE_HIP_OK;
         const int64_t m = max_len();
         if (m == 0) return CRANE_HIP_E_INVALID;
@@ -327,6 +345,7 @@ class PagedKv {
     }
 
     int prefill(const void* q, int Hq, int S, float scale, int flags, void* out, hipStream_t st) {
+        if (f8_) return CRANE_HIP_E_DTYPE;
         if (S < 0) return CRANE_HIP_E_INVALID;
         if (batch_.empty() || S == 0) return CRANE_HIP_OK;
         for (int id : batch_)
@@ -338,14 +357,34 @@ class PagedKv {
                                             max_len() - S, B(), S, Hq, Hkv_, D_, scale, flags, out, dtype_, st);
     }
 
+    // Attention of the batch's last S rows over a cache in 8 bits.
+    size_t attention_f8_workspace(int Hq, int S) const {
+        return f8_ ? crane_hip_attn_paged_f8_workspace(max_len(), B(), S, Hq, Hkv_, D_, dtype_) : 0;
+    }
+    int attention_f8(const void* q, int Hq, int S, float scale, int flags, void* ws, size_t ws_bytes, void* out,
+                     hipStream_t st) const {
+        if (!f8_) return CRANE_HIP_E_DTYPE;
+        if (S < 0) return CRANE_HIP_E_INVALID;
+        if (batch_.empty() || S == 0) return CRANE_HIP_OK;
+        for (int id : batch_)
+            if (S > 1 && seqs_[id].len < S) return CRANE_HIP_E_INVALID;  // every sequence holds its S new rows
+        if (max_len() == 0) return CRANE_HIP_E_INVALID;
+        return crane_hip_attn_paged_f8(q, k_pool_, v_pool_, k_scale_, v_scale_, n_pages_, P_, d_table_, max_pps_,
+                                       d_len_, max_len(), B(), S, Hq, Hkv_, D_, scale, flags, ws, ws_bytes, out, dtype_,
+                                       st);
+    }
+
     int read_seq(int id, void* k, void* v, hipStream_t st) {
         if (!live(id)) return CRANE_HIP_E_INVALID;
         const Seq& s = seqs_[id];
         if (s.len == 0) return CRANE_HIP_OK;
         if (!k || !v) return CRANE_HIP_E_INVALID;
         if (!aligned16(k) || !aligned16(v)) return CRANE_HIP_E_ALIGN;
-        int rc = upload_one(s.pages, st);
+        int rc = upload_one(s, st);
         if (rc) return rc;
+        if (f8_)
+            return crane_hip_read_paged_f8(k_pool_, v_pool_, k_scale_, v_scale_, n_pages_, P_, d_one_, max_pps_,
+                                           d_one_ + max_pps_, s.len, 1, Hkv_, D_, k, v, dtype_, st);
         const int64_t n_chunks = (int64_t)Hkv_ * s.len * (int64_t)(row_bytes() / 16);
         hipLaunchKernelGGL(gather_rows_kernel, dim3((unsigned)((n_chunks + 255) / 256)), dim3(256), 0, st,
                            (const uint8_t*)k_pool_, (const uint8_t*)v_pool_, (uint8_t*)k, (uint8_t*)v, one_rows(), Hkv_,
@@ -360,6 +399,7 @@ class PagedKv {
         Seq& s = seqs_[id];
         const int64_t need = (len + P_ - 1) / P_;
         if (need > max_pps_ || len > 0x7fffffffLL) return CRANE_HIP_E_CAPACITY;
+        if (!rows_fit(1, len)) return CRANE_HIP_E_INVALID;
         // A page other sequences hold is not written: it is given up for another.
         int64_t kept = 0, back = 0;
         for (int32_t p : s.pages) {
@@ -381,7 +421,7 @@ class PagedKv {
         s.pages.swap(pages);
         s.len = len;
         if (len == 0) return CRANE_HIP_OK;
-        const int rc = upload_one(s.pages, st);
+        const int rc = upload_one(s, st);
         return rc ? rc : scatter(k, v, one_rows(), nullptr, 1, len, st);
     }
 
@@ -513,11 +553,13 @@ class PagedKv {
         return B() ? sum / B() : 0;
     }
     size_t shared_workspace(int Hq, int S) const {
+        if (f8_) return 0;
         return crane_hip_attn_shared_workspace(batch_groups_.data(), n_groups_, max_len(), max_own(), mean_own(), B(),
                                                S, Hq, Hkv_, D_, dtype_);
     }
     int attention_shared(const void* q, int Hq, int S, float scale, int flags, void* ws, size_t ws_bytes, void* out,
                          hipStream_t st) const {
+        if (f8_) return CRANE_HIP_E_DTYPE;
         if (S < 0) return CRANE_HIP_E_INVALID;
         if (batch_.empty() || S == 0) return CRANE_HIP_OK;
         for (int id : batch_)
@@ -530,14 +572,22 @@ class PagedKv {
     }
 
     bool same_shape(const PagedKv& o) const {
-        return Hkv_ == o.Hkv_ && D_ == o.D_ && dtype_ == o.dtype_ && P_ == o.P_ && n_pages_ == o.n_pages_;
+        return Hkv_ == o.Hkv_ && D_ == o.D_ && es_ == o.es_ && f8_ == o.f8_ && P_ == o.P_ && n_pages_ == o.n_pages_;
     }
     int max_seqs() const { return max_seqs_; }
-    void* k_pool() const { return k_pool_; }
-    void* v_pool() const { return v_pool_; }
-    int copy_into(std::vector<void*>& pools, const Copies& c, hipStream_t st) const {
-        return crane_hip_copy_pages(pools.data(), (int)pools.size(), n_pages_, P_, Hkv_, D_, c.src.data(), c.dst.data(),
-                                    c.rows.data(), (int)c.src.size(), dtype_, st);
+    // The pools a page copy goes over: of rows, and of a cache in 8 bits the scales.
+    void add_pools(std::vector<void*>* rows, std::vector<void*>* scales) const {
+        rows->insert(rows->end(), {k_pool_, v_pool_});
+        if (f8_) scales->insert(scales->end(), {k_scale_, v_scale_});
+    }
+    int copy_into(const std::vector<void*>& rows, const std::vector<void*>& scales, const Copies& c,
+                  hipStream_t st) const {
+        const int n = (int)c.src.size();
+        const int rc = copy_page_rows(rows.data(), (int)rows.size(), n_pages_, P_, Hkv_, (int)row_bytes(), c.src.data(),
+                                      c.dst.data(), c.rows.data(), n, st);
+        return rc ? rc
+                  : copy_page_rows(scales.data(), (int)scales.size(), n_pages_, 1, 1, (int)page_scales(), c.src.data(),
+                                   c.dst.data(), nullptr, n, st);
     }
 
     void views(void** k, void** v, const int32_t** table, int64_t* stride, const int32_t** dlen) const {
@@ -546,6 +596,10 @@ class PagedKv {
         if (table) *table = d_table_;
         if (stride) *stride = max_pps_;
         if (dlen) *dlen = d_len_;
+    }
+    void scales(void** k, void** v) const {
+        if (k) *k = k_scale_;
+        if (v) *v = v_scale_;
     }
 
   private:
@@ -578,16 +632,21 @@ class PagedKv {
 
     PagedRows one_rows() const { return PagedRows{d_one_, max_pps_, n_pages_, P_}; }
 
-    // One sequence's page ids into the single-row table d_one_.
-    int upload_one(const std::vector<int32_t>& pages, hipStream_t st) {
-        std::vector<int32_t> row((size_t)max_pps_, -1);
-        std::copy(pages.begin(), pages.end(), row.begin());
+    // One sequence's page ids into the single-row table d_one_, its length behind them.
+    int upload_one(const Seq& s, hipStream_t st) {
+        std::vector<int32_t> row((size_t)max_pps_ + 1, -1);
+        std::copy(s.pages.begin(), s.pages.end(), row.begin());
+        row.back() = (int32_t)s.len;
         int rc = hip_rc(hipMemcpyAsync(d_one_, row.data(), sizeof(int32_t) * row.size(), hipMemcpyHostToDevice, st));
         return rc ? rc : hip_rc(hipStreamSynchronize(st));  // `row` is a local staging buffer
     }
 
+    // Whether one launch takes S rows of B sequences (of any length) in 8 bits.
+    bool rows_fit(int B, int64_t S) const { return !f8_ || f8_rows_units(B, S, Hkv_) <= kMostUnits8; }
+
     int scatter(const void* k, const void* v, const PagedRows& rows, const int32_t* start, int B, int64_t S,
                 hipStream_t st) {
+        if (f8_) return f8_write_rows(k, v, k_pool_, v_pool_, k_scale_, v_scale_, rows, start, B, S, Hkv_, dtype_, st);
         const int64_t n_chunks = (int64_t)B * Hkv_ * S * (int64_t)(row_bytes() / 16);
         if ((n_chunks + 255) / 256 > 0x7fffffffLL || S > 0x7fffffffLL) return CRANE_HIP_E_INVALID;
         hipLaunchKernelGGL(scatter_rows_kernel, dim3((unsigned)((n_chunks + 255) / 256)), dim3(256), 0, st,
@@ -597,24 +656,27 @@ class PagedKv {
     }
 
     void release() {
-        for (void* p : {k_pool_, v_pool_, (void*)d_table_, (void*)d_len_, (void*)d_start_, (void*)d_one_,
-                        (void*)d_groups_})
+        for (void* p : {k_pool_, v_pool_, k_scale_, v_scale_, (void*)d_table_, (void*)d_len_, (void*)d_start_,
+                        (void*)d_one_, (void*)d_groups_})
             if (p) (void)hipFree(p);
-        k_pool_ = v_pool_ = nullptr;
+        k_pool_ = v_pool_ = k_scale_ = v_scale_ = nullptr;
         d_table_ = d_len_ = d_start_ = d_one_ = d_groups_ = nullptr;
     }
 
-    int Hkv_, D_, dtype_;
-    size_t es_;
+    int Hkv_, D_, dtype_;  // dtype_: of q and of the rows that come in and go out
+    bool f8_;
+    size_t es_;  // bytes of a value in the pools
     int P_;
     int64_t n_pages_;
     int max_seqs_, max_pps_;
     void* k_pool_ = nullptr;
     void* v_pool_ = nullptr;
+    void* k_scale_ = nullptr;     // in 8 bits only
+    void* v_scale_ = nullptr;
     int32_t* d_table_ = nullptr;  // current batch: B rows of max_pps_ page ids
     int32_t* d_len_ = nullptr;    // current batch lengths
     int32_t* d_start_ = nullptr;  // prefill chunk starts
-    int32_t* d_one_ = nullptr;    // one sequence's page ids (read_seq / write_seq)
+    int32_t* d_one_ = nullptr;    // one sequence's page ids and length (read_seq / write_seq)
     int32_t* d_groups_ = nullptr;  // current batch: groups, their members, shared rows (when there are groups)
     std::vector<int32_t> free_;
     std::vector<int32_t> refs_;   // owners of every page
@@ -631,8 +693,8 @@ using crane::PagedKv;
 
 struct crane_pkv {
     PagedKv impl;
-    crane_pkv(int Hkv, int D, int dtype, int P, int64_t n_pages, int max_seqs, int max_pps)
-        : impl(Hkv, D, dtype, P, n_pages, max_seqs, max_pps) {}
+    crane_pkv(int Hkv, int D, int dtype, bool f8, int P, int64_t n_pages, int max_seqs, int max_pps)
+        : impl(Hkv, D, dtype, f8, P, n_pages, max_seqs, max_pps) {}
 };
 
 namespace {
@@ -654,15 +716,14 @@ int copy_all(crane_pkv* const* caches, const std::vector<PLAN>& plans, hipStream
     for (size_t i = 0; i < plans.size(); ++i) {
         if (done[i] || plans[i].copies.src.empty()) continue;
         const PagedKv& first = caches[i]->impl;
-        std::vector<void*> pools;
+        std::vector<void*> rows, scales;
         for (size_t j = i; j < plans.size(); ++j) {
             const PagedKv& c = caches[j]->impl;
             if (done[j] || !c.same_shape(first) || !(plans[j].copies == plans[i].copies)) continue;
             done[j] = 1;
-            pools.push_back(c.k_pool());
-            pools.push_back(c.v_pool());
+            c.add_pools(&rows, &scales);
         }
-        const int rc = first.copy_into(pools, plans[i].copies, st);
+        const int rc = first.copy_into(rows, scales, plans[i].copies, st);
         if (rc) return rc;
     }
     return CRANE_HIP_OK;
@@ -743,8 +804,10 @@ extern "C" int crane_pkv_attention_shared(const crane_pkv* pkv, const void* q, i
                : CRANE_HIP_E_INVALID;
 }
 
-extern "C" int crane_pkv_create(int Hkv, int D, int dtype, int page_rows, int64_t n_pages, int max_seqs,
-                                int max_pages_per_seq, crane_pkv** out) {
+namespace {
+
+int create(int Hkv, int D, int dtype, bool f8, int page_rows, int64_t n_pages, int max_seqs, int max_pages_per_seq,
+           crane_pkv** out) {
     if (!out) return CRANE_HIP_E_INVALID;
     *out = nullptr;
     if (dtype != CRANE_HIP_F32 && dtype != CRANE_HIP_BF16) return CRANE_HIP_E_DTYPE;
@@ -754,14 +817,44 @@ extern "C" int crane_pkv_create(int Hkv, int D, int dtype, int page_rows, int64_
     int32_t dummy = 0;  // the table pointer is not known yet; only the sizes are checked here
     const int rc = crane::check_paged(n_pages, page_rows, &dummy, max_pages_per_seq, Hkv);
     if (rc) return rc;
-    crane_pkv* p = new (std::nothrow) crane_pkv(Hkv, D, dtype, page_rows, n_pages, max_seqs, max_pages_per_seq);
-    if (!p) return CRANE_HIP_E_INVALID;
-    const int irc = p->impl.init();
-    if (irc) {
-        delete p;
+    if (f8 && (int64_t)Hkv * page_rows > 0x7fffffffLL) return CRANE_HIP_E_INVALID;  // a page's scales are one copied row
+    try {
+        std::unique_ptr<crane_pkv> p(
+            new crane_pkv(Hkv, D, dtype, f8, page_rows, n_pages, max_seqs, max_pages_per_seq));
+        const int irc = p->impl.init();
+        if (!irc) *out = p.release();
         return irc;
+    } catch (...) {  // no memory
+        return CRANE_HIP_E_INVALID;
     }
-    *out = p;
+}
+
+}  // namespace
+
+extern "C" int crane_pkv_create(int Hkv, int D, int dtype, int page_rows, int64_t n_pages, int max_seqs,
+                                int max_pages_per_seq, crane_pkv** out) {
+    return create(Hkv, D, dtype, false, page_rows, n_pages, max_seqs, max_pages_per_seq, out);
+}
+
+extern "C" int crane_pkv_create_f8(int Hkv, int D, int dtype, int page_rows, int64_t n_pages, int max_seqs,
+                                   int max_pages_per_seq, crane_pkv** out) {
+    return create(Hkv, D, dtype, true, page_rows, n_pages, max_seqs, max_pages_per_seq, out);
+}
+
+extern "C" size_t crane_pkv_attention_f8_workspace(const crane_pkv* pkv, int Hq, int S) {
+    return pkv ? pkv->impl.attention_f8_workspace(Hq, S) : 0;
+}
+
+extern "C" int crane_pkv_attention_f8(const crane_pkv* pkv, const void* q, int Hq, int S, float scale, int flags,
+                                      void* workspace, size_t ws_bytes, void* out, void* stream) {
+    return pkv ? pkv->impl.attention_f8(q, Hq, S, scale, flags, workspace, ws_bytes, out, (hipStream_t)stream)
+               : CRANE_HIP_E_INVALID;
+}
+
+extern "C" int crane_pkv_scales_f8(const crane_pkv* pkv, void** k_scale, void** v_scale) {
+    if (!pkv) return CRANE_HIP_E_INVALID;
+    if (!pkv->impl.f8()) return CRANE_HIP_E_DTYPE;
+    pkv->impl.scales(k_scale, v_scale);
     return CRANE_HIP_OK;
 }
 

@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "common.h"
+#include "page_copies.h"
 #include "page_groups.h"
 #include "../../include/crane_shared.h"
 
@@ -19,8 +20,8 @@ namespace {
 constexpr int kPools = 128;      // pools per launch: K and V of 64 layers
 constexpr int kPairs = 128;      // pairs per launch
 constexpr int kThreads = 256;
-constexpr int kBlockBytes = 16 * kThreads;  // bytes of one head's run per workgroup
 
+typedef unsigned int u32x2_v __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4_v __attribute__((ext_vector_type(4)));
 
 struct CopyArgs {
@@ -33,16 +34,18 @@ struct CopyArgs {
 // to 8 others, 267 MB in all: 36 us, 65 with plain stores; 97 pages to 97, 407 MB: 59 us
 // for 76), and with 2, 4, 8 or 16 loads issued ahead of the stores the first of these
 // takes 44 to 47 us, the second the same.
+// V: what a thread moves, 16 bytes, or 8 where rows are no multiple of that.
 // grid: (heads x blocks of a run, pairs, pools)
+template <typename V>
 __global__ __launch_bounds__(kThreads) void copy_pages_kernel(CopyArgs a, int blocks, int Hkv, int64_t run_bytes,
                                                               int row_bytes) {
     const int head = blockIdx.x / blocks, block = blockIdx.x % blocks;
-    const int64_t at = (int64_t)block * kBlockBytes + 16 * threadIdx.x;
+    const int64_t at = ((int64_t)block * kThreads + threadIdx.x) * sizeof(V);
     if (at >= (int64_t)a.rows[blockIdx.y] * row_bytes) return;
     uint8_t* pool = a.pool[blockIdx.z];
     const uint8_t* src = pool + ((int64_t)a.src[blockIdx.y] * Hkv + head) * run_bytes;
     uint8_t* dst = pool + ((int64_t)a.dst[blockIdx.y] * Hkv + head) * run_bytes;
-    __builtin_nontemporal_store(*reinterpret_cast<const u32x4_v*>(src + at), reinterpret_cast<u32x4_v*>(dst + at));
+    __builtin_nontemporal_store(*reinterpret_cast<const V*>(src + at), reinterpret_cast<V*>(dst + at));
 }
 
 // The lists sorted form a tree: a node is a run of them with `common` first pages in
@@ -188,20 +191,14 @@ extern "C" int crane_hip_group_prefixes(const int32_t* table, int64_t stride, co
     return CRANE_HIP_OK;
 }
 
-extern "C" int crane_hip_copy_pages(void* const* pools, int n_pools, int64_t n_pages, int page_rows, int Hkv, int D,
-                                    const int32_t* src, const int32_t* dst, const int32_t* rows, int n, int dtype,
-                                    void* stream) {
-    if (dtype != CRANE_HIP_F32 && dtype != CRANE_HIP_BF16) return CRANE_HIP_E_DTYPE;
-    if (D != kHeadDim) return CRANE_HIP_E_HEAD_DIM;
-    if (n_pools < 0 || n < 0 || Hkv <= 0 || Hkv > 65535) return CRANE_HIP_E_INVALID;
-    int32_t dummy = 0;  // no block table here; only the pool sizes are checked
-    int rc = check_paged(n_pages, page_rows, &dummy, 1, Hkv);
-    if (rc) return rc;
+int crane::copy_page_rows(void* const* pools, int n_pools, int64_t n_pages, int page_rows, int Hkv, int row_bytes,
+                          const int32_t* src, const int32_t* dst, const int32_t* rows, int n, hipStream_t stream) {
     if (n == 0 || n_pools == 0) return CRANE_HIP_OK;
     if (!pools || !src || !dst) return CRANE_HIP_E_INVALID;
+    const int unit = row_bytes % 16 ? 8 : 16;
     for (int i = 0; i < n_pools; ++i) {
         if (!pools[i]) return CRANE_HIP_E_INVALID;
-        if (!aligned16(pools[i])) return CRANE_HIP_E_ALIGN;
+        if ((uintptr_t)pools[i] % unit) return CRANE_HIP_E_ALIGN;
     }
     int max_rows = 0;
     for (int i = 0; i < n; ++i) {
@@ -220,9 +217,8 @@ extern "C" int crane_hip_copy_pages(void* const* pools, int n_pools, int64_t n_p
         return CRANE_HIP_E_INVALID;
     }
     if (max_rows == 0) return CRANE_HIP_OK;
-    const int row_bytes = kHeadDim * elem_size(dtype);
-    const int64_t run = (int64_t)page_rows * row_bytes;
-    const int64_t blocks = ((int64_t)max_rows * row_bytes + kBlockBytes - 1) / kBlockBytes;
+    const int64_t run = (int64_t)page_rows * row_bytes, block = (int64_t)unit * kThreads;
+    const int64_t blocks = ((int64_t)max_rows * row_bytes + block - 1) / block;
     if (blocks * Hkv > 0xffffffffLL / kThreads) return CRANE_HIP_E_INVALID;  // a grid's threads: 32 bits
     CopyArgs a;
     for (int p0 = 0; p0 < n_pools; p0 += kPools) {
@@ -235,11 +231,29 @@ extern "C" int crane_hip_copy_pages(void* const* pools, int n_pools, int64_t n_p
                 a.dst[i] = dst[i0 + i];
                 a.rows[i] = rows ? rows[i0 + i] : page_rows;
             }
-            hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(blocks * Hkv), (unsigned)ni, (unsigned)np),
-                               dim3(kThreads), 0, (hipStream_t)stream, a, (int)blocks, Hkv, run, row_bytes);
-            rc = launch_status(hipGetLastError());
+            const dim3 grid((unsigned)(blocks * Hkv), (unsigned)ni, (unsigned)np);
+            if (unit == 16)
+                hipLaunchKernelGGL(copy_pages_kernel<u32x4_v>, grid, dim3(kThreads), 0, stream, a, (int)blocks, Hkv, run,
+                                   row_bytes);
+            else
+                hipLaunchKernelGGL(copy_pages_kernel<u32x2_v>, grid, dim3(kThreads), 0, stream, a, (int)blocks, Hkv, run,
+                                   row_bytes);
+            const int rc = launch_status(hipGetLastError());
             if (rc) return rc;
         }
     }
     return CRANE_HIP_OK;
+}
+
+extern "C" int crane_hip_copy_pages(void* const* pools, int n_pools, int64_t n_pages, int page_rows, int Hkv, int D,
+                                    const int32_t* src, const int32_t* dst, const int32_t* rows, int n, int dtype,
+                                    void* stream) {
+    if (dtype != CRANE_HIP_F32 && dtype != CRANE_HIP_BF16) return CRANE_HIP_E_DTYPE;
+    if (D != kHeadDim) return CRANE_HIP_E_HEAD_DIM;
+    if (n_pools < 0 || n < 0 || Hkv <= 0 || Hkv > 65535) return CRANE_HIP_E_INVALID;
+    int32_t dummy = 0;  // no block table here; only the pool sizes are checked
+    const int rc = check_paged(n_pages, page_rows, &dummy, 1, Hkv);
+    if (rc) return rc;
+    return copy_page_rows(pools, n_pools, n_pages, page_rows, Hkv, kHeadDim * elem_size(dtype), src, dst, rows, n,
+                          (hipStream_t)stream);
 }

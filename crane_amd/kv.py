@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 from ._lib import CraneHipError, check
-from .ops import (HEAD_DIM, PREFILL_CAUSAL, _ORDERS, _dev, _dtype_code, _on_device, _prefill_flags, _ptr,
+from .ops import (F8_BLOCK_ROWS, HEAD_DIM, PREFILL_CAUSAL, _ORDERS, _dev, _dtype_code, _on_device, _prefill_flags, _ptr,
                   _rope_inputs, _stream)
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
@@ -226,19 +226,30 @@ class PagedKvCache:
     (set_batch) and the ops below act on it.  No KV row moves when a batch is
     set up or torn down, or when a sequence grows: Crane's pad/stack/extract
     copies (qwen3/modeling.rs:973-1102) and update_kv_cache's reallocation copy
-    (:333-355) have no counterpart here."""
+    (:333-355) have no counterpart here.
+
+    kv_dtype=torch.float8_e4m3fn holds the rows in 8 bits with a scale for every 32 of
+    them (ops.f8_pools); dtype is then that of q and of the rows that come in and go
+    out.  Appends quantise, decode and prefill are ops.attention_paged_f8;
+    attention_shared, score_mode and long_rows_one_rounding are refused."""
 
     def __init__(self, num_kv_heads: int, n_pages: int, dtype: torch.dtype = torch.bfloat16,
                  page_rows: int = 256, max_seqs: int = 64, max_pages_per_seq: int = 128,
-                 device: Optional[torch.device] = None, head_dim: int = HEAD_DIM):
+                 device: Optional[torch.device] = None, head_dim: int = HEAD_DIM,
+                 kv_dtype: Optional[torch.dtype] = None):
         if dtype not in _DT:
             raise CraneHipError(_lib.E_DTYPE, f"KV cache dtype {dtype}")
+        self.kv_dtype = dtype if kv_dtype is None else kv_dtype
+        if self.kv_dtype not in (dtype, torch.float8_e4m3fn):
+            raise CraneHipError(_lib.E_DTYPE, f"rows of {dtype} held as {kv_dtype}")
+        self._f8 = self.kv_dtype == torch.float8_e4m3fn
         self.num_kv_heads, self.dtype, self.page_rows, self.n_pages = num_kv_heads, dtype, page_rows, n_pages
         self.max_seqs, self.max_pages_per_seq = max_seqs, max_pages_per_seq
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
         handle = ctypes.c_void_p()
-        check(_lib.lib().crane_pkv_create(num_kv_heads, head_dim, _DT[dtype], page_rows, n_pages, max_seqs,
-                                          max_pages_per_seq, ctypes.byref(handle)), "crane_pkv_create")
+        create = _lib.lib().crane_pkv_create_f8 if self._f8 else _lib.lib().crane_pkv_create
+        check(create(num_kv_heads, head_dim, _DT[dtype], page_rows, n_pages, max_seqs, max_pages_per_seq,
+                     ctypes.byref(handle)), "crane_pkv_create")
         self._h = handle
         self._destroy = _lib.lib().crane_pkv_destroy  # bound now: usable during interpreter shutdown
         self._batch: List[int] = []
@@ -283,7 +294,7 @@ class PagedKvCache:
 
     @property
     def bytes(self) -> int:
-        """Bytes of the K and V pools."""
+        """Bytes of the K and V pools, scales included."""
         return int(_lib.lib().crane_pkv_bytes(self._h))
 
     @property
@@ -306,9 +317,18 @@ class PagedKvCache:
         return k.value, v.value, tbl.value, stride.value, dlen.value
 
     def pools(self):
-        """(K, V) tensors [n_pages, Hkv, page_rows, D] viewing the pools."""
+        """(K, V) tensors [n_pages, Hkv, page_rows, D] viewing the pools; of a cache in 8
+        bits (K, V, K scales, V scales) as ops.f8_pools has them."""
         k, v, _, _, _ = self._views()
         shape = (self.n_pages, self.num_kv_heads, self.page_rows, HEAD_DIM)
+        if self._f8:
+            ks, vs = ctypes.c_void_p(), ctypes.c_void_p()
+            check(_lib.lib().crane_pkv_scales_f8(self._h, ctypes.byref(ks), ctypes.byref(vs)), "crane_pkv_scales_f8")
+            blocks = shape[:2] + (self.page_rows // F8_BLOCK_ROWS,)
+            return tuple(torch.as_tensor(_DeviceView(p, s, "|u1"), device=self.device).view(t)
+                         for p, s, t in ((k, shape, torch.float8_e4m3fn), (v, shape, torch.float8_e4m3fn),
+                                         (ks.value, blocks, torch.float8_e8m0fnu),
+                                         (vs.value, blocks, torch.float8_e8m0fnu)))
         ts = "<f4" if self.dtype == torch.float32 else "<i2"
         out = []
         for p in (k, v):
@@ -357,6 +377,10 @@ class PagedKvCache:
         (score_mode as in ops.attention_decode)."""
         from .ops import decode_workspace, score_mode_code
         _check_q(q, 3, len(self._batch), self.dtype, self.device)
+        if self._f8:
+            if score_mode is not None:
+                raise CraneHipError(_lib.E_INVALID, "score_mode with a cache in 8 bits")
+            return self._attention("crane_pkv_attention_f8", q, scale, True, workspace)
         q = q.contiguous()
         B, Hq, D = q.shape
         need = _lib.lib().crane_hip_attn_decode_workspace(B, Hq, self.num_kv_heads, D, max(self.lengths),
@@ -377,6 +401,10 @@ class PagedKvCache:
         sequence) over its rows; [B, S, Hq*D].  long_rows_one_rounding as in
         ops.attention_prefill."""
         _check_q(q, 4, len(self._batch), self.dtype, self.device)
+        if self._f8:
+            if long_rows_one_rounding:
+                raise CraneHipError(_lib.E_INVALID, "long_rows_one_rounding with a cache in 8 bits")
+            return self._attention("crane_pkv_attention_f8", q, scale, causal, None)
         B, Hq, S, D = q.shape
         out = torch.empty((B, S, Hq * D), dtype=q.dtype, device=q.device)
         check(_lib.lib().crane_pkv_prefill(self._h, q.contiguous().data_ptr(), Hq, S, scale if scale else D ** -0.5,
@@ -390,20 +418,25 @@ class PagedKvCache:
         once for all that share them (ops.attention_shared_paged): q [B, Hq, D] (a
         decode step) gives [B, 1, Hq*D], q [B, Hq, S, D] gives [B, S, Hq*D]."""
         _check_q(q, 4 if q.dim() == 4 else 3, len(self._batch), self.dtype, self.device)
+        return self._attention("crane_pkv_attention_shared", q, scale, causal, workspace)
+
+    def _attention(self, name: str, q: torch.Tensor, scale: Optional[float], causal: bool,
+                   workspace: Optional[torch.Tensor]) -> torch.Tensor:
         q = q.contiguous()
         B, Hq, S = q.shape[0], q.shape[1], q.shape[2] if q.dim() == 4 else 1
         lib = _lib.lib()
-        need = lib.crane_pkv_shared_workspace(self._h, Hq, S)
+        sizes = lib.crane_pkv_attention_f8_workspace if self._f8 else lib.crane_pkv_shared_workspace
+        need = sizes(self._h, Hq, S)
         if workspace is not None:
             _dev(q, workspace)
         elif need:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         out = torch.empty((B, S, Hq * HEAD_DIM), dtype=q.dtype, device=q.device)
-        check(_on_device(q.device, lib.crane_pkv_attention_shared, (
+        check(_on_device(q.device, getattr(lib, name), (
             self._h, q.data_ptr(), Hq, S, HEAD_DIM ** -0.5 if scale is None else scale,
             PREFILL_CAUSAL if causal else 0, _ptr(workspace),
             workspace.numel() * workspace.element_size() if workspace is not None else 0, out.data_ptr(),
-            _stream(q.device))), "crane_pkv_attention_shared")
+            _stream(q.device))), name)
         return out
 
     def read_sequence(self, sid: int):

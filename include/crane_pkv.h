@@ -51,6 +51,14 @@ typedef struct crane_pkv crane_pkv;
  * max_seqs live sequences of up to max_pages_per_seq pages each. */
 int crane_pkv_create(int Hkv, int D, int dtype, int page_rows, int64_t n_pages, int max_seqs,
                      int max_pages_per_seq, crane_pkv** out);
+/* The same with rows held in 8 bits (crane_f8.h; Hkv * page_rows < 2^31): dtype is that
+ * of q and of the rows that come in and go out.  update, append_qkv and write_seq quantise
+ * as crane_hip_qknorm_rope_append_paged_f8 does, read_seq gives the codes' values, fork,
+ * truncate and compact keep codes and scales (a block cut to fewer rows keeps its scale).
+ * Attention is crane_pkv_attention_f8; decode, prefill and attention_shared return
+ * CRANE_HIP_E_DTYPE. */
+int crane_pkv_create_f8(int Hkv, int D, int dtype, int page_rows, int64_t n_pages, int max_seqs,
+                        int max_pages_per_seq, crane_pkv** out);
 void crane_pkv_destroy(crane_pkv* pkv);
 
 /* A new, empty sequence; its id is in [0, max_seqs). */
@@ -62,7 +70,7 @@ int crane_pkv_seq_free(crane_pkv* pkv, int seq_id);
 int64_t crane_pkv_seq_len(const crane_pkv* pkv, int seq_id);
 /* Pages on the free list. */
 int64_t crane_pkv_free_pages(const crane_pkv* pkv);
-/* Bytes of the K and V pools. */
+/* Bytes of the K and V pools, scales included. */
 uint64_t crane_pkv_bytes(const crane_pkv* pkv);
 
 /* Make seq_ids[0..B) (distinct live sequences, B <= max_seqs) the batch that
@@ -90,6 +98,15 @@ int crane_pkv_decode(const crane_pkv* pkv, const void* q, int Hq, float scale, i
  * CRANE_HIP_PREFILL_* bits of crane_hip_attn_prefill (1 = causal). */
 int crane_pkv_prefill(crane_pkv* pkv, const void* q, int Hq, int S, float scale, int flags, void* out,
                       void* stream);
+
+/* Attention of the last S rows of every batch sequence of a cache in 8 bits (q
+ * [B, Hq, S, D]; S = 1 is a decode step): crane_hip_attn_paged_f8, where the arguments
+ * and results are described.  With S > 1 every sequence holds S rows or more; with S = 1
+ * some sequence has rows, and one without gets zeros.  The workspace's size follows the
+ * batch and its lengths; 0: none is needed. */
+size_t crane_pkv_attention_f8_workspace(const crane_pkv* pkv, int Hq, int S);
+int crane_pkv_attention_f8(const crane_pkv* pkv, const void* q, int Hq, int S, float scale, int flags,
+                           void* workspace, size_t ws_bytes, void* out, void* stream);
 
 /* ---- Sequences that share pages.  fork, truncate and compact take n caches (the
  * layers of a model, of one device, driven with the same ids): all are changed, their
@@ -136,6 +153,9 @@ int crane_pkv_write_seq(crane_pkv* pkv, int seq_id, const void* k, const void* v
  * lengths (int32 [B]). */
 int crane_pkv_views(const crane_pkv* pkv, void** k_pool, void** v_pool, const int32_t** block_table,
                     int64_t* table_stride, const int32_t** dev_len);
+
+/* The pools of scales of a cache in 8 bits (crane_pkv_views gives the codes'). */
+int crane_pkv_scales_f8(const crane_pkv* pkv, void** k_scale, void** v_scale);
 
 #ifdef __cplusplus
 }
