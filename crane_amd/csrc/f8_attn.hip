@@ -193,16 +193,28 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint8_t* pool,
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(pool) + t.off, (short)0, t.bytes, 0x00020000);
 }
 
-// The scales of a tile's two blocks, as f32 (read through the constant address space: one
-// scalar load).  A byte of a block without rows may be anything; 254 keeps 0 times it 0.
+// The scales of a tile's two blocks, as f32.  A byte of a block without rows may be
+// anything; 254 keeps 0 times it 0.
 struct Scales {
     float of[2];
-    __device__ __forceinline__ void load(const uint8_t* pool, int64_t tile_off) {
-        const int64_t at = tile_off / (kRow * kBlockRows8);  // even
-        typedef const __attribute__((address_space(4))) uint32_t* words_t;
-        const uint32_t w = ((words_t)(uintptr_t)pool)[at >> 2] >> (8 * (at & 2));
+    // The first of them among the pool's: even.
+    static __device__ __forceinline__ int64_t at(int64_t tile_off) { return tile_off / (kRow * kBlockRows8); }
+    // From the aligned word that they are in.
+    __device__ __forceinline__ void set(uint32_t word, int64_t tile_off) {
+        const uint32_t w = word >> (8 * (at(tile_off) & 2));
         of[0] = scale_of(min(w & 255u, 254u));
         of[1] = scale_of(min((w >> 8) & 255u, 254u));
+    }
+    // That word: by one scalar load (through the constant address space) ...
+    __device__ __forceinline__ void load(const uint8_t* pool, int64_t tile_off) {
+        typedef const __attribute__((address_space(4))) uint32_t* words_t;
+        set(((words_t)(uintptr_t)pool)[at(tile_off) >> 2], tile_off);
+    }
+    // ... or by a vector load, for later.
+    static __device__ __forceinline__ uint32_t fetch(const uint8_t* pool, int64_t tile_off) {
+        const uint8_t* from = pool + (at(tile_off) & ~(int64_t)3);
+        return __builtin_amdgcn_raw_buffer_load_b32(
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), (short)0, 4, 0x00020000), 0, 0, 0);
     }
 };
 
@@ -564,7 +576,9 @@ template <int RT, int W> union StreamLds {
 // Workgroup x's item of `units` (pair, kv head) units with `tiles` row tiles each.  Ids that
 // are equal mod 8 run on one XCD: where the units come in eights it gets all tiles of a
 // unit, one after the other, and reads their keys through its own L2.  Otherwise a unit's
-// tiles are on all XCDs (4 units of 66 tiles, 6000 keys: on 4 XCDs 88 us, on all 52).
+// tiles are on all XCDs (4 units of 66 tiles, 6000 keys: on 4 XCDs 88 us, on all 52).  The
+// last tiles, which see most keys of a causal call, go first (8 prompts of 2048 tokens:
+// 297 us to 281).
 struct Item8 {
     int block, kvh, pair;
     __device__ __forceinline__ Item8(const Args8& a, int x) {
@@ -576,6 +590,7 @@ struct Item8 {
             block = rem >> 3;
             unit = 8 * c + (rem & 7);
         }
+        block = a.tiles - 1 - block;
         pair = unit / a.Hkv;
         kvh = unit - pair * a.Hkv;
     }
@@ -697,7 +712,14 @@ __global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1
 //
 // 32 rows to a wave and every wave on the same tile: the workgroup reads K and V once for
 // 128 rows.  Tiles are copied one ahead into the other of two buffers, a quarter of each by
-// every wave.  v_mfma_f32_32x32x16_bf16 (half the instructions and operand reads of the
+// every wave.  All of a tile's K is read before the first product, all of its V before the
+// softmax that hides it, and only then is the next tile's copy started: a transposed read
+// waits for every copy under way (the compiler cannot tell them apart).  With reads one
+// ahead of their use, copies started first and the scales by scalar loads 12 prompts' 1024
+// tokens over 9000 keys (28 / 4 heads, 2688 workgroups) took 1239 us, so 1130; with the
+// products' phases above the softmax in the CU's priority 1121 (1.0 PFLOP/s).  What is left
+// is the issue of instructions that are no products: without the conversions of codes
+// (timing only) 11% less, without the exponentials 8%.  v_mfma_f32_32x32x16_bf16 (half the instructions and operand reads of the
 // 16-row product for the same work): lane (i, h) = (lane % 32, lane / 32) holds, for query
 // row i, rows 8 a + 4 h + c of a product (register 4 a + c).  A's row x is key 16 (x / 16)
 // + 8 (x / 4 % 2) + 4 (x / 8 % 2) + x % 4 of 32, so that the lane holds keys 16 s + 8 h +
@@ -749,17 +771,19 @@ template <typename T> struct BlockRows {
     }
     // s[u][8 t + e]: the raw score of key 32 u + 16 t + 8 h + e.
     __device__ __forceinline__ void scores(f32x16_v (&s)[2], const Scales& ks, uint32_t buf) const {
+        u32x4_v k[2][4];
+#pragma unroll
+        for (int z = 0; z < 8; ++z) k[z >> 2][z & 3] = key(z >> 2, z & 3, buf);
+        __builtin_amdgcn_sched_barrier(0);  // all reads under way before the first is waited for
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const u32x4_v w = key(u, x, buf);
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
-                    s[u] = product(widen(w[2 * y], w[2 * y + 1], ks.of[u]), q[2 * x + y], s[u]);
-            }
+                    s[u] = product(widen(k[u][x][2 * y], k[u][x][2 * y + 1], ks.of[u]), q[2 * x + y], s[u]);
         }
     }
     __device__ __forceinline__ void mask(f32x16_v (&s)[2], int j, int hi) const {
@@ -799,7 +823,7 @@ template <typename T> struct BlockRows {
             }
         l += sum;
     }
-    template <class VALUE> __device__ __forceinline__ void accumulate(const f32x16_v (&p)[2], const Scales& vs, VALUE value) {
+    __device__ __forceinline__ void accumulate(const f32x16_v (&p)[2], const Scales& vs, const uint2 (&v)[2][2][4]) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -810,10 +834,7 @@ template <typename T> struct BlockRows {
                 Parts<T> w;
                 w.set(x);
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const uint2 y = value(u, t, d);
-                    o[d] = product(widen(y.x, y.y, vs.of[u]), w, o[d]);
-                }
+                for (int d = 0; d < 4; ++d) o[d] = product(widen(v[u][t][d].x, v[u][t][d].y, vs.of[u]), w, o[d]);
             }
     }
     // As Rows8::settle_nan; key j + 32 u + 16 t + 8 h + e.
@@ -878,7 +899,14 @@ __global__ __launch_bounds__(256, 2) void f8_block_kernel(Args8 a) {
         }
     };
     Pages8::Tile tile{0, 0};
-    if (end > 0) copy(tile = tile_at(0), 0);
+    uint32_t k_scales = 0, v_scales = 0;
+    auto start = [&](int j, int buf) __attribute__((always_inline)) {
+        if (j >= end) return;
+        copy(tile = tile_at(j), buf);
+        k_scales = Scales::fetch(a.k_scale, tile.off);
+        v_scales = Scales::fetch(a.v_scale, tile.off);
+    };
+    start(0, 0);
     const int r = row0 + st.i, s_of = min(r, R - 1) / a.G, head = min(r, R - 1) - s_of * a.G;
     const int at = r < R ? (int)(((int64_t)b * a.Hq + x.kvh * a.G + head) * a.S + s_of) : -1;
     const int hi = min(a.limit(n, s_of), end);
@@ -887,30 +915,33 @@ __global__ __launch_bounds__(256, 2) void f8_block_kernel(Args8 a) {
         st.q[y].load(reinterpret_cast<const T*>(a.q) + (int64_t)max(at, 0) * kHeadDim + 32 * (y >> 1) + 16 * st.h + 8 * (y & 1));
     for (int j = 0, half = 0; j < end; j += kTile, half ^= 1) {
         const uint32_t buf = half * kTileBytes;
-        Scales ks, vs;
-        ks.load(a.k_scale, tile.off);
-        vs.load(a.v_scale, tile.off);
         wait_memory();
         __syncthreads();  // the tile is there, and the one before it is used
-        if (j + kTile < end) copy(tile = tile_at(j + kTile), half ^ 1);
-        if (j >= max_hi) continue;  // none of the wave's rows
+        Scales ks, vs;
+        ks.set(__builtin_amdgcn_readfirstlane(k_scales), tile.off);
+        vs.set(__builtin_amdgcn_readfirstlane(v_scales), tile.off);
+        if (j >= max_hi) {  // none of the wave's rows
+            start(j + kTile, half ^ 1);
+            continue;
+        }
         f32x16_v s[2];
+        uint2 v[2][2][4];
+        __builtin_amdgcn_s_setprio(1);
         st.scores(s, ks, buf);
+#pragma unroll
+        for (int z = 0; z < 16; ++z) v[z >> 3][(z >> 2) & 1][z & 3] = st.value(z >> 3, (z >> 2) & 1, z & 3, buf);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        start(j + kTile, half ^ 1);
         const bool masked = j + kTile > min(min_hi, end);
         if (masked) st.mask(s, j, hi);
         st.settle(s, a.c);
         if (st.big) st.template weights<true>(s, a.c);
         else st.template weights<false>(s, a.c);
-        auto value = [&](int u, int t2, int d) __attribute__((always_inline)) { return st.value(u, t2, d, buf); };
-        if (masked && min_hi < end) {
-            uint2 v[2][2][4];
-#pragma unroll
-            for (int z = 0; z < 16; ++z) v[z >> 3][(z >> 2) & 1][z & 3] = value(z >> 3, (z >> 2) & 1, z & 3);
-            st.settle_nan(v, j, hi);
-            st.accumulate(s, vs, [&](int u, int t2, int d) __attribute__((always_inline)) { return v[u][t2][d]; });
-        } else {
-            st.accumulate(s, vs, value);
-        }
+        if (masked && min_hi < end) st.settle_nan(v, j, hi);
+        __builtin_amdgcn_s_setprio(1);
+        st.accumulate(s, vs, v);
+        __builtin_amdgcn_s_setprio(0);
     }
 
     const float l = halves_sum(st.l);
@@ -1002,12 +1033,13 @@ struct Plan8 {
 Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv, bool bf16) {
     Plan8 p{};
     const int64_t R = (int64_t)S * (Hq / Hkv), slots = 2 * kCus;  // two workgroups a CU, of any form
-    // The block form where its workgroups, whose waves all walk all keys, fill the device several
-    // times over.  8 prompts of 2048 tokens at 28 / 4 heads (3584 of them) 338 us, 402 in the
-    // stream form; 1024 tokens of 12 prompts of 9000 (2688) 1331 for 1368, of 4 (896) 494 for 441.
-    // f32: 16 times 256 tokens (1024 of them) 459 for 496, 4 times (256) 165 for 155.
+    // The block form where its workgroups, whose waves all walk all keys, fill the device.  1024
+    // tokens of 2 prompts of 1024 at 32 / 8 heads (512 of them) 40 us, 45 in the stream form, of
+    // 8192 267 for 285; of 1 prompt (256) 28 for 25, 167 for 143; 256 tokens of 7 to 3000 (448)
+    // 74 for 74, of 6 (384) 73 for 67.  f32, 256 tokens: 8 prompts (512) 184 for 224, 4 (256) 160
+    // for 150.
     const int64_t blocks = B * Hkv * ceil_div(R, 128);
-    p.block = blocks >= (bf16 ? 3 : 2) * slots;
+    p.block = blocks >= slots;
     p.rows = p.block ? 128 : R <= 16 ? 16 : 32;
     p.tiles = ceil_div(R, p.rows);
     const int64_t heads = Hkv * p.tiles;
