@@ -163,7 +163,8 @@ __device__ __forceinline__ Cut cut_at(const Args8& a, const Lengths& raw, int pa
 struct Pages8 {
     const int32_t* row;
     int stride, ids, page0, P, lane;
-    __device__ __forceinline__ Pages8(const Args8& a, int ln) : stride((int)a.rows.stride), P(a.rows.page_rows), lane(ln) {}
+    __device__ __forceinline__ Pages8(const Args8& a, int ln)
+        : stride((int)a.rows.stride), P(a.rows.page_rows), lane(ln) {}
     __device__ __forceinline__ void open(const Args8& a, int b, int begin) {
         row = a.rows.table + (int64_t)b * a.rows.stride;
         load(stride <= 64 ? 0 : begin / P);
@@ -515,6 +516,11 @@ template <typename T, int RT> struct Rows8 {
 // A wave copies its next tile of K and V (8 KiB each) into LDS of its own while it works
 // on the one in its registers: the copies are asynchronous, take whole 128-byte rows, and
 // hold no registers, which the reads could not do for the layouts the products want.
+//
+// Decode is bound by memory where there is enough of it: 8 sequences of 32768 rows at 64 / 8
+// heads (537 MB) 85.6 us, 6.3 TB/s, of which 78 are this kernel's at 6.9; 32 of 512 to 4096
+// at 32 / 8 (163 MB) 33.5, of which 4 are the first dependent loads (lengths, page, rows), 24
+// the rows at that rate and 4 the join; 1 of 300, whole, 6.2.
 template <typename T, int RT> struct Stream : Rows8<T, RT> {
     typedef Rows8<T, RT> Base;
     TileReads reads;
@@ -563,20 +569,23 @@ template <typename T, int RT> struct Stream : Rows8<T, RT> {
     }
 };
 
-// The LDS of a workgroup of W waves: their tiles, then their results.
-template <int RT, int W> union StreamLds {
+// The LDS of a workgroup: its waves' tiles, then their results.  (8 waves a workgroup where
+// no more than one a CU is launched took 6.4 us for 6.2 at 1 token of 300, 10.0 for 9.8 at
+// 2 of 1000, 14.1 for 13.1 at 16 times 8 of 1000.)
+constexpr int kWaves8 = 4;
+template <int RT> union StreamLds {
     static constexpr int kStride = kHeadDim + 4;  // f32 per row: 16 rows at one column hit different banks
-    __attribute__((aligned(1024))) uint8_t tile[W][2 * kTileBytes];
+    __attribute__((aligned(1024))) uint8_t tile[kWaves8][2 * kTileBytes];
     struct {
-        float o[W][16 * RT][kStride];
-        float m[W][16 * RT], l[W][16 * RT];
+        float o[kWaves8][16 * RT][kStride];
+        float m[kWaves8][16 * RT], l[kWaves8][16 * RT];
     } join;
 };
 
 // Workgroup x's item of `units` (pair, kv head) units with `tiles` row tiles each.  Ids that
 // are equal mod 8 run on one XCD: where the units come in eights it gets all tiles of a
 // unit, one after the other, and reads their keys through its own L2.  Otherwise a unit's
-// tiles are on all XCDs (4 units of 66 tiles, 6000 keys: on 4 XCDs 88 us, on all 52).  The
+// tiles are on all XCDs (4 units of 66 tiles, 6000 keys: on 4 XCDs 88 us, on all 65).  The
 // last tiles, which see most keys of a causal call, go first (8 prompts of 2048 tokens:
 // 297 us to 281).
 struct Item8 {
@@ -596,9 +605,9 @@ struct Item8 {
     }
 };
 
-template <typename T, int RT, int W>
-__global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1) void f8_stream_kernel(Args8 a) {
-    __shared__ StreamLds<RT, W> sm;
+template <typename T, int RT>
+__global__ __launch_bounds__(64 * kWaves8, RT == 1 || sizeof(T) == 2 ? 2 : 1) void f8_stream_kernel(Args8 a) {
+    __shared__ StreamLds<RT> sm;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Item8 x(a, blockIdx.x);
@@ -644,7 +653,7 @@ __global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1
 
     int at[RT], hi[RT];
     st.open(a, b, x.kvh, row0, n, end, at, hi);
-    constexpr int kStride = W * kTile;
+    constexpr int kStride = kWaves8 * kTile;
     for (; j < end; j += kStride) {
         st.ks.load(a.k_scale, tile.off);
         st.vs.load(a.v_scale, tile.off);
@@ -679,15 +688,15 @@ __global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1
     }
     __syncthreads();
     // 16 threads per row, 8 dims each.
-    for (int r = tid >> 4; r < 16 * RT && row0 + r < R; r += 4 * W) {
+    for (int r = tid >> 4; r < 16 * RT && row0 + r < R; r += 4 * kWaves8) {
         const int s = (row0 + r) / a.G, h = row0 + r - s * a.G, d = 8 * (tid & 15);
         const int place = (int)(((int64_t)b * a.Hq + x.kvh * a.G + h) * a.S + s);
         float top = sm.join.m[0][r];
 #pragma unroll
-        for (int w = 1; w < W; ++w) top = fmaxf(top, sm.join.m[w][r]);
+        for (int w = 1; w < kWaves8; ++w) top = fmaxf(top, sm.join.m[w][r]);
         float l = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
+        for (int w = 0; w < kWaves8; ++w) {
             const float f = fast_exp2((sm.join.m[w][r] - top) * a.c);
             float z[8];
             load8(&sm.join.o[w][r][d], z);
@@ -719,9 +728,11 @@ __global__ __launch_bounds__(64 * W, RT == 1 || sizeof(T) == 2 || W == 8 ? 2 : 1
 // tokens over 9000 keys (28 / 4 heads, 2688 workgroups) took 1239 us, so 1130; with the
 // products' phases above the softmax in the CU's priority 1121 (1.0 PFLOP/s).  What is left
 // is the issue of instructions that are no products: without the conversions of codes
-// (timing only) 11% less, without the exponentials 8%.  v_mfma_f32_32x32x16_bf16 (half the instructions and operand reads of the
-// 16-row product for the same work): lane (i, h) = (lane % 32, lane / 32) holds, for query
-// row i, rows 8 a + 4 h + c of a product (register 4 a + c).  A's row x is key 16 (x / 16)
+// (timing only) 11% less, without the exponentials 8%.
+//
+// v_mfma_f32_32x32x16_bf16 (half the instructions and operand reads of the 16-row product
+// for the same work): lane (i, h) = (lane % 32, lane / 32) holds, for query row i, rows 8 a
+// + 4 h + c of a product (register 4 a + c).  A's row x is key 16 (x / 16)
 // + 8 (x / 4 % 2) + 4 (x / 8 % 2) + x % 4 of 32, so that the lane holds keys 16 s + 8 h +
 // (0 .. 7), s = 0, 1: P^T of two products with V^T, whose bytes are one transposed read
 // each.
@@ -841,7 +852,10 @@ template <typename T> struct BlockRows {
     __device__ __forceinline__ void settle_nan(uint2 (&v)[2][2][4], int j, int hi) {
         uint32_t bad = 0;
 #pragma unroll
-        for (int x = 0; x < 16; ++x) bad |= nan_codes(v[x >> 3][(x >> 2) & 1][x & 3].x) | nan_codes(v[x >> 3][(x >> 2) & 1][x & 3].y);
+        for (int x = 0; x < 16; ++x) {
+            const uint2 c = v[x >> 3][(x >> 2) & 1][x & 3];
+            bad |= nan_codes(c.x) | nan_codes(c.y);
+        }
         if (!__any(bad != 0)) return;
         constexpr int kNone = 0x7fffffff;
 #pragma unroll
@@ -868,7 +882,7 @@ template <typename T> struct BlockRows {
 };
 
 template <typename T>
-__global__ __launch_bounds__(256, 2) void f8_block_kernel(Args8 a) {
+__global__ __launch_bounds__(64 * kWaves8, 2) void f8_block_kernel(Args8 a) {
     __shared__ BlockLds sm;
     constexpr int kRows = 128;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -912,7 +926,8 @@ __global__ __launch_bounds__(256, 2) void f8_block_kernel(Args8 a) {
     const int hi = min(a.limit(n, s_of), end);
 #pragma unroll
     for (int y = 0; y < 8; ++y)
-        st.q[y].load(reinterpret_cast<const T*>(a.q) + (int64_t)max(at, 0) * kHeadDim + 32 * (y >> 1) + 16 * st.h + 8 * (y & 1));
+        st.q[y].load(reinterpret_cast<const T*>(a.q) + (int64_t)max(at, 0) * kHeadDim + 32 * (y >> 1) + 16 * st.h +
+                     8 * (y & 1));
     for (int j = 0, half = 0; j < end; j += kTile, half ^= 1) {
         const uint32_t buf = half * kTileBytes;
         wait_memory();
@@ -1021,16 +1036,16 @@ __global__ __launch_bounds__(P == 1 ? 256 : 64 * P) void f8_join_kernel(Args8 a,
     Elem<T>::store(out + 1, n == 0 ? 0.f : x1 / den);
 }
 
-// How a call is launched: its form, the rows of a workgroup, its waves, and whether and into
-// how many chunks at most the sequences are cut.
+// How a call is launched: its form, the rows of a workgroup, and whether and into how many
+// chunks at most the sequences are cut.
 struct Plan8 {
     bool block;
-    int rows, waves;
+    int rows;
     int64_t tiles, pairs, items;
     size_t ml_off, cut_off, total;
 };
 
-Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv, bool bf16) {
+Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv) {
     Plan8 p{};
     const int64_t R = (int64_t)S * (Hq / Hkv), slots = 2 * kCus;  // two workgroups a CU, of any form
     // The block form where its workgroups, whose waves all walk all keys, fill the device.  1024
@@ -1040,14 +1055,15 @@ Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv, bool bf16) {
     // for 150.
     const int64_t blocks = B * Hkv * ceil_div(R, 128);
     p.block = blocks >= slots;
+    // Up to 16 rows half the accumulators: 32 decode steps (4 rows) 34.4 us, 36.3 with 32 rows a
+    // wave; f32 (7 rows) 10.9 for 14.1.
     p.rows = p.block ? 128 : R <= 16 ? 16 : 32;
     p.tiles = ceil_div(R, p.rows);
     const int64_t heads = Hkv * p.tiles;
-    // Cut where the sequences are fewer than the device holds and longer than the second kernel is
-    // worth (1 sequence of 1000 rows at 32 / 8 heads: 8.3 us whole, 9.4 cut; 4 of 2000: 14.7 and
-    // 10.1); whole ones up to one a CU have 8 waves.
-    if (!p.block && B <= kMostCut && B * heads < slots && max_kv > 1024) p.pairs = slots / heads;
-    p.waves = !p.block && !p.pairs && (bf16 || p.rows == 16) && B * heads <= kCus ? 8 : 4;
+    // Cut where the device holds more of them at once, and they are longer than the second kernel is
+    // worth (1 sequence of 1000 rows at 32 / 8 heads: 8.7 us whole, 9.2 cut; 4 of 2000: 14.2 and
+    // 10.0).
+    if (!p.block && B <= kMostCut && slots / heads > B && max_kv > 1024) p.pairs = slots / heads;
     p.items = (p.pairs ? p.pairs : B) * heads;
     const size_t rows = (size_t)(p.pairs * heads * p.rows);
     p.ml_off = rows * kHeadDim * sizeof(float);
@@ -1057,23 +1073,21 @@ Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv, bool bf16) {
 }
 
 template <typename T> int launch8(const Args8& a, const Plan8& p, int64_t n_rows, hipStream_t st) {
-    const dim3 grid((unsigned)p.items), threads(64 * p.waves);
-#define CRANE_F8_CASE(rt, w)                                           \
-    if (!p.block && p.rows == 16 * rt && p.waves == w)                 \
-        hipLaunchKernelGGL((f8_stream_kernel<T, rt, w>), grid, threads, 0, st, a);
-    CRANE_F8_CASE(1, 4)
-    CRANE_F8_CASE(1, 8)
-    CRANE_F8_CASE(2, 4)
-    if constexpr (sizeof(T) == 2) {
-        CRANE_F8_CASE(2, 8)
-    }
-#undef CRANE_F8_CASE
+    const dim3 grid((unsigned)p.items), threads(64 * kWaves8);
     if (p.block) hipLaunchKernelGGL(f8_block_kernel<T>, grid, threads, 0, st, a);
+    else if (p.rows == 32) hipLaunchKernelGGL((f8_stream_kernel<T, 2>), grid, threads, 0, st, a);
+    else hipLaunchKernelGGL((f8_stream_kernel<T, 1>), grid, threads, 0, st, a);
     int rc = launch_status(hipGetLastError());
     if (rc || !p.pairs) return rc;
-    if (p.pairs <= kJoinRegs * a.B)
-        hipLaunchKernelGGL((f8_join_kernel<T, 1>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a, (int)n_rows);
-    else if (p.pairs <= 4 * kJoinRegs * a.B)
+    // About a sequence's chunks, a wave for up to kJoinRegs of them: 1 sequence of 32768 rows at 64 /
+    // 8 heads (64 chunks) takes 34.0 us in all with 1 wave a row, 21.4 with 4, 19.7 with 16; of 8000
+    // at 32 / 8 (32) 13.3, 10.5, 11.0; 4 of 2000 (8) 9.8, 10.2, 10.7; 32 of up to 8192 (2) 33.5,
+    // 35.0, 38.2.
+    const int64_t chunks = std::min(p.pairs / a.B, ceil_div(a.max_kv, kLeastChunk * kTile));
+    if (chunks <= kJoinRegs)
+        hipLaunchKernelGGL((f8_join_kernel<T, 1>), dim3((unsigned)((n_rows + 3) / 4)), dim3(256), 0, st, a,
+                           (int)n_rows);
+    else if (chunks <= 4 * kJoinRegs)
         hipLaunchKernelGGL((f8_join_kernel<T, 4>), dim3((unsigned)n_rows), dim3(256), 0, st, a, (int)n_rows);
     else
         hipLaunchKernelGGL((f8_join_kernel<T, 16>), dim3((unsigned)n_rows), dim3(1024), 0, st, a, (int)n_rows);
@@ -1098,8 +1112,8 @@ using namespace crane;
 
 extern "C" size_t crane_hip_attn_paged_f8_workspace(int64_t max_kv, int B, int S, int Hq, int Hkv, int D, int dtype) {
     if (check_sizes8(max_kv, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0 || max_kv <= 0) return 0;
-    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16);
-    return p.items <= kMostThreads / (64 * p.waves) ? p.total : 0;
+    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv);
+    return p.items <= kMostThreads / (64 * kWaves8) ? p.total : 0;
 }
 
 extern "C" int crane_hip_attn_paged_f8(const void* q, const void* k_pool, const void* v_pool, const void* k_scale,
@@ -1118,8 +1132,8 @@ extern "C" int crane_hip_attn_paged_f8(const void* q, const void* k_pool, const 
     if (!q || !kv_len || !out) return CRANE_HIP_E_INVALID;
     if ((rc = check_pools8(k_pool, v_pool, k_scale, v_scale))) return rc;
     if (!aligned16(q) || !aligned16(out)) return CRANE_HIP_E_ALIGN;
-    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16);
-    if (p.items > kMostThreads / (64 * p.waves)) return CRANE_HIP_E_INVALID;
+    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv);
+    if (p.items > kMostThreads / (64 * kWaves8)) return CRANE_HIP_E_INVALID;
     if (p.total && (!workspace || ws_bytes < p.total || !aligned16(workspace))) return CRANE_HIP_E_WORKSPACE;
     Args8 a;
     a.q = q;

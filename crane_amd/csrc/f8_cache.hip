@@ -44,7 +44,8 @@ __device__ __forceinline__ void store_streamed(float* p, const float (&x)[4]) {
     __builtin_nontemporal_store(w, reinterpret_cast<u32x4_v*>(p));
 }
 __device__ __forceinline__ void store_streamed(bf16_t* p, const float (&x)[8]) {
-    const u32x4_v w = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    const u32x4_v w = {pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                       pack_bf16x2(x[6], x[7])};
     __builtin_nontemporal_store(w, reinterpret_cast<u32x4_v*>(p));
 }
 
@@ -103,7 +104,8 @@ struct RowValues {
     float a[8], b[8];  // dims 8l .., 64 + 8l ..
 };
 
-template <typename T> __device__ __forceinline__ void norm(RowValues& x, const float (&w1)[8], const float (&w2)[8], float eps) {
+template <typename T>
+__device__ __forceinline__ void norm(RowValues& x, const float (&w1)[8], const float (&w2)[8], float eps) {
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -179,7 +181,9 @@ template <bool STREAM, typename T> __device__ __forceinline__ void q_item(const 
     put8<STREAM>(dst + 64 + 8 * l, x.b);
 }
 
-// S = 1: every head row is an item of 8 lanes.  grid: q items, then k and v items.
+// S = 1: every head row is an item of 8 lanes (1 sequence 3.6 us, 4.2 through the blocks
+// kernel, whose workgroups hold 31 idle rows; 32 sequences at 32 / 8 heads 3.7 for 4.8: a
+// launch, and the rows' latency).  grid: q items, then k and v items.
 template <typename T> __global__ __launch_bounds__(256) void f8_append_token_kernel(Append<T> p) {
     const int l = threadIdx.x & 7;
     if ((int64_t)blockIdx.x < p.q_blocks) return q_item<false>(p, (int64_t)blockIdx.x * kItems + (threadIdx.x >> 3), l);
@@ -217,7 +221,9 @@ template <typename T> __global__ __launch_bounds__(256) void f8_append_token_ker
 }
 
 // Any S.  ROWS: k_rows and v_rows in place of qkv's.  The rows and q, each touched once, go
-// past the caches (8 prompts of 4096 tokens: 105 us to 99).  grid: q items, then one workgroup per (sequence, block, k or v head).
+// past the caches: 8 prompts of 4096 tokens, 28 / 4 heads (302 MB read, 268 MB written) 105
+// us to 98, 5.8 TB/s: the memory is the bound (a large copy reaches 5.2).  grid: q items,
+// then one workgroup per (sequence, block, k or v head).
 template <typename T, bool ROWS> __global__ __launch_bounds__(256) void f8_append_blocks_kernel(Append<T> p) {
     const int l = threadIdx.x & 7, r = threadIdx.x >> 3;
     if ((int64_t)blockIdx.x < p.q_blocks) return q_item<true>(p, (int64_t)blockIdx.x * kItems + r, l);
@@ -294,6 +300,8 @@ template <typename T> int launch_rows(Append<T> p, int B, hipStream_t st) {
 // Codes to values.  A workgroup takes 64 rows of a head (two blocks, within one page), a
 // thread 16 bytes of values at a time, so that a wave's stores are whole lines side by
 // side; all its loads are issued before the first store.  The stores go past the caches.
+// 16 sequences of 512 to 4096 rows, 8 heads, to bf16 (347 MB): 48 us, 7.2 TB/s (8-byte
+// stores through the caches 75); one of 333 to f32: 4.1, a launch and two dependent loads.
 // grid: (row tiles of all heads, k and v)
 constexpr int kReadRows = 2 * kBlockRows8;
 template <typename T>

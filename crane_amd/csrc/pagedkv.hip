@@ -817,7 +817,8 @@ int create(int Hkv, int D, int dtype, bool f8, int page_rows, int64_t n_pages, i
     int32_t dummy = 0;  // the table pointer is not known yet; only the sizes are checked here
     const int rc = crane::check_paged(n_pages, page_rows, &dummy, max_pages_per_seq, Hkv);
     if (rc) return rc;
-    if (f8 && (int64_t)Hkv * page_rows > 0x7fffffffLL) return CRANE_HIP_E_INVALID;  // a page's scales are one copied row
+    // a page's scales are one copied row
+    if (f8 && (int64_t)Hkv * page_rows > 0x7fffffffLL) return CRANE_HIP_E_INVALID;
     try {
         std::unique_ptr<crane_pkv> p(
             new crane_pkv(Hkv, D, dtype, f8, page_rows, n_pages, max_seqs, max_pages_per_seq));

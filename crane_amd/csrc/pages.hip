@@ -233,11 +233,11 @@ int crane::copy_page_rows(void* const* pools, int n_pools, int64_t n_pages, int 
             }
             const dim3 grid((unsigned)(blocks * Hkv), (unsigned)ni, (unsigned)np);
             if (unit == 16)
-                hipLaunchKernelGGL(copy_pages_kernel<u32x4_v>, grid, dim3(kThreads), 0, stream, a, (int)blocks, Hkv, run,
-                                   row_bytes);
+                hipLaunchKernelGGL(copy_pages_kernel<u32x4_v>, grid, dim3(kThreads), 0, stream, a, (int)blocks, Hkv,
+                                   run, row_bytes);
             else
-                hipLaunchKernelGGL(copy_pages_kernel<u32x2_v>, grid, dim3(kThreads), 0, stream, a, (int)blocks, Hkv, run,
-                                   row_bytes);
+                hipLaunchKernelGGL(copy_pages_kernel<u32x2_v>, grid, dim3(kThreads), 0, stream, a, (int)blocks, Hkv,
+                                   run, row_bytes);
             const int rc = launch_status(hipGetLastError());
             if (rc) return rc;
         }

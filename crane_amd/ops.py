@@ -656,7 +656,8 @@ def f8_pools(n_pages: int, num_kv_heads: int, page_rows: int = PAGE_ALIGN, devic
     scales 1."""
     shape = (n_pages, num_kv_heads, page_rows)
     codes = [torch.zeros(shape + (HEAD_DIM,), dtype=torch.uint8, device=device) for _ in "kv"]
-    scales = [torch.full(shape[:2] + (page_rows // F8_BLOCK_ROWS,), 127, dtype=torch.uint8, device=device) for _ in "kv"]
+    blocks = shape[:2] + (page_rows // F8_BLOCK_ROWS,)
+    scales = [torch.full(blocks, 127, dtype=torch.uint8, device=device) for _ in "kv"]
     return tuple([t.view(torch.float8_e4m3fn) for t in codes] + [t.view(torch.float8_e8m0fnu) for t in scales])
 
 
