@@ -272,6 +272,22 @@ def test_append_rows_of_wider_tensors(gpu):
     assert all(torch.equal(a, b) for a, b in zip(*outs))
 
 
+@gpu_test
+@pytest.mark.parametrize("S", [1, 5])
+def test_append_before_the_first_row(gpu, S):
+    """Rows before row 0 are not written; those from it on are, as in an empty sequence."""
+    from crane_amd import ops
+    cos, sin = (x.to(gpu) for x in tables(64, torch.bfloat16))
+    qkv = torch.randn((1, S, 3 * D), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(gpu)
+    got, want = ([x.clone() for x in Cache(1, [0], 1, ahead=S).to(gpu)[0]] for _ in "ab")
+    table = Cache(1, [0], 1, ahead=S).to(gpu)[1]
+    ops.qk_norm_rope_append_paged_f8(qkv, cos, sin, ints([7], gpu), got, table, ints([-3], gpu), 1)
+    if S > 3:
+        ops.qk_norm_rope_append_paged_f8(qkv[:, 3:].contiguous(), cos, sin, ints([10], gpu), want, table,
+                                         ints([0], gpu), 1)
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got, want))
+
+
 # ------------------------------------------------------------------ attention
 
 def reference(c, q, lens, scale, causal):
@@ -373,6 +389,13 @@ def test_chunk_of_many(gpu, dtype, B, S, Hq, Hkv, P, causal):
     """As many query rows as run in blocks of 128 that share their keys."""
     lens = [0, S // 2, S, S + 1] + [S + 37 * b % 300 for b in range(4, B)]
     check_attention(gpu, dtype, lens, S, Hq, Hkv, P, causal=causal, seed=B)
+
+
+@gpu_test
+@pytest.mark.parametrize("lens,S,Hq", [([17000] + [3] * 256, 1, 2), ([17000, 16385, 70], 3, 2), ([17000, 30], 128, 256)])
+def test_more_pages_than_lanes(gpu, lens, S, Hq):
+    """Sequences of 67 pages: whole, cut, and in blocks of 128 rows."""
+    check_attention(gpu, "bf16", lens, S, Hq, 1, seed=S)
 
 
 @gpu_test
@@ -597,6 +620,40 @@ def test_captured_step(gpu, B, Hq, Hkv, S):
         for graph, pools, out in graphs:
             assert all(torch.equal(a, b) for a, b in zip(out, want)), turn_
             assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(pools, mine))
+
+
+@gpu_test
+@pytest.mark.parametrize("S", [1, 30])
+def test_captured_attention_follows_the_lengths(gpu, S):
+    """One captured call, its bound the longest there may be, replayed as the lengths change, in
+    a workspace that others write to between the replays."""
+    from crane_amd import _lib, ops
+    top = 6000
+    c = Cache(3, [top, 5000, 40], 2)
+    pools, table = c.to(gpu)
+    n = ints([top, 5000, 40], gpu)
+    q = torch.randn((3, 4, S, D), device=gpu).bfloat16()
+    need = _lib.lib().crane_hip_attn_paged_f8_workspace(top, 3, S, 4, 2, D, _lib.BF16)
+    assert need > 0
+    ws = torch.empty(need, dtype=torch.uint8, device=gpu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.attention_paged_f8(q, pools, table, n, top, workspace=ws)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.attention_paged_f8(q, pools, table, n, top, workspace=ws)
+    for lens in ([top, 5000, 40], [1, 0, 7], [300, 4097, 0], [0, 0, 0], [64, 4999, 33], [top, 5000, 40]):
+        n.copy_(ints(lens, gpu))
+        ws.fill_(0xff)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.attention_paged_f8(q, pools, table, n, top)), lens
+        ref, mag, slack = reference(c, q.cpu(), lens, D ** -0.5, True)
+        tol = HALF["bf16"] * (ref.abs() + mag) + mag * slack
+        assert ((out.cpu().double() - ref).abs() <= tol).all(), lens
 
 
 @gpu_test
