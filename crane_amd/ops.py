@@ -661,36 +661,42 @@ def f8_pools(n_pages: int, num_kv_heads: int, page_rows: int = PAGE_ALIGN, devic
     return tuple([t.view(torch.float8_e4m3fn) for t in codes] + [t.view(torch.float8_e8m0fnu) for t in scales])
 
 
-def _f8_call(index: int, call, *args) -> int:
-    """call(*args, stream) with the device `index` current and its current stream (_on_device and
-    _stream, for callers that have the index and no device object)."""
+def _f8_stream(index: int) -> int:
+    """_stream, for callers that have the device's index and no device object."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _f8_call(index: int, call, args: tuple) -> int:
+    """_on_device, likewise."""
     if torch._C._cuda_getDevice() == index:
-        return call(*args, torch._C._cuda_getCurrentRawStream(index))
+        return call(*args)
     with torch.cuda.device(index):
-        return call(*args, torch._C._cuda_getCurrentRawStream(index))
+        return call(*args)
 
 
 def _f8_args(pools: Sequence[torch.Tensor], block_table: torch.Tensor, kv_len: torch.Tensor, B: int, index: int):
     """Checks of the pools, the block table and the lengths [B] on the device `index`: (K codes,
-    V codes, K scales, V scales, the pools' shape)."""
+    V codes, K scales, V scales, n_pages, Hkv, page_rows, pages of a row of the table)."""
     try:
         k, v, ks, vs = pools
     except ValueError:
         raise CraneHipError(_lib.E_INVALID, "pools must be (K codes, V codes, K scales, V scales)") from None
-    shape, tb = k.shape, block_table.shape
+    shape, tb, e4m3, e8m0 = k.shape, block_table.shape, torch.float8_e4m3fn, torch.float8_e8m0fnu
     # One expression for what every call passes; the cases that fail it are told apart below.
     if index == k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == block_table.get_device() == \
-            kv_len.get_device() and index >= 0 and \
-            len(shape) == 4 and shape[3] == HEAD_DIM and v.shape == shape and shape[2] % F8_BLOCK_ROWS == 0 and \
-            ks.shape == vs.shape == (shape[0], shape[1], shape[2] // F8_BLOCK_ROWS) and \
-            k.dtype is v.dtype is torch.float8_e4m3fn and ks.dtype is vs.dtype is torch.float8_e8m0fnu and \
-            block_table.dtype is kv_len.dtype is torch.int32 and len(tb) == 2 and tb[0] == B == kv_len.numel() and \
-            k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and \
-            block_table.is_contiguous() and kv_len.is_contiguous():
-        return k, v, ks, vs, shape
+            kv_len.get_device() and index >= 0 and len(shape) == 4 and len(tb) == 2:
+        n_pages, Hkv, page_rows, D = shape
+        rows, stride = tb
+        if D == HEAD_DIM and v.shape == shape and page_rows % F8_BLOCK_ROWS == 0 and \
+                ks.shape == vs.shape == (n_pages, Hkv, page_rows // F8_BLOCK_ROWS) and \
+                k.dtype is v.dtype is e4m3 and ks.dtype is vs.dtype is e8m0 and \
+                block_table.dtype is kv_len.dtype is torch.int32 and rows == B == kv_len.numel() and \
+                k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and \
+                block_table.is_contiguous() and kv_len.is_contiguous():
+            return k, v, ks, vs, n_pages, Hkv, page_rows, stride
     if _dev(k, v, ks, vs, block_table, kv_len).index != index:
         raise CraneHipError(_lib.E_INVALID, "tensors on different devices")
-    if not (k.dtype == v.dtype == torch.float8_e4m3fn and ks.dtype == vs.dtype == torch.float8_e8m0fnu):
+    if not (k.dtype == v.dtype == e4m3 and ks.dtype == vs.dtype == e8m0):
         raise CraneHipError(_lib.E_DTYPE, "pools must be float8_e4m3fn, scales float8_e8m0fnu")
     if len(shape) != 4 or shape[3] != HEAD_DIM or v.shape != shape or shape[2] % F8_BLOCK_ROWS:
         raise CraneHipError(_lib.E_INVALID, "pools must be [n_pages, Hkv, page_rows, D]")
@@ -718,8 +724,7 @@ def qk_norm_rope_append_paged_f8(qkv: torch.Tensor, cos: torch.Tensor, sin: torc
         raise CraneHipError(_lib.E_INVALID, "qkv must be [B, S, (Hq+2Hkv)*D]")
     B, S, width = shape
     index = qkv.get_device()
-    k, v, ks, vs, pshape = _f8_args(pools, block_table, cache_len, B, index)
-    n_pages, Hkv, page_rows, _ = pshape
+    k, v, ks, vs, n_pages, Hkv, page_rows, stride = _f8_args(pools, block_table, cache_len, B, index)
     dt, table = _dtype_code_of(dtype), cos.shape
     # What _rope_inputs checks, in one expression where the rows are contiguous.
     if (positions is cache_len or (positions.dtype is torch.int32 and positions.numel() == B and
@@ -727,9 +732,11 @@ def qk_norm_rope_append_paged_f8(qkv: torch.Tensor, cos: torch.Tensor, sin: torc
             qkv.is_contiguous() and width == (num_heads + 2 * Hkv) * HEAD_DIM and \
             index == cos.get_device() == sin.get_device() and cos.dtype is sin.dtype is dtype and \
             len(table) == 2 and table[1] == HEAD_DIM // 2 and sin.shape == table and cos.is_contiguous() and \
-            sin.is_contiguous() and order in _ORDERS and all([
-                w is None or (w.dtype is dtype and w.numel() == HEAD_DIM and w.get_device() == index and w.is_contiguous())
-                for w in (q_norm_w, k_norm_w)]):
+            sin.is_contiguous() and order in _ORDERS and \
+            (q_norm_w is None or (q_norm_w.dtype is dtype and q_norm_w.numel() == HEAD_DIM and
+                                  q_norm_w.get_device() == index and q_norm_w.is_contiguous())) and \
+            (k_norm_w is None or (k_norm_w.dtype is dtype and k_norm_w.numel() == HEAD_DIM and
+                                  k_norm_w.get_device() == index and k_norm_w.is_contiguous())):
         row_stride = width
     else:
         _rope_inputs(qkv, (num_heads + 2 * Hkv) * HEAD_DIM, cos, sin, positions, q_norm_w, k_norm_w, order)
@@ -737,11 +744,12 @@ def qk_norm_rope_append_paged_f8(qkv: torch.Tensor, cos: torch.Tensor, sin: torc
     q_out = qkv.new_empty((B, num_heads, S, HEAD_DIM))
     if B == 0:  # an empty block table has no address
         return q_out
-    rc = _f8_call(index, _lib.lib().crane_hip_qknorm_rope_append_paged_f8, qkv.data_ptr(), row_stride, _ptr(q_norm_w),
-                  _ptr(k_norm_w), eps, _ORDERS[order], cos.data_ptr(), sin.data_ptr(), HEAD_DIM // 2, table[0],
-                  positions.data_ptr(), q_out.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-                  n_pages, page_rows, block_table.data_ptr(), block_table.shape[1], cache_len.data_ptr(), B, S,
-                  num_heads, Hkv, HEAD_DIM, dt)
+    rc = _f8_call(index, _lib.lib().crane_hip_qknorm_rope_append_paged_f8, (
+        qkv.data_ptr(), row_stride, None if q_norm_w is None else q_norm_w.data_ptr(),
+        None if k_norm_w is None else k_norm_w.data_ptr(), eps, _ORDERS[order], cos.data_ptr(), sin.data_ptr(),
+        HEAD_DIM // 2, table[0], positions.data_ptr(), q_out.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
+        vs.data_ptr(), n_pages, page_rows, block_table.data_ptr(), stride, cache_len.data_ptr(), B, S, num_heads, Hkv,
+        HEAD_DIM, dt, _f8_stream(index)))
     if rc:
         check(rc, "qk_norm_rope_append_paged_f8")
     return q_out
@@ -775,8 +783,7 @@ def attention_paged_f8(q: torch.Tensor, pools: Sequence[torch.Tensor], block_tab
     if D != HEAD_DIM:
         raise CraneHipError(_lib.E_HEAD_DIM, "q must be [B, Hq, 128] or [B, Hq, S, 128]")
     index = q.get_device()
-    k, v, ks, vs, pshape = _f8_args(pools, block_table, kv_len, B, index)
-    n_pages, Hkv, page_rows, _ = pshape
+    k, v, ks, vs, n_pages, Hkv, page_rows, stride = _f8_args(pools, block_table, kv_len, B, index)
     if not q.is_contiguous():
         _contig(q, "q")
     dt = _dtype_code_of(q.dtype)
@@ -792,10 +799,11 @@ def attention_paged_f8(q: torch.Tensor, pools: Sequence[torch.Tensor], block_tab
     elif need:
         workspace = q.new_empty(need // q.element_size())  # need is a multiple of 16
         ws = workspace.data_ptr()
-    rc = _f8_call(index, _lib.lib().crane_hip_attn_paged_f8, q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(),
-                  vs.data_ptr(), n_pages, page_rows, block_table.data_ptr(), block_table.shape[1], kv_len.data_ptr(),
-                  max_kv, B, S, Hq, Hkv, HEAD_DIM, _SCALE if scale is None else scale,
-                  PREFILL_CAUSAL if causal else 0, ws, need, out.data_ptr(), dt)
+    rc = _f8_call(index, _lib.lib().crane_hip_attn_paged_f8, (
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), n_pages, page_rows,
+        block_table.data_ptr(), stride, kv_len.data_ptr(), max_kv, B, S, Hq, Hkv, HEAD_DIM,
+        _SCALE if scale is None else scale, PREFILL_CAUSAL if causal else 0, ws, need, out.data_ptr(), dt,
+        _f8_stream(index)))
     if rc:
         check(rc, "attention_paged_f8")
     return out
@@ -807,18 +815,17 @@ def read_paged_f8(pools: Sequence[torch.Tensor], block_table: torch.Tensor, kv_l
     [B, Hkv, max_kv, D] in `dtype` (exact in bf16 too), zeros from kv_len on."""
     B = block_table.shape[0] if block_table.dim() else 0
     index = block_table.get_device()
-    k, v, ks, vs, pshape = _f8_args(pools, block_table, kv_len, B, index)
-    n_pages, Hkv, page_rows, _ = pshape
+    k, v, ks, vs, n_pages, Hkv, page_rows, stride = _f8_args(pools, block_table, kv_len, B, index)
     dt = _dtype_code_of(dtype)
     if max_kv < 0:
         raise CraneHipError(_lib.E_INVALID, f"max_kv {max_kv}")
-    k_out = torch.empty((B, Hkv, max_kv, HEAD_DIM), dtype=dtype, device=block_table.device)
+    k_out = block_table.new_empty((B, Hkv, max_kv, HEAD_DIM), dtype=dtype)
     v_out = torch.empty_like(k_out)
     if B == 0:  # an empty block table has no address
         return k_out, v_out
-    rc = _f8_call(index, _lib.lib().crane_hip_read_paged_f8, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-                  n_pages, page_rows, block_table.data_ptr(), block_table.shape[1], kv_len.data_ptr(), max_kv, B, Hkv,
-                  HEAD_DIM, k_out.data_ptr(), v_out.data_ptr(), dt)
+    rc = _f8_call(index, _lib.lib().crane_hip_read_paged_f8, (
+        k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), n_pages, page_rows, block_table.data_ptr(), stride,
+        kv_len.data_ptr(), max_kv, B, Hkv, HEAD_DIM, k_out.data_ptr(), v_out.data_ptr(), dt, _f8_stream(index)))
     if rc:
         check(rc, "read_paged_f8")
     return k_out, v_out
