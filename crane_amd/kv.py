@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 from ._lib import CraneHipError, check
-from .ops import (F8_BLOCK_ROWS, HEAD_DIM, PREFILL_CAUSAL, _ORDERS, _dev, _dtype_code, _on_device, _prefill_flags, _ptr,
+from .ops import (F8_BLOCK_ROWS, HEAD_DIM, PREFILL_CAUSAL, _ORDERS, _contig, _dev, _dtype_code, _on_device, _prefill_flags, _ptr,
                   _rope_inputs, _stream)
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
@@ -347,10 +347,16 @@ class PagedKvCache:
 
     # ------------------------------------------------------------ ops
 
+    def _check_device(self, *ts: torch.Tensor) -> None:
+        if any(not t.is_cuda or self.device.index not in (None, t.get_device()) for t in ts):
+            raise CraneHipError(_lib.E_INVALID, f"tensors on {[str(t.device) for t in ts]}, cache on {self.device}")
+
     def update_kv_cache(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """Append k, v [B, Hkv, S, D] at every batch sequence's length."""
-        if k.shape != v.shape or k.dim() != 4 or k.shape[0] != len(self._batch) or k.shape[1] != self.num_kv_heads:
+        if k.shape != v.shape or k.dim() != 4 or k.shape[0] != len(self._batch) or \
+                k.shape[1] != self.num_kv_heads or k.shape[3] != HEAD_DIM:
             raise CraneHipError(_lib.E_INVALID, "k, v must be [B, Hkv, S, D] matching the batch")
+        self._check_device(k, v)
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise CraneHipError(_lib.E_DTYPE, f"k/v dtype {k.dtype} != cache dtype {self.dtype}")
         k, v = k.contiguous(), v.contiguous()
@@ -429,6 +435,7 @@ class PagedKvCache:
         need = sizes(self._h, Hq, S)
         if workspace is not None:
             _dev(q, workspace)
+            _contig(workspace, "workspace")
         elif need:
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         out = torch.empty((B, S, Hq * HEAD_DIM), dtype=q.dtype, device=q.device)
@@ -454,6 +461,7 @@ class PagedKvCache:
         """Replace a sequence's rows by k, v [Hkv, len, D] (set_kv_caches)."""
         if k.shape != v.shape or k.dim() != 3 or k.shape[0] != self.num_kv_heads or k.shape[2] != HEAD_DIM:
             raise CraneHipError(_lib.E_INVALID, "k, v must be [Hkv, len, D]")
+        self._check_device(k, v)
         if k.dtype != self.dtype or v.dtype != self.dtype:
             raise CraneHipError(_lib.E_DTYPE, f"k/v dtype {k.dtype} != cache dtype {self.dtype}")
         k, v = k.contiguous(), v.contiguous()

@@ -795,6 +795,7 @@ def attention_paged_f8(q: torch.Tensor, pools: Sequence[torch.Tensor], block_tab
     ws = None
     if workspace is not None:
         _dev(q, workspace)
+        _contig(workspace, "workspace")
         need, ws = workspace.numel() * workspace.element_size(), workspace.data_ptr()
     elif need:
         workspace = q.new_empty(need // q.element_size())  # need is a multiple of 16

@@ -77,7 +77,8 @@ size_t crane_hip_attn_paged_f8_workspace(int64_t max_kv, int B, int S, int Hq, i
  *          NULL when that is 0
  * out      [B, S, Hq*D]
  *
- * Scores, softmax and sums are f32; bf16 calls round the probabilities before the
+ * Scores, softmax and sums are f32 (sums of V's values up to 2^90 do not overflow: weights
+ * are up to 2^16 before the division); bf16 calls round the probabilities before the
  * product with V, f32 calls split q and the probabilities into three bf16 parts, which
  * hold all of their bits.  The order of the sums follows the sizes: two runs of one call
  * give the same bits. */

@@ -696,6 +696,10 @@ def test_given_workspace(gpu):
     with pytest.raises(_lib.CraneHipError) as e:
         ops.attention_paged_f8(q, pools, table, ints(lens, gpu), 5000, workspace=ws[:need - 16])
     assert e.value.code == _lib.E_WORKSPACE
+    for bad in (ws[:1].expand(need), torch.empty(2 * need, dtype=torch.uint8, device=gpu)[::2]):
+        with pytest.raises(_lib.CraneHipError) as e:
+            ops.attention_paged_f8(q, pools, table, ints(lens, gpu), 5000, workspace=bad)
+        assert e.value.code == _lib.E_INVALID
 
 
 # ------------------------------------------------------------------ refusals

@@ -251,6 +251,15 @@ def test_sizes_and_refusals(gpu):
     assert L.crane_pkv_attention_f8_workspace(plain._h, 2, 1) == 0
     a, b = ctypes.c_void_p(), ctypes.c_void_p()
     assert L.crane_pkv_scales_f8(plain._h, ctypes.byref(a), ctypes.byref(b)) == _lib.E_DTYPE
+    # rows on the host, of another width, and a workspace that is not what its size says
+    one = z[None, :, :1]
+    refused(_lib.E_INVALID, lambda: c.update_kv_cache(one.cpu(), one.cpu()))
+    refused(_lib.E_INVALID, lambda: c.update_kv_cache(one, one.cpu()))
+    refused(_lib.E_INVALID, lambda: c.update_kv_cache(one[..., :64], one[..., :64]))
+    other = c.add_sequence()
+    refused(_lib.E_INVALID, lambda: c.write_sequence(other, z.cpu(), z.cpu()))
+    refused(_lib.E_INVALID, lambda: c.decode(q, workspace=torch.empty(1, device=gpu).expand(1 << 20)))
+    c.free_sequence(other)
     # a batch without rows, and a full cache: nothing changes
     empty = c.add_sequence()
     c.set_batch([empty])
