@@ -824,15 +824,15 @@ template <typename T> struct BlockRows {
         }
     }
     template <bool BIG> __device__ __forceinline__ void weights(f32x16_v (&s)[2], float c) {
-        float sum = 0.f;
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 s[u][r] = fast_exp2(BIG ? (s[u][r] - m) * c : __builtin_fmaf(s[u][r], c, -mc));
-                sum += s[u][r];
+                sum[u] += s[u][r];
             }
-        l += sum;
+        l += sum[0] + sum[1];
     }
     __device__ __forceinline__ void accumulate(const f32x16_v (&p)[2], const Scales& vs, const uint2 (&v)[2][2][4]) {
 #pragma unroll
@@ -1051,7 +1051,7 @@ Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv) {
     // The block form where its workgroups, whose waves all walk all keys, fill the device.  1024
     // tokens of 2 prompts of 1024 at 32 / 8 heads (512 of them) 40 us, 45 in the stream form, of
     // 8192 267 for 285; of 1 prompt (256) 28 for 25, 167 for 143; 256 tokens of 7 to 3000 (448)
-    // 74 for 74, of 6 (384) 73 for 67.  f32, 256 tokens: 8 prompts (512) 184 for 224, 4 (256) 160
+    // 74 for 74, of 6 (384) 73 for 67.  f32, 256 tokens: 8 prompts (512) 180 for 224, 4 (256) 160
     // for 150.
     const int64_t blocks = B * Hkv * ceil_div(R, 128);
     p.block = blocks >= slots;
