@@ -606,7 +606,7 @@ struct Item8 {
 };
 
 template <typename T, int RT>
-__global__ __launch_bounds__(64 * kWaves8, RT == 1 || sizeof(T) == 2 ? 2 : 1) void f8_stream_kernel(Args8 a) {
+__global__ __launch_bounds__(64 * kWaves8, 2) void f8_stream_kernel(Args8 a) {
     __shared__ StreamLds<RT> sm;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1045,25 +1045,38 @@ struct Plan8 {
     size_t ml_off, cut_off, total;
 };
 
-Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv) {
+Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv, bool bf16) {
     Plan8 p{};
     const int64_t R = (int64_t)S * (Hq / Hkv), slots = 2 * kCus;  // two workgroups a CU, of any form
-    // The block form where its workgroups, whose waves all walk all keys, fill the device.  1024
-    // tokens of 2 prompts of 1024 at 32 / 8 heads (512 of them) 40 us, 45 in the stream form, of
-    // 8192 267 for 285; of 1 prompt (256) 28 for 25, 167 for 143; 256 tokens of 7 to 3000 (448)
-    // 74 for 74, of 6 (384) 73 for 67.  f32, 256 tokens: 8 prompts (512) 180 for 224, 4 (256) 160
-    // for 150.
+    // The block form where its workgroups, whose waves all walk all keys, fill the device: bf16,
+    // 1024 tokens of 2 prompts of 1024 at 32 / 8 heads (512 of them) 40 us, 45 in the stream form,
+    // of 8192 267 for 285; of 1 prompt (256) 28 for 25, 167 for 143; 256 tokens of 7 to 3000 (448)
+    // 74 for 74.  f32, whose 16 rows a wave hide more: 1024 tokens of 8 prompts of 1024 at 28 / 4
+    // (1792) 210 for 279, 256 tokens of 16 to 3000 (1024) 370 for 360.
     const int64_t blocks = B * Hkv * ceil_div(R, 128);
-    p.block = blocks >= slots;
-    // Up to 16 rows half the accumulators: 32 decode steps (4 rows) 34.4 us, 36.3 with 32 rows a
-    // wave; f32 (7 rows) 10.9 for 14.1.
-    p.rows = p.block ? 128 : R <= 16 ? 16 : 32;
+    p.block = blocks >= (bf16 ? 1 : 3) * slots;
+    // Else 16 or 32 rows a wave.  16 leave room for loads under way, 32 widen the codes once for
+    // twice the rows.  f32 takes 16: its q has three parts, and 32 rows spill (256 tokens of 4 to
+    // 3000 113 us for 151, 9 to 40 tokens of 4 to 4000 22 to 41 for 35 to 56).  bf16 takes 16 up to
+    // 16 rows (32 decode steps of 4 rows 34.4 for 36.3); past 32 while that is a workgroup a CU at
+    // most (8 sequences of 1000 to 4000 at 32 / 8 heads: 16 tokens, 256 of them, 22.6 for 26.4, 20
+    // tokens, 320 of them, 37.6 for 28.2); and from 17 to 32, where it reads the keys twice, while
+    // the chunks are short (5 tokens, 28 / 4: 4 sequences of up to 5000 15.7 for 17.1; 32 / 8: 4 of
+    // 16000 32.5 for 29.0, 16 of 5000 32.4 for 28.1).
+    auto most = [&](int rows) { return slots / (Hkv * ceil_div(R, rows)); };  // chunks that fit at once
+    const bool half = !bf16 || R <= 16 ||
+                      (R > 32 ? B * Hkv * ceil_div(R, 16) <= kCus : B * max_kv <= 1024 * most(16));
+    p.rows = p.block ? 128 : half ? 16 : 32;
     p.tiles = ceil_div(R, p.rows);
     const int64_t heads = Hkv * p.tiles;
     // Cut where the device holds more of them at once, and they are longer than the second kernel is
     // worth (1 sequence of 1000 rows at 32 / 8 heads: 8.7 us whole, 9.2 cut; 4 of 2000: 14.2 and
-    // 10.0).
-    if (!p.block && B <= kMostCut && slots / heads > B && max_kv > 1024) p.pairs = slots / heads;
+    // 10.0).  Decode, bound by memory: 40 of up to 4096 (1.6 chunks each fit) 44.7 whole, 37.5 cut,
+    // 56 (1.1) 49.6 and 51.9; f32 likewise.  bf16 past 16 rows is bound by instructions, and a
+    // workgroup a CU does: 24 tokens of 8 of up to 4000 (2.7) 28.4 whole, 32.0 cut, 5 tokens of 16
+    // of up to 5000 (4) 33.4 and 28.1.
+    const bool cut = bf16 && R > 16 ? most(p.rows) >= 3 * B : 2 * most(p.rows) > 3 * B;
+    if (!p.block && B <= kMostCut && cut && max_kv > 1024) p.pairs = most(p.rows);
     p.items = (p.pairs ? p.pairs : B) * heads;
     const size_t rows = (size_t)(p.pairs * heads * p.rows);
     p.ml_off = rows * kHeadDim * sizeof(float);
@@ -1075,8 +1088,8 @@ Plan8 plan8(int64_t max_kv, int B, int S, int Hq, int Hkv) {
 template <typename T> int launch8(const Args8& a, const Plan8& p, int64_t n_rows, hipStream_t st) {
     const dim3 grid((unsigned)p.items), threads(64 * kWaves8);
     if (p.block) hipLaunchKernelGGL(f8_block_kernel<T>, grid, threads, 0, st, a);
-    else if (p.rows == 32) hipLaunchKernelGGL((f8_stream_kernel<T, 2>), grid, threads, 0, st, a);
-    else hipLaunchKernelGGL((f8_stream_kernel<T, 1>), grid, threads, 0, st, a);
+    else if (p.rows == 16) hipLaunchKernelGGL((f8_stream_kernel<T, 1>), grid, threads, 0, st, a);
+    else hipLaunchKernelGGL((f8_stream_kernel<bf16_t, 2>), grid, threads, 0, st, a);
     int rc = launch_status(hipGetLastError());
     if (rc || !p.pairs) return rc;
     // About a sequence's chunks, a wave for up to kJoinRegs of them: 1 sequence of 32768 rows at 64 /
@@ -1112,7 +1125,7 @@ using namespace crane;
 
 extern "C" size_t crane_hip_attn_paged_f8_workspace(int64_t max_kv, int B, int S, int Hq, int Hkv, int D, int dtype) {
     if (check_sizes8(max_kv, B, S, Hq, Hkv, D, dtype) || B == 0 || S == 0 || max_kv <= 0) return 0;
-    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv);
+    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16);
     return p.items <= kMostThreads / (64 * kWaves8) ? p.total : 0;
 }
 
@@ -1132,7 +1145,7 @@ extern "C" int crane_hip_attn_paged_f8(const void* q, const void* k_pool, const 
     if (!q || !kv_len || !out) return CRANE_HIP_E_INVALID;
     if ((rc = check_pools8(k_pool, v_pool, k_scale, v_scale))) return rc;
     if (!aligned16(q) || !aligned16(out)) return CRANE_HIP_E_ALIGN;
-    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv);
+    const Plan8 p = plan8(max_kv, B, S, Hq, Hkv, dtype == CRANE_HIP_BF16);
     if (p.items > kMostThreads / (64 * kWaves8)) return CRANE_HIP_E_INVALID;
     if (p.total && (!workspace || ws_bytes < p.total || !aligned16(workspace))) return CRANE_HIP_E_WORKSPACE;
     Args8 a;

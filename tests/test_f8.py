@@ -382,6 +382,19 @@ def test_sequences_cut_into_chunks(gpu, dtype, lens, S, Hq, Hkv, max_kv):
 
 
 @gpu_test
+@pytest.mark.parametrize("dtype,lens,S,Hq,Hkv", [
+    ("bf16", [3000, 70, 2100, 0, 3000, 12, 1500, 900, 3000, 41, 2999, 3000], 5, 32, 8),  # 32 rows a wave, cut
+    ("bf16", [3000], 66, 64, 8), ("bf16", [4000] * 3 + [300], 20, 32, 8),                # the same, R > 32; whole
+    ("bf16", [2500, 1300, 20], 12, 16, 4), ("bf16", [1500] * 8, 9, 32, 8),               # 16 rows a wave, cut; whole
+    ("bf16", [2000, 1999], 5, 28, 4),
+    ("f32", [3000, 17, 2100], 12, 16, 4), ("f32", [1500] * 6, 24, 32, 8), ("f32", [2000], 150, 16, 2)])
+def test_rows_of_a_wave(gpu, dtype, lens, S, Hq, Hkv):
+    """16 and 32 query rows a wave, over sequences that are cut and that are not."""
+    check_attention(gpu, dtype, lens, S, Hq, Hkv, seed=S)
+    check_attention(gpu, dtype, lens, S, Hq, Hkv, seed=S, causal=False)
+
+
+@gpu_test
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dtype,B,S,Hq,Hkv,P", [("bf16", 13, 260, 56, 8, 256), ("bf16", 50, 129, 32, 8, 512),
                                                  ("f32", 9, 260, 56, 8, 256), ("f32", 70, 40, 32, 8, 256)])
