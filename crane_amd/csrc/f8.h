@@ -35,7 +35,7 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv) {
     }
     return make_uint2(w[0], w[1]);
 }
-// The values of four codes, times nothing.
+// Four codes' values, at scale 1.
 __device__ __forceinline__ void values4(uint32_t w, float* x) {
     const f32x2_v a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
     x[0] = a[0];

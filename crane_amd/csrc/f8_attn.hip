@@ -330,7 +330,7 @@ __device__ __forceinline__ int copy_from(int x, int lane) {
     const int row = 8 * x + (lane >> 3);
     return row * kRow + 16 * ((lane & 7) ^ permute8(row));
 }
-// A lane's reads of tiles that start at k and v.
+// A lane's reads of a tile that starts at k and v.
 struct TileReads {
     uint32_t k, v;
     __device__ __forceinline__ TileReads(uint32_t k_lds, uint32_t v_lds, int lane) {
@@ -340,13 +340,11 @@ struct TileReads {
     }
     // Dims 64 half + 16 g .. of the key that is row i of product kt = 2 u + b (4 rows on, or 4
     // chunks, bit 2 of the chunk flips).
-    __device__ __forceinline__ u32x4_v key(int kt, int half, uint32_t buf) const {
-        return lds_read16((k ^ (((kt & 1) ^ half) << 6)) + buf + 32 * (kt >> 1) * kRow + 4 * (kt & 1) * kRow);
+    __device__ __forceinline__ u32x4_v key(int kt, int half) const {
+        return lds_read16((k ^ (((kt & 1) ^ half) << 6)) + 32 * (kt >> 1) * kRow + 4 * (kt & 1) * kRow);
     }
     // Keys 32 u + 8 g .. of dim 16 n + i.
-    __device__ __forceinline__ uint2 value(int u, int n, uint32_t buf) const {
-        return lds_read_tr8((v ^ (16 * n)) + buf + 32 * u * kRow);
-    }
+    __device__ __forceinline__ uint2 value(int u, int n) const { return lds_read_tr8((v ^ (16 * n)) + 32 * u * kRow); }
 };
 
 // A wave's 16 RT query rows: their q and their running results.
@@ -549,11 +547,11 @@ template <typename T, int RT> struct Stream : Rows8<T, RT> {
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) k[kt][half] = reads.key(kt, half, 0);
+            for (int half = 0; half < 2; ++half) k[kt][half] = reads.key(kt, half);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int n = 0; n < 8; ++n) v[u][n] = reads.value(u, n, 0);
+            for (int n = 0; n < 8; ++n) v[u][n] = reads.value(u, n);
     }
     // The tile in registers, of keys from j on.  Every row sees the keys before min_hi.
     __device__ __forceinline__ void step(const Args8& a, int j, const int (&hi)[RT], int min_hi, int end) {
