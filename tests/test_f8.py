@@ -405,6 +405,21 @@ def test_chunk_of_many(gpu, dtype, B, S, Hq, Hkv, P, causal):
 
 
 @gpu_test
+@pytest.mark.parametrize("seed", range(40))
+def test_drawn_calls(gpu, seed):
+    """Sizes drawn over what the rules for rows, cuts and blocks tell apart."""
+    g = torch.Generator().manual_seed(100 + seed)
+    pick = lambda lo, hi: int(lo * (hi / lo) ** float(torch.rand((), generator=g)))  # noqa: E731
+    Hkv, G, S = pick(1, 9), pick(1, 17), 1 if seed % 3 == 0 else pick(2, 300)
+    longest = pick(300, 5000)
+    B = min(pick(1, 60), max(1, int(2e8 / (Hkv * G * S * longest))))
+    lens = [0 if float(torch.rand((), generator=g)) < 0.1 else pick(1, longest + 1) for _ in range(B)]
+    lens[0] = longest
+    check_attention(gpu, "f32" if seed % 4 == 1 else "bf16", lens, S, Hkv * G, Hkv, 256 * pick(1, 3), seed % 5 != 2,
+                    seed=seed, max_kv=longest if seed % 2 else None)
+
+
+@gpu_test
 @pytest.mark.parametrize("lens,S,Hq", [([17000] + [3] * 256, 1, 2), ([17000, 16385, 70], 3, 2), ([17000, 30], 128, 256)])
 def test_more_pages_than_lanes(gpu, lens, S, Hq):
     """Sequences of 67 pages: whole, cut, and in blocks of 128 rows."""
