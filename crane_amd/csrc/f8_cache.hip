@@ -197,14 +197,19 @@ template <typename T> __global__ __launch_bounds__(256) void f8_append_token_ker
     load_row<false>(x, p, b, p.Hq + hh, l);
     const int64_t off = p.rows.offset(b, p.Hkv, h, j);
     if (off < 0) return;
-    if (!is_v) {
-        if (pos < 0 || pos >= p.table_rows) return;
-        norm_rope(x, p, p.kw, pos, l);
-    }
     const int64_t at = off / kHeadDim / kBlockRows8;
     uint8_t* scale = (is_v ? p.v_scale : p.k_scale) + at;
     uint8_t* block = (is_v ? p.v_pool : p.k_pool) + at * kBlockRows8 * kHeadDim;
-    const int held = (int)(j % kBlockRows8), need = scale_byte(group8_max(largest(x)));
+    const int held = (int)(j % kBlockRows8);
+    if (!is_v) {
+        if (pos < 0 || pos >= p.table_rows) {
+            // the rows that come after it in the block keep to its scale
+            if (l == 0 && !held) *scale = kLeastScale;
+            return;
+        }
+        norm_rope(x, p, p.kw, pos, l);
+    }
+    const int need = scale_byte(group8_max(largest(x)));
     const int had = held ? *scale : 0, byte = max(need, had);
     if (byte > had && held) {
         const float down = scale_of(max(127 + had - byte, 0));
@@ -259,9 +264,12 @@ template <typename T, bool ROWS> __global__ __launch_bounds__(256) void f8_appen
     if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
     __syncthreads();
     const float amax = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-    if (amax < 0.f) return;  // no row is written
     const int64_t at = off / kHeadDim / kBlockRows8;
     uint8_t* scale = (is_v ? p.v_scale : p.k_scale) + at;
+    if (amax < 0.f) {  // no row is written: a block that begins with them gets a scale all the same
+        if (first >= len && threadIdx.x == 0) *scale = kLeastScale;
+        return;
+    }
     uint8_t* row = (is_v ? p.v_pool : p.k_pool) + off + r * kHeadDim;
     const int had = first < len ? *scale : 0, byte = max(scale_byte(amax), had);
     if (fresh) store_codes(row, x, byte, l);

@@ -46,8 +46,8 @@ extern "C" {
  *           the scale grew, the codes of the block's older rows are rounded to it
  *           (exactly, but for those that get subnormal)
  * A new row of q and k whose position is outside the tables is not written, and has no
- * part in the scale.  Nothing else is written: rows behind cache_len[b] + S keep their
- * codes.  A page that rows land in must be in one row of the block table only. */
+ * part in the scale (of a block that begins with such rows alone it is 2^-100).  Nothing
+ * else is written: rows behind cache_len[b] + S keep their codes.  A page that rows land in must be in one row of the block table only. */
 int crane_hip_qknorm_rope_append_paged_f8(const void* qkv, int64_t qkv_row_stride, const void* q_norm_w,
                                           const void* k_norm_w, float eps, int order, const void* cos,
                                           const void* sin, int64_t cs_stride, int64_t table_rows,

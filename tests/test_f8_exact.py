@@ -23,6 +23,41 @@ def set_rows(c, which, b, x, byte=127):
         c.scales[which, page, :, :-(-m // BLOCK)] = byte
 
 
+# ------------------------------------------------------------------ the append
+
+@gpu_test
+@pytest.mark.parametrize("stale", [0xff, 254, 200, 0])
+@pytest.mark.parametrize("skipped", [1, 2, 5, 40])
+@pytest.mark.parametrize("S", [1, 3])
+def test_block_that_begins_with_rows_that_are_not_written(gpu, S, skipped, stale):
+    """New rows whose positions are outside the tables begin blocks, over scales that earlier
+    owners left; the rows that come after them are as in blocks of the smallest scale."""
+    from crane_amd import ops
+    lens = [64, 0, 32]
+    cos, sin = (x.to(gpu) for x in f8.tables(200, torch.bfloat16))
+    g = torch.Generator().manual_seed(skipped)
+    first, then = (torch.randn((3, n, 8 * D), generator=g).to(gpu, torch.bfloat16) for n in (skipped, S))
+    outs = []
+    for byte in (stale, f8.FLOOR):
+        c = f8.Cache(2, lens, 2, ahead=skipped + S)
+        for b, n in enumerate(lens):
+            page, block = c.block(b, torch.arange(n, n + skipped + S, BLOCK))
+            c.scales[0, page, :, block] = byte
+        pools, table = c.to(gpu)
+        at = ints(lens, gpu)
+        ops.qk_norm_rope_append_paged_f8(first, cos, sin, ints([300, -skipped, 1000], gpu), pools, table, at, 4)
+        at = at + skipped
+        ops.qk_norm_rope_append_paged_f8(then, cos, sin, at, pools, table, at, 4)
+        outs.append(pools)
+    for b, n in enumerate(lens):
+        page, row = c.at(b, torch.arange(n + skipped, n + skipped + S))
+        for which in (0, 1):
+            codes, want = (p[which].view(torch.uint8).cpu()[page, :, row] for p in outs)
+            assert torch.equal(codes, want) and ((codes & 0x7f) != 0x7f).all() and (codes & 0x7f).any()
+            scales, want = (p[2 + which].view(torch.uint8).cpu()[page, :, row // BLOCK] for p in outs)
+            assert torch.equal(scales, want)
+
+
 # ------------------------------------------------------------------ attention
 
 @gpu_test
