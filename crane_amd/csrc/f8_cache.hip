@@ -160,7 +160,20 @@ __device__ __forceinline__ float largest(const RowValues& x) {
     return m;
 }
 
-__device__ __forceinline__ void store_codes(uint8_t* row, const RowValues& x, int byte, int l) {
+// Rounding to 4 bits takes magnitudes past 1.9375 2^127 to 2^128, which no type holds: under
+// scales that reach that far finite values stop at the largest code below it, 1.875 2^127.
+constexpr float kMostValue = 0x1.ep127f;
+constexpr int kLargeScale = 247;  // 448 times the next smaller scale is finite
+__device__ __forceinline__ void hold_finite(float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (fabsf(x[i]) < INFINITY) x[i] = fminf(fmaxf(x[i], -kMostValue), kMostValue);
+}
+__device__ __forceinline__ void store_codes(uint8_t* row, RowValues& x, int byte, int l) {
+    if (byte >= kLargeScale) {
+        hold_finite(x.a);
+        hold_finite(x.b);
+    }
     const float inv = scale_of(254 - byte);
     *reinterpret_cast<uint2*>(row + 8 * l) = codes8(x.a, inv);
     *reinterpret_cast<uint2*>(row + 64 + 8 * l) = codes8(x.b, inv);

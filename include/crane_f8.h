@@ -11,8 +11,8 @@
  * torch.float8_e4m3fn) and, for each, a pool of scales [n_pages, Hkv, page_rows / 32] of
  * one byte (torch.float8_e8m0fnu): byte x stands for 2^(x - 127) and is the scale of 32
  * rows of a head, a block.  A value is its code times its block's scale, which bf16
- * holds exactly.  Scale bytes are 1 to 254 (the append writes 27 and more); others give
- * unspecified values.  Rows are addressed as in the paged launchers: row j of sequence b
+ * holds exactly.  Scale bytes are 1 to 254 (the append writes 27 and more) and values finite,
+ * below 2^128; others give unspecified values.  Rows are addressed as in the paged launchers: row j of sequence b
  * is row j % page_rows of page block_table[b * table_stride + j / page_rows].
  *
  * Conventions are those of crane_hip.h: 0 or a CRANE_HIP_E_* status, arguments checked on
@@ -42,12 +42,14 @@ extern "C" {
  *   scale   the smallest 2^e >= 2^-100 with |x| <= 448 2^e for every finite x of the new
  *           rows; where the block holds rows of the sequence already, no smaller than
  *           its scale
- *   codes   x 2^-e rounded to nearest even; a NaN or an infinity becomes a NaN.  Where
- *           the scale grew, the codes of the block's older rows are rounded to it
- *           (exactly, but for those that get subnormal)
+ *   codes   x 2^-e rounded to nearest even, to 1.875 2^127 where that would be 2^128; a
+ *           NaN or an infinity becomes a NaN.  Where the scale grew, the codes of the
+ *           block's older rows are rounded to it (exactly, but for those that get
+ *           subnormal)
  * A new row of q and k whose position is outside the tables is not written, and has no
  * part in the scale (of a block that begins with such rows alone it is 2^-100).  Nothing
- * else is written: rows behind cache_len[b] + S keep their codes.  A page that rows land in must be in one row of the block table only. */
+ * else is written: rows behind cache_len[b] + S keep their codes.  A page that rows land in
+ * must be in one row of the block table only. */
 int crane_hip_qknorm_rope_append_paged_f8(const void* qkv, int64_t qkv_row_stride, const void* q_norm_w,
                                           const void* k_norm_w, float eps, int order, const void* cos,
                                           const void* sin, int64_t cs_stride, int64_t table_rows,

@@ -58,7 +58,54 @@ def test_block_that_begins_with_rows_that_are_not_written(gpu, S, skipped, stale
             assert torch.equal(scales, want)
 
 
+@gpu_test
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("S", [1, 3])
+@pytest.mark.parametrize("held", [0, 5])
+def test_finite_values_stay_finite(gpu, dtype, S, held):
+    """The largest values of the types: their codes times their scales are finite too, and read
+    so; an infinity is a NaN."""
+    from crane_amd import ops
+    t = DTYPES[dtype]
+    top = 2.0 ** 127
+    x = torch.tensor([torch.finfo(t).max, -torch.finfo(t).max, 1.9375 * top, 1.921875 * top, 1.875 * top, -1.8125 * top,
+                      1.78125 * top, 3e38, 1e38, -1e36, math.inf, math.nan], dtype=torch.float64).to(t)
+    want = torch.tensor([1.875, -1.875, 1.875, 1.875, 1.875, -1.75, 1.75, 1.75, 0.5625, -0.00585937500, math.nan, math.nan],
+                        dtype=torch.float64) * top
+    c = f8.Cache(2, [held], 1, ahead=S)
+    pools, table = c.to(gpu)
+    cos, sin = (y.to(gpu) for y in f8.tables(64, t))
+    qkv = torch.zeros((1, S, 3 * D), dtype=t)
+    qkv[0, S - 1, 2 * D:2 * D + len(x)] = x
+    at = ints([held], gpu)
+    ops.qk_norm_rope_append_paged_f8(qkv.to(gpu), cos, sin, at, pools, table, at, 1, order="rope_only")
+    v = ops.read_paged_f8(pools, table, at + S, held + S, torch.float32)[1][0, 0, held + S - 1, :len(x)]
+    assert torch.equal(torch.nan_to_num(v.cpu().double(), nan=7.0), torch.nan_to_num(want, nan=7.0))
+
+
 # ------------------------------------------------------------------ attention
+
+@gpu_test
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("S,G", [(6, 3), (140, 3), (500, 400)])
+def test_hidden_largest_values_reach_nobody(gpu, dtype, S, G):
+    """A chunk whose last token's v is the largest there is: earlier queries get what they get
+    with zeros in its place."""
+    from crane_amd import ops
+    t, n = DTYPES[dtype], S + 90
+    c = f8.Cache(8, [90], 1, ahead=S)
+    pools, table = c.to(gpu)
+    cos, sin = (x.to(gpu) for x in f8.tables(n, t))
+    qkv = torch.randn((1, S, (G + 2) * D), generator=torch.Generator().manual_seed(1)).to(t)
+    qkv[0, S - 1, (G + 1) * D:] = torch.finfo(t).max
+    at = ints([90], gpu)
+    q = ops.qk_norm_rope_append_paged_f8(qkv.to(gpu), cos, sin, at, pools, table, at, G)
+    got = ops.attention_paged_f8(q, pools, table, at + S, n)
+    page, row = (int(x) for x in c.at(0, n - 1))
+    pools[1].view(torch.uint8)[page, :, row] = 0
+    want = ops.attention_paged_f8(q, pools, table, at + S, n)
+    assert torch.isfinite(got[:, :-1]).all() and torch.equal(got[:, :-1], want[:, :-1])
+
 
 @gpu_test
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
