@@ -16,6 +16,10 @@ typedef float f32x2_v __attribute__((ext_vector_type(2)));
 
 // 2^(byte - 127) of a scale byte in 1 .. 254; 0 for 0.
 __device__ __forceinline__ float scale_of(int byte) { return __uint_as_float((uint32_t)byte << 23); }
+// 1 over it, subnormal for 254.
+__device__ __forceinline__ float inverse_scale(int byte) {
+    return byte < 254 ? scale_of(254 - byte) : __uint_as_float(0x400000u);
+}
 
 // The byte of the smallest scale 2^e with amax <= 448 2^e (448 = 1.75 2^8, the largest
 // code), from the bits of a finite amax >= 0.

@@ -174,7 +174,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, RowValues& x, int byte
         hold_finite(x.a);
         hold_finite(x.b);
     }
-    const float inv = scale_of(254 - byte);
+    const float inv = inverse_scale(byte);
     *reinterpret_cast<uint2*>(row + 8 * l) = codes8(x.a, inv);
     *reinterpret_cast<uint2*>(row + 64 + 8 * l) = codes8(x.b, inv);
 }

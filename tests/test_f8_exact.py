@@ -83,6 +83,29 @@ def test_finite_values_stay_finite(gpu, dtype, S, held):
     assert torch.equal(torch.nan_to_num(v.cpu().double(), nan=7.0), torch.nan_to_num(want, nan=7.0))
 
 
+@gpu_test
+@pytest.mark.parametrize("byte", [1, 26, 247, 253, 254])
+@pytest.mark.parametrize("S", [1, 3])
+def test_append_to_scales_that_no_append_writes(gpu, S, byte):
+    """Rows that join a block whose scale is any of the format's: the smallest, below the append's
+    own, and the largest."""
+    from crane_amd import ops
+    c = f8.Cache(2, [5], 1, ahead=S)
+    page, block = (int(x) for x in c.block(0, 0))
+    c.scales[1, page, :, block] = byte
+    pools, table = c.to(gpu)
+    qkv = torch.zeros((1, S, 3 * D))
+    x = torch.tensor([1.5, 1.0, -1.25, 0.75]) * 2.0 ** min(byte - 127, 127)
+    qkv[0, S - 1, 2 * D:2 * D + 4] = x
+    cos, sin = (y.to(gpu) for y in f8.tables(64, torch.float32))
+    at = ints([5], gpu)
+    ops.qk_norm_rope_append_paged_f8(qkv.to(gpu), cos, sin, at, pools, table, at, 1, order="rope_only")
+    have = int(pools[3].view(torch.uint8)[page, 0, block])
+    assert have == max(byte, f8.FLOOR)
+    want = f8.encode(x.double(), torch.tensor(have))
+    assert torch.equal(pools[1].view(torch.uint8)[page, 0, 5 + S - 1, :4].cpu(), want)
+
+
 # ------------------------------------------------------------------ attention
 
 @gpu_test
