@@ -29,6 +29,10 @@ namespace {
 
 constexpr float kNoMax = -FLT_MAX;  // m before the first key (finite: exp2(-inf - m) is 0, not NaN)
 constexpr float kSlack = 16.f, kMostMax = 0x1p26f;  // see Rows8
+// What the rounding of mc = m c leaves of it (0 where nobody counts from mc, see Rows8).
+__device__ __forceinline__ float left_of(float m, float mc, float c) {
+    return fabsf(mc) <= kMostMax ? __builtin_fmaf(m, c, -mc) : 0.f;
+}
 constexpr int kTile = 64;           // keys of a tile: two blocks, within one page
 constexpr int kRow = kHeadDim;      // bytes of a row of codes
 constexpr int kTileBytes = kTile * kRow;
@@ -362,7 +366,8 @@ template <typename T, int RT> struct Rows8 {
     Parts<T> q[RT][4];    // dims 16 g .., 16 g + 8 .., 64 + 16 g .., 64 + 16 g + 8 ..
     f32x4_v o[RT][8];     // dims 16 n + 4 g + r of row i
     f32x4_v l[RT];        // the sum over all keys, in all four
-    float m[RT], mc[RT];  // the raw score p's exponent counts from, and m c (0 before the first key)
+    float m[RT], mc[RT];  // the raw score p's exponent counts from, and m c rounded ..
+    float left[RT];       // .. and what that leaves: weights are exp2((s - m) c + left)  (all 0 before the first key)
     float limit[RT];      // a score past this moves m
     bool big;             // some m c has lost bits below 1: its row's exponents are (s - m) c
 
@@ -376,7 +381,7 @@ template <typename T, int RT> struct Rows8 {
 #pragma unroll
             for (int r = 0; r < 4; ++r) l[t][r] = 0.f;
             m[t] = limit[t] = kNoMax;
-            mc[t] = 0.f;
+            mc[t] = left[t] = 0.f;
         }
     }
     // This lane's rows of those from row0 on: their places in q [B, Hq, S] (-1: none), the keys
@@ -436,9 +441,11 @@ template <typename T, int RT> struct Rows8 {
 #pragma unroll
             for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
             if (__any(mx > limit[t])) {
-                const float to = fmaxf(m[t], groups_max(mx)), f = fast_exp2((m[t] - to) * c);
-                m[t] = to;
+                const float to = fmaxf(m[t], groups_max(mx)), was = left[t];
                 mc[t] = to == kNoMax ? 0.f : to * c;
+                left[t] = to == kNoMax ? 0.f : left_of(to, mc[t], c);
+                const float f = fast_exp2(__builtin_fmaf(m[t] - to, c, left[t] - was));
+                m[t] = to;
                 limit[t] = to == kNoMax ? kNoMax : to + kSlack / c;
                 big = __any(big || !(fabsf(mc[t]) <= kMostMax));
 #pragma unroll
@@ -450,16 +457,18 @@ template <typename T, int RT> struct Rows8 {
             }
         }
     }
-    // Weights p = exp2((s - m) c) in place of the scores.  s c - m c is one product with one
-    // rounding, which leaves every weight of the row the factor exp2(the rounding of m c); o / l
-    // takes that out again, but it overflows or vanishes where half a step of m c passes a
-    // hundred: past kMostMax (`big`) the difference is taken first.
+    // Weights p in place of the scores.  s c - mc is one product with one rounding, which leaves
+    // every weight the factor exp2(left), the rounding of m c; o / l takes that out again where
+    // one m stays, and where it moves, or results of several m are joined, `left` does (m c of
+    // 2^20 has half a step of 2^-5: a factor of 1.02).  It overflows or vanishes where half a
+    // step of m c passes a hundred: past kMostMax (`big`) the difference is taken first.
     template <bool BIG> __device__ __forceinline__ void weights(float (&s)[RT][16], float c) const {
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                s[t][e] = fast_exp2(BIG ? (s[t][e] - m[t]) * c : __builtin_fmaf(s[t][e], c, -mc[t]));
+                s[t][e] = fast_exp2(BIG ? __builtin_fmaf(s[t][e] - m[t], c, left[t])
+                                        : __builtin_fmaf(s[t][e], c, -mc[t]));
     }
     // o += P V, and l with it: a product of ones sums the weights as they are rounded.
     // value(u, n) as TileReads::value.
@@ -584,7 +593,7 @@ template <int RT> union StreamLds {
     __attribute__((aligned(1024))) uint8_t tile[kWaves8][2 * kTileBytes];
     struct {
         float o[kWaves8][16 * RT][kStride];
-        float m[kWaves8][16 * RT], l[kWaves8][16 * RT];
+        float m[kWaves8][16 * RT], left[kWaves8][16 * RT], l[kWaves8][16 * RT];
     } join;
 };
 
@@ -682,6 +691,7 @@ __global__ __launch_bounds__(64 * kWaves8, 2) void f8_stream_kernel(Args8 a) {
     for (int t = 0; t < RT; ++t) {
         if (st.g == 0) {
             sm.join.m[wave][16 * t + st.i] = st.m[t];
+            sm.join.left[wave][16 * t + st.i] = st.left[t];
             sm.join.l[wave][16 * t + st.i] = st.l[t][0];
         }
 #pragma unroll
@@ -703,7 +713,7 @@ __global__ __launch_bounds__(64 * kWaves8, 2) void f8_stream_kernel(Args8 a) {
         float l = 0.f, y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < kWaves8; ++w) {
-            const float f = fast_exp2((sm.join.m[w][r] - top) * a.c);
+            const float f = fast_exp2(__builtin_fmaf(sm.join.m[w][r] - top, a.c, -sm.join.left[w][r]));
             float z[8];
             load8(&sm.join.o[w][r][d], z);
             l += f * sm.join.l[w][r];
@@ -770,10 +780,10 @@ template <typename T> struct BlockRows {
     // parts hold all of their bits, over the lane's own keys (a product would spill more).
     static constexpr bool kProductSum = Parts<T>::kN == 1;
     std::conditional_t<kProductSum, f32x16_v, float> l;
-    float m, mc, limit;   // as Rows8
+    float m, mc, left, limit;  // as Rows8
     bool big;
     __device__ __forceinline__ BlockRows(int lane, const BlockLds& sm)
-        : i(lane & 31), h(lane >> 5), l{}, m(kNoMax), mc(0.f), limit(kNoMax), big(false) {
+        : i(lane & 31), h(lane >> 5), l{}, m(kNoMax), mc(0.f), left(0.f), limit(kNoMax), big(false) {
         const int k_row = (i & 16) | ((i & 4) << 1) | ((i & 8) >> 1) | (i & 3), v_row = 8 * h + ((lane & 15) >> 1);
         k_at = lds_at(sm.k) + k_row * kRow + 16 * (h ^ permute8_block(k_row));
         v_at = lds_at(sm.v) + v_row * kRow + 16 * (((lane >> 4) & 1) ^ permute8_block(v_row)) + 8 * (lane & 1);
@@ -825,9 +835,11 @@ template <typename T> struct BlockRows {
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
         if (__any(mx > limit)) {
-            const float to = fmaxf(m, halves_max(mx)), f = fast_exp2((m - to) * c);
-            m = to;
+            const float to = fmaxf(m, halves_max(mx)), was = left;
             mc = to == kNoMax ? 0.f : to * c;
+            left = to == kNoMax ? 0.f : left_of(to, mc, c);
+            const float f = fast_exp2(__builtin_fmaf(m - to, c, left - was));
+            m = to;
             limit = to == kNoMax ? kNoMax : to + kSlack / c;
             big = __any(big || !(fabsf(mc) <= kMostMax));
             if constexpr (kProductSum) {
@@ -848,7 +860,7 @@ template <typename T> struct BlockRows {
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[u][r] = fast_exp2(BIG ? (s[u][r] - m) * c : __builtin_fmaf(s[u][r], c, -mc));
+                s[u][r] = fast_exp2(BIG ? __builtin_fmaf(s[u][r] - m, c, left) : __builtin_fmaf(s[u][r], c, -mc));
                 if constexpr (!kProductSum) sum[u] += s[u][r];
             }
         if constexpr (!kProductSum) l += sum[0] + sum[1];

@@ -155,3 +155,48 @@ def test_rows_of_one_value(gpu, dtype, lens, S, Hq, Hkv):
         assert torch.equal(got.cpu().double(), want)
     else:
         assert ((got.cpu().double() - want).abs() <= (max(lens) + 64) * 2.0 ** -24 * want.abs()).all()
+
+
+def large_scores(c, lens, S, Hq, seed, rising):
+    """Keys whose scores are 2^20 + d, d whole numbers up to 11 in any order or up to 48 and
+    rising, all exact in f32, for queries of (2^20, 1, 0 ..); (q, [d] per sequence)."""
+    g = torch.Generator().manual_seed(seed)
+    steps = torch.tensor([*range(17), *range(18, 33, 2), *range(36, 49, 4)])
+    ds = []
+    for b, n in enumerate(lens):
+        d = steps[torch.arange(n) * len(steps) // max(n, 1)] if rising else torch.randint(0, 12, (n,), generator=g)
+        k = torch.zeros((n, D))
+        k[:, 0], k[:, 1] = 1.0, d.float()
+        set_rows(c, 0, b, k)
+        ds.append(d.double())
+    q = torch.zeros((len(lens), Hq, S, D))
+    q[..., 0], q[..., 1] = 2.0 ** 20, 1.0
+    return q, ds
+
+
+@gpu_test
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("lens,S,Hq,Hkv", FORMS)
+def test_weights_of_large_scores(gpu, dtype, lens, S, Hq, Hkv, rising):
+    """Scores near 2^20, where half a step of f32 is 2^-5 and a weight that far off 2%: the maxima
+    that tiles, waves and chunks count from differ, and their partial results have to join
+    as if there was no rounding.  A weight's exponent, 24 at most where the weight counts, is off
+    by 4 of its half steps (scale, log2 e, their product, the result's)."""
+    from crane_amd import ops
+    c = f8.Cache(5, lens, Hkv)
+    q, ds = large_scores(c, lens, S, Hq, 6, rising)
+    scale = float(torch.tensor(0.7))
+    pools, table = c.to(gpu)
+    got = ops.attention_paged_f8(q.to(gpu, DTYPES[dtype]), pools, table, ints(lens, gpu), max(lens), scale).cpu().double()
+    for b, n in enumerate(lens):
+        v = c.rows(1, b, n)
+        w = torch.exp(scale * (ds[b] - ds[b].max()))[None, :, None]
+        at = torch.arange(n - S, n)
+        den = w.cumsum(1)[:, at]
+        ref, mag = ((w * x).cumsum(1)[:, at] / den for x in (v, v.abs()))
+        tol = f8.HALF[dtype] * (ref.abs() + mag) + mag * (2 * 24 * 4 + n + 64) * 2.0 ** -24
+        have = got[b].view(S, Hkv, Hq // Hkv, D)
+        for i in range(Hq // Hkv):
+            bad = ~((have[:, :, i].transpose(0, 1) - ref).abs() <= tol)
+            assert not bad.any(), (b, i, float(((have[:, :, i].transpose(0, 1) - ref).abs() / tol).max()))
