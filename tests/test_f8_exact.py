@@ -200,3 +200,47 @@ def test_weights_of_large_scores(gpu, dtype, lens, S, Hq, Hkv, rising):
         for i in range(Hq // Hkv):
             bad = ~((have[:, :, i].transpose(0, 1) - ref).abs() <= tol)
             assert not bad.any(), (b, i, float(((have[:, :, i].transpose(0, 1) - ref).abs() / tol).max()))
+
+
+# Of f32 attention in the norm, random rows.  A weight's exponent is up to 16 in size and rounded
+# once, uniformly within 2^-20 (a root mean square of 3.8e-7 of the weight), its score is a sum
+# of 12 such steps of sums a quarter as large (3.3e-7), exp2, the weights' product and the sums
+# are off by a few half steps of 1 (2e-7); half as much again for the inputs at hand.
+NORM = 8e-7 * 1.5
+
+
+def parts(x, n):
+    """The first n bf16 parts of f32 values, each the rounding of what the ones before leave."""
+    out = torch.zeros_like(x)
+    for _ in range(n):
+        out = out + (x - out).bfloat16().float()
+    return out
+
+
+@pytest.mark.parametrize("n", [33, 700, 5000])
+@pytest.mark.parametrize("q_parts,w_parts", [(3, 3), (2, 3), (3, 2)])
+def test_the_norm_tells_parts_apart(n, q_parts, w_parts):
+    """With two bf16 parts of q or of the weights the result is past the bound, with three it is
+    a tenth of it (everything else exact)."""
+    c = f8.Cache(1, [n], 1)
+    q = 1.5 * torch.randn((1, 4, 1, D), generator=torch.Generator().manual_seed(2))
+    ref, _, _ = f8.reference(c, q, [n], D ** -0.5, True)
+    s = parts(q[0, :, 0], q_parts).double() @ c.rows(0, 0, n)[0].T * D ** -0.5
+    w = torch.exp(s - s.amax(1, keepdim=True))
+    out = parts(w.float(), w_parts).double() @ c.rows(1, 0, n)[0] / w.sum(1, keepdim=True)
+    off = (out.view(-1) - ref.view(-1)).norm() / ref.norm()
+    assert off < NORM / 10 if q_parts == w_parts == 3 else off > NORM
+
+
+@gpu_test
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,S,Hq,Hkv", FORMS)
+def test_f32_keeps_its_bits(gpu, lens, S, Hq, Hkv, causal):
+    """f32 calls carry q and the weights in three parts: within a bound that two exceed."""
+    from crane_amd import ops
+    c = f8.Cache(7, lens, Hkv)
+    q = 1.5 * torch.randn((len(lens), Hq, S, D), generator=torch.Generator().manual_seed(8))
+    pools, table = c.to(gpu)
+    got = ops.attention_paged_f8(q.to(gpu), pools, table, ints(lens, gpu), max(lens), causal=causal).cpu().double()
+    ref, _, _ = f8.reference(c, q, lens, D ** -0.5, causal)
+    assert (got - ref).norm() <= NORM * ref.norm(), float((got - ref).norm() / ref.norm())
