@@ -67,8 +67,8 @@ size_t crane_hip_attn_paged_f8_workspace(int64_t max_kv, int B, int S, int Hq, i
  *
  * q        [B, Hq, S, D] (S = 1: a decode step's [B, Hq, D])
  * kv_len   [B] int32, device: rows of every sequence, its S new ones included; query i
- *          sits at row kv_len[b] - S + i.  kv_len[b] <= max_kv; rows past max_kv are
- *          not attended
+ *          sits at row kv_len[b] - S + i.  kv_len[b] <= max_kv (a longer sequence is
+ *          taken as one of max_kv rows)
  * flags    CRANE_HIP_PREFILL_CAUSAL: query i sees rows [0, kv_len[b] - S + i]; 0: every
  *          query sees all kv_len[b] rows.  A query that sees none gets zeros.  Rows a
  *          query does not see have no influence on it, whatever they hold.  Rows of a

@@ -202,6 +202,19 @@ def test_weights_of_large_scores(gpu, dtype, lens, S, Hq, Hkv, rising):
             assert not bad.any(), (b, i, float(((have[:, :, i].transpose(0, 1) - ref).abs() / tol).max()))
 
 
+@gpu_test
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("S,Hq,bound", [(1, 4, 300), (5, 4, 300), (40, 2, 1100), (200, 400, 256)])
+def test_a_longer_sequence_counts_as_the_bound(gpu, S, Hq, bound, causal):
+    """Chunks of a sequence past max_kv: its queries sit at the last rows of max_kv."""
+    from crane_amd import ops
+    c = f8.Cache(2, [1400, 90], 1)
+    pools, table = c.to(gpu)
+    q = torch.randn((2, Hq, S, D), generator=torch.Generator().manual_seed(3)).to(gpu, torch.bfloat16)
+    a, b = (ops.attention_paged_f8(q, pools, table, ints([n, 90], gpu), bound, causal=causal) for n in (1400, bound))
+    assert torch.equal(a, b)
+
+
 # Of f32 attention in the norm, random rows.  A weight's exponent is up to 16 in size and rounded
 # once, uniformly within 2^-20 (a root mean square of 3.8e-7 of the weight), its score is a sum
 # of 12 such steps of sums a quarter as large (3.3e-7), exp2, the weights' product and the sums
