@@ -1169,7 +1169,7 @@ extern "C" int crane_hip_attn_paged_f8(const void* q, const void* k_pool, const 
     int rc = check_sizes8(max_kv, B, S, Hq, Hkv, D, dtype);
     if (rc) return rc;
     if (flags & ~CRANE_HIP_PREFILL_CAUSAL) return CRANE_HIP_E_INVALID;
-    if (!(scale > 0.0f) || !__builtin_isfinite(scale)) return CRANE_HIP_E_INVALID;
+    if (!(scale > 0.0f) || !__builtin_isfinite(scale * kLog2e)) return CRANE_HIP_E_INVALID;
     if ((rc = check_paged(n_pages, page_rows, block_table, table_stride, Hkv))) return rc;
     if (max_kv <= 0) return CRANE_HIP_E_INVALID;
     if (max_kv > table_stride * page_rows) return CRANE_HIP_E_CAPACITY;

@@ -73,7 +73,7 @@ size_t crane_hip_attn_paged_f8_workspace(int64_t max_kv, int B, int S, int Hq, i
  *          query sees all kv_len[b] rows.  A query that sees none gets zeros.  Rows a
  *          query does not see have no influence on it, whatever they hold.  Rows of a
  *          page id outside [0, n_pages) count as zeros
- * scale    of the scores, positive
+ * scale    of the scores, positive, its product with log2 e finite
  * workspace device scratch of crane_hip_attn_paged_f8_workspace(...) bytes, 16-byte
  *          aligned, any contents; calls that overlap in time must not share one.  May be
  *          NULL when that is 0

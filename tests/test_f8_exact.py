@@ -257,3 +257,9 @@ def test_f32_keeps_its_bits(gpu, lens, S, Hq, Hkv, causal):
     got = ops.attention_paged_f8(q.to(gpu), pools, table, ints(lens, gpu), max(lens), causal=causal).cpu().double()
     ref, _, _ = f8.reference(c, q, lens, D ** -0.5, causal)
     assert (got - ref).norm() <= NORM * ref.norm(), float((got - ref).norm() / ref.norm())
+
+
+@pytest.mark.parametrize("scale,code", [(3.4e38, 1), (2.4e38, 1), (2.3e38, 0), (1e-45, 0)])
+def test_scales_whose_product_overflows_are_refused(scale, code):
+    """In base 2 the exponents' factor is scale log2 e: past 2^128 every weight would be NaN."""
+    assert f8._attn(scale=scale) == code
