@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "attn_lanes.h"
 #include "f8.h"
 #include "shared_plan.h"
 
@@ -36,8 +37,6 @@ __device__ __forceinline__ float left_of(float m, float mc, float c) {
 constexpr int kTile = 64;           // keys of a tile: two blocks, within one page
 constexpr int kRow = kHeadDim;      // bytes of a row of codes
 constexpr int kTileBytes = kTile * kRow;
-
-typedef unsigned int u32x4_v __attribute__((ext_vector_type(4)));
 
 struct Args8 {
     const void* q;
@@ -68,11 +67,6 @@ struct Args8 {
         return ((int64_t)b * S + s) * Hq + (bh - b * Hq);
     }
 };
-
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
-    return (int64_t)((uint64_t)hi << 32 | lo);
-}
 
 // The sequences' chunks.  All are cut into chunks of the same number of tiles, few enough
 // of them that there are no more than `pairs` in all: as many workgroups as the device
@@ -296,23 +290,6 @@ template <typename T, typename C> __device__ __forceinline__ C product(u32x4_v a
 }
 __device__ __forceinline__ u32x4_v ones() { return u32x4_v{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}; }
 
-// Maximum over the four lane groups of a query row; every lane gets it.  (A row swap of a
-// value with itself leaves each row's value in one result and its neighbour's in the
-// other.)
-__device__ __forceinline__ float groups_max(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t v = __float_as_uint(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-    const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
-// LDS byte addresses, and reads at them.
-__device__ __forceinline__ uint32_t lds_at(const void* p) {
-    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
-}
-__device__ __forceinline__ u32x4_v lds_read16(uint32_t at) {
-    return *(const __attribute__((address_space(3))) u32x4_v*)(uintptr_t)at;
-}
 typedef int i32x2_v __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2_v lds_i32x2_v;
 // Within 16 lanes, lane x gets column x of the 8 rows x 16 columns of bytes that the lanes
@@ -759,17 +736,6 @@ struct BlockLds {
 // The chunk permutation of these tiles: 16 rows of a K read, and 8 rows x 2 chunks of a V
 // read, do not meet in a bank.
 __device__ __forceinline__ int permute8_block(int row) { return ((row >> 3) & 1) | (row & 6); }
-
-__device__ __forceinline__ float halves_max(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float halves_sum(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 
 template <typename T> struct BlockRows {
     const int i, h;

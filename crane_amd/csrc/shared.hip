@@ -57,7 +57,7 @@
 #include <cstring>
 #include <type_traits>
 
-#include "common.h"
+#include "attn_lanes.h"
 #include "shared_plan.h"
 #include "../../include/crane_shared.h"
 
@@ -72,7 +72,6 @@ constexpr size_t kHalfLds = 81920;   // half of a CU's LDS
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* base, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
 }
-typedef unsigned int u32x4_v __attribute__((ext_vector_type(4)));
 // NT: read once, streamed past the caches.
 template <bool NT = false> __device__ __forceinline__ u32x4_v buf_load16(__amdgpu_buffer_rsrc_t r, int off) {
     return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? 2 : 0);
@@ -156,13 +155,6 @@ template <bool SHARED> struct Segment {
         return ((int64_t)x.b * a.Hq + kvh * a.G + x.h) * a.S + x.s;
     }
 };
-
-// A wave-uniform value the compiler holds in vector registers (a buffer resource made
-// of such would be read lane by lane).
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
-    return (int64_t)((uint64_t)hi << 32 | lo);
-}
 
 // A chunk's pages, one id per lane: those from the chunk's first on, or the whole table
 // row where it fits (then the load waits for nothing).
@@ -340,17 +332,6 @@ template <typename T> struct Row {
         return sizeof(T) == 2 ? 32 * g + 8 * r + n0 : 16 * n0 + 16 * g + 4 * r;
     }
 };
-
-// Maximum over the four lane groups of a query row; every lane gets it.  (A row swap
-// of a value with itself leaves each row's value in one result and its neighbour's in
-// the other.)
-__device__ __forceinline__ float groups_max(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t v = __float_as_uint(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-    const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
 
 // p = exp2(s c - m) of the step's scores; MOVE: m moved to the largest so far first, and
 // o and l scaled to it.
@@ -709,13 +690,6 @@ template <int N> __device__ __forceinline__ void wait_copies() {
     __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
-// LDS reads at byte addresses.
-__device__ __forceinline__ uint32_t lds_at(const void* p) {
-    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
-}
-__device__ __forceinline__ u32x4_v lds_read16(uint32_t at) {
-    return *(const __attribute__((address_space(3))) u32x4_v*)(uintptr_t)at;
-}
 typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4_v;
 typedef __attribute__((address_space(3))) s16x4_v lds_s16x4_v;
 // Within 16 lanes, lane x gets column x of the 4 rows x 16 columns of bf16 that the
@@ -727,17 +701,6 @@ __device__ __forceinline__ f32x16_v mfma(u32x4_v a, u32x4_v b, f32x16_v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_v, a), __builtin_bit_cast(bf16x8_v, b), c,
                                                    0, 0, 0);
 }
-__device__ __forceinline__ float halves_max(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float halves_sum(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // A wave's share of a block: Q, o, m and l of its 32 rows, and one tile's work.  Lane
 // (n, h) = (lane % 32, lane / 32) holds, for row n, keys 32 b + 8 (r / 4) + 4 h + r % 4 in
 // register r of score block b, and dims 32 d + 8 (r / 4) + 4 h + r % 4 in register r of
