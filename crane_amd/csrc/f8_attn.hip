@@ -243,12 +243,13 @@ __device__ __forceinline__ f32x16_v mfma(u32x4_v a, u32x4_v b, f32x16_v c) {
 // Eight values as an MFMA operand: bf16 calls round them once, f32 calls carry them in
 // three parts, each the rounding of what the ones before leave.
 //
-// The weights of bf16 calls in one part: results are 0.0019 to 0.0023 off (relative, in the
-// norm), 0.00166 where only they themselves are rounded.  A second part reaches that and is
-// a product, two subtractions and a conversion more: 8 sequences of 32768 rows 86.3 us to
-// 87.2, 32 of up to 4096 33.4 to 34.6, 5 drafted tokens of 16 28.2 to 30.2, 1 of 300 6.2 to
-// 6.7, 1024 tokens of 4 prompts over 9000 keys 405 to 562.  The sum that divides is of the
-// weights as they are rounded, so that what a rounding moves all weights by goes out again.
+// The weights of bf16 calls in one part: results are 0.0017 to 0.0023 off (relative, in the
+// norm; 0.00166 is the rounding of the results themselves), against values that a cache in 8
+// bits holds to 0.026.  A second part reaches 0.00166 and is a product, two subtractions and
+// a conversion more: 8 sequences of 32768 rows 86.3 us to 87.2, 32 of up to 4096 33.4 to
+// 34.6, 5 drafted tokens of 16 28.2 to 30.2, 1 of 300 6.2 to 6.7, 1024 tokens of 4 prompts
+// over 5000 to 9000 keys 405 to 562.  The sum that divides is of the weights as they are
+// rounded, so that what a rounding moves all weights by goes out again.
 template <typename T> struct Parts;
 template <> struct Parts<bf16_t> {
     static constexpr int kN = 1;
@@ -512,7 +513,7 @@ template <typename T, int RT> struct Rows8 {
 // Decode is bound by memory where there is enough of it: 8 sequences of 32768 rows at 64 / 8
 // heads (537 MB) 85.6 us, 6.3 TB/s, of which 78 are this kernel's at 6.9; 32 of 512 to 4096
 // at 32 / 8 (163 MB) 33.5, of which 4 are the first dependent loads (lengths, page, rows), 24
-// the rows at that rate and 4 the join; 1 of 300, whole, 6.2.
+// the rows at that rate and 4 the join; 1 of 300, whole, 6.3.
 template <typename T, int RT> struct Stream : Rows8<T, RT> {
     typedef Rows8<T, RT> Base;
     TileReads reads;
@@ -718,10 +719,11 @@ __global__ __launch_bounds__(64 * kWaves8, 2) void f8_stream_kernel(Args8 a) {
 // softmax that hides it, and only then is the next tile's copy started: a transposed read
 // waits for every copy under way (the compiler cannot tell them apart).  With reads one
 // ahead of their use, copies started first and the scales by scalar loads 12 prompts' 1024
-// tokens over 9000 keys (28 / 4 heads, 2688 workgroups) took 1239 us, so 1130; with the
-// products' phases above the softmax in the CU's priority 1121 (1.0 PFLOP/s).  What is left
-// is the issue of instructions that are no products: without the conversions of codes
-// (timing only) 11% less, without the exponentials 8%.
+// tokens over 5000 to 9000 keys (28 / 4 heads, 2688 workgroups) took 1239 us, so 1130; with
+// the products' phases above the softmax in the CU's priority 1121 (1.0 PFLOP/s, as over
+// 9000 keys each), with the weights' sum as a product 0.7% more.  What is left is the issue
+// of instructions that are no products: without the conversions of codes (timing only) 11%
+// less, without the exponentials 8%.
 //
 // v_mfma_f32_32x32x16_bf16 (half the instructions and operand reads of the 16-row product
 // for the same work): lane (i, h) = (lane % 32, lane / 32) holds, for query row i, rows 8 a

@@ -18,8 +18,8 @@ import torch
 
 from . import _lib
 from ._lib import CraneHipError, check
-from .ops import (F8_BLOCK_ROWS, HEAD_DIM, PREFILL_CAUSAL, _ORDERS, _contig, _dev, _dtype_code, _on_device, _prefill_flags, _ptr,
-                  _rope_inputs, _stream)
+from .ops import (F8_BLOCK_ROWS, HEAD_DIM, PREFILL_CAUSAL, _ORDERS, _contig, _dev, _dtype_code, _on_device,
+                  _prefill_flags, _ptr, _rope_inputs, _stream)
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 

@@ -110,7 +110,8 @@ int crane_pkv_attention_f8(const crane_pkv* pkv, const void* q, int Hq, int S, f
 
 /* ---- Sequences that share pages.  fork, truncate and compact take n caches (the
  * layers of a model, of one device, driven with the same ids): all are changed, their
- * copies in one launch where they need the same ones, or none (a launch error aside).
+ * copies in one launch where they need the same ones (in 8 bits two: codes and scales),
+ * or none (a launch error aside).
  * They do not synchronise; work queued on other streams that still reads the pages
  * concerned is the caller's to order. */
 
